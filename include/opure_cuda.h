@@ -283,6 +283,80 @@ opure_status opure_gemv(opure_ctx *ctx, const opure_gemv_args *a);
 opure_status opure_argmax_decode(opure_ctx *ctx, const unsigned long long *keys, uint32_t n,
                                  uint32_t *out_idx, float *out_val);
 
+/* ---- microscaled (MX) linear layers ----------------------------------------------------
+ * Matrices whose rows are cut into blocks of 32 values that share one power-of-two scale
+ * (the Open Compute Project's Microscaling Formats, MXFP4 and MXFP8). The reference has one
+ * scale per tensor at most (GEMV_Quant, shaders/Opure_GEMV_Quant.usf:52-93); these calls are
+ * an addition: 4-bit weights at 0.53 bytes each, and 8- or 4-bit activations, multiplied on
+ * the tensor cores' block-scaled formats.
+ *
+ * Layout. kp = cols rounded up to a multiple of 128; columns cols .. kp - 1 hold code 0, and
+ * blocks of nothing else scale 0.
+ *   codes   row-major. OPURE_MX_FP8: E4M3, one byte each, kp bytes per row. OPURE_MX_FP4:
+ *           E2M1, two per byte, the even column in the low half, kp / 2 bytes per row.
+ *   scales  E8M0: byte b stands for 2^(b - 127), 255 for NaN. Tiles of 128 rows x 4 blocks
+ *           (128 columns), 512 bytes each, tile (r / 128) * (kp / 128) + k / 128, and in it
+ *           byte (r % 32) * 16 + (r / 32 % 4) * 4 + k / 32 % 4. Rows that fill the last tile
+ *           are never written, and what they hold has no effect.
+ * codes must be 32-byte aligned, scales 16-byte aligned (opure_alloc gives 256).
+ *
+ * A block's scale is 2^(floor(log2 m) - e), m its largest magnitude and e the exponent of
+ * the format's largest value (2 or 8), at least 2^-127; values are divided by it, rounded to
+ * the nearest code (ties to even) and limited to the format's largest value (6 or 448). A
+ * block that holds an infinity or NaN gets scale 255 and codes 0: all of it reads as NaN. */
+typedef enum opure_type { OPURE_F32 = 0, OPURE_F16 = 1, OPURE_BF16 = 2 } opure_type;
+enum { OPURE_MX_FP4 = 4, OPURE_MX_FP8 = 8 }; /* bits per code */
+typedef struct opure_mx_matrix {
+    uint8_t *codes;
+    uint8_t *scales;
+    uint32_t rows, cols;
+    uint32_t format;           /* OPURE_MX_FP4 or OPURE_MX_FP8                    */
+} opure_mx_matrix;
+/* Bytes of the two parts (0 for an unknown format). */
+size_t opure_mx_code_bytes(uint32_t format, uint32_t rows, uint32_t cols);
+size_t opure_mx_scale_bytes(uint32_t rows, uint32_t cols);
+
+/* x [out->rows][x_stride] of an opure_type, x_stride >= out->cols, to MX. */
+opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, size_t x_stride,
+                               const opure_mx_matrix *out);
+/* The values that an MX matrix stands for, rounded to an opure_type: y [x->rows][y_stride]. */
+opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void *y, uint32_t y_type,
+                                 size_t y_stride);
+
+/* s = x + residual;  out = MX(s / sqrt(mean(s^2) + eps) * gain), per row, s in fp32: the
+ * residual add (Opure_AddRes.usf:29-43) and RMSNorm (Opure_RMSNorm.usf:31-79) before a
+ * linear layer in one pass. residual and sum share x's type and stride. */
+typedef struct opure_mx_norm_args {
+    const void *x;             /* [out.rows][x_stride]                            */
+    uint32_t x_type;           /* opure_type                                      */
+    size_t x_stride;           /* >= out.cols                                     */
+    const void *residual;      /* or NULL: s = x                                  */
+    void *sum;                 /* or NULL: s is not kept. May be x or residual     */
+    const uint16_t *gain;      /* [out.cols] fp16, or NULL (identity)             */
+    float eps;
+    opure_mx_matrix out;       /* either format                                   */
+} opure_mx_norm_args;
+opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a);
+
+/* y[i][r] = sum_k x[i][k] w[r][k] in fp32, w in OPURE_MX_FP4, x in either format, with one
+ * of opure_gemv's epilogues:
+ *   OPURE_EPI_STORE   y = acc
+ *   OPURE_EPI_ADD     y = residual + acc (residual may be y; same type and stride)
+ *   OPURE_EPI_SWIGLU  w is [gate; up] (w.rows even): out = MX(silu(gate) * up), the next
+ *                     product's x, out.cols = w.rows / 2; y is not used
+ * Any number of rows, from one token to a long prompt. */
+typedef struct opure_mx_gemm_args {
+    opure_mx_matrix w;         /* [rows][cols]                                    */
+    opure_mx_matrix x;         /* [tokens][cols]                                  */
+    uint32_t epilogue;
+    uint32_t y_type;           /* opure_type of y and residual                    */
+    void *y;                   /* [x.rows][y_stride], y_stride >= w.rows          */
+    size_t y_stride;
+    const void *residual;      /* OPURE_EPI_ADD                                   */
+    opure_mx_matrix out;       /* OPURE_EPI_SWIGLU: [x.rows][w.rows / 2]          */
+} opure_mx_gemm_args;
+opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a);
+
 /* ---- decode-step bookkeeping ----------------------------------------------------
  * A decode step computes one token vector per entry. opure_step_begin / opure_step_end
  * bracket the per-layer kernels of a step so that a captured step graph replays with no

@@ -19,6 +19,9 @@ W_F16, W_Q8 = 0, 1
 PRO_NONE, PRO_RMSNORM = 0, 1
 EPI_STORE, EPI_ADD, EPI_SWIGLU, EPI_ARGMAX = 0, 1, 2, 3
 SPEC_GREEDY, SPEC_REJECTION = 0, 1
+F32, F16, BF16 = 0, 1, 2
+VALUE_TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+MX_FP4, MX_FP8 = 4, 8
 
 P, u8, u32, u64, f32, i32, sz = (C.c_void_p, C.c_uint8, C.c_uint32, C.c_uint64, C.c_float,
                                  C.c_int32, C.c_size_t)
@@ -70,6 +73,21 @@ class SampleArgs(C.Structure):
                 ("out", P), ("keys", P)]
 
 
+class MxMatrix(C.Structure):
+    """A microscaled matrix (opure_mx_matrix): device pointers of its codes and scales."""
+    _fields_ = [("codes", P), ("scales", P), ("rows", u32), ("cols", u32), ("format", u32)]
+
+
+class MxNormArgs(C.Structure):
+    _fields_ = [("x", P), ("x_type", u32), ("x_stride", sz), ("residual", P), ("sum", P),
+                ("gain", P), ("eps", f32), ("out", MxMatrix)]
+
+
+class MxGemmArgs(C.Structure):
+    _fields_ = [("w", MxMatrix), ("x", MxMatrix), ("epilogue", u32), ("y_type", u32), ("y", P),
+                ("y_stride", sz), ("residual", P), ("out", MxMatrix)]
+
+
 class DeviceInfo(C.Structure):
     _fields_ = [("device", i32), ("sm_count", i32), ("cc_major", i32), ("cc_minor", i32),
                 ("hbm_bytes", u64), ("l2_bytes", u64), ("smem_per_block_optin", u32),
@@ -109,6 +127,8 @@ _SIGS = {
     "opure_peer_create": [P, P, u32, u32, P], "opure_peer_destroy": [P, P, P],
     "opure_peer_info": [P, P, P, P], "opure_gemv_allreduce": [P, P, P],
     "opure_peer_argmax": [P, P, P, u32, u32],
+    "opure_mx_quantize": [P, P, u32, sz, P], "opure_mx_dequantize": [P, P, P, u32, sz],
+    "opure_mx_rmsnorm": [P, P], "opure_mx_gemm": [P, P],
 }
 
 
@@ -133,6 +153,10 @@ def lib() -> C.CDLL:
         L.opure_attention_scratch_bytes.restype = sz
         L.opure_packed_bytes.argtypes = [u32, u32]
         L.opure_packed_bytes.restype = sz
+        L.opure_mx_code_bytes.argtypes = [u32, u32, u32]
+        L.opure_mx_code_bytes.restype = sz
+        L.opure_mx_scale_bytes.argtypes = [u32, u32]
+        L.opure_mx_scale_bytes.restype = sz
         _lib = L
     return _lib
 
@@ -168,6 +192,16 @@ def attention_scratch_bytes(n, n_q, n_heads, n_kv, head_dim, max_ctx, split_toke
 def packed_bytes(nvec: int, length: int) -> int:
     """Bytes of a chained tensor-core operand (fp16 hi/lo pairs of nvec vectors)."""
     return int(lib().opure_packed_bytes(nvec, length))
+
+
+def mx_code_bytes(fmt: int, rows: int, cols: int) -> int:
+    """Bytes of the codes of a microscaled matrix (rows padded to 128 columns)."""
+    return int(lib().opure_mx_code_bytes(fmt, rows, cols))
+
+
+def mx_scale_bytes(rows: int, cols: int) -> int:
+    """Bytes of its scales (tiles of 128 rows x 128 columns, 512 bytes each)."""
+    return int(lib().opure_mx_scale_bytes(rows, cols))
 
 
 class DeviceBuffer:
@@ -263,6 +297,24 @@ class Ctx:
 
     def sample_filtered(self, args: SampleArgs):
         check(lib().opure_sample_filtered(self.h, C.byref(args)), "opure_sample_filtered")
+
+    def mx_matrix(self, rows: int, cols: int, fmt: int) -> MxMatrix:
+        """Device memory for a microscaled matrix, owned by the context."""
+        codes, scales = self.buffer(mx_code_bytes(fmt, rows, cols)), self.buffer(mx_scale_bytes(rows, cols))
+        return MxMatrix(codes.ptr, scales.ptr, rows, cols, fmt)
+
+    def mx_quantize(self, x: int, x_type: int, x_stride: int, out: MxMatrix):
+        """x (device pointer, rows of x_stride values of x_type) to microscaled form."""
+        check(lib().opure_mx_quantize(self.h, x, x_type, x_stride, C.byref(out)), "opure_mx_quantize")
+
+    def mx_dequantize(self, x: MxMatrix, y: int, y_type: int, y_stride: int):
+        check(lib().opure_mx_dequantize(self.h, C.byref(x), y, y_type, y_stride), "opure_mx_dequantize")
+
+    def mx_rmsnorm(self, args: MxNormArgs):
+        check(lib().opure_mx_rmsnorm(self.h, C.byref(args)), "opure_mx_rmsnorm")
+
+    def mx_gemm(self, args: MxGemmArgs):
+        check(lib().opure_mx_gemm(self.h, C.byref(args)), "opure_mx_gemm")
 
     def call(self, name: str, *args):
         check(getattr(lib(), name)(self.h, *args), name)
