@@ -7,6 +7,9 @@ namespace opure {
 // Tensor-core GEMV workspace: up to 256 vectors x 16384 columns packed as fp16 pairs
 // (16 MiB), their scales and split-K tickets, and 32 MiB of split-K partial sums.
 constexpr size_t kTcWorkspaceBytes = size_t(48) << 20;
+// Its first part, the packed vectors: written anew by every call that uses it, so scratch for
+// other kernels too (what follows it has to stay zero between calls).
+constexpr size_t kScratchBytes = size_t(16) << 20;
 }  // namespace opure
 
 struct opure_ctx {

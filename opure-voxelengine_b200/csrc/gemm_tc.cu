@@ -60,6 +60,7 @@ constexpr size_t kScaleOff = kPackOff + kPackBytes;
 constexpr size_t kTicketOff = kScaleOff + kMaxN * 4;
 constexpr size_t kPartialOff = (kTicketOff + kMaxTickets * 4 + 255) & ~size_t(255);
 static_assert(kPartialOff < kTcWorkspaceBytes, "workspace layout");
+static_assert(kPackOff == 0 && kPackBytes == kScratchBytes, "scratch that other kernels may use");
 
 // ---- PTX wrappers -------------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y,

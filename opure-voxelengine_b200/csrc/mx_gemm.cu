@@ -2,105 +2,309 @@
 // the linear layer's epilogues (store, residual add, SwiGLU with an MX result).
 //
 // With block b's scales sx and sw and its codes' values cx and cw,
-//   y[i][r] = sum_b sx[i][b] sw[r][b] (sum_{k in b} cx[i][k] cw[r][k]).
-// The products of codes are exact in fp16; sums are fp32.
+//   y[i][r] = sum_b sx[i][b] sw[r][b] (sum_{k in b} cx[i][k] cw[r][k]),
+// which is what tcgen05.mma kind::mxf8f6f4 computes 32 columns at a time, with fp32 sums: the
+// tokens are its M side (128 TMEM lanes), weight rows its N side. 4-bit codes cross HBM and L2
+// packed; TMA spreads them into the byte-wide slots that this kind reads.
+//
+// mx_gemm_kernel  one CTA per (128 tokens, 128 weight rows, K split). Thread 0 streams 128
+//     columns a stage (codes by tiled TMA, scale tiles by bulk copies) into a ring of
+//     shared-memory stages; thread 32 copies the scale tiles to TMEM and issues the MMAs. A K
+//     split is a thread-block cluster: each CTA leaves its sums in its own shared memory and the
+//     CTAs share the epilogue, each adding the splits of its part in rank order over distributed
+//     shared memory, so that results do not depend on timing. In SwiGLU a tile is 64 gate rows
+//     and the 64 up rows that go with them.
+// All waits are bounded (1 s); a timeout is reported in the ctx status word.
+#include <cudaTypedefs.h>
+
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "mx.cuh"
+#include "tcgen05.cuh"
 
 namespace opure {
 namespace {
 
+constexpr uint32_t kM = 128;       // tokens per tile = TMEM lanes
+constexpr uint32_t kN = 128;       // weight rows per tile
+constexpr uint32_t kK = 128;       // columns per stage: one 128-byte swizzled row of byte slots
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMaxSplits = 8;  // portable cluster size
+constexpr uint32_t kBBytes = kN * kK;
+constexpr uint32_t kScaleBytes = 2048;  // per stage: x tile, w (or gate) tile, up tile; keeps 1 KB alignment
+constexpr uint32_t kScaleCols = 12;     // TMEM columns of a stage's scales
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kRow = kN + 4;       // floats per row of the shared partial sums
+static_assert(kN + kMaxStages * kScaleCols <= kTmemCols, "TMEM columns");
+
 struct GemmParams {
-    const uint8_t *w, *ws, *x, *xs;
-    uint32_t n, rows, cols, x_format;
+    const uint8_t *ws, *us, *xs;  // scale tiles: weights (or gate rows), up rows, tokens
+    uint32_t n, rows, kblocks, splits, stages;
+    uint32_t a_rows;              // token rows that a stage holds: multiple of 8, at most 128
+    uint32_t half;                // SwiGLU: first up row = result columns
+    uint32_t x_format;
     void *y;
     size_t y_stride;
     const void *residual;
-    uint8_t *out, *outs;  // OPURE_EPI_SWIGLU
+    uint8_t *out, *outs;          // SwiGLU
+    DeviceStatus *st;
 };
 
-// Dot product of token i and weight row r; every lane of the warp gets it. A lane takes every
-// 32nd block.
-__device__ __forceinline__ float dot(const GemmParams &p, uint32_t i, uint32_t r) {
-    const uint32_t lane = threadIdx.x & 31u, blocks = (p.cols + kMxBlock - 1) / kMxBlock;
-    float acc = 0.f;
-    for (uint32_t b = lane; b < blocks; b += 32) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p.w + r * mx_row_bytes(OPURE_MX_FP4, p.cols) + b * 16);
-        const uint32_t wv[4] = {w.x, w.y, w.z, w.w};
-        uint32_t xv[8];
-        const uint8_t *xr = p.x + i * mx_row_bytes(p.x_format, p.cols) + b * (4 * p.x_format);
-        for (uint32_t j = 0; j < p.x_format; ++j) xv[j] = reinterpret_cast<const uint32_t *>(xr)[j];
-        float t = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t hw[4], hx[4];
-            mx_unpack_fp4(wv[j], hw);
-            if (p.x_format == OPURE_MX_FP4) {
-                mx_unpack_fp4(xv[j], hx);
-            } else {
-                mx_unpack_fp8(xv[2 * j], hx[0], hx[1]);
-                mx_unpack_fp8(xv[2 * j + 1], hx[2], hx[3]);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float2 a = h2f2(hw[q]), c = h2f2(hx[q]);
-                t = fmaf(a.x, c.x, t);
-                t = fmaf(a.y, c.y, t);
-            }
-        }
-        acc = fmaf(t * mx_scale_value(p.xs[mx_scale_offset(p.cols, i, b)]),
-                   mx_scale_value(p.ws[mx_scale_offset(p.cols, r, b)]), acc);
-    }
-    return warp_sum(acc);
-}
-
-// One warp per (token, 32 result columns): lane j keeps column j.
-template <int EPI, typename T>
-__global__ void __launch_bounds__(256) mx_gemm_kernel(GemmParams p) {
-    grid_dependency_wait();
-    grid_dependents_launch();
+// Quantises 32 values, one per lane, and stores them as one block of `row` (codes) and `scale`.
+template <uint32_t FMT>
+__device__ __forceinline__ void store_block(float v, uint8_t *codes, uint8_t *scale) {
     const uint32_t lane = threadIdx.x & 31u;
-    const uint32_t out_rows = EPI == OPURE_EPI_SWIGLU ? p.rows / 2 : p.rows;
-    const uint32_t units = EPI == OPURE_EPI_SWIGLU ? mx_kp(out_rows) / 32 : (out_rows + 31) / 32;
-    const uint64_t unit = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-    const uint64_t i64 = unit / units;
-    if (i64 >= p.n) return;
-    const uint32_t i = uint32_t(i64), r0 = uint32_t(unit - i64 * units) * 32;
-    float v = 0.f;
-    for (uint32_t j = 0; j < 32 && r0 + j < out_rows; ++j) {
-        float d = dot(p, i, r0 + j);
-        if constexpr (EPI == OPURE_EPI_SWIGLU) {
-            const float up = dot(p, i, out_rows + r0 + j);
-            d = d * (1.0f / (1.0f + expf(-d))) * up;
-        }
-        if (lane == j) v = d;
-    }
-    if constexpr (EPI == OPURE_EPI_SWIGLU) {
-        uint32_t m = __float_as_uint(v) & 0x7fffffffu;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const bool fp4 = std::is_same_v<T, uint32_t>;
-        const uint32_t byte = fp4 ? mx_scale_byte<OPURE_MX_FP4>(m) : mx_scale_byte<OPURE_MX_FP8>(m);
-        v = byte == 255u ? 0.f : v * mx_inverse(byte);
+    const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
+    v = byte == 255u ? 0.f : v * mx_inverse(byte);
+    if constexpr (FMT == OPURE_MX_FP4) {
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = __shfl_sync(0xffffffffu, v, (lane % 4) * 8 + j);
-        uint8_t *row = p.out + i * mx_row_bytes(fp4 ? OPURE_MX_FP4 : OPURE_MX_FP8, out_rows);
-        if (lane < 4) {
-            if (fp4)
-                reinterpret_cast<uint32_t *>(row)[r0 / 8 + lane] = mx_pack_fp4(f);
-            else
-                reinterpret_cast<uint2 *>(row)[r0 / 8 + lane] =
-                    make_uint2(mx_pack_fp8(f[0], f[1], f[2], f[3]), mx_pack_fp8(f[4], f[5], f[6], f[7]));
-        }
-        if (lane == 0) p.outs[mx_scale_offset(out_rows, i, r0 / kMxBlock)] = uint8_t(byte);
-    } else if (r0 + lane < out_rows) {
-        const size_t o = i * p.y_stride + r0 + lane;
-        if constexpr (EPI == OPURE_EPI_ADD) v += to_f32(static_cast<const T *>(p.residual)[o]);
-        static_cast<T *>(p.y)[o] = from_f32<T>(v);
+        if (lane < 4) reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp4(f);
+    } else {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = __shfl_sync(0xffffffffu, v, (lane % 8) * 4 + j);
+        if (lane < 8) reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp8(f[0], f[1], f[2], f[3]);
     }
+    if (lane == 0) *scale = uint8_t(byte);
+}
+
+__device__ __forceinline__ float silu(float g) { return g * (1.0f / (1.0f + expf(-g))); }
+
+// T: the type of y, or for SwiGLU uint8_t (E4M3) or uint32_t (E2M1).
+template <int EPI, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, GemmParams p) {
+    constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
+    constexpr uint32_t kTileRows = kSwiglu ? kN / 2 : kN;  // result columns per tile
+    extern __shared__ uint8_t dsm[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ uint32_t issued_s, consumed_s;
+    __shared__ int fail;
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t tile = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+    const uint32_t m0 = blockIdx.y * kM, r0 = tile * kTileRows;
+    const uint32_t kb0 = uint32_t(uint64_t(p.kblocks) * split / p.splits);
+    const uint32_t nk = uint32_t(uint64_t(p.kblocks) * (split + 1) / p.splits) - kb0;
+    const uint32_t a_bytes = p.a_rows * kK, stage_bytes = kBBytes + kScaleBytes + a_bytes;
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
+    // Stage: [B 16 KB][scales 2 KB][A]. The MMA reads 128 rows of A whatever a_rows is; rows past
+    // a_rows are other bytes of this allocation (the launch adds room after the last stage) and
+    // only reach accumulator lanes of tokens that are not there.
+    auto b_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes; };
+    auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes; };
+    auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&done, 1);
+        fail = 0;
+        issued_s = 0;
+        consumed_s = 0;
+        tc::prefetch_map(&wmap);
+        tc::prefetch_map(&xmap);
+    }
+    if (warp == 2) tc::alloc(&tmem_base, kTmemCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dependency_wait();
+    grid_dependents_launch();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t i = 0;
+            for (; i < nk; ++i) {
+                const uint32_t s = i % p.stages, kb = kb0 + i;
+                if (i >= p.stages && !mbar_wait(&empty[s], ((i / p.stages) & 1u) ^ 1u)) {
+                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 80, blockIdx.x);
+                    fail = 1;
+                    break;
+                }
+                // A spreading copy counts the bytes that it reads, not the slots that it fills.
+                mbar_expect_tx(&full[s], kBBytes / 2 + a_bytes * p.x_format / 8 + kMxTileBytes * (kSwiglu ? 3 : 2));
+                tc::load_2d(b_tile(s), &wmap, kb * kK, r0, &full[s]);
+                if (kSwiglu) tc::load_2d(b_tile(s) + kBBytes / 2, &wmap, kb * kK, p.half + r0, &full[s]);
+                bulk_load(sf_tile(s) + 512, p.ws + (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
+                if (kSwiglu)
+                    bulk_load(sf_tile(s) + 1024, p.us + (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
+                tc::load_2d(a_tile(s), &xmap, kb * kK, m0, &full[s]);
+                bulk_load_keep(sf_tile(s), p.xs + (size_t(m0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
+            }
+            issued_s = i;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc =
+                tc::idesc_mx(p.x_format == OPURE_MX_FP8 ? tc::kE4M3 : tc::kE2M1, tc::kE2M1, kSwiglu ? kN / 2 : kN);
+            // In SwiGLU a tile's 64 rows are the first or the second half of their scale tile.
+            const uint32_t shift = kSwiglu ? r0 / 32 % 4 : 0;
+            uint32_t i = 0;
+            for (; i < nk; ++i) {
+                const uint32_t s = i % p.stages;
+                if (!mbar_wait(&full[s], (i / p.stages) & 1u)) {
+                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 81, blockIdx.x);
+                    fail = 1;
+                    break;
+                }
+                tc::fence_after();
+                // Each stage has TMEM columns of its own for its scales, so a copy never meets
+                // an MMA that still reads them: the stage was freed by that MMA's commit.
+                const uint32_t sf = tmem + kN + s * kScaleCols, sfs = smem_addr(sf_tile(s));
+                tc::copy_scales(sf, tc::desc_scales(sfs));
+                tc::copy_scales(sf + 4, tc::desc_scales(sfs + 512));
+                if (kSwiglu) tc::copy_scales(sf + 8, tc::desc_scales(sfs + 1024));
+                const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
+#pragma unroll
+                for (uint32_t k = 0; k < kK / 32; ++k) {
+                    const uint32_t id = idesc | tc::idesc_block(k), acc = (i | k) != 0;
+                    tc::mma_mxf8f6f4(tmem, da + 2 * k, db + 2 * k, id, sf, sf + 4 + shift, acc);
+                    if (kSwiglu)
+                        tc::mma_mxf8f6f4(tmem + kN / 2, da + 2 * k, db + 2 * k + (kBBytes / 2 >> 4), id, sf, sf + 8 + shift, acc);
+                }
+                tc::commit(&empty[s]);
+            }
+            consumed_s = i;
+            tc::commit(&done);
+        }
+        __syncwarp();
+    }
+    if (!mbar_wait(&done, 0)) {
+        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 82, blockIdx.x);
+        fail = 1;
+    }
+    tc::fence_after();
+    __syncthreads();
+    const bool failed = fail;
+    if (failed && threadIdx.x == 0)  // leave no copy in flight into this CTA's shared memory
+        for (uint32_t i = consumed_s; i < issued_s; ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u);
+
+    // Accumulators -> shared memory (every stage is done with): part[token][column]. Warps w and
+    // w + 4 share TMEM lanes 32 (w % 4) ..; each takes half of the columns.
+    float *part = reinterpret_cast<float *>(base);
+    const uint32_t n = min(p.n - m0, kM);
+    const uint32_t quarter = warp & 3u;
+    if (!failed && quarter * 32 < n) {
+        for (uint32_t c = (warp >> 2) * (kN / 2), e = c + kN / 2; c < e; c += 32) {
+            uint32_t r[32];
+            tc::ld32(tmem + ((quarter * 32) << 16) + c, r);
+            tc::wait_ld();
+            float4 *dst = reinterpret_cast<float4 *>(part + (quarter * 32 + lane) * kRow + c);
+            if (quarter * 32 + lane < n)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                         __uint_as_float(r[4 * j + 3]));
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 2) tc::dealloc(tmem, kTmemCols);
+    if (p.splits > 1) tc::cluster_sync();
+
+    // Epilogue: a warp takes 32 result columns of a token, a lane one of them.
+    constexpr uint32_t kChunks = kTileRows / 32;
+    auto sum = [&](uint32_t at) {
+        if (p.splits == 1) return part[at];
+        float v = 0.f;
+        const uint32_t a = smem_addr(part + at);
+        for (uint32_t q = 0; q < p.splits; ++q) v += tc::ld_cluster_f32(tc::map_rank(a, q));
+        return v;
+    };
+    for (uint32_t u = split + p.splits * warp; !failed && u < n * kChunks; u += p.splits * (kThreads / 32)) {
+        const uint32_t i = u / kChunks, c = u % kChunks * 32 + lane, col = r0 + c;
+        float v = sum(i * kRow + c);
+        if constexpr (kSwiglu) {
+            v = silu(v) * sum(i * kRow + kN / 2 + c);
+            if (col >= p.half) v = 0.f;  // gate rows past the half are up rows
+            if (col - lane < mx_kp(p.half)) {
+                constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
+                store_block<kF>(v, p.out + (m0 + i) * mx_row_bytes(kF, p.half) + (col - lane) * kF / 8,
+                                p.outs + mx_scale_offset(p.half, m0 + i, (col - lane) / 32));
+            }
+        } else if (col < p.rows) {
+            const size_t o = (m0 + i) * p.y_stride + col;
+            if constexpr (EPI == OPURE_EPI_ADD) v += to_f32(static_cast<const T *>(p.residual)[o]);
+            static_cast<T *>(p.y)[o] = from_f32<T>(v);
+        }
+    }
+    if (p.splits > 1) tc::cluster_sync();  // the others have read this CTA's sums
+}
+
+// Scale tiles of rows [first, first + rows) of a matrix, as a matrix of their own: what the up
+// half needs when it does not start on a tile. One thread per (row, 128 columns).
+__global__ void __launch_bounds__(256)
+    mx_move_scales_kernel(const uint8_t *src, uint8_t *dst, uint32_t first, uint32_t rows, uint32_t kblocks) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const uint64_t t = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    const uint32_t kb = uint32_t(t / rows), r = uint32_t(t - uint64_t(kb) * rows);
+    if (kb >= kblocks) return;
+    const uint32_t cols = kblocks * 128;
+    *reinterpret_cast<uint32_t *>(dst + mx_scale_offset(cols, r, kb * 4)) =
+        *reinterpret_cast<const uint32_t *>(src + mx_scale_offset(cols, first + r, kb * 4));
+}
+
+// ---- host -------------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+// Codes as byte slots in shared memory: boxes of 128 columns x box_rows rows, 128-byte swizzle.
+// E2M1 is spread by the copy: 16 codes (8 bytes) to 16 bytes.
+bool make_map(CUtensorMap *m, const opure_mx_matrix &a, uint32_t box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {mx_kp(a.cols), a.rows};
+    const cuuint64_t strides[1] = {mx_row_bytes(a.format, a.cols)};
+    const cuuint32_t box[2] = {kK, box_rows};
+    const cuuint32_t es[2] = {1, 1};
+    return fn(m, a.format == OPURE_MX_FP4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.codes,
+              dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int EPI, typename T>
+opure_status launch_gemm(opure_ctx *ctx, const CUtensorMap &wm, const CUtensorMap &xm, const GemmParams &p, uint32_t tiles,
+                         size_t smem) {
+    auto *kernel = mx_gemm_kernel<EPI, T>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return cuda_status(e);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles * p.splits, (p.n + kM - 1) / kM);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, wm, xm, p);
+    return e == cudaSuccess ? OPURE_OK : cuda_status(e);
 }
 
 }  // namespace
@@ -127,17 +331,54 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     }
     if (a->x.rows == 0 || a->w.rows == 0) return OPURE_OK;
     if (!swiglu && (!a->y || (a->epilogue == OPURE_EPI_ADD && !a->residual))) return OPURE_ERR_INVALID_ARG;
-    GemmParams p{a->w.codes, a->w.scales, a->x.codes, a->x.scales, a->x.rows, a->w.rows, a->w.cols, a->x.format,
-                 a->y, a->y_stride, a->residual, a->out.codes, a->out.scales};
-    const uint64_t units = uint64_t(a->x.rows) * (swiglu ? mx_kp(a->w.rows / 2) / 32 : ceil_div(a->w.rows, 32));
-    if ((units + 7) / 8 > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
-    auto go = [&](auto kernel) { return launch(ctx, kernel, dim3(ceil_div(units, 8)), dim3(256), 0, true, p); };
+
+    GemmParams p{};
+    p.n = a->x.rows;
+    p.rows = a->w.rows;
+    p.half = a->w.rows / 2;
+    p.kblocks = mx_kp(a->w.cols) / kK;
+    p.x_format = a->x.format;
+    p.ws = a->w.scales;
+    p.xs = a->x.scales;
+    p.y = a->y;
+    p.y_stride = a->y_stride;
+    p.residual = a->residual;
+    p.out = a->out.codes;
+    p.outs = a->out.scales;
+    p.st = ctx->status;
+    if (p.n > 65535u * kM) return OPURE_ERR_UNSUPPORTED;
+    const uint32_t tiles = swiglu ? mx_kp(p.half) / (kN / 2) : ceil_div(p.rows, kN);
+    const uint32_t mtiles = ceil_div(p.n, kM);
+    // As many K splits as fill the SMs once.
+    p.splits = std::max(1u, std::min({kMaxSplits, p.kblocks, uint32_t(ctx->sm_count) / std::max(1u, tiles * mtiles)}));
+    p.a_rows = std::min(kM, (p.n + 7) & ~7u);
+    const uint32_t stage_bytes = kBBytes + kScaleBytes + p.a_rows * kK;
+    // After the ring: 1 KB to align it, and the rest of the last stage's 128 rows of A. The
+    // partial sums share it. Below 114 KB two CTAs would fit an SM, which all of TMEM does not.
+    const size_t tail = 1024 + size_t(kM - p.a_rows) * kK, budget = std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024;
+    p.stages = std::min<uint32_t>({kMaxStages, uint32_t((budget - tail) / stage_bytes), ceil_div(p.kblocks, p.splits)});
+    const size_t smem = std::max<size_t>({p.stages * stage_bytes + tail, 1024 + size_t(kM) * kRow * 4, 116 * 1024});
+    if (swiglu) {
+        if (p.half % 128 == 0) {
+            p.us = p.ws + size_t(p.half / 128) * p.kblocks * kMxTileBytes;
+        } else {
+            if (opure_mx_scale_bytes(p.half, a->w.cols) > kScratchBytes) return OPURE_ERR_UNSUPPORTED;
+            uint8_t *us = static_cast<uint8_t *>(ctx->ws);
+            s = launch(ctx, mx_move_scales_kernel, dim3(ceil_div(uint64_t(p.half) * p.kblocks, 256)), dim3(256), 0, true, p.ws, us,
+                       p.half, p.half, p.kblocks);
+            if (s) return s;
+            p.us = us;
+        }
+    }
+    CUtensorMap wm, xm;
+    if (!make_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
     if (swiglu)
-        return a->out.format == OPURE_MX_FP4 ? go(mx_gemm_kernel<OPURE_EPI_SWIGLU, uint32_t>)
-                                             : go(mx_gemm_kernel<OPURE_EPI_SWIGLU, uint8_t>);
+        return a->out.format == OPURE_MX_FP4 ? launch_gemm<OPURE_EPI_SWIGLU, uint32_t>(ctx, wm, xm, p, tiles, smem)
+                                             : launch_gemm<OPURE_EPI_SWIGLU, uint8_t>(ctx, wm, xm, p, tiles, smem);
     return with_type(a->y_type, [&](auto t) {
         using T = decltype(t);
-        return a->epilogue == OPURE_EPI_ADD ? go(mx_gemm_kernel<OPURE_EPI_ADD, T>) : go(mx_gemm_kernel<OPURE_EPI_STORE, T>);
+        return a->epilogue == OPURE_EPI_ADD ? launch_gemm<OPURE_EPI_ADD, T>(ctx, wm, xm, p, tiles, smem)
+                                            : launch_gemm<OPURE_EPI_STORE, T>(ctx, wm, xm, p, tiles, smem);
     });
 }
 
