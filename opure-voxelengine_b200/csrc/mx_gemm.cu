@@ -15,14 +15,10 @@
 //     shared memory, so that results do not depend on timing. In SwiGLU a tile is 64 gate rows
 //     and the 64 up rows that go with them.
 // All waits are bounded (1 s); a timeout is reported in the ctx status word.
-#include <cudaTypedefs.h>
-
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
-#include "mx.cuh"
-#include "tcgen05.cuh"
+#include "mx_gemm.cuh"
 
 namespace opure {
 namespace {
@@ -72,8 +68,6 @@ __device__ __forceinline__ void store_block(float v, uint8_t *codes, uint8_t *sc
     }
     if (lane == 0) *scale = uint8_t(byte);
 }
-
-__device__ __forceinline__ float silu(float g) { return g * (1.0f / (1.0f + expf(-g))); }
 
 // T: the type of y, or for SwiGLU uint8_t (E4M3) or uint32_t (E2M1).
 template <int EPI, typename T>
@@ -147,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0) {
             const uint32_t idesc =
-                tc::idesc_mx(p.x_format == OPURE_MX_FP8 ? tc::kE4M3 : tc::kE2M1, tc::kE2M1, kSwiglu ? kN / 2 : kN);
+                tc::idesc_mx(p.x_format == OPURE_MX_FP8 ? tc::kE4M3 : tc::kE2M1, tc::kE2M1, kM, kSwiglu ? kN / 2 : kN);
             // In SwiGLU a tile's 64 rows are the first or the second half of their scale tile.
             const uint32_t shift = kSwiglu ? r0 / 32 % 4 : 0;
             uint32_t i = 0;
@@ -257,33 +251,6 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host -------------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
-}
-
-// Codes as byte slots in shared memory: boxes of 128 columns x box_rows rows, 128-byte swizzle.
-// E2M1 is spread by the copy: 16 codes (8 bytes) to 16 bytes.
-bool make_map(CUtensorMap *m, const opure_mx_matrix &a, uint32_t box_rows) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[2] = {mx_kp(a.cols), a.rows};
-    const cuuint64_t strides[1] = {mx_row_bytes(a.format, a.cols)};
-    const cuuint32_t box[2] = {kK, box_rows};
-    const cuuint32_t es[2] = {1, 1};
-    return fn(m, a.format == OPURE_MX_FP4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a.codes,
-              dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int EPI, typename T>
 opure_status launch_gemm(opure_ctx *ctx, const CUtensorMap &wm, const CUtensorMap &xm, const GemmParams &p, uint32_t tiles,
                          size_t smem) {
@@ -370,8 +337,9 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
             p.us = us;
         }
     }
+    if (mx_gemm_pair_suits(ctx, a)) return mx_gemm_pair(ctx, a, p.us);
     CUtensorMap wm, xm;
-    if (!make_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
+    if (!make_slot_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_slot_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
     if (swiglu)
         return a->out.format == OPURE_MX_FP4 ? launch_gemm<OPURE_EPI_SWIGLU, uint32_t>(ctx, wm, xm, p, tiles, smem)
                                              : launch_gemm<OPURE_EPI_SWIGLU, uint8_t>(ctx, wm, xm, p, tiles, smem);

@@ -1,0 +1,457 @@
+// mx_gemm_pair.cu -- the product of microscaled matrices for many tokens: persistent pairs of
+// SMs (cta_group::2), each working through tiles of 256 tokens x 256 weight rows.
+//
+// Bound by the tensor cores. With 8-bit tokens the weights' 4-bit codes are spread into byte
+// slots by TMA (kind::mxf8f6f4, 128 columns a stage); with 4-bit tokens both sides stay packed
+// (kind::mxf4, twice the rate, 256 columns a stage). In a pair each CTA holds 128 rows of either
+// operand, so that an SM's shared memory feeds 256 x 256 results from 32 KB a stage: a single
+// CTA's 128 x 256 tile would need 48 KB, and both its reads and TMA's writes would pass what
+// shared memory delivers.
+//
+//   warp 0   loads: codes, scale tiles; every load of either CTA completes on the even CTA's
+//            barrier
+//   warp 1   (even CTA) copies scale tiles to TMEM and issues the MMAs
+//   warps 4-11  results: two accumulators alternate, so that a tile's results leave while the
+//            next is computed. TMEM's 512 columns hold two of 256 and 48 of scales by letting the
+//            two overlap by 48 columns, which are read first; then the next tile may begin.
+//
+// Results go through shared memory: whole rows of 128 bytes that TMA stores, or, where y's
+// alignment or the residual forbids it, 32 columns of a row at a time by a warp. In SwiGLU the
+// even CTA holds gate rows and the odd CTA the up rows that go with them; a thread owns a token's
+// 32 columns, which is a block of the MX result.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "mx_gemm.cuh"
+
+namespace opure {
+namespace {
+
+constexpr uint32_t kTile = 256;    // tokens and weight rows per tile
+constexpr uint32_t kHalf = 128;    // of each, per CTA
+constexpr uint32_t kStages = 5;
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kEpiWarp = 4, kEpiWarps = 8;
+constexpr uint32_t kOperand = kHalf * 128;  // bytes of a CTA's part of one operand of a stage
+constexpr uint32_t kSlab = 4096;            // result staging per warp: 32 rows of 128 bytes
+constexpr uint32_t kTmemCols = 512, kScaleCol = 464, kAcc1 = 208;  // accumulator 0 starts at column 0
+
+template <uint32_t XF>
+struct Shape {
+    static constexpr uint32_t kBlocks = XF == OPURE_MX_FP8 ? 1 : 2;  // scale tiles (128 columns) per stage
+    static constexpr uint32_t kScaleBytes = kBlocks * 3 * kMxTileBytes;
+    static constexpr uint32_t kStageBytes = 2 * kOperand + kScaleBytes;
+    static constexpr uint32_t kScaleCols = kBlocks * 12;
+    static constexpr uint32_t kSlots = (kTmemCols - kScaleCol) / kScaleCols;  // scales of that many stages at once
+    // Bytes that arrive per CTA and stage; a copy that spreads codes counts what it reads.
+    static constexpr uint32_t kTx = kOperand + (XF == OPURE_MX_FP8 ? kOperand / 2 : kOperand) + kScaleBytes;
+    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStageBytes + kEpiWarps * kSlab;
+};
+
+struct PairParams {
+    uint32_t n, rows, half, kblocks, mtiles, ntiles;
+    void *y;
+    size_t y_stride;
+    const void *residual;
+    uint8_t *out, *outs;
+    bool tma_store;
+    DeviceStatus *st;
+};
+
+// 32 values of a thread -> 32 codes in global memory (dst 16-byte aligned); returns the scale byte.
+template <uint32_t FMT>
+__device__ __forceinline__ uint32_t quantize_block(float (&v)[32], uint8_t *dst, bool in) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    const uint32_t byte = mx_scale_byte<FMT>(m);
+    const float inv = mx_inverse(byte);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
+    if constexpr (FMT == OPURE_MX_FP4) {
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = v[8 * j + q];
+            c[j] = mx_pack_fp4(f);
+        }
+        if (in) *reinterpret_cast<uint4 *>(dst) = make_uint4(c[0], c[1], c[2], c[3]);
+    } else {
+        uint32_t c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = mx_pack_fp8(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        if (in) {
+            reinterpret_cast<uint4 *>(dst)[0] = make_uint4(c[0], c[1], c[2], c[3]);
+            reinterpret_cast<uint4 *>(dst)[1] = make_uint4(c[4], c[5], c[6], c[7]);
+        }
+    }
+    return byte;
+}
+
+// The results' warps stop together when one of their lanes gives up.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, phase));
+}
+
+template <uint32_t XF, int EPI, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
+                        const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap usmap,
+                        const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap ymap, PairParams p) {
+    using S = Shape<XF>;
+    constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
+    constexpr uint32_t kResult = kSwiglu ? kHalf : kTile;  // result columns per tile
+    extern __shared__ uint8_t dsm[];
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], drained;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int fail;
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = tc::cluster_rank();
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
+    auto a_tile = [&](uint32_t s) { return base + s * 2 * kOperand; };
+    auto b_tile = [&](uint32_t s) { return base + s * 2 * kOperand + kOperand; };
+    uint8_t *slabs = base + kStages * 2 * kOperand;
+    auto sf_tile = [&](uint32_t s) { return slabs + kEpiWarps * kSlab + s * S::kScaleBytes; };
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&acc_full[0], 1);
+        mbar_init(&acc_full[1], 1);
+        mbar_init(&drained, 2 * kEpiWarps);
+        fail = 0;
+        tc::prefetch_map(&wmap);
+        tc::prefetch_map(&xmap);
+        tc::prefetch_map(&wsmap);
+        tc::prefetch_map(&xsmap);
+    }
+    if (warp == 2) tc::alloc_pair(&tmem_base, kTmemCols);
+    tc::fence_before();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dependency_wait();
+    grid_dependents_launch();
+
+    const uint32_t tiles = p.mtiles * p.ntiles, pairs = gridDim.x / 2, first = blockIdx.x / 2;
+    const uint32_t stages = (p.kblocks + S::kBlocks - 1) / S::kBlocks;  // per tile
+    uint32_t issued = 0, consumed = 0;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            for (uint32_t t = first; ok && t < tiles; t += pairs) {
+                const uint32_t m0 = t % p.mtiles * kTile + rank * kHalf, r0 = t / p.mtiles * kResult;
+                // This CTA's half of the weight rows, and the scale tiles of both halves.
+                const uint32_t w_row = kSwiglu ? (rank ? p.half + r0 : r0) : r0 + rank * kHalf;
+                const uint32_t x_sf = m0 / 128 * p.kblocks, g_sf = r0 / 128 * p.kblocks;
+                for (uint32_t i = 0; i < stages; ++i, ++issued) {
+                    const uint32_t s = issued % kStages;
+                    if (issued >= kStages && !mbar_wait(&empty[s], ((issued / kStages) & 1u) ^ 1u)) {
+                        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 84, blockIdx.x);
+                        fail = 1;
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = tc::map_rank(smem_addr(&full[s]), 0);
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kTx);
+                    const uint32_t kb = i * S::kBlocks;
+                    tc::load_2d_pair(a_tile(s), &xmap, i * 128, m0, bar);
+                    tc::load_2d_pair(b_tile(s), &wmap, i * 128, w_row, bar);
+                    uint8_t *sf = sf_tile(s);
+                    tc::load_2d_pair(sf, &xsmap, 0, x_sf + kb, bar);
+                    tc::load_2d_pair(sf + S::kBlocks * kMxTileBytes, &wsmap, 0, g_sf + kb, bar);
+                    if (kSwiglu)
+                        tc::load_2d_pair(sf + 2 * S::kBlocks * kMxTileBytes, &usmap, 0, g_sf + kb, bar);
+                    else
+                        tc::load_2d_pair(sf + 2 * S::kBlocks * kMxTileBytes, &wsmap, 0, g_sf + p.kblocks + kb, bar);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = XF == OPURE_MX_FP8 ? tc::idesc_mx(tc::kE4M3, tc::kE2M1, kTile, kTile)
+                                                          : tc::idesc_mx(tc::kPackedE2M1, tc::kPackedE2M1, kTile, kTile);
+            bool ok = true;
+            uint32_t lt = 0;
+            for (uint32_t t = first; ok && t < tiles; t += pairs, ++lt) {
+                const uint32_t acc = tmem + (lt & 1u) * kAcc1;
+                // The tile before last has left this accumulator, and the last one the columns
+                // that the two share.
+                if (lt && !mbar_wait(&drained, (lt - 1) & 1u)) {
+                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 85, blockIdx.x);
+                    fail = 1;
+                    break;
+                }
+                tc::fence_after();
+                for (uint32_t i = 0; i < stages; ++i, ++consumed) {
+                    const uint32_t s = consumed % kStages;
+                    // This stage's columns for scales are free once the MMAs of kSlots stages ago
+                    // are done (their commit).
+                    const uint32_t old = consumed - S::kSlots;
+                    if (!mbar_wait(&full[s], (consumed / kStages) & 1u) ||
+                        (consumed >= S::kSlots && !mbar_wait(&empty[old % kStages], (old / kStages) & 1u))) {
+                        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 86, blockIdx.x);
+                        fail = 1;
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after();
+                    const uint32_t sfa = tmem + kScaleCol + consumed % S::kSlots * S::kScaleCols, sfb = sfa + S::kBlocks * 4;
+                    const uint32_t src = smem_addr(sf_tile(s));
+#pragma unroll
+                    for (uint32_t b = 0; b < S::kBlocks; ++b) {
+                        tc::copy_scales_pair(sfa + b * 4, tc::desc_scales(src + b * kMxTileBytes));
+                        tc::copy_scales_pair(sfb + b * 8, tc::desc_scales(src + (S::kBlocks + b) * kMxTileBytes));
+                        tc::copy_scales_pair(sfb + b * 8 + 4, tc::desc_scales(src + (2 * S::kBlocks + b) * kMxTileBytes));
+                    }
+                    const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const uint32_t more = (i | k) != 0;
+                        if constexpr (XF == OPURE_MX_FP8)
+                            tc::mma_mxf8f6f4_pair(acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k), sfa, sfb, more);
+                        else if (i * 2 + k / 2 < p.kblocks)
+                            tc::mma_mxf4_pair(acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k % 2 * 2), sfa + k / 2 * 4,
+                                              sfb + k / 2 * 8, more);
+                    }
+                    tc::commit_pair(&empty[s]);
+                }
+                if (ok) tc::commit_pair(&acc_full[lt & 1u]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= kEpiWarp) {
+        const uint32_t quarter = warp & 3u, part = (warp - kEpiWarp) >> 2;  // TMEM lanes, half of the columns
+        const uint32_t drain_bar = tc::map_rank(smem_addr(&drained), 0);
+        uint8_t *slab = slabs + (warp - kEpiWarp) * kSlab;
+        uint32_t lt = 0;
+        for (uint32_t t = first; t < tiles; t += pairs, ++lt) {
+            const uint32_t b = lt & 1u;
+            const uint32_t row0 = t % p.mtiles * kTile + rank * kHalf + quarter * 32, row = row0 + lane;
+            const uint32_t r0 = t / p.mtiles * kResult;
+            const uint32_t acc = tmem + b * kAcc1 + ((quarter * 32) << 16);
+            if (!warp_wait(&acc_full[b], (lt >> 1) & 1u)) {
+                if (lane == 0 && !fail) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 87, blockIdx.x);
+                fail = 1;
+                break;
+            }
+            tc::fence_after();
+            // Accumulator 0 shares its last 48 columns, accumulator 1 its first 48: the half
+            // of the warps that has them reads them before anything else, then lets the next
+            // tile begin. The other half does so at once: it has left the tile before this one.
+            auto release = [&] {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::arrive_cluster(drain_bar);
+            };
+            if (part == b) release();
+            if constexpr (kSwiglu) {
+                // Blocks 2 part and 2 part + 1 of the tile's four: gate columns 32 j, up 128 + 32 j.
+                constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
+                uint32_t pre[2][32], cur[32];
+                const uint32_t c0 = part * 64, shared_side = b ? 0 : kHalf, other_side = kHalf - shared_side;
+                tc::ld32(acc + shared_side + c0, pre[0]);
+                tc::ld32(acc + shared_side + c0 + 32, pre[1]);
+                tc::ld32(acc + other_side + c0, cur);
+                tc::wait_ld();
+                if (part != b) release();  // accumulator 0: up blocks 2, 3; accumulator 1: gate blocks 0, 1
+                uint32_t bytes = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) {
+                    if (j) {
+                        tc::ld32(acc + other_side + c0 + 32, cur);
+                        tc::wait_ld();
+                    }
+                    const uint32_t col = r0 + c0 + 32 * j;
+                    float v[32];
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        const float x0 = __uint_as_float(pre[j][q]), x1 = __uint_as_float(cur[q]);
+                        v[q] = b ? silu(x0) * x1 : silu(x1) * x0;
+                        if (col + q >= p.half) v[q] = 0.f;  // gate rows past the half are up rows
+                    }
+                    const bool in = row < p.n && col < mx_kp(p.half);
+                    bytes |= quantize_block<kF>(v, p.out + row * mx_row_bytes(kF, p.half) + size_t(col) * kF / 8, in) << (8 * j);
+                }
+                if (row < p.n && r0 + c0 < mx_kp(p.half))
+                    *reinterpret_cast<uint16_t *>(p.outs + mx_scale_offset(p.half, row, (r0 + c0) / 32)) = uint16_t(bytes);
+            } else {
+                // Twice 64 columns, the shared ones first.
+                const bool back = part == 1 && b == 0;
+#pragma unroll 1
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t v[2][32];
+                    const uint32_t c = part * kHalf + (back ? 1 - h : h) * 64;
+                    tc::ld32(acc + c, v[0]);
+                    tc::ld32(acc + c + 32, v[1]);
+                    tc::wait_ld();
+                    if (h == 0 && part != b) release();
+                    const uint32_t col = r0 + c;
+                    if (EPI == OPURE_EPI_STORE && p.tma_store) {
+                        constexpr uint32_t kCols = 128 / sizeof(T);  // columns of a slab row
+#pragma unroll
+                        for (uint32_t q = 0; q < 64 / kCols; ++q) {
+                            if (lane == 0) tc::store_wait_read();
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t e = 0; e < 8; ++e) {  // 16 bytes each
+                                uint4 u;
+                                T *h8 = reinterpret_cast<T *>(&u);
+#pragma unroll
+                                for (uint32_t k = 0; k < 16 / sizeof(T); ++k) {
+                                    const uint32_t at = q * kCols + e * (16 / sizeof(T)) + k;
+                                    h8[k] = from_f32<T>(__uint_as_float(v[at / 32][at % 32]));
+                                }
+                                *reinterpret_cast<uint4 *>(slab + lane * 128 + ((e ^ (lane & 7u)) << 4)) = u;
+                            }
+                            tc::fence_async_shared();
+                            __syncwarp();
+                            if (lane == 0 && row0 < p.n && col + q * kCols < p.rows) tc::store_2d(&ymap, col + q * kCols, row0, slab);
+                        }
+                    } else {
+                        float *f = reinterpret_cast<float *>(slab);
+#pragma unroll
+                        for (uint32_t q = 0; q < 2; ++q) {
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t k = 0; k < 32; ++k) f[lane * 32 + (k ^ lane)] = __uint_as_float(v[q][k]);
+                            __syncwarp();
+                            const uint32_t cc = col + q * 32 + lane;
+                            if (cc < p.rows) {
+                                for (uint32_t r = 0; r < 32; r += 8) {
+                                    float res[8];
+#pragma unroll
+                                    for (uint32_t k = 0; k < 8; ++k) {
+                                        res[k] = 0.f;
+                                        if (EPI == OPURE_EPI_ADD && row0 + r + k < p.n)
+                                            res[k] = to_f32(static_cast<const T *>(p.residual)[(row0 + r + k) * p.y_stride + cc]);
+                                    }
+#pragma unroll
+                                    for (uint32_t k = 0; k < 8; ++k)
+                                        if (row0 + r + k < p.n)
+                                            static_cast<T *>(p.y)[(row0 + r + k) * p.y_stride + cc] =
+                                                from_f32<T>(f[(r + k) * 32 + (lane ^ (r + k))] + res[k]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (EPI == OPURE_EPI_STORE && p.tma_store && lane == 0) tc::store_wait();
+        __syncwarp();
+    }
+    tc::fence_before();
+    __syncthreads();
+    // After a failure: leave no copy in flight into the pair's shared memory.
+    if (fail && threadIdx.x == 0 && rank == 0)
+        for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_wait(&full[i % kStages], (i / kStages) & 1u);
+    tc::cluster_sync();
+    if (warp == 2) tc::dealloc_pair(tmem, kTmemCols);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+template <uint32_t XF, int EPI, typename T>
+opure_status launch_pair(opure_ctx *ctx, const CUtensorMap (&m)[6], const PairParams &p) {
+    auto *kernel = mx_gemm_pair_kernel<XF, EPI, T>;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<XF>::kSmem));
+    if (e != cudaSuccess) return cuda_status(e);
+    const uint32_t pairs = std::min(uint32_t(ctx->sm_count) / 2, p.mtiles * p.ntiles);
+    return launch(ctx, kernel, dim3(2 * pairs), dim3(kThreads), Shape<XF>::kSmem, true, m[0], m[1], m[2], m[3], m[4], m[5], p);
+}
+
+}  // namespace
+
+bool make_map(CUtensorMap *m, CUtensorMapDataType type, const void *p, uint64_t cols, uint64_t rows, uint64_t row_bytes,
+              uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_bytes};
+    const cuuint32_t box[2] = {box_cols, box_rows}, es[2] = {1, 1};
+    return fn(m, type, 2, const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool mx_gemm_pair_suits(const opure_ctx *ctx, const opure_mx_gemm_args *a) {
+    const bool swiglu = a->epilogue == OPURE_EPI_SWIGLU;
+    const uint64_t ntiles = swiglu ? mx_kp(a->w.rows / 2) / kHalf : (uint64_t(a->w.rows) + kTile - 1) / kTile;
+    return a->x.rows > kHalf && (uint64_t(a->x.rows) + kTile - 1) / kTile * ntiles * 4 >= uint32_t(ctx->sm_count);
+}
+
+opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *us) {
+    const bool swiglu = a->epilogue == OPURE_EPI_SWIGLU, fp8 = a->x.format == OPURE_MX_FP8;
+    PairParams p{};
+    p.n = a->x.rows;
+    p.rows = a->w.rows;
+    p.half = a->w.rows / 2;
+    p.kblocks = mx_kp(a->w.cols) / 128;
+    p.mtiles = (p.n + kTile - 1) / kTile;
+    p.ntiles = swiglu ? mx_kp(p.half) / kHalf : (p.rows + kTile - 1) / kTile;
+    p.y = a->y;
+    p.y_stride = a->y_stride;
+    p.residual = a->residual;
+    p.out = a->out.codes;
+    p.outs = a->out.scales;
+    p.st = ctx->status;
+    // Maps: w, x, scale tiles of w, of its up half and of x (128 words each), y.
+    CUtensorMap m[6] = {};
+    const uint32_t blocks = fp8 ? 1 : 2;
+    auto codes = [&](CUtensorMap *t, const opure_mx_matrix &q) {
+        if (fp8) return make_slot_map(t, q, kHalf);
+        const size_t bytes = mx_row_bytes(q.format, q.cols);
+        return make_map(t, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, bytes, q.rows, bytes, 128, kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    auto scales = [&](CUtensorMap *t, const uint8_t *s, uint32_t rows) {
+        return make_map(t, CU_TENSOR_MAP_DATA_TYPE_UINT32, s, 128, (uint64_t(rows) + 127) / 128 * p.kblocks, kMxTileBytes, 128,
+                        blocks, CU_TENSOR_MAP_SWIZZLE_NONE);
+    };
+    if (!codes(&m[0], a->w) || !codes(&m[1], a->x) || !scales(&m[2], a->w.scales, p.rows) ||
+        !scales(&m[3], swiglu ? us : a->w.scales, swiglu ? p.half : p.rows) || !scales(&m[4], a->x.scales, p.n))
+        return OPURE_ERR_UNSUPPORTED;
+    m[5] = m[4];
+    if (a->epilogue == OPURE_EPI_STORE && rows_aligned16(a->y, a->y_type, a->y_stride)) {
+        const uint32_t size = type_bytes(a->y_type);
+        const CUtensorMapDataType type = a->y_type == OPURE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : a->y_type == OPURE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        p.tma_store = make_map(&m[5], type, a->y, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    auto go = [&](auto t, auto epi) {
+        using T = decltype(t);
+        constexpr int kEpi = decltype(epi)::value;
+        return fp8 ? launch_pair<OPURE_MX_FP8, kEpi, T>(ctx, m, p) : launch_pair<OPURE_MX_FP4, kEpi, T>(ctx, m, p);
+    };
+    if (swiglu) {
+        const std::integral_constant<int, OPURE_EPI_SWIGLU> epi;
+        return a->out.format == OPURE_MX_FP4 ? go(uint32_t(), epi) : go(uint8_t(), epi);
+    }
+    return with_type(a->y_type, [&](auto t) {
+        return a->epilogue == OPURE_EPI_ADD ? go(t, std::integral_constant<int, OPURE_EPI_ADD>())
+                                            : go(t, std::integral_constant<int, OPURE_EPI_STORE>());
+    });
+}
+
+}  // namespace opure

@@ -49,11 +49,11 @@ __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-// Element formats of kind::mxf8f6f4 in the instruction descriptor.
-constexpr uint32_t kE4M3 = 0, kE2M1 = 5;
-// Instruction descriptor: M = 128, E8M0 scales; the scale's byte (block within a column) is or'ed in.
-constexpr __host__ __device__ uint32_t idesc_mx(uint32_t a_format, uint32_t b_format, uint32_t n) {
-    return (a_format << 7) | (b_format << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+// Element formats in the instruction descriptor: of kind::mxf8f6f4, and E2M1 of kind::mxf4.
+constexpr uint32_t kE4M3 = 0, kE2M1 = 5, kPackedE2M1 = 1;
+// Instruction descriptor with E8M0 scales; the scale's byte (block within a column) is or'ed in.
+constexpr __host__ __device__ uint32_t idesc_mx(uint32_t a_format, uint32_t b_format, uint32_t m, uint32_t n) {
+    return (a_format << 7) | (b_format << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24);
 }
 __device__ __forceinline__ uint32_t idesc_block(uint32_t b) { return (b << 4) | (b << 29); }
 
@@ -86,6 +86,71 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ---- CTA pairs (cta_group::2) ---------------------------------------------------------------
+// The even CTA of a pair issues; D spans both CTAs' TMEM (128 rows each), each CTA's shared
+// memory holds its 128 rows of A and its half of B's rows, at the same offsets in both.
+
+// A load into this CTA that completes on an mbarrier of either CTA of the pair (a cluster address).
+__device__ __forceinline__ void load_2d_pair(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void alloc_pair(uint32_t *dst, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// Scale tile to TMEM in both CTAs, each from its own shared memory.
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// K = 32 of byte slots, one scale per row.
+__device__ __forceinline__ void mma_mxf8f6f4_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                  uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// K = 64 of packed E2M1 on both sides, two scales per row.
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// Arrives on `bar` of both CTAs once every tcgen05 operation this thread issued before has completed.
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_addr(bar)),
+                 "h"(uint16_t(3))
+                 : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- TMA stores ----------------------------------------------------------------------------
+__device__ __forceinline__ void store_2d(const CUtensorMap *map, uint32_t x, uint32_t y, const void *src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(smem_addr(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- clusters --------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
