@@ -236,18 +236,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.splits > 1) tc::cluster_sync();  // the others have read this CTA's sums
 }
 
-// Scale tiles of rows [first, first + rows) of a matrix, as a matrix of their own: what the up
-// half needs when it does not start on a tile. One thread per (row, 128 columns).
-__global__ void __launch_bounds__(256)
-    mx_move_scales_kernel(const uint8_t *src, uint8_t *dst, uint32_t first, uint32_t rows, uint32_t kblocks) {
+// Scale tiles of the two halves of a matrix, each as a matrix of its own, one after the other:
+// what SwiGLU needs when the second half does not start on a tile. One thread per (row, 128
+// columns).
+__global__ void __launch_bounds__(256) mx_split_scales_kernel(const uint8_t *src, uint8_t *dst, uint32_t half, uint32_t kblocks) {
     grid_dependency_wait();
     grid_dependents_launch();
     const uint64_t t = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    const uint32_t kb = uint32_t(t / rows), r = uint32_t(t - uint64_t(kb) * rows);
+    const uint32_t kb = uint32_t(t / (2 * half)), r = uint32_t(t - uint64_t(kb) * (2 * half));
     if (kb >= kblocks) return;
     const uint32_t cols = kblocks * 128;
-    *reinterpret_cast<uint32_t *>(dst + mx_scale_offset(cols, r, kb * 4)) =
-        *reinterpret_cast<const uint32_t *>(src + mx_scale_offset(cols, first + r, kb * 4));
+    if (r >= half) dst += size_t((half + 127) / 128) * kblocks * kMxTileBytes;
+    *reinterpret_cast<uint32_t *>(dst + mx_scale_offset(cols, r >= half ? r - half : r, kb * 4)) =
+        *reinterpret_cast<const uint32_t *>(src + mx_scale_offset(cols, r, kb * 4));
 }
 
 // ---- host -------------------------------------------------------------------------------
@@ -326,18 +327,18 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.stages = std::min<uint32_t>({kMaxStages, uint32_t((budget - tail) / stage_bytes), ceil_div(p.kblocks, p.splits)});
     const size_t smem = std::max<size_t>({p.stages * stage_bytes + tail, 1024 + size_t(kM) * kRow * 4, 116 * 1024});
     if (swiglu) {
-        if (p.half % 128 == 0) {
-            p.us = p.ws + size_t(p.half / 128) * p.kblocks * kMxTileBytes;
-        } else {
-            if (opure_mx_scale_bytes(p.half, a->w.cols) > kScratchBytes) return OPURE_ERR_UNSUPPORTED;
-            uint8_t *us = static_cast<uint8_t *>(ctx->ws);
-            s = launch(ctx, mx_move_scales_kernel, dim3(ceil_div(uint64_t(p.half) * p.kblocks, 256)), dim3(256), 0, true, p.ws, us,
-                       p.half, p.half, p.kblocks);
+        const size_t side = opure_mx_scale_bytes(p.half, a->w.cols);
+        if (p.half % 128) {
+            if (2 * side > kScratchBytes) return OPURE_ERR_UNSUPPORTED;
+            uint8_t *split = static_cast<uint8_t *>(ctx->ws);
+            s = launch(ctx, mx_split_scales_kernel, dim3(ceil_div(uint64_t(p.rows) * p.kblocks, 256)), dim3(256), 0, true, p.ws, split,
+                       p.half, p.kblocks);
             if (s) return s;
-            p.us = us;
+            p.ws = split;
         }
+        p.us = p.ws + side;
     }
-    if (mx_gemm_pair_suits(ctx, a)) return mx_gemm_pair(ctx, a, p.us);
+    if (mx_gemm_pair_suits(ctx, a)) return mx_gemm_pair(ctx, a, p.ws);
     CUtensorMap wm, xm;
     if (!make_slot_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_slot_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
     if (swiglu)

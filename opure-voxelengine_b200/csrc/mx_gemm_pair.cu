@@ -101,8 +101,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
 template <uint32_t XF, int EPI, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
-                        const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap usmap,
-                        const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap ymap, PairParams p) {
+                        const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap,
+                        const __grid_constant__ CUtensorMap ymap, PairParams p) {
     using S = Shape<XF>;
     constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
     constexpr uint32_t kResult = kSwiglu ? kHalf : kTile;  // result columns per tile
@@ -146,75 +146,74 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint32_t issued = 0, consumed = 0;
 
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            for (uint32_t t = first; ok && t < tiles; t += pairs) {
-                const uint32_t m0 = t % p.mtiles * kTile + rank * kHalf, r0 = t / p.mtiles * kResult;
-                // This CTA's half of the weight rows, and the scale tiles of both halves.
-                const uint32_t w_row = kSwiglu ? (rank ? p.half + r0 : r0) : r0 + rank * kHalf;
-                const uint32_t x_sf = m0 / 128 * p.kblocks, g_sf = r0 / 128 * p.kblocks;
-                for (uint32_t i = 0; i < stages; ++i, ++issued) {
-                    const uint32_t s = issued % kStages;
-                    if (issued >= kStages && !mbar_wait(&empty[s], ((issued / kStages) & 1u) ^ 1u)) {
-                        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 84, blockIdx.x);
-                        fail = 1;
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t bar = tc::map_rank(smem_addr(&full[s]), 0);
+        const bool one = tc::elect();
+        const uint32_t full0 = tc::map_rank(smem_addr(&full[0]), 0);
+        uint32_t s = 0, phase = 1;  // the first round finds every stage free
+        bool ok = true;
+        for (uint32_t t = first; ok && t < tiles; t += pairs) {
+            const uint32_t m0 = t % p.mtiles * kTile + rank * kHalf, r0 = t / p.mtiles * kResult;
+            // This CTA's half of the weight rows, and the scale tiles of both halves.
+            const uint32_t w_row = kSwiglu ? (rank ? p.half + r0 : r0) : r0 + rank * kHalf;
+            for (uint32_t i = 0; i < stages; ++i, ++issued) {
+                if (issued >= kStages && !mbar_wait(&empty[s], phase)) {
+                    if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 84, blockIdx.x);
+                    fail = 1;
+                    ok = false;
+                    break;
+                }
+                const uint32_t bar = full0 + s * 8, kb = i * S::kBlocks;
+                if (one) {
                     if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kTx);
-                    const uint32_t kb = i * S::kBlocks;
                     tc::load_2d_pair(a_tile(s), &xmap, i * 128, m0, bar);
                     tc::load_2d_pair(b_tile(s), &wmap, i * 128, w_row, bar);
-                    uint8_t *sf = sf_tile(s);
-                    tc::load_2d_pair(sf, &xsmap, 0, x_sf + kb, bar);
-                    tc::load_2d_pair(sf + S::kBlocks * kMxTileBytes, &wsmap, 0, g_sf + kb, bar);
-                    if (kSwiglu)
-                        tc::load_2d_pair(sf + 2 * S::kBlocks * kMxTileBytes, &usmap, 0, g_sf + kb, bar);
-                    else
-                        tc::load_2d_pair(sf + 2 * S::kBlocks * kMxTileBytes, &wsmap, 0, g_sf + p.kblocks + kb, bar);
+                    tc::load_4d_pair(sf_tile(s), &xsmap, 0, kb, m0 / 128, 0, bar);
+                    tc::load_4d_pair(sf_tile(s) + S::kBlocks * kMxTileBytes, &wsmap, 0, kb, r0 / 128, 0, bar);
+                }
+                __syncwarp();
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
         }
-        __syncwarp();
     } else if (warp == 1 && rank == 0) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = XF == OPURE_MX_FP8 ? tc::idesc_mx(tc::kE4M3, tc::kE2M1, kTile, kTile)
-                                                          : tc::idesc_mx(tc::kPackedE2M1, tc::kPackedE2M1, kTile, kTile);
-            bool ok = true;
-            uint32_t lt = 0;
-            for (uint32_t t = first; ok && t < tiles; t += pairs, ++lt) {
-                const uint32_t acc = tmem + (lt & 1u) * kAcc1;
-                // The tile before last has left this accumulator, and the last one the columns
-                // that the two share.
-                if (lt && !mbar_wait(&drained, (lt - 1) & 1u)) {
-                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 85, blockIdx.x);
+        constexpr uint32_t idesc = XF == OPURE_MX_FP8 ? tc::idesc_mx(tc::kE4M3, tc::kE2M1, kTile, kTile)
+                                                      : tc::idesc_mx(tc::kPackedE2M1, tc::kPackedE2M1, kTile, kTile);
+        const bool one = tc::elect();
+        const uint32_t tbase = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t da0 = tc::desc_sw128(smem_addr(a_tile(0))), ds0 = tc::desc_scales(smem_addr(sf_tile(0)));
+        uint32_t s = 0, phase = 0, slot = 0, old = 0, old_phase = 0, lt = 0;
+        bool ok = true;
+        for (uint32_t t = first; ok && t < tiles; t += pairs, ++lt) {
+            const uint32_t acc = tbase + (lt & 1u) * kAcc1;
+            // The tile before last has left this accumulator, and the last one the columns
+            // that the two share.
+            if (lt && !mbar_wait(&drained, (lt - 1) & 1u)) {
+                if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 85, blockIdx.x);
+                fail = 1;
+                break;
+            }
+            for (uint32_t i = 0; i < stages; ++i, ++consumed) {
+                // This stage's columns for scales are free once the MMAs of kSlots stages ago
+                // are done (their commit).
+                if (!mbar_wait(&full[s], phase) || (consumed >= S::kSlots && !mbar_wait(&empty[old], old_phase))) {
+                    if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 86, blockIdx.x);
                     fail = 1;
+                    ok = false;
                     break;
                 }
                 tc::fence_after();
-                for (uint32_t i = 0; i < stages; ++i, ++consumed) {
-                    const uint32_t s = consumed % kStages;
-                    // This stage's columns for scales are free once the MMAs of kSlots stages ago
-                    // are done (their commit).
-                    const uint32_t old = consumed - S::kSlots;
-                    if (!mbar_wait(&full[s], (consumed / kStages) & 1u) ||
-                        (consumed >= S::kSlots && !mbar_wait(&empty[old % kStages], (old / kStages) & 1u))) {
-                        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 86, blockIdx.x);
-                        fail = 1;
-                        ok = false;
-                        break;
-                    }
-                    tc::fence_after();
-                    const uint32_t sfa = tmem + kScaleCol + consumed % S::kSlots * S::kScaleCols, sfb = sfa + S::kBlocks * 4;
-                    const uint32_t src = smem_addr(sf_tile(s));
+                const uint32_t sfa = tbase + kScaleCol + slot * S::kScaleCols, sfb = sfa + S::kBlocks * 4;
+                const uint64_t da = da0 + s * (2 * kOperand >> 4), db = da + (kOperand >> 4);
+                const uint64_t ds = ds0 + s * (S::kScaleBytes >> 4);
+                constexpr uint32_t kTile16 = kMxTileBytes >> 4;
+                if (one) {
 #pragma unroll
                     for (uint32_t b = 0; b < S::kBlocks; ++b) {
-                        tc::copy_scales_pair(sfa + b * 4, tc::desc_scales(src + b * kMxTileBytes));
-                        tc::copy_scales_pair(sfb + b * 8, tc::desc_scales(src + (S::kBlocks + b) * kMxTileBytes));
-                        tc::copy_scales_pair(sfb + b * 8 + 4, tc::desc_scales(src + (2 * S::kBlocks + b) * kMxTileBytes));
+                        tc::copy_scales_pair(sfa + b * 4, ds + b * kTile16);
+                        tc::copy_scales_pair(sfb + b * 8, ds + (S::kBlocks + b) * kTile16);
+                        tc::copy_scales_pair(sfb + b * 8 + 4, ds + (2 * S::kBlocks + b) * kTile16);
                     }
-                    const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t more = (i | k) != 0;
@@ -225,11 +224,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                               sfb + k / 2 * 8, more);
                     }
                     tc::commit_pair(&empty[s]);
+                    if (i + 1 == stages) tc::commit_pair(&acc_full[lt & 1u]);
                 }
-                if (ok) tc::commit_pair(&acc_full[lt & 1u]);
+                __syncwarp();
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+                if (++slot == S::kSlots) slot = 0;
+                if (consumed >= S::kSlots && ++old == kStages) {
+                    old = 0;
+                    old_phase ^= 1;
+                }
             }
         }
-        __syncwarp();
     } else if (warp >= kEpiWarp) {
         const uint32_t quarter = warp & 3u, part = (warp - kEpiWarp) >> 2;  // TMEM lanes, half of the columns
         const uint32_t drain_bar = tc::map_rank(smem_addr(&drained), 0);
@@ -374,24 +382,25 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 template <uint32_t XF, int EPI, typename T>
-opure_status launch_pair(opure_ctx *ctx, const CUtensorMap (&m)[6], const PairParams &p) {
+opure_status launch_pair(opure_ctx *ctx, const CUtensorMap (&m)[5], const PairParams &p) {
     auto *kernel = mx_gemm_pair_kernel<XF, EPI, T>;
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<XF>::kSmem));
     if (e != cudaSuccess) return cuda_status(e);
     const uint32_t pairs = std::min(uint32_t(ctx->sm_count) / 2, p.mtiles * p.ntiles);
-    return launch(ctx, kernel, dim3(2 * pairs), dim3(kThreads), Shape<XF>::kSmem, true, m[0], m[1], m[2], m[3], m[4], m[5], p);
+    return launch(ctx, kernel, dim3(2 * pairs), dim3(kThreads), Shape<XF>::kSmem, true, m[0], m[1], m[2], m[3], m[4], p);
 }
 
 }  // namespace
 
-bool make_map(CUtensorMap *m, CUtensorMapDataType type, const void *p, uint64_t cols, uint64_t rows, uint64_t row_bytes,
-              uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+bool make_map(CUtensorMap *m, CUtensorMapDataType type, uint32_t rank, const void *p, const uint64_t *dims, const uint64_t *strides,
+              const uint32_t *box, CUtensorMapSwizzle swizzle) {
     auto fn = encode_fn();
     if (!fn) return false;
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_cols, box_rows}, es[2] = {1, 1};
-    return fn(m, type, 2, const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    static_assert(sizeof(cuuint64_t) == sizeof(uint64_t) && sizeof(cuuint32_t) == sizeof(uint32_t), "map dimensions");
+    return fn(m, type, rank, const_cast<void *>(p), reinterpret_cast<const cuuint64_t *>(dims),
+              reinterpret_cast<const cuuint64_t *>(strides), box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -401,7 +410,7 @@ bool mx_gemm_pair_suits(const opure_ctx *ctx, const opure_mx_gemm_args *a) {
     return a->x.rows > kHalf && (uint64_t(a->x.rows) + kTile - 1) / kTile * ntiles * 4 >= uint32_t(ctx->sm_count);
 }
 
-opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *us) {
+opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *w_scales) {
     const bool swiglu = a->epilogue == OPURE_EPI_SWIGLU, fp8 = a->x.format == OPURE_MX_FP8;
     PairParams p{};
     p.n = a->x.rows;
@@ -416,28 +425,32 @@ opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uin
     p.out = a->out.codes;
     p.outs = a->out.scales;
     p.st = ctx->status;
-    // Maps: w, x, scale tiles of w, of its up half and of x (128 words each), y.
-    CUtensorMap m[6] = {};
-    const uint32_t blocks = fp8 ? 1 : 2;
+    // Maps: w, x, their scale tiles, y.
+    CUtensorMap m[5] = {};
     auto codes = [&](CUtensorMap *t, const opure_mx_matrix &q) {
         if (fp8) return make_slot_map(t, q, kHalf);
         const size_t bytes = mx_row_bytes(q.format, q.cols);
         return make_map(t, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.codes, bytes, q.rows, bytes, 128, kHalf, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    auto scales = [&](CUtensorMap *t, const uint8_t *s, uint32_t rows) {
-        return make_map(t, CU_TENSOR_MAP_DATA_TYPE_UINT32, s, 128, (uint64_t(rows) + 127) / 128 * p.kblocks, kMxTileBytes, 128,
-                        blocks, CU_TENSOR_MAP_SWIZZLE_NONE);
+    // Scale tiles as [sides][rows of tiles][tiles][128 words]: boxes of a stage's tiles of one row
+    // of tiles (x), of two neighbouring ones (w), or of one in either half of w (SwiGLU).
+    const uint32_t blocks = fp8 ? 1 : 2;
+    auto scales = [&](CUtensorMap *t, const uint8_t *s, uint32_t rows, uint32_t sides, uint32_t box_rows) {
+        const uint64_t row = uint64_t(p.kblocks) * kMxTileBytes, tile_rows = (uint64_t(rows) + 127) / 128;
+        const uint64_t dims[4] = {128, p.kblocks, tile_rows, sides}, strides[3] = {kMxTileBytes, row, row * tile_rows};
+        const uint32_t box[4] = {128, blocks, box_rows, sides};
+        return make_map(t, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, s, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
     };
-    if (!codes(&m[0], a->w) || !codes(&m[1], a->x) || !scales(&m[2], a->w.scales, p.rows) ||
-        !scales(&m[3], swiglu ? us : a->w.scales, swiglu ? p.half : p.rows) || !scales(&m[4], a->x.scales, p.n))
+    if (!codes(&m[0], a->w) || !codes(&m[1], a->x) || !scales(&m[2], w_scales, swiglu ? p.half : p.rows, swiglu ? 2 : 1, swiglu ? 1 : 2) ||
+        !scales(&m[3], a->x.scales, p.n, 1, 1))
         return OPURE_ERR_UNSUPPORTED;
-    m[5] = m[4];
+    m[4] = m[3];
     if (a->epilogue == OPURE_EPI_STORE && rows_aligned16(a->y, a->y_type, a->y_stride)) {
         const uint32_t size = type_bytes(a->y_type);
         const CUtensorMapDataType type = a->y_type == OPURE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : a->y_type == OPURE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        p.tma_store = make_map(&m[5], type, a->y, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        p.tma_store = make_map(&m[4], type, a->y, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     }
     auto go = [&](auto t, auto epi) {
         using T = decltype(t);

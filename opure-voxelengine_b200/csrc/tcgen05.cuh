@@ -29,6 +29,15 @@ __device__ __forceinline__ void alloc(uint32_t *dst, uint32_t ncols) {
 __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
+// One lane of a converged warp. The loops that issue loads and MMAs run on all lanes, and only
+// the instructions themselves on this one: addresses and descriptors then stay in uniform
+// registers, where the instructions want them (a loop inside "if (lane == 0)" moved each there
+// and took 1,000 cycles for 4 MMAs that execute in 512).
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -97,6 +106,14 @@ __device__ __forceinline__ void load_2d_pair(void *dst, const CUtensorMap *map, 
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
         "[%4];" ::"r"(smem_addr(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void load_4d_pair(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t w,
+                                             uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void alloc_pair(uint32_t *dst, uint32_t ncols) {
