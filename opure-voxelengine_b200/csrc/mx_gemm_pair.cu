@@ -61,37 +61,47 @@ struct PairParams {
     DeviceStatus *st;
 };
 
+// The largest of three magnitudes; NaN if one is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // 32 values of a thread -> 32 codes in global memory (dst 16-byte aligned); returns the scale byte.
 template <uint32_t FMT>
 __device__ __forceinline__ uint32_t quantize_block(float (&v)[32], uint8_t *dst, bool in) {
-    uint32_t m = 0;
+    float m = max_abs3(v[0], v[1], 0.f);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-    const uint32_t byte = mx_scale_byte<FMT>(m);
+    for (int j = 2; j < 32; j += 2) m = max_abs3(m, v[j], v[j + 1]);
+    const uint32_t byte = mx_scale_byte<FMT>(__float_as_uint(m) & 0x7fffffffu);
     const float inv = mx_inverse(byte);
+    const uint32_t keep = byte == 255u ? 0u : ~0u;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
-    if constexpr (FMT == OPURE_MX_FP4) {
-        uint32_t c[4];
+    for (int j = 0; j < 32; ++j) v[j] *= inv;
+    constexpr int kWords = FMT == OPURE_MX_FP4 ? 4 : 8;
+    uint32_t c[kWords];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kWords; ++j) {
+        if constexpr (FMT == OPURE_MX_FP4) {
             float f[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) f[q] = v[8 * j + q];
-            c[j] = mx_pack_fp4(f);
-        }
-        if (in) *reinterpret_cast<uint4 *>(dst) = make_uint4(c[0], c[1], c[2], c[3]);
-    } else {
-        uint32_t c[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = mx_pack_fp8(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        if (in) {
-            reinterpret_cast<uint4 *>(dst)[0] = make_uint4(c[0], c[1], c[2], c[3]);
-            reinterpret_cast<uint4 *>(dst)[1] = make_uint4(c[4], c[5], c[6], c[7]);
+            c[j] = mx_pack_fp4(f) & keep;
+        } else {
+            c[j] = mx_pack_fp8(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]) & keep;
         }
     }
+    if (in)
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4) reinterpret_cast<uint4 *>(dst)[j / 4] = make_uint4(c[j], c[j + 1], c[j + 2], c[j + 3]);
     return byte;
 }
+
+// silu(g) u with the hardware's exp2 and reciprocal, each within 2 units of fp32's last place
+// (exp's argument times log2 e adds |g| 2^-24): far below a step of the 8-bit result, and a
+// third of the instructions of expf and a rounded division.
+__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 // The results' warps stop together when one of their lanes gives up.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
@@ -282,11 +292,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     const uint32_t col = r0 + c0 + 32 * j;
                     float v[32];
+                    if (b) {
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) {
-                        const float x0 = __uint_as_float(pre[j][q]), x1 = __uint_as_float(cur[q]);
-                        v[q] = b ? silu(x0) * x1 : silu(x1) * x0;
-                        if (col + q >= p.half) v[q] = 0.f;  // gate rows past the half are up rows
+                        for (int q = 0; q < 32; ++q) v[q] = swiglu(__uint_as_float(pre[j][q]), __uint_as_float(cur[q]));
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) v[q] = swiglu(__uint_as_float(cur[q]), __uint_as_float(pre[j][q]));
+                    }
+                    if (col + 32 > p.half) {
+#pragma unroll
+                        for (int q = 0; q < 32; ++q)
+                            if (col + q >= p.half) v[q] = 0.f;  // gate rows past the half are up rows
                     }
                     const bool in = row < p.n && col < mx_kp(p.half);
                     bytes |= quantize_block<kF>(v, p.out + row * mx_row_bytes(kF, p.half) + size_t(col) * kF / 8, in) << (8 * j);
