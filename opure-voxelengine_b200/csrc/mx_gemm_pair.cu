@@ -12,8 +12,8 @@
 //            barrier
 //   warp 1   (even CTA) copies scale tiles to TMEM and issues the MMAs
 //   warps 4-11  results: two accumulators alternate, so that a tile's results leave while the
-//            next is computed. TMEM's 512 columns hold two of 256 and 48 of scales by letting the
-//            two overlap by 48 columns, which are read first; then the next tile may begin.
+//            next is computed. TMEM's 512 columns hold two of 256 and 128 of scales by letting
+//            the two overlap by 128 columns, which are read first; then the next tile may begin.
 //
 // Results go through shared memory: whole rows of 128 bytes that TMA stores, or, where y's
 // alignment or the residual forbids it, 32 columns of a row at a time by a warp. In SwiGLU the
@@ -37,7 +37,7 @@ constexpr uint32_t kThreads = 384;
 constexpr uint32_t kEpiWarp = 4, kEpiWarps = 8;
 constexpr uint32_t kOperand = kHalf * 128;  // bytes of a CTA's part of one operand of a stage
 constexpr uint32_t kSlab = 4096;            // result staging per warp: 32 rows of 128 bytes
-constexpr uint32_t kTmemCols = 512, kScaleCol = 464, kAcc1 = 208;  // accumulator 0 starts at column 0
+constexpr uint32_t kTmemCols = 512, kAcc1 = 128, kScaleCol = 384;  // accumulator 0 starts at column 0
 
 template <uint32_t XF>
 struct Shape {
@@ -45,7 +45,9 @@ struct Shape {
     static constexpr uint32_t kScaleBytes = kBlocks * 3 * kMxTileBytes;
     static constexpr uint32_t kStageBytes = 2 * kOperand + kScaleBytes;
     static constexpr uint32_t kScaleCols = kBlocks * 12;
-    static constexpr uint32_t kSlots = (kTmemCols - kScaleCol) / kScaleCols;  // scales of that many stages at once
+    // Each stage has TMEM columns of its own for its scales, so a copy never meets an MMA that
+    // still reads them: that MMA's commit freed the stage.
+    static_assert(kStages * kScaleCols <= kTmemCols - kScaleCol, "TMEM columns");
     // Bytes that arrive per CTA and stage; a copy that spreads codes counts what it reads.
     static constexpr uint32_t kTx = kOperand + (XF == OPURE_MX_FP8 ? kOperand / 2 : kOperand) + kScaleBytes;
     static constexpr size_t kSmem = 1024 + size_t(kStages) * kStageBytes + kEpiWarps * kSlab;
@@ -153,7 +155,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     const uint32_t tiles = p.mtiles * p.ntiles, pairs = gridDim.x / 2, first = blockIdx.x / 2;
     const uint32_t stages = (p.kblocks + S::kBlocks - 1) / S::kBlocks;  // per tile
-    uint32_t issued = 0, consumed = 0;
+    uint32_t issued = 0;
 
     if (warp == 0) {
         const bool one = tc::elect();
@@ -192,7 +194,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool one = tc::elect();
         const uint32_t tbase = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t da0 = tc::desc_sw128(smem_addr(a_tile(0))), ds0 = tc::desc_scales(smem_addr(sf_tile(0)));
-        uint32_t s = 0, phase = 0, slot = 0, old = 0, old_phase = 0, lt = 0;
+        uint32_t s = 0, phase = 0, lt = 0;
         bool ok = true;
         for (uint32_t t = first; ok && t < tiles; t += pairs, ++lt) {
             const uint32_t acc = tbase + (lt & 1u) * kAcc1;
@@ -203,20 +205,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 fail = 1;
                 break;
             }
-            for (uint32_t i = 0; i < stages; ++i, ++consumed) {
-                // This stage's columns for scales are free once the MMAs of kSlots stages ago
-                // are done (their commit).
-                if (!mbar_wait(&full[s], phase) || (consumed >= S::kSlots && !mbar_wait(&empty[old], old_phase))) {
+            for (uint32_t i = 0; i < stages; ++i) {
+                if (!mbar_wait(&full[s], phase)) {
                     if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 86, blockIdx.x);
                     fail = 1;
                     ok = false;
                     break;
                 }
                 tc::fence_after();
-                const uint32_t sfa = tbase + kScaleCol + slot * S::kScaleCols, sfb = sfa + S::kBlocks * 4;
+                const uint32_t sfa = tbase + kScaleCol + s * S::kScaleCols, sfb = sfa + S::kBlocks * 4;
                 const uint64_t da = da0 + s * (2 * kOperand >> 4), db = da + (kOperand >> 4);
                 const uint64_t ds = ds0 + s * (S::kScaleBytes >> 4);
                 constexpr uint32_t kTile16 = kMxTileBytes >> 4;
+                uint64_t *const release = &empty[s];
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1;
+                }
                 if (one) {
 #pragma unroll
                     for (uint32_t b = 0; b < S::kBlocks; ++b) {
@@ -233,23 +238,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             tc::mma_mxf4_pair(acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k % 2 * 2), sfa + k / 2 * 4,
                                               sfb + k / 2 * 8, more);
                     }
-                    tc::commit_pair(&empty[s]);
+                    tc::commit_pair(release);
                     if (i + 1 == stages) tc::commit_pair(&acc_full[lt & 1u]);
                 }
                 __syncwarp();
-                if (++s == kStages) {
-                    s = 0;
-                    phase ^= 1;
-                }
-                if (++slot == S::kSlots) slot = 0;
-                if (consumed >= S::kSlots && ++old == kStages) {
-                    old = 0;
-                    old_phase ^= 1;
-                }
             }
         }
     } else if (warp >= kEpiWarp) {
-        const uint32_t quarter = warp & 3u, part = (warp - kEpiWarp) >> 2;  // TMEM lanes, half of the columns
+        const uint32_t quarter = warp & 3u, part = (warp - kEpiWarp) >> 2;  // TMEM lanes, 64 columns of either half
         const uint32_t drain_bar = tc::map_rank(smem_addr(&drained), 0);
         uint8_t *slab = slabs + (warp - kEpiWarp) * kSlab;
         uint32_t lt = 0;
@@ -264,25 +260,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 break;
             }
             tc::fence_after();
-            // Accumulator 0 shares its last 48 columns, accumulator 1 its first 48: the half
-            // of the warps that has them reads them before anything else, then lets the next
-            // tile begin. The other half does so at once: it has left the tile before this one.
+            // Accumulator 0 shares its last 128 columns, accumulator 1 its first 128. Each warp has
+            // 64 of them and 64 others; it reads the shared ones first and lets the next tile begin.
             auto release = [&] {
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) tc::arrive_cluster(drain_bar);
             };
-            if (part == b) release();
+            const uint32_t shared_side = b ? 0 : kHalf, other_side = kHalf - shared_side, c0 = part * 64;
             if constexpr (kSwiglu) {
                 // Blocks 2 part and 2 part + 1 of the tile's four: gate columns 32 j, up 128 + 32 j.
                 constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
                 uint32_t pre[2][32], cur[32];
-                const uint32_t c0 = part * 64, shared_side = b ? 0 : kHalf, other_side = kHalf - shared_side;
                 tc::ld32(acc + shared_side + c0, pre[0]);
                 tc::ld32(acc + shared_side + c0 + 32, pre[1]);
+                tc::wait_ld();
+                release();
                 tc::ld32(acc + other_side + c0, cur);
                 tc::wait_ld();
-                if (part != b) release();  // accumulator 0: up blocks 2, 3; accumulator 1: gate blocks 0, 1
                 uint32_t bytes = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < 2; ++j) {
@@ -310,16 +305,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (row < p.n && r0 + c0 < mx_kp(p.half))
                     *reinterpret_cast<uint16_t *>(p.outs + mx_scale_offset(p.half, row, (r0 + c0) / 32)) = uint16_t(bytes);
             } else {
-                // Twice 64 columns, the shared ones first.
-                const bool back = part == 1 && b == 0;
 #pragma unroll 1
                 for (uint32_t h = 0; h < 2; ++h) {
                     uint32_t v[2][32];
-                    const uint32_t c = part * kHalf + (back ? 1 - h : h) * 64;
+                    const uint32_t c = (h ? other_side : shared_side) + c0;
                     tc::ld32(acc + c, v[0]);
                     tc::ld32(acc + c + 32, v[1]);
                     tc::wait_ld();
-                    if (h == 0 && part != b) release();
+                    if (h == 0) release();
                     const uint32_t col = r0 + c;
                     if (EPI == OPURE_EPI_STORE && p.tma_store) {
                         constexpr uint32_t kCols = 128 / sizeof(T);  // columns of a slab row
