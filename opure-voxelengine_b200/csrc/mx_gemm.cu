@@ -7,9 +7,9 @@
 // tokens are its M side (128 TMEM lanes), weight rows its N side. 4-bit codes cross HBM and L2
 // packed; TMA spreads them into the byte-wide slots that this kind reads.
 //
-// mx_gemm_kernel  one CTA per (128 tokens, 128 weight rows, K split). Thread 0 streams 128
+// mx_gemm_kernel  one CTA per (128 tokens, 128 weight rows, K split). Warps 0 and 3 stream 128
 //     columns a stage (codes by tiled TMA, scale tiles by bulk copies) into a ring of
-//     shared-memory stages; thread 32 copies the scale tiles to TMEM and issues the MMAs. A K
+//     shared-memory stages; warp 1 copies the scale tiles to TMEM and issues the MMAs. A K
 //     split is a thread-block cluster: each CTA leaves its sums in its own shared memory and the
 //     CTAs share the epilogue, each adding the splits of its part in rank order over distributed
 //     shared memory, so that results do not depend on timing. In SwiGLU a tile is 64 gate rows
@@ -27,12 +27,13 @@ constexpr uint32_t kM = 128;       // tokens per tile = TMEM lanes
 constexpr uint32_t kN = 128;       // weight rows per tile
 constexpr uint32_t kK = 128;       // columns per stage: one 128-byte swizzled row of byte slots
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMaxStages = 10;
 constexpr uint32_t kMaxSplits = 8;  // portable cluster size
 constexpr uint32_t kBBytes = kN * kK;
 constexpr uint32_t kScaleBytes = 2048;  // per stage: x tile, w (or gate) tile, up tile; keeps 1 KB alignment
 constexpr uint32_t kScaleCols = 12;     // TMEM columns of a stage's scales
-constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmemCols = 256;
+constexpr size_t kHalfSmem = 112 * 1024;  // dynamic shared memory of two CTAs on an SM
 constexpr uint32_t kRow = kN + 4;       // floats per row of the shared partial sums
 static_assert(kN + kMaxStages * kScaleCols <= kTmemCols, "TMEM columns");
 
@@ -71,14 +72,14 @@ __device__ __forceinline__ void store_block(float v, uint8_t *codes, uint8_t *sc
 
 // T: the type of y, or for SwiGLU uint8_t (E4M3) or uint32_t (E2M1).
 template <int EPI, typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, GemmParams p) {
     constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
     constexpr uint32_t kTileRows = kSwiglu ? kN / 2 : kN;  // result columns per tile
     extern __shared__ uint8_t dsm[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_base;
-    __shared__ uint32_t issued_s, consumed_s;
+    __shared__ uint32_t issued_s[2], consumed_s;
     __shared__ int fail;
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -97,13 +98,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < p.stages; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 2);
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
         fail = 0;
-        issued_s = 0;
-        consumed_s = 0;
+        issued_s[0] = issued_s[1] = consumed_s = 0;
         tc::prefetch_map(&wmap);
         tc::prefetch_map(&xmap);
     }
@@ -115,64 +115,78 @@ __global__ void __launch_bounds__(kThreads, 1)
     grid_dependency_wait();
     grid_dependents_launch();
 
-    if (warp == 0) {
-        if (lane == 0) {
-            uint32_t i = 0;
-            for (; i < nk; ++i) {
-                const uint32_t s = i % p.stages, kb = kb0 + i;
-                if (i >= p.stages && !mbar_wait(&empty[s], ((i / p.stages) & 1u) ^ 1u)) {
-                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 80, blockIdx.x);
-                    fail = 1;
-                    break;
-                }
+    if (warp == 0 || warp == 3) {
+        // Warp 0 loads the weights, warp 3 the tokens.
+        const bool one = tc::elect();
+        uint32_t s = 0, phase = 1, i = 0;
+        for (; i < nk; ++i) {
+            if (i >= p.stages && !mbar_wait(&empty[s], phase)) {
+                if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 80, blockIdx.x);
+                fail = 1;
+                break;
+            }
+            const uint32_t kb = kb0 + i;
+            if (one && warp == 0) {
                 // A spreading copy counts the bytes that it reads, not the slots that it fills.
-                mbar_expect_tx(&full[s], kBBytes / 2 + a_bytes * p.x_format / 8 + kMxTileBytes * (kSwiglu ? 3 : 2));
+                mbar_expect_tx(&full[s], kBBytes / 2 + kMxTileBytes * (kSwiglu ? 2 : 1));
                 tc::load_2d(b_tile(s), &wmap, kb * kK, r0, &full[s]);
                 if (kSwiglu) tc::load_2d(b_tile(s) + kBBytes / 2, &wmap, kb * kK, p.half + r0, &full[s]);
-                bulk_load(sf_tile(s) + 512, p.ws + (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
-                if (kSwiglu)
-                    bulk_load(sf_tile(s) + 1024, p.us + (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
+                const size_t tile = (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes;
+                bulk_load(sf_tile(s) + 512, p.ws + tile, kMxTileBytes, &full[s]);
+                if (kSwiglu) bulk_load(sf_tile(s) + 1024, p.us + tile, kMxTileBytes, &full[s]);
+            }
+            if (one && warp == 3) {
+                mbar_expect_tx(&full[s], a_bytes * p.x_format / 8 + kMxTileBytes);
                 tc::load_2d(a_tile(s), &xmap, kb * kK, m0, &full[s]);
                 bulk_load_keep(sf_tile(s), p.xs + (size_t(m0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
             }
-            issued_s = i;
+            __syncwarp();
+            if (++s == p.stages) {
+                s = 0;
+                phase ^= 1;
+            }
         }
-        __syncwarp();
+        if (one) issued_s[warp / 3] = i;
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc =
-                tc::idesc_mx(p.x_format == OPURE_MX_FP8 ? tc::kE4M3 : tc::kE2M1, tc::kE2M1, kM, kSwiglu ? kN / 2 : kN);
-            // In SwiGLU a tile's 64 rows are the first or the second half of their scale tile.
-            const uint32_t shift = kSwiglu ? r0 / 32 % 4 : 0;
-            uint32_t i = 0;
-            for (; i < nk; ++i) {
-                const uint32_t s = i % p.stages;
-                if (!mbar_wait(&full[s], (i / p.stages) & 1u)) {
-                    report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 81, blockIdx.x);
-                    fail = 1;
-                    break;
-                }
-                tc::fence_after();
-                // Each stage has TMEM columns of its own for its scales, so a copy never meets
-                // an MMA that still reads them: the stage was freed by that MMA's commit.
-                const uint32_t sf = tmem + kN + s * kScaleCols, sfs = smem_addr(sf_tile(s));
-                tc::copy_scales(sf, tc::desc_scales(sfs));
-                tc::copy_scales(sf + 4, tc::desc_scales(sfs + 512));
-                if (kSwiglu) tc::copy_scales(sf + 8, tc::desc_scales(sfs + 1024));
-                const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
+        const bool one = tc::elect();
+        const uint32_t idesc =
+            tc::idesc_mx(p.x_format == OPURE_MX_FP8 ? tc::kE4M3 : tc::kE2M1, tc::kE2M1, kM, kSwiglu ? kN / 2 : kN);
+        // In SwiGLU a tile's 64 rows are the first or the second half of their scale tile.
+        const uint32_t shift = kSwiglu ? r0 / 32 % 4 : 0, tbase = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t s = 0, phase = 0, i = 0;
+        for (; i < nk; ++i) {
+            if (!mbar_wait(&full[s], phase)) {
+                if (one) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 81, blockIdx.x);
+                fail = 1;
+                break;
+            }
+            tc::fence_after();
+            // Each stage has TMEM columns of its own for its scales, so a copy never meets an
+            // MMA that still reads them: the stage was freed by that MMA's commit.
+            const uint32_t sf = tbase + kN + s * kScaleCols;
+            const uint64_t ds = tc::desc_scales(smem_addr(sf_tile(s)));
+            const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
+            if (one) {
+                tc::copy_scales(sf, ds);
+                tc::copy_scales(sf + 4, ds + (512 >> 4));
+                if (kSwiglu) tc::copy_scales(sf + 8, ds + (1024 >> 4));
 #pragma unroll
                 for (uint32_t k = 0; k < kK / 32; ++k) {
                     const uint32_t id = idesc | tc::idesc_block(k), acc = (i | k) != 0;
-                    tc::mma_mxf8f6f4(tmem, da + 2 * k, db + 2 * k, id, sf, sf + 4 + shift, acc);
+                    tc::mma_mxf8f6f4(tbase, da + 2 * k, db + 2 * k, id, sf, sf + 4 + shift, acc);
                     if (kSwiglu)
-                        tc::mma_mxf8f6f4(tmem + kN / 2, da + 2 * k, db + 2 * k + (kBBytes / 2 >> 4), id, sf, sf + 8 + shift, acc);
+                        tc::mma_mxf8f6f4(tbase + kN / 2, da + 2 * k, db + 2 * k + (kBBytes / 2 >> 4), id, sf, sf + 8 + shift, acc);
                 }
                 tc::commit(&empty[s]);
+                if (i + 1 == nk) tc::commit(&done);
             }
-            consumed_s = i;
-            tc::commit(&done);
+            __syncwarp();
+            if (++s == p.stages) {
+                s = 0;
+                phase ^= 1;
+            }
         }
-        __syncwarp();
+        consumed_s = i;
     }
     if (!mbar_wait(&done, 0)) {
         report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 82, blockIdx.x);
@@ -182,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     const bool failed = fail;
     if (failed && threadIdx.x == 0)  // leave no copy in flight into this CTA's shared memory
-        for (uint32_t i = consumed_s; i < issued_s; ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u);
+        for (uint32_t i = consumed_s; i < max(issued_s[0], issued_s[1]); ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u);
 
     // Accumulators -> shared memory (every stage is done with): part[token][column]. Warps w and
     // w + 4 share TMEM lanes 32 (w % 4) ..; each takes half of the columns.
@@ -322,10 +336,12 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.a_rows = std::min(kM, (p.n + 7) & ~7u);
     const uint32_t stage_bytes = kBBytes + kScaleBytes + p.a_rows * kK;
     // After the ring: 1 KB to align it, and the rest of the last stage's 128 rows of A. The
-    // partial sums share it. Below 114 KB two CTAs would fit an SM, which all of TMEM does not.
-    const size_t tail = 1024 + size_t(kM - p.a_rows) * kK, budget = std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024;
+    // partial sums share it. More CTAs than SMs go two to an SM, which TMEM's 512 columns allow
+    // and, above 75 KB each, no third.
+    const size_t tail = 1024 + size_t(kM - p.a_rows) * kK;
+    const size_t budget = tiles * mtiles * p.splits > uint32_t(ctx->sm_count) ? kHalfSmem : std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024;
     p.stages = std::min<uint32_t>({kMaxStages, uint32_t((budget - tail) / stage_bytes), ceil_div(p.kblocks, p.splits)});
-    const size_t smem = std::max<size_t>({p.stages * stage_bytes + tail, 1024 + size_t(kM) * kRow * 4, 116 * 1024});
+    const size_t smem = std::max<size_t>({p.stages * stage_bytes + tail, 1024 + size_t(kM) * kRow * 4, 80 * 1024});
     if (swiglu) {
         const size_t side = opure_mx_scale_bytes(p.half, a->w.cols);
         if (p.half % 128) {
