@@ -10,10 +10,10 @@
 // mx_gemm_kernel  one CTA per (128 tokens, 128 weight rows, K split). Warps 0 and 3 stream 128
 //     columns a stage (codes by tiled TMA, scale tiles by bulk copies) into a ring of
 //     shared-memory stages; warp 1 copies the scale tiles to TMEM and issues the MMAs. A K
-//     split is a thread-block cluster: each CTA leaves its sums in its own shared memory and the
-//     CTAs share the epilogue, each adding the splits of its part in rank order over distributed
-//     shared memory, so that results do not depend on timing. In SwiGLU a tile is 64 gate rows
-//     and the 64 up rows that go with them.
+//     split is a thread-block cluster whose CTAs share the epilogue: each sends its sums to the
+//     CTAs that finish them (st.async, counted by the receiver's mbarrier; nobody waits for a
+//     reader), which add the splits in rank order, so that results do not depend on timing. In
+//     SwiGLU a tile is 64 gate rows and the 64 up rows that go with them.
 // All waits are bounded (1 s); a timeout is reported in the ctx status word.
 #include <algorithm>
 #include <type_traits>
@@ -34,7 +34,7 @@ constexpr uint32_t kScaleBytes = 2048;  // per stage: x tile, w (or gate) tile, 
 constexpr uint32_t kScaleCols = 12;     // TMEM columns of a stage's scales
 constexpr uint32_t kTmemCols = 256;
 constexpr size_t kHalfSmem = 112 * 1024;  // dynamic shared memory of two CTAs on an SM
-constexpr uint32_t kRow = kN + 4;       // floats per row of the shared partial sums
+constexpr uint32_t kUnit = 512;           // partial sums of 4 tokens x 32 columns, bytes
 static_assert(kN + kMaxStages * kScaleCols <= kTmemCols, "TMEM columns");
 
 struct GemmParams {
@@ -42,6 +42,8 @@ struct GemmParams {
     uint32_t n, rows, kblocks, splits, stages;
     uint32_t a_rows;              // token rows that a stage holds: multiple of 8, at most 128
     uint32_t half;                // SwiGLU: first up row = result columns
+    uint32_t sums_offset;         // of the received sums, past the ring
+    bool vec;                     // rows of y and residual allow accesses of 4 values
     uint32_t x_format;
     void *y;
     size_t y_stride;
@@ -50,22 +52,24 @@ struct GemmParams {
     DeviceStatus *st;
 };
 
-// Quantises 32 values, one per lane, and stores them as one block of `row` (codes) and `scale`.
+// Quantises a block held as 4 values in each of 8 neighbouring lanes; `codes` is the block's
+// place in its row. All lanes of the warp call it; only those with `in` store.
 template <uint32_t FMT>
-__device__ __forceinline__ void store_block(float v, uint8_t *codes, uint8_t *scale) {
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-    v = byte == 255u ? 0.f : v * mx_inverse(byte);
+__device__ __forceinline__ void store_block(const float (&v)[4], uint8_t *codes, uint8_t *scale, bool in) {
+    const uint32_t lane = threadIdx.x & 7u;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t byte = mx_scale_byte<FMT>(m), keep = byte == 255u ? 0u : ~0u;
+    const float inv = mx_inverse(byte);
+    if (!in) return;
     if constexpr (FMT == OPURE_MX_FP4) {
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __shfl_sync(0xffffffffu, v, (lane % 4) * 8 + j);
-        if (lane < 4) reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp4(f);
+        const float f[8] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+        reinterpret_cast<uint16_t *>(codes)[lane] = uint16_t(mx_pack_fp4(f) & keep);
     } else {
-        float f[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = __shfl_sync(0xffffffffu, v, (lane % 8) * 4 + j);
-        if (lane < 8) reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp8(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv) & keep;
     }
     if (lane == 0) *scale = uint8_t(byte);
 }
@@ -76,8 +80,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, GemmParams p) {
     constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
     constexpr uint32_t kTileRows = kSwiglu ? kN / 2 : kN;  // result columns per tile
+    constexpr uint32_t kChunks = kTileRows / 32, kSides = kSwiglu ? 2 : 1;
     extern __shared__ uint8_t dsm[];
-    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done, recv;
     __shared__ uint32_t tmem_base;
     __shared__ uint32_t issued_s[2], consumed_s;
     __shared__ int fail;
@@ -95,6 +100,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto b_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes; };
     auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes; };
     auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
+    // Results in units of 4 tokens x 32 columns. Unit u is finished by CTA u % splits, whose
+    // sums[u / splits][split][side] receive every split's part. Not in the ring: a CTA that is
+    // done with its split sends while this one still computes.
+    uint8_t *sums = base + p.sums_offset;
+    const uint32_t n = min(p.n - m0, kM), units = (n + 3) / 4 * kChunks;
+    const uint32_t own_units = (units + p.splits - 1 - split) / p.splits;
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < p.stages; ++s) {
@@ -102,6 +113,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             mbar_init(&empty[s], 1);
         }
         mbar_init(&done, 1);
+        mbar_init(&recv, 1);
+        mbar_expect_tx(&recv, own_units * p.splits * kSides * kUnit);
         fail = 0;
         issued_s[0] = issued_s[1] = consumed_s = 0;
         tc::prefetch_map(&wmap);
@@ -112,6 +125,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
+    tc::cluster_arrive();  // this CTA's recv is ready
     grid_dependency_wait();
     grid_dependents_launch();
 
@@ -198,56 +212,79 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (failed && threadIdx.x == 0)  // leave no copy in flight into this CTA's shared memory
         for (uint32_t i = consumed_s; i < max(issued_s[0], issued_s[1]); ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u);
 
-    // Accumulators -> shared memory (every stage is done with): part[token][column]. Warps w and
-    // w + 4 share TMEM lanes 32 (w % 4) ..; each takes half of the columns.
-    float *part = reinterpret_cast<float *>(base);
-    const uint32_t n = min(p.n - m0, kM);
-    const uint32_t quarter = warp & 3u;
+    // Accumulators -> the CTAs that finish them. Warps w and w + 4 share TMEM lanes 32 (w % 4) ..
+    // (tokens); each takes half of the columns.
+    tc::cluster_wait();
+    const uint32_t quarter = warp & 3u, part = warp >> 2, token = quarter * 32 + lane;
     if (!failed && quarter * 32 < n) {
-        for (uint32_t c = (warp >> 2) * (kN / 2), e = c + kN / 2; c < e; c += 32) {
-            uint32_t r[32];
-            tc::ld32(tmem + ((quarter * 32) << 16) + c, r);
-            tc::wait_ld();
-            float4 *dst = reinterpret_cast<float4 *>(part + (quarter * 32 + lane) * kRow + c);
-            if (quarter * 32 + lane < n)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    dst[j] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
-                                         __uint_as_float(r[4 * j + 3]));
+        for (uint32_t c = 0; c < 2; ++c) {
+            uint32_t r[32];
+            tc::ld32(tmem + ((quarter * 32) << 16) + part * (kN / 2) + c * 32, r);
+            tc::wait_ld();
+            if (token < (n + 3) / 4 * 4) {
+                const uint32_t u = token / 4 * kChunks + (kSwiglu ? c : part * 2 + c);
+                const uint32_t at = ((u / p.splits * p.splits + split) * kSides + (kSwiglu ? part : 0)) * kUnit + token % 4 * 128;
+                const uint32_t dst = tc::map_rank(smem_addr(sums + at), u % p.splits);
+                const uint32_t bar = tc::map_rank(smem_addr(&recv), u % p.splits);
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) tc::st_async_f4(dst + j * 16, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3], bar);
+            }
+        }
+    }
+    const bool got = mbar_wait(&recv, 0);
+    if (!got && threadIdx.x == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 83, blockIdx.x);
+
+    // Epilogue: a warp takes a unit, a lane 4 columns of a token.
+    for (uint32_t l = warp; got && l < own_units; l += kThreads / 32) {
+        const uint32_t u = l * p.splits + split, i = m0 + u / kChunks * 4 + lane / 8;
+        const uint32_t col = r0 + u % kChunks * 32 + lane % 8 * 4;
+        float v[kSides][4] = {};
+#pragma unroll
+        for (uint32_t q = 0; q < kMaxSplits; ++q) {
+            if (q >= p.splits) break;
+#pragma unroll
+            for (uint32_t s = 0; s < kSides; ++s) {
+                const float4 f = lds_f4(reinterpret_cast<const float *>(sums + ((l * p.splits + q) * kSides + s) * kUnit) + lane * 4);
+                v[s][0] += f.x; v[s][1] += f.y; v[s][2] += f.z; v[s][3] += f.w;
+            }
+        }
+        if constexpr (kSwiglu) {
+            constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                v[0][j] = col + j < p.half ? silu(v[0][j]) * v[1][j] : 0.f;  // gate rows past the half are up rows
+            const uint32_t block = col / 32 * 32;
+            store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(block) * kF / 8,
+                            p.outs + mx_scale_offset(p.half, i, block / 32), i < p.n && block < mx_kp(p.half));
+        } else if (i < p.n) {
+            T *y = static_cast<T *>(p.y) + i * p.y_stride + col;
+            const T *res = static_cast<const T *>(p.residual) + i * p.y_stride + col;
+            const uint32_t m = col < p.rows ? min(p.rows - col, 4u) : 0u;
+            if (p.vec && m == 4) {
+                struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
+                if constexpr (EPI == OPURE_EPI_ADD) {
+                    const Quad q = *reinterpret_cast<const Quad *>(res);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) v[0][j] += to_f32(q.v[j]);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) o.v[j] = from_f32<T>(v[0][j]);
+                *reinterpret_cast<Quad *>(y) = o;
+            } else {
+                for (uint32_t j = 0; j < m; ++j) {
+                    if constexpr (EPI == OPURE_EPI_ADD) v[0][j] += to_f32(res[j]);
+                    y[j] = from_f32<T>(v[0][j]);
+                }
+            }
         }
     }
     tc::fence_before();
     __syncthreads();
     if (warp == 2) tc::dealloc(tmem, kTmemCols);
-    if (p.splits > 1) tc::cluster_sync();
-
-    // Epilogue: a warp takes 32 result columns of a token, a lane one of them.
-    constexpr uint32_t kChunks = kTileRows / 32;
-    auto sum = [&](uint32_t at) {
-        if (p.splits == 1) return part[at];
-        float v = 0.f;
-        const uint32_t a = smem_addr(part + at);
-        for (uint32_t q = 0; q < p.splits; ++q) v += tc::ld_cluster_f32(tc::map_rank(a, q));
-        return v;
-    };
-    for (uint32_t u = split + p.splits * warp; !failed && u < n * kChunks; u += p.splits * (kThreads / 32)) {
-        const uint32_t i = u / kChunks, c = u % kChunks * 32 + lane, col = r0 + c;
-        float v = sum(i * kRow + c);
-        if constexpr (kSwiglu) {
-            v = silu(v) * sum(i * kRow + kN / 2 + c);
-            if (col >= p.half) v = 0.f;  // gate rows past the half are up rows
-            if (col - lane < mx_kp(p.half)) {
-                constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
-                store_block<kF>(v, p.out + (m0 + i) * mx_row_bytes(kF, p.half) + (col - lane) * kF / 8,
-                                p.outs + mx_scale_offset(p.half, m0 + i, (col - lane) / 32));
-            }
-        } else if (col < p.rows) {
-            const size_t o = (m0 + i) * p.y_stride + col;
-            if constexpr (EPI == OPURE_EPI_ADD) v += to_f32(static_cast<const T *>(p.residual)[o]);
-            static_cast<T *>(p.y)[o] = from_f32<T>(v);
-        }
-    }
-    if (p.splits > 1) tc::cluster_sync();  // the others have read this CTA's sums
+    // Nobody reads another CTA's memory, so a CTA may leave when it has all of its sums. One that
+    // gave up waiting stays until the others have left or gave up too: they may still send.
+    if (!got) tc::cluster_sync();
 }
 
 // Scale tiles of the two halves of a matrix, each as a matrix of its own, one after the other:
@@ -335,13 +372,22 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.splits = std::max(1u, std::min({kMaxSplits, p.kblocks, uint32_t(ctx->sm_count) / std::max(1u, tiles * mtiles)}));
     p.a_rows = std::min(kM, (p.n + 7) & ~7u);
     const uint32_t stage_bytes = kBBytes + kScaleBytes + p.a_rows * kK;
-    // After the ring: 1 KB to align it, and the rest of the last stage's 128 rows of A. The
-    // partial sums share it. More CTAs than SMs go two to an SM, which TMEM's 512 columns allow
-    // and, above 75 KB each, no third.
-    const size_t tail = 1024 + size_t(kM - p.a_rows) * kK;
-    const size_t budget = tiles * mtiles * p.splits > uint32_t(ctx->sm_count) ? kHalfSmem : std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024;
-    p.stages = std::min<uint32_t>({kMaxStages, uint32_t((budget - tail) / stage_bytes), ceil_div(p.kblocks, p.splits)});
-    const size_t smem = std::max<size_t>({p.stages * stage_bytes + tail, 1024 + size_t(kM) * kRow * 4, 80 * 1024});
+    // After the ring: the rest of the last stage's 128 rows of A, and the received sums (without a
+    // split they take the ring's place, which is done with by then); before it 1 KB to align it.
+    const uint32_t chunks = swiglu ? kN / 64 : kN / 32, units = ceil_div(std::min(p.n, kM), 4) * chunks;
+    const size_t sums = size_t(ceil_div(units, p.splits)) * p.splits * (swiglu ? 2 : 1) * kUnit;
+    const size_t tail = size_t(kM - p.a_rows) * kK, fixed = 1024 + tail + (p.splits > 1 ? sums : 0);
+    auto stages_in = [&](size_t bytes) {
+        return std::min<uint32_t>({kMaxStages, uint32_t((bytes - fixed) / stage_bytes), ceil_div(p.kblocks, p.splits)});
+    };
+    // More CTAs than SMs go two to an SM (TMEM's 512 columns allow it and, above 75 KB each, no
+    // third) where that leaves each a ring of at least 4 stages, or all that it needs.
+    p.stages = stages_in(std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024);
+    if (tiles * mtiles * p.splits > uint32_t(ctx->sm_count) && stages_in(kHalfSmem) >= std::min(4u, p.stages))
+        p.stages = stages_in(kHalfSmem);
+    p.sums_offset = p.splits > 1 ? p.stages * stage_bytes + uint32_t(tail) : 0;
+    const size_t smem = std::max<size_t>({1024 + p.stages * stage_bytes + tail, 1024 + p.sums_offset + sums, 80 * 1024});
+    p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
     if (swiglu) {
         const size_t side = opure_mx_scale_bytes(p.half, a->w.cols);
         if (p.half % 128) {
