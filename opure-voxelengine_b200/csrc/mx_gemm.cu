@@ -52,28 +52,6 @@ struct GemmParams {
     DeviceStatus *st;
 };
 
-// Quantises a block held as 4 values in each of 8 neighbouring lanes; `codes` is the block's
-// place in its row. All lanes of the warp call it; only those with `in` store.
-template <uint32_t FMT>
-__device__ __forceinline__ void store_block(const float (&v)[4], uint8_t *codes, uint8_t *scale, bool in) {
-    const uint32_t lane = threadIdx.x & 7u;
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t byte = mx_scale_byte<FMT>(m), keep = byte == 255u ? 0u : ~0u;
-    const float inv = mx_inverse(byte);
-    if (!in) return;
-    if constexpr (FMT == OPURE_MX_FP4) {
-        const float f[8] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-        reinterpret_cast<uint16_t *>(codes)[lane] = uint16_t(mx_pack_fp4(f) & keep);
-    } else {
-        reinterpret_cast<uint32_t *>(codes)[lane] = mx_pack_fp8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv) & keep;
-    }
-    if (lane == 0) *scale = uint8_t(byte);
-}
-
 // T: the type of y, or for SwiGLU uint8_t (E4M3) or uint32_t (E2M1).
 template <int EPI, typename T>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -102,7 +80,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
     // Results in units of 4 tokens x 32 columns. Unit u is finished by CTA u % splits, whose
     // sums[u / splits][split][side] receive every split's part. Not in the ring: a CTA that is
-    // done with its split sends while this one still computes.
+    // done with its split sends while this one still computes. A token's eight pieces of 16 bytes
+    // stand in an order of its own (piece ^ token % 8), so that 32 tokens' stores spread over all
+    // banks.
     uint8_t *sums = base + p.sums_offset;
     const uint32_t n = min(p.n - m0, kM), units = (n + 3) / 4 * kChunks;
     const uint32_t own_units = (units + p.splits - 1 - split) / p.splits;
@@ -228,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const uint32_t dst = tc::map_rank(smem_addr(sums + at), u % p.splits);
                 const uint32_t bar = tc::map_rank(smem_addr(&recv), u % p.splits);
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) tc::st_async_f4(dst + j * 16, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3], bar);
+                for (uint32_t j = 0; j < 8; ++j) tc::st_async_f4(dst + ((j ^ (lane & 7u)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3], bar);
             }
         }
     }
@@ -239,13 +219,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (uint32_t l = warp; got && l < own_units; l += kThreads / 32) {
         const uint32_t u = l * p.splits + split, i = m0 + u / kChunks * 4 + lane / 8;
         const uint32_t col = r0 + u % kChunks * 32 + lane % 8 * 4;
+        const uint32_t piece = lane / 8 * 128 + ((lane ^ (u / kChunks * 4 + lane / 8)) & 7u) * 16;
         float v[kSides][4] = {};
 #pragma unroll
         for (uint32_t q = 0; q < kMaxSplits; ++q) {
             if (q >= p.splits) break;
 #pragma unroll
             for (uint32_t s = 0; s < kSides; ++s) {
-                const float4 f = lds_f4(reinterpret_cast<const float *>(sums + ((l * p.splits + q) * kSides + s) * kUnit) + lane * 4);
+                const float4 f = lds_f4(reinterpret_cast<const float *>(sums + ((l * p.splits + q) * kSides + s) * kUnit + piece));
                 v[s][0] += f.x; v[s][1] += f.y; v[s][2] += f.z; v[s][3] += f.w;
             }
         }
@@ -258,25 +239,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(block) * kF / 8,
                             p.outs + mx_scale_offset(p.half, i, block / 32), i < p.n && block < mx_kp(p.half));
         } else if (i < p.n) {
-            T *y = static_cast<T *>(p.y) + i * p.y_stride + col;
-            const T *res = static_cast<const T *>(p.residual) + i * p.y_stride + col;
-            const uint32_t m = col < p.rows ? min(p.rows - col, 4u) : 0u;
-            if (p.vec && m == 4) {
-                struct alignas(4 * sizeof(T)) Quad { T v[4]; } o;
-                if constexpr (EPI == OPURE_EPI_ADD) {
-                    const Quad q = *reinterpret_cast<const Quad *>(res);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) v[0][j] += to_f32(q.v[j]);
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) o.v[j] = from_f32<T>(v[0][j]);
-                *reinterpret_cast<Quad *>(y) = o;
-            } else {
-                for (uint32_t j = 0; j < m; ++j) {
-                    if constexpr (EPI == OPURE_EPI_ADD) v[0][j] += to_f32(res[j]);
-                    y[j] = from_f32<T>(v[0][j]);
-                }
-            }
+            const size_t at = i * p.y_stride + col;
+            store_quad<EPI>(v[0], static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at,
+                            col < p.rows ? min(p.rows - col, 4u) : 0u, p.vec);
         }
     }
     tc::fence_before();
@@ -400,6 +365,7 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
         }
         p.us = p.ws + side;
     }
+    if (mx_gemv_suits(a)) return mx_gemv(ctx, a, p.ws, p.us);
     if (mx_gemm_pair_suits(ctx, a)) return mx_gemm_pair(ctx, a, p.ws);
     CUtensorMap wm, xm;
     if (!make_slot_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_slot_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
