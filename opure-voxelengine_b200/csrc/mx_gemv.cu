@@ -3,21 +3,23 @@
 //
 // Bound by memory: a weight is 0.53 bytes and used once per token. At the measured 6.45 TB/s an SM
 // gets 23 bytes, 43 weights, a clock, so that about 3 lane instructions per weight is all that its
-// 128 lanes have. mma.sync m16n8k16 (fp16 in, fp32 out) takes the multiplications: 16 weight rows,
-// up to 8 tokens, half a block of 32 columns. The codes' values are exact in fp16, and a block's
-// sum is scaled by both scales in fp32. The tensor-core kernels' fixed costs (TMEM, tensor maps,
-// a single issuing thread) are what this kernel avoids: there one token took 2 to 3 times as long.
+// 128 lanes have. mma.sync m16n8k16 (fp16 in, fp32 out) takes the multiplications; the codes'
+// values are exact in fp16, and a block's sum is scaled by both scales in fp32. The tensor-core
+// kernels' fixed costs (TMEM, tensor maps, a single issuing thread) are what this kernel avoids.
 //
-// A warp reads 16 rows x 128 columns at once: lane 4 g + t holds block t (16 bytes) of rows g and
-// g + 8. mma.sync wants a row's block spread over the four lanes t; which columns a lane holds
-// does not matter as long as weights and tokens agree, so four words are exchanged among the four
-// lanes and lane t takes columns 8 t .. 8 t + 7 of every block.
+// A warp reads 16 weight rows x 128 columns as lane 4 g + t holding block t (16 bytes) of rows g
+// and g + 8, and feeds that to the MMA as it stands: each MMA then sums over columns of all four
+// blocks. The token side keeps the blocks apart. Its 8 columns are 2 tokens x 4 blocks, column
+// 4 j + b having token j's values in the k slots of lanes t = b and zeros elsewhere, so that after
+// the 8 MMAs of a piece D[row][4 j + b] is the sum over block b alone. Nothing is moved between
+// lanes, and a piece is scaled once: 1.1 instructions per weight for 1 or 2 tokens. (With a block's
+// 8 columns per MMA taken by 8 tokens, four words had to be exchanged among lanes and every block
+// scaled by itself: 2.8 per weight.)
 //
-// A CTA is tiles x splits warps: `tiles` tiles of 16 rows (SwiGLU: 32 gate rows and the up rows that
-// go with them), each shared by `splits` warps that take every splits'th 128 columns and are added
-// in order through shared memory.
+// A CTA is units x splits warps: a unit is 16 MT rows (in SwiGLU the CTA's units are 32 gate rows
+// and the 32 up rows that go with them), shared by `splits` warps that take every splits'th 128
+// columns and are added in order through shared memory.
 #include <algorithm>
-#include <type_traits>
 
 #include "mx_gemm.cuh"
 
@@ -26,11 +28,11 @@ namespace {
 
 constexpr uint32_t kMaxTokens = 8;
 constexpr uint32_t kMaxWarps = 16;
-constexpr uint32_t kAhead = 4;  // 128-column pieces that a warp has in flight
 
 struct GemvParams {
     const uint8_t *w, *ws, *us, *x, *xs;
-    uint32_t n, rows, cols, half, tiles, splits;
+    uint32_t n, rows, cols, half, units, splits;
+    uint32_t epilogue, y_type, out_format;
     void *y;
     size_t y_stride;
     const void *residual;
@@ -46,167 +48,193 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 // Two scale bytes as fp32.
-__device__ __forceinline__ void scale_pair(uint32_t bytes, float &s0, float &s1) {
+__device__ __forceinline__ void scale_pair(uint16_t bytes, float &s0, float &s1) {
     uint32_t b;
-    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(b) : "h"(uint16_t(bytes)));
+    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(b) : "h"(bytes));
     s0 = __uint_as_float(b << 16);
     s1 = __uint_as_float(b & 0xffff0000u);
 }
 
-// Word j of lane t <-> word t of lane j, among four neighbouring lanes.
-__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
-    const uint32_t t = threadIdx.x & 3u;
-    {
-        const bool up = t & 2u;
-        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? w[0] : w[2], 2), r1 = __shfl_xor_sync(0xffffffffu, up ? w[1] : w[3], 2);
-        if (up) {
-            w[0] = r0;
-            w[1] = r1;
-        } else {
-            w[2] = r0;
-            w[3] = r1;
-        }
-    }
-    {
-        const bool up = t & 1u;
-        const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? w[0] : w[1], 1), r1 = __shfl_xor_sync(0xffffffffu, up ? w[2] : w[3], 1);
-        if (up) {
-            w[0] = r0;
-            w[2] = r1;
-        } else {
-            w[1] = r0;
-            w[3] = r1;
-        }
-    }
-}
-
-// What a warp reads of 128 columns.
+// Weights of 16 MT rows x 128 columns: block t of rows g and g + 8 of each tile, and the scales of
+// the two blocks whose sums this lane gets.
+template <uint32_t MT>
+struct Weights {
+    uint4 w[2 * MT];
+    uint16_t s[2 * MT];
+};
+// Two tokens' 128 columns: this lane's block of its token (or zeros), and two blocks' scales.
 template <uint32_t XF>
-struct Piece {
-    uint4 w[2];            // block t of rows g, g + 8
-    uint32_t sw[2];        // four scales of each
-    uint32_t x[4][XF / 4];  // columns 8 t .. of token g in each block
-    uint32_t sx[2];        // four scales of tokens 2 t, 2 t + 1
+struct Tokens {
+    uint4 x[XF / 4];
+    uint16_t s;
 };
 
-// T: the type of y, or for SwiGLU uint8_t (E4M3) or uint32_t (E2M1).
-template <uint32_t XF, int EPI, typename T>
+// MT: tiles of 16 rows per warp. NP: pairs of tokens.
+template <uint32_t XF, uint32_t MT, uint32_t NP>
 __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
-    constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
-    __shared__ float part[kMaxWarps][16][kMaxTokens];
+    constexpr uint32_t kAhead = MT == 1 ? 4 : 3;  // pieces of weights in flight
+    constexpr uint32_t kRows = 16 * MT;
+    __shared__ float part[kMaxWarps][kRows][2 * NP + 1];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    const uint32_t tile = warp / p.splits, split = warp % p.splits;
+    const uint32_t unit = warp / p.splits, split = warp % p.splits;
     const uint32_t pieces = mx_kp(p.cols) / 128;
-    // This warp's rows. In SwiGLU tiles 0 and 1 are gate rows, 2 and 3 up rows, whose scale tiles
-    // are counted from the first up row.
-    const uint32_t c0 = blockIdx.x * (kSwiglu ? 32 : p.tiles * 16);  // first result column of the CTA
-    const uint32_t local = c0 + (kSwiglu ? tile % 2 : tile) * 16 + g;
-    const uint32_t limit = kSwiglu ? p.half : p.rows, first = kSwiglu && tile >= 2 ? p.half : 0;
-    const uint8_t *scales = first ? p.us : p.ws;
-    const uint8_t *w[2], *sw[2];
+    const bool swiglu = p.epilogue == OPURE_EPI_SWIGLU;
+    // This warp's rows. In SwiGLU the first 32 / kRows units are gate rows, the others up rows,
+    // whose scale tiles are counted from the first up row.
+    constexpr uint32_t kGate = 32 / kRows;
+    const bool up = swiglu && unit >= kGate;
+    const uint32_t c0 = blockIdx.x * (swiglu ? 32 : p.units * kRows);  // first result column of the CTA
+    const uint32_t local = c0 + (up ? unit - kGate : unit) * kRows + g;
+    const uint32_t limit = swiglu ? p.half : p.rows, first = up ? p.half : 0;
+    const size_t row_bytes = mx_row_bytes(OPURE_MX_FP4, p.cols);
+    const uint8_t *w[2 * MT], *ws[2 * MT];
 #pragma unroll
-    for (uint32_t j = 0; j < 2; ++j) {
+    for (uint32_t j = 0; j < 2 * MT; ++j) {
         const uint32_t r = min(local + 8 * j, limit - 1);  // rows past the end repeat the last one
-        w[j] = p.w + size_t(first + r) * mx_row_bytes(OPURE_MX_FP4, p.cols) + t * 16;
-        sw[j] = scales + mx_scale_offset(p.cols, r, 0);
+        w[j] = p.w + (first + r) * row_bytes + t * 16;
+        ws[j] = (up ? p.us : p.ws) + mx_scale_offset(p.cols, r, 0) + t % 2 * 2;
     }
-    // Weights may be asked for before the kernel that this one waits for has ended: into L2 only,
-    // where a late write of theirs would show.
-    if (t == 0)
+    // The weights may be asked for before the kernel that this one waits for has ended, into L2
+    // only, where a late write of its would show.
+    if (t == 0 && split < pieces)
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i)
-            if (split + i * p.splits < pieces)
-#pragma unroll
-                for (uint32_t j = 0; j < 2; ++j)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(w[j] + size_t(split + i * p.splits) * 64));
+        for (uint32_t j = 0; j < 2 * MT; ++j) asm volatile("prefetch.global.L2 [%0];" ::"l"(w[j] + size_t(split) * 64));
     grid_dependency_wait();
     grid_dependents_launch();
 
-    const uint8_t *x = p.x + size_t(min(g, p.n - 1)) * mx_row_bytes(XF, p.cols) + t * XF;
-    const uint8_t *sx[2];
+    // Column g of the MMA is block g % 4 of token g / 4 of the pair: the lanes t = g % 4 hold it.
+    // D's columns 2 t and 2 t + 1 are blocks 2 t % 4 and the next of token t / 2.
+    const uint8_t *x = p.x + t * (4 * XF), *xs = p.xs + t % 2 * 2;
+    const size_t x_bytes = mx_row_bytes(XF, p.cols);
+    auto load_weights = [&](Weights<MT> &in, uint32_t k) {
 #pragma unroll
-    for (uint32_t j = 0; j < 2; ++j) sx[j] = p.xs + mx_scale_offset(p.cols, min(2 * t + j, p.n - 1), 0);
-    float acc[4] = {};
-    for (uint32_t k0 = split; k0 < pieces; k0 += kAhead * p.splits) {
-        Piece<XF> in[kAhead];
+        for (uint32_t j = 0; j < 2 * MT; ++j) {
+            in.w[j] = ldg_stream(w[j] + size_t(k) * 64);
+            in.s[j] = *reinterpret_cast<const uint16_t *>(ws[j] + size_t(k) * kMxTileBytes);
+        }
+    };
+    auto load_tokens = [&](Tokens<XF> &in, uint32_t pair, uint32_t k) {
+        const uint32_t token = pair * 2 + g / 4, of = min(pair * 2 + t / 2, p.n - 1);
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t k = min(k0 + i * p.splits, pieces - 1);
+        for (uint32_t j = 0; j < XF / 4; ++j) {
+            in.x[j] = make_uint4(0, 0, 0, 0);
+            if (t == g % 4 && token < p.n)
+                in.x[j] = *reinterpret_cast<const uint4 *>(x + token * x_bytes + size_t(k) * (16 * XF) + j * 16);
+        }
+        in.s = *reinterpret_cast<const uint16_t *>(xs + mx_scale_offset(p.cols, of, 0) + size_t(k) * kMxTileBytes);
+    };
+    float acc[NP][2 * MT] = {};
+    auto compute = [&](const Weights<MT> &wt, const Tokens<XF> &tk, float (&sum)[2 * MT]) {
+        // The tokens' 32 values per lane as fp16 pairs, in the order of the weights' codes.
+        uint32_t b[16];
+        const uint32_t *c = reinterpret_cast<const uint32_t *>(tk.x);
 #pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                in[i].w[j] = ldg_stream(w[j] + size_t(k) * 64);
-                in[i].sw[j] = *reinterpret_cast<const uint32_t *>(sw[j] + size_t(k) * kMxTileBytes);
-                in[i].sx[j] = *reinterpret_cast<const uint32_t *>(sx[j] + size_t(k) * kMxTileBytes);
+        for (uint32_t q = 0; q < 4; ++q) {
+            uint32_t h[4];
+            if constexpr (XF == OPURE_MX_FP4) {
+                mx_unpack_fp4(c[q], h);
+            } else {
+                mx_unpack_fp8(c[2 * q], h[0], h[1]);
+                mx_unpack_fp8(c[2 * q + 1], h[2], h[3]);
             }
 #pragma unroll
-            for (uint32_t b = 0; b < 4; ++b) {
-                const uint32_t *s = reinterpret_cast<const uint32_t *>(x + size_t(k) * (16 * XF) + b * (4 * XF));
+            for (uint32_t j = 0; j < 4; ++j) b[4 * q + j] = h[j];
+        }
+        float x0, x1;
+        scale_pair(tk.s, x0, x1);
 #pragma unroll
-                for (uint32_t j = 0; j < XF / 4; ++j) in[i].x[b][j] = s[j];
+        for (uint32_t m = 0; m < MT; ++m) {
+            float d[4] = {};
+            const uint32_t lo[4] = {wt.w[2 * m].x, wt.w[2 * m].y, wt.w[2 * m].z, wt.w[2 * m].w};
+            const uint32_t hi[4] = {wt.w[2 * m + 1].x, wt.w[2 * m + 1].y, wt.w[2 * m + 1].z, wt.w[2 * m + 1].w};
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                uint32_t a0[4], a1[4];
+                mx_unpack_fp4(lo[q], a0);
+                mx_unpack_fp4(hi[q], a1);
+                mma_f16(d, a0[0], a1[0], a0[1], a1[1], b[4 * q], b[4 * q + 1]);
+                mma_f16(d, a0[2], a1[2], a0[3], a1[3], b[4 * q + 2], b[4 * q + 3]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                float s0, s1;
+                scale_pair(wt.s[2 * m + j], s0, s1);
+                sum[2 * m + j] = fmaf(d[2 * j] * x0, s0, fmaf(d[2 * j + 1] * x1, s1, sum[2 * m + j]));
             }
         }
+    };
+    Weights<MT> in[kAhead];
+    Tokens<XF> tk[kAhead];  // one pair: in flight beside the weights
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (split + i * p.splits < pieces) {
+            load_weights(in[i], split + i * p.splits);
+            if (NP == 1) load_tokens(tk[i], 0, split + i * p.splits);
+        }
+    for (uint32_t k0 = split; k0 < pieces; k0 += kAhead * p.splits) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
-            if (k0 + i * p.splits >= pieces) break;
-            uint32_t lo[4] = {in[i].w[0].x, in[i].w[0].y, in[i].w[0].z, in[i].w[0].w};
-            uint32_t hi[4] = {in[i].w[1].x, in[i].w[1].y, in[i].w[1].z, in[i].w[1].w};
-            transpose4(lo);
-            transpose4(hi);
-            float fw[2][4], fx[2][4];
+            const uint32_t k = k0 + i * p.splits, next = k + kAhead * p.splits;
+            if (k >= pieces) break;
 #pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                scale_pair(in[i].sw[j], fw[j][0], fw[j][1]);
-                scale_pair(in[i].sw[j] >> 16, fw[j][2], fw[j][3]);
-                scale_pair(in[i].sx[j], fx[j][0], fx[j][1]);
-                scale_pair(in[i].sx[j] >> 16, fx[j][2], fx[j][3]);
+            for (uint32_t pair = 0; pair < NP; ++pair) {
+                if (NP > 1) load_tokens(tk[i], pair, k);
+                compute(in[i], tk[i], acc[pair]);
             }
-#pragma unroll
-            for (uint32_t b = 0; b < 4; ++b) {
-                uint32_t a0[4], a1[4], bx[4];
-                mx_unpack_fp4(lo[b], a0);
-                mx_unpack_fp4(hi[b], a1);
-                if constexpr (XF == OPURE_MX_FP4) {
-                    mx_unpack_fp4(in[i].x[b][0], bx);
-                } else {
-                    mx_unpack_fp8(in[i].x[b][0], bx[0], bx[1]);
-                    mx_unpack_fp8(in[i].x[b][1], bx[2], bx[3]);
-                }
-                float d[4] = {};
-                mma_f16(d, a0[0], a1[0], a0[1], a1[1], bx[0], bx[1]);
-                mma_f16(d, a0[2], a1[2], a0[3], a1[3], bx[2], bx[3]);
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) acc[j] = fmaf(d[j] * fx[j & 1][b], fw[j >> 1][b], acc[j]);
+            if (next < pieces) {
+                load_weights(in[i], next);
+                if (NP == 1) load_tokens(tk[i], 0, next);
             }
         }
     }
+    // Lanes t and t ^ 1 hold two blocks each of one token.
 #pragma unroll
-    for (uint32_t j = 0; j < 2; ++j)
-        *reinterpret_cast<float2 *>(&part[warp][g + 8 * j][2 * t]) = make_float2(acc[2 * j], acc[2 * j + 1]);
+    for (uint32_t pair = 0; pair < NP; ++pair)
+#pragma unroll
+        for (uint32_t j = 0; j < 2 * MT; ++j) {
+            const float v = acc[pair][j] + __shfl_xor_sync(0xffffffffu, acc[pair][j], 1);
+            if (t % 2 == 0) part[warp][g + 8 * j][pair * 2 + t / 2] = v;
+        }
     __syncthreads();
 
     // Results: a thread takes 4 neighbouring columns of a token.
     auto sum = [&](uint32_t column, uint32_t token) {
         float v = 0.f;
-        for (uint32_t q = 0; q < p.splits; ++q) v += part[column / 16 * p.splits + q][column % 16][token];
+        for (uint32_t q = 0; q < p.splits; ++q) v += part[column / kRows * p.splits + q][column % kRows][token];
         return v;
     };
-    const uint32_t quads = kSwiglu ? 8 : p.tiles * 4;
+    const uint32_t quads = (swiglu ? 32 : p.units * kRows) / 4;
     const uint32_t all = (quads * p.n + 31) / 32 * 32;  // whole warps
     for (uint32_t u = threadIdx.x; u < all; u += blockDim.x) {
+        const bool real = u / quads < p.n;
         const uint32_t token = min(u / quads, p.n - 1), c = u % quads * 4, col = c0 + c;
         float v[4];
-        if constexpr (kSwiglu) {
-            constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) v[j] = col + j < p.half ? silu(sum(c + j, token)) * sum(32 + c + j, token) : 0.f;
-            store_block<kF>(v, p.out + token * mx_row_bytes(kF, p.half) + size_t(c0) * kF / 8,
-                            p.outs + mx_scale_offset(p.half, token, c0 / 32), u / quads < p.n);
-        } else if (u / quads < p.n) {
+        for (uint32_t j = 0; j < 4; ++j) v[j] = sum(c + j, token);
+        if (swiglu) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) v[j] = sum(c + j, token);
+            for (uint32_t j = 0; j < 4; ++j) v[j] = col + j < p.half ? silu(v[j]) * sum(32 + c + j, token) : 0.f;
+            uint8_t *scale = p.outs + mx_scale_offset(p.half, token, c0 / 32);
+            if (p.out_format == OPURE_MX_FP4)
+                store_block<OPURE_MX_FP4>(v, p.out + token * mx_row_bytes(OPURE_MX_FP4, p.half) + size_t(c0) / 2, scale, real);
+            else
+                store_block<OPURE_MX_FP8>(v, p.out + token * mx_row_bytes(OPURE_MX_FP8, p.half) + c0, scale, real);
+        } else if (real) {
             const size_t at = token * p.y_stride + col;
-            store_quad<EPI>(v, static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at,
-                            col < p.rows ? min(p.rows - col, 4u) : 0u, p.vec);
+            const uint32_t m = col < p.rows ? min(p.rows - col, 4u) : 0u;
+            auto store = [&](auto type) {
+                using T = decltype(type);
+                if (p.epilogue == OPURE_EPI_ADD)
+                    store_quad<OPURE_EPI_ADD>(v, static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at, m, p.vec);
+                else
+                    store_quad<OPURE_EPI_STORE>(v, static_cast<T *>(p.y) + at, static_cast<const T *>(nullptr), m, p.vec);
+            };
+            if (p.y_type == OPURE_F32)
+                store(float());
+            else if (p.y_type == OPURE_F16)
+                store(__half());
+            else
+                store(__nv_bfloat16());
         }
     }
 }
@@ -227,34 +255,33 @@ opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t 
     p.rows = a->w.rows;
     p.cols = a->w.cols;
     p.half = a->w.rows / 2;
+    p.epilogue = a->epilogue;
+    p.y_type = a->y_type;
+    p.out_format = a->out.format;
     p.y = a->y;
     p.y_stride = a->y_stride;
     p.residual = a->residual;
     p.out = a->out.codes;
     p.outs = a->out.scales;
     p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
-    // About 16 warps per SM, each with 128 columns at least; CTAs of at least 4 warps.
-    const uint32_t pieces = mx_kp(p.cols) / 128;
+    const uint32_t pieces = mx_kp(p.cols) / 128, sms = uint32_t(ctx->sm_count);
     const uint32_t row_tiles = swiglu ? mx_kp(p.half) / 32 * 4 : ceil_div(p.rows, 16);
+    // Two tiles per warp halve the work on the tokens' side where rows alone give every SM 8 warps;
+    // with fewer rows one, and K splits up to about 16 warps per SM.
+    const bool two = row_tiles >= sms * 16;
+    const uint32_t units_all = two ? (row_tiles + 1) / 2 : row_tiles, cta_units = swiglu ? (two ? 2 : 4) : 1;
     p.splits = 1;
-    while (row_tiles * p.splits < uint32_t(ctx->sm_count) * 16 && p.splits * 2 <= pieces && p.splits * (swiglu ? 4 : 1) < kMaxWarps)
-        p.splits *= 2;
-    p.tiles = swiglu ? 4 : std::max(1u, 4 / p.splits);
-    const dim3 grid(swiglu ? mx_kp(p.half) / 32 : ceil_div(row_tiles, p.tiles)), block(32 * p.tiles * p.splits);
-    auto go = [&](auto t, auto epi) {
-        using T = decltype(t);
-        constexpr int kEpi = decltype(epi)::value;
-        return fp8 ? launch(ctx, mx_gemv_kernel<OPURE_MX_FP8, kEpi, T>, grid, block, 0, true, p)
-                   : launch(ctx, mx_gemv_kernel<OPURE_MX_FP4, kEpi, T>, grid, block, 0, true, p);
+    while (!two && units_all * p.splits < sms * 16 && p.splits * 2 <= pieces && p.splits * 2 * cta_units <= kMaxWarps) p.splits *= 2;
+    p.units = swiglu ? cta_units : std::max(1u, 4 / p.splits);
+    const dim3 grid(swiglu ? mx_kp(p.half) / 32 : ceil_div(units_all, p.units)), block(32 * p.units * p.splits);
+    auto go = [&](auto kernel) { return launch(ctx, kernel, grid, block, 0, true, p); };
+    auto pick = [&](auto pairs) {
+        constexpr uint32_t NP = decltype(pairs)::value;
+        if (fp8) return two ? go(mx_gemv_kernel<OPURE_MX_FP8, 2, NP>) : go(mx_gemv_kernel<OPURE_MX_FP8, 1, NP>);
+        return two ? go(mx_gemv_kernel<OPURE_MX_FP4, 2, NP>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, NP>);
     };
-    if (swiglu) {
-        const std::integral_constant<int, OPURE_EPI_SWIGLU> epi;
-        return a->out.format == OPURE_MX_FP4 ? go(uint32_t(), epi) : go(uint8_t(), epi);
-    }
-    return with_type(a->y_type, [&](auto t) {
-        return a->epilogue == OPURE_EPI_ADD ? go(t, std::integral_constant<int, OPURE_EPI_ADD>())
-                                            : go(t, std::integral_constant<int, OPURE_EPI_STORE>());
-    });
+    if (p.n <= 2) return pick(std::integral_constant<uint32_t, 1>());
+    return p.n <= 4 ? pick(std::integral_constant<uint32_t, 2>()) : pick(std::integral_constant<uint32_t, 4>());
 }
 
 }  // namespace opure
