@@ -1,9 +1,7 @@
 // mx.cu -- to and from microscaled (MX) form: quantise, dequantise, and RMSNorm with the
 // residual's addition and an MX result.
 //
-// All three are bound by memory: a value is read once and its code written once. A lane owns
-// 8 neighbouring values (one 16-byte load of 16-bit values, two of fp32), 4 lanes a block of
-// 32, 16 lanes the four blocks whose scales make one 4-byte word of a scale tile.
+// All three are bound by memory: a value is read once and its code written once.
 #include <algorithm>
 #include <type_traits>
 
@@ -13,99 +11,130 @@ namespace opure {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kUnitCols = 256;  // columns that a warp takes at once
-constexpr uint32_t kUnits = 4;       // how many times: loads of all are in flight together
 
-// A warp's units: pieces of 256 columns, row after row.
-struct Units {
-    uint32_t row, piece, per_row;
-    __device__ __forceinline__ Units(uint32_t cols) {
-        per_row = (mx_kp(cols) + kUnitCols - 1) / kUnitCols;
-        const uint32_t unit = (blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kUnits;
-        row = unit / per_row;
-        piece = unit - row * per_row;
-    }
-    // This lane's first column in the current unit, then on to the next one.
-    __device__ __forceinline__ uint32_t column() const { return piece * kUnitCols + (threadIdx.x & 31u) * 8; }
-    __device__ __forceinline__ void next() {
-        if (++piece == per_row) {
-            piece = 0;
-            ++row;
-        }
+// To and from MX, a lane owns 16 neighbouring values, 8 lanes the 128 columns whose four scales
+// make one word of a scale tile: a group. Groups are counted row after row, so that no lane idles
+// at a row's end. At 8 values a lane the same kernels were bound by instructions (half of them
+// for the scale and the addresses): 65 us for 49152 x 2048 fp16, against 40 us for the bytes.
+struct Groups {
+    uint32_t rows, per_row, magic;  // magic: per_row's reciprocal
+    __device__ __forceinline__ bool at(uint32_t group, uint32_t &row, uint32_t &c) const {
+        // floor(group / per_row) or one more (group < 2^31, magic rounded up), then corrected.
+        row = per_row == 1 ? group : __umulhi(group, magic);
+        if (row * per_row > group) --row;
+        c = (group - row * per_row) * 128 + (threadIdx.x & 7u) * 16;
+        return row < rows;
     }
 };
 
-template <typename T, uint32_t FMT, bool VEC>
+template <typename T, uint32_t FMT, bool VEC, uint32_t U>
 __global__ void __launch_bounds__(kThreads)
-    mx_quantize_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, uint32_t rows, uint32_t cols) {
+    mx_quantize_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {
     grid_dependency_wait();
     grid_dependents_launch();
-    const uint32_t kp = mx_kp(cols);
-    float v[kUnits][8];
-    Units u(cols), w = u;
+    const uint32_t first = (blockIdx.x * U * kThreads + threadIdx.x) / 8;
+    uint32_t raw[U][4 * sizeof(T)];
+    uint32_t row[U], c[U];
+    bool in[U];
 #pragma unroll
-    for (uint32_t i = 0; i < kUnits; ++i, u.next()) {
-        const uint32_t c = u.column(), n = u.row < rows && c < cols ? min(cols - c, 8u) : 0u;
-        const T *p = x + size_t(u.row) * stride + c;
-        if (VEC && n == 8)
-            load8(p, v[i]);
-        else
-            load8_part(p, n, v[i]);
+    for (uint32_t i = 0; i < U; ++i) {
+        in[i] = groups.at(first + i * (kThreads / 8), row[i], c[i]);
+        const T *p = x + size_t(row[i]) * stride + c[i];
+        if (VEC && in[i] && c[i] + 16 <= cols) {
+            load16(p, raw[i]);
+        } else {
+            T *r = reinterpret_cast<T *>(raw[i]);
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) r[j] = in[i] && c[i] + j < cols ? p[j] : from_f32<T>(0.f);
+        }
     }
 #pragma unroll
-    for (uint32_t i = 0; i < kUnits; ++i, w.next()) {
-        const uint32_t c = w.column();
-        const bool in = w.row < rows && c < kp;
-        const uint32_t byte = mx_store_octet<FMT>(v[i], codes + size_t(w.row) * mx_row_bytes(FMT, cols), c / 8, in);
-        const uint32_t word = mx_scale_word(byte);
-        if (in && threadIdx.x % 16 == 0)
-            *reinterpret_cast<uint32_t *>(scales + mx_scale_offset(cols, w.row, c / kMxBlock)) = word;
+    for (uint32_t i = 0; i < U; ++i) {
+        float v[16];
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) v[j] = to_f32(reinterpret_cast<const T *>(raw[i])[j]);
+        float f = max_abs3(v[0], v[1], 0.f);
+#pragma unroll
+        for (uint32_t j = 2; j < 16; j += 2) f = max_abs3(f, v[j], v[j + 1]);
+        uint32_t m = __float_as_uint(f) & 0x7fffffffu;
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const uint32_t byte = mx_scale_byte<FMT>(m), keep = byte == 255u ? 0u : ~0u;
+        const float inv = mx_inverse(byte);
+        uint32_t s = byte << (4u * (threadIdx.x & 6u));
+        s |= __shfl_xor_sync(0xffffffffu, s, 2);
+        s |= __shfl_xor_sync(0xffffffffu, s, 4);
+        if (!in[i]) continue;
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) v[j] *= inv;
+        uint8_t *dst = codes + size_t(row[i]) * mx_row_bytes(FMT, cols) + size_t(c[i]) * FMT / 8;
+        if constexpr (FMT == OPURE_MX_FP4) {
+            const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+            const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(mx_pack_fp4(lo) & keep, mx_pack_fp4(hi) & keep);
+        } else {
+            *reinterpret_cast<uint4 *>(dst) =
+                make_uint4(mx_pack_fp8(v[0], v[1], v[2], v[3]) & keep, mx_pack_fp8(v[4], v[5], v[6], v[7]) & keep,
+                           mx_pack_fp8(v[8], v[9], v[10], v[11]) & keep, mx_pack_fp8(v[12], v[13], v[14], v[15]) & keep);
+        }
+        if (threadIdx.x % 8 == 0) *reinterpret_cast<uint32_t *>(scales + mx_scale_offset(cols, row[i], c[i] / kMxBlock)) = s;
     }
 }
 
-template <typename T, uint32_t FMT, bool VEC>
+template <typename T, uint32_t FMT, bool VEC, uint32_t U>
 __global__ void __launch_bounds__(kThreads)
-    mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, uint32_t rows, uint32_t cols) {
-    using Word = std::conditional_t<FMT == OPURE_MX_FP4, uint32_t, uint2>;  // 8 codes
+    mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, Groups groups, uint32_t cols) {
     grid_dependency_wait();
     grid_dependents_launch();
-    Word code[kUnits];
-    uint8_t scale[kUnits];
-    Units u(cols), w = u;
+    const uint32_t first = (blockIdx.x * U * kThreads + threadIdx.x) / 8;
+    using Word = std::conditional_t<FMT == OPURE_MX_FP4, uint2, uint4>;  // 16 codes
+    Word code[U];
+    uint8_t scale[U];
+    uint32_t row[U], c[U];
+    bool in[U];
 #pragma unroll
-    for (uint32_t i = 0; i < kUnits; ++i, u.next()) {
-        const uint32_t c = u.column();
-        code[i] = Word{};
-        scale[i] = 0;
-        if (u.row < rows && c < cols) {
-            code[i] = reinterpret_cast<const Word *>(codes + size_t(u.row) * mx_row_bytes(FMT, cols))[c / 8];
-            scale[i] = scales[mx_scale_offset(cols, u.row, c / kMxBlock)];
+    for (uint32_t i = 0; i < U; ++i) {
+        in[i] = groups.at(first + i * (kThreads / 8), row[i], c[i]) && c[i] < cols;
+        if (in[i]) {
+            code[i] = *reinterpret_cast<const Word *>(codes + size_t(row[i]) * mx_row_bytes(FMT, cols) + size_t(c[i]) * FMT / 8);
+            scale[i] = scales[mx_scale_offset(cols, row[i], c[i] / kMxBlock)];
         }
     }
 #pragma unroll
-    for (uint32_t i = 0; i < kUnits; ++i, w.next()) {
-        const uint32_t c = w.column();
-        if (w.row >= rows || c >= cols) continue;
+    for (uint32_t i = 0; i < U; ++i) {
+        if (!in[i]) continue;
         const float s = mx_scale_value(scale[i]);
-        uint32_t h[4];
-        if constexpr (FMT == OPURE_MX_FP4) {
-            mx_unpack_fp4(code[i], h);
-        } else {
-            mx_unpack_fp8(code[i].x, h[0], h[1]);
-            mx_unpack_fp8(code[i].y, h[2], h[3]);
-        }
-        float v[8];
+        uint32_t h[8];
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&code[i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = h2f2(h[j]);
-            v[2 * j] = f.x * s;
-            v[2 * j + 1] = f.y * s;
+        for (uint32_t q = 0; q < 2; ++q) {
+            uint32_t f[4];
+            if constexpr (FMT == OPURE_MX_FP4) {
+                mx_unpack_fp4(w[q], f);
+            } else {
+                mx_unpack_fp8(w[2 * q], f[0], f[1]);
+                mx_unpack_fp8(w[2 * q + 1], f[2], f[3]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) h[4 * q + j] = f[j];
         }
-        T *p = y + size_t(w.row) * stride + c;
-        if (VEC && cols - c >= 8)
-            store8(p, v);
-        else
-            store8_part(p, min(cols - c, 8u), v);
+        uint32_t raw[4 * sizeof(T)];
+        T *r = reinterpret_cast<T *>(raw);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const float2 f = h2f2(h[j]);
+            r[2 * j] = from_f32<T>(f.x * s);
+            r[2 * j + 1] = from_f32<T>(f.y * s);
+        }
+        T *p = y + size_t(row[i]) * stride + c[i];
+        if (VEC && c[i] + 16 <= cols) {
+#pragma unroll
+            for (uint32_t j = 0; j < sizeof(T) / 2; ++j)
+                stg256(reinterpret_cast<uint8_t *>(p) + 32 * j, *reinterpret_cast<const uint32_t(*)[8]>(raw + 8 * j));
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j)
+                if (c[i] + j < cols) p[j] = r[j];
+        }
     }
 }
 
@@ -211,11 +240,20 @@ __global__ void __launch_bounds__(1024) mx_rmsnorm_kernel(NormParams p) {
     }
 }
 
-// Blocks of kThreads that cover a matrix; 0 when there would be too many units to count.
-uint32_t unit_blocks(const opure_mx_matrix &m) {
-    const uint64_t units = uint64_t(m.rows) * ceil_div(mx_kp(m.cols), kUnitCols);
-    const uint64_t per_block = kThreads / 32 * kUnits;
-    return units < 0xffffffffu - per_block ? uint32_t((units + per_block - 1) / per_block) : 0u;
+// The groups of a matrix, and how many each lane takes: two where that still fills every SM, so
+// that more loads are in flight; one in smaller calls, where latency counts.
+bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
+    g.rows = m.rows;
+    g.per_row = mx_kp(m.cols) / 128;
+    g.magic = g.per_row == 1 ? 0 : uint32_t(0xffffffffu / g.per_row + 1);
+    const uint64_t groups = uint64_t(m.rows) * g.per_row;
+    if (groups >= (uint64_t(1) << 31) - kThreads) return false;
+    per_lane = groups >= uint64_t(ctx->sm_count) * 8 * kThreads / 8 ? 2 : 1;
+    blocks = ceil_div(groups * 8, kThreads * per_lane);
+    return true;
+}
+bool rows_aligned32(const void *p, uint32_t type, size_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % 32 == 0 && stride * type_bytes(type) % 32 == 0;
 }
 
 }  // namespace
@@ -241,18 +279,23 @@ opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, s
     if (!out || !mx_valid(*out) || !type_aligned(x, x_type) || x_stride < out->cols) return OPURE_ERR_INVALID_ARG;
     if (out->rows == 0) return OPURE_OK;
     if (!x) return OPURE_ERR_INVALID_ARG;
-    const uint32_t blocks = unit_blocks(*out);
-    if (!blocks) return OPURE_ERR_UNSUPPORTED;
-    const bool vec = rows_aligned16(x, x_type, x_stride);
+    Groups groups;
+    uint32_t per_lane, blocks;
+    if (!make_groups(ctx, *out, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
+    const bool vec = rows_aligned32(x, x_type, x_stride);
     return with_type(x_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
             return launch(ctx, kernel, dim3(blocks), dim3(kThreads), 0, true, static_cast<const T *>(x), x_stride,
-                          out->codes, out->scales, out->rows, out->cols);
+                          out->codes, out->scales, groups, out->cols);
         };
-        if (out->format == OPURE_MX_FP4)
-            return vec ? go(mx_quantize_kernel<T, OPURE_MX_FP4, true>) : go(mx_quantize_kernel<T, OPURE_MX_FP4, false>);
-        return vec ? go(mx_quantize_kernel<T, OPURE_MX_FP8, true>) : go(mx_quantize_kernel<T, OPURE_MX_FP8, false>);
+        auto pick = [&](auto format) {
+            constexpr uint32_t F = decltype(format)::value;
+            if (per_lane == 1) return vec ? go(mx_quantize_kernel<T, F, true, 1>) : go(mx_quantize_kernel<T, F, false, 1>);
+            return vec ? go(mx_quantize_kernel<T, F, true, 2>) : go(mx_quantize_kernel<T, F, false, 2>);
+        };
+        return out->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
+                                           : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
     });
 }
 
@@ -262,18 +305,23 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
     if (!x || !mx_valid(*x) || !type_aligned(y, y_type) || y_stride < x->cols) return OPURE_ERR_INVALID_ARG;
     if (x->rows == 0) return OPURE_OK;
     if (!y) return OPURE_ERR_INVALID_ARG;
-    const uint32_t blocks = unit_blocks(*x);
-    if (!blocks) return OPURE_ERR_UNSUPPORTED;
-    const bool vec = rows_aligned16(y, y_type, y_stride);
+    Groups groups;
+    uint32_t per_lane, blocks;
+    if (!make_groups(ctx, *x, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
+    const bool vec = rows_aligned32(y, y_type, y_stride);
     return with_type(y_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
             return launch(ctx, kernel, dim3(blocks), dim3(kThreads), 0, true, static_cast<const uint8_t *>(x->codes),
-                          static_cast<const uint8_t *>(x->scales), static_cast<T *>(y), y_stride, x->rows, x->cols);
+                          static_cast<const uint8_t *>(x->scales), static_cast<T *>(y), y_stride, groups, x->cols);
         };
-        if (x->format == OPURE_MX_FP4)
-            return vec ? go(mx_dequantize_kernel<T, OPURE_MX_FP4, true>) : go(mx_dequantize_kernel<T, OPURE_MX_FP4, false>);
-        return vec ? go(mx_dequantize_kernel<T, OPURE_MX_FP8, true>) : go(mx_dequantize_kernel<T, OPURE_MX_FP8, false>);
+        auto pick = [&](auto format) {
+            constexpr uint32_t F = decltype(format)::value;
+            if (per_lane == 1) return vec ? go(mx_dequantize_kernel<T, F, true, 1>) : go(mx_dequantize_kernel<T, F, false, 1>);
+            return vec ? go(mx_dequantize_kernel<T, F, true, 2>) : go(mx_dequantize_kernel<T, F, false, 2>);
+        };
+        return x->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
+                                         : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
     });
 }
 

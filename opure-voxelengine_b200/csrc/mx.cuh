@@ -120,6 +120,23 @@ __device__ __forceinline__ void store8(T *p, const float (&f)[8]) {
         *reinterpret_cast<uint4 *>(p) = u;
     }
 }
+// 16 neighbouring values in 32-byte loads and stores (p 32-byte aligned).
+__device__ __forceinline__ void ldg256(const void *p, uint32_t (&r)[8]) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void stg256(void *p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, uint32_t (&raw)[4 * sizeof(T)]) {
+#pragma unroll
+    for (uint32_t j = 0; j < sizeof(T) / 2; ++j) ldg256(reinterpret_cast<const uint8_t *>(p) + 32 * j, *reinterpret_cast<uint32_t(*)[8]>(raw + 8 * j));
+}
 // The first `n` of 8 neighbouring values, zeros after them; any alignment.
 template <typename T>
 __device__ __forceinline__ void load8_part(const T *p, uint32_t n, float (&f)[8]) {
@@ -133,25 +150,31 @@ __device__ __forceinline__ void store8_part(T *p, uint32_t n, const float (&f)[8
         if (uint32_t(j) < n) p[j] = from_f32<T>(f[j]);
 }
 
+// The largest of three magnitudes; NaN if one is.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Quantises a block held as 8 values in each of 4 neighbouring lanes and stores this lane's
 // codes at `codes` (the row's base), columns 8 oct .. 8 oct + 7. Returns the scale byte. All
 // lanes of the warp call it; only those with `in` store.
 template <uint32_t FMT>
 __device__ __forceinline__ uint32_t mx_store_octet(float (&v)[8], uint8_t *codes, uint32_t oct, bool in) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+    const float f = max_abs3(max_abs3(v[0], v[1], v[2]), max_abs3(v[3], v[4], v[5]), max_abs3(v[6], v[7], 0.f));
+    uint32_t m = __float_as_uint(f) & 0x7fffffffu;
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t byte = mx_scale_byte<FMT>(m);
+    const uint32_t byte = mx_scale_byte<FMT>(m), keep = byte == 255u ? 0u : ~0u;
     const float inv = mx_inverse(byte);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
+    for (int j = 0; j < 8; ++j) v[j] *= inv;
     if constexpr (FMT == OPURE_MX_FP4) {
-        const uint32_t c = mx_pack_fp4(v);
+        const uint32_t c = mx_pack_fp4(v) & keep;
         if (in) reinterpret_cast<uint32_t *>(codes)[oct] = c;
     } else {
-        const uint2 c = make_uint2(mx_pack_fp8(v[0], v[1], v[2], v[3]), mx_pack_fp8(v[4], v[5], v[6], v[7]));
+        const uint2 c = make_uint2(mx_pack_fp8(v[0], v[1], v[2], v[3]) & keep, mx_pack_fp8(v[4], v[5], v[6], v[7]) & keep);
         if (in) reinterpret_cast<uint2 *>(codes)[oct] = c;
     }
     return byte;

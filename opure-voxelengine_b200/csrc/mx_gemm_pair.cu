@@ -63,13 +63,6 @@ struct PairParams {
     DeviceStatus *st;
 };
 
-// The largest of three magnitudes; NaN if one is.
-__device__ __forceinline__ float max_abs3(float a, float b, float c) {
-    float r;
-    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 // 32 values of a thread -> 32 codes in global memory (dst 16-byte aligned); returns the scale byte.
 template <uint32_t FMT>
 __device__ __forceinline__ uint32_t quantize_block(float (&v)[32], uint8_t *dst, bool in) {
