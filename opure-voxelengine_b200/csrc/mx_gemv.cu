@@ -1,4 +1,4 @@
-// mx_gemv.cu -- the product of microscaled matrices for at most 8 tokens: decode's weight
+// mx_gemv.cu -- the product of microscaled matrices for at most 4 tokens: decode's weight
 // streaming.
 //
 // Bound by memory: a weight is 0.53 bytes and used once per token. At the measured 6.45 TB/s an SM
@@ -26,7 +26,7 @@
 namespace opure {
 namespace {
 
-constexpr uint32_t kMaxTokens = 8;
+constexpr uint32_t kMaxTokens = 4;
 constexpr uint32_t kMaxWarps = 16;
 
 struct GemvParams {
@@ -239,6 +239,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
     }
 }
 
+// Units and splits per CTA: the least estimated time. 16 warps of this kernel's registers fit an
+// SM. A wave of CTAs costs its fixed part (about 500 cycles) and a memory latency (700) for every
+// round of pieces in flight; an SM takes about 120 cycles for a piece of two tiles and 75 for one.
+void choose(GemvParams &p, uint32_t pieces, uint32_t units_all, uint32_t cta_units, bool two, uint32_t sms) {
+    uint64_t best = ~uint64_t(0);
+    for (uint32_t u = cta_units ? cta_units : 1; u <= (cta_units ? cta_units : kMaxWarps); ++u)
+        for (uint32_t s = 1; u * s <= kMaxWarps && s <= pieces; ++s) {
+            if (u * s < 4 && s < pieces && !cta_units) continue;  // CTAs of 4 warps at least
+            const uint64_t ctas = ceil_div(units_all, u), resident = uint64_t(sms) * (kMaxWarps / (u * s));
+            const uint64_t waves = (ctas + resident - 1) / resident;
+            const uint64_t rounds = ceil_div(ceil_div(pieces, s), two ? 3 : 4);
+            const uint64_t cost = waves * (500 + 700 * rounds) + (ctas + sms - 1) / sms * u * pieces * (two ? 120 : 75);
+            if (cost < best) {
+                best = cost;
+                p.units = u;
+                p.splits = s;
+            }
+        }
+}
+
 }  // namespace
 
 bool mx_gemv_suits(const opure_mx_gemm_args *a) { return a->x.rows <= kMaxTokens; }
@@ -266,22 +286,15 @@ opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t 
     p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
     const uint32_t pieces = mx_kp(p.cols) / 128, sms = uint32_t(ctx->sm_count);
     const uint32_t row_tiles = swiglu ? mx_kp(p.half) / 32 * 4 : ceil_div(p.rows, 16);
-    // Two tiles per warp halve the work on the tokens' side where rows alone give every SM 8 warps;
-    // with fewer rows one, and K splits up to about 16 warps per SM.
-    const bool two = row_tiles >= sms * 16;
-    const uint32_t units_all = two ? (row_tiles + 1) / 2 : row_tiles, cta_units = swiglu ? (two ? 2 : 4) : 1;
-    p.splits = 1;
-    while (!two && units_all * p.splits < sms * 16 && p.splits * 2 <= pieces && p.splits * 2 * cta_units <= kMaxWarps) p.splits *= 2;
-    p.units = swiglu ? cta_units : std::max(1u, 4 / p.splits);
-    const dim3 grid(swiglu ? mx_kp(p.half) / 32 : ceil_div(units_all, p.units)), block(32 * p.units * p.splits);
+    // Two tiles per warp halve the work on the tokens' side; one where that would leave SMs empty.
+    const bool two = p.n <= 2 && (swiglu || row_tiles >= 2 * sms);
+    const uint32_t units_all = two ? (row_tiles + 1) / 2 : row_tiles;
+    choose(p, pieces, units_all, swiglu ? (two ? 2 : 4) : 0, two, sms);
+    const dim3 grid(ceil_div(units_all, p.units)), block(32 * p.units * p.splits);
     auto go = [&](auto kernel) { return launch(ctx, kernel, grid, block, 0, true, p); };
-    auto pick = [&](auto pairs) {
-        constexpr uint32_t NP = decltype(pairs)::value;
-        if (fp8) return two ? go(mx_gemv_kernel<OPURE_MX_FP8, 2, NP>) : go(mx_gemv_kernel<OPURE_MX_FP8, 1, NP>);
-        return two ? go(mx_gemv_kernel<OPURE_MX_FP4, 2, NP>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, NP>);
-    };
-    if (p.n <= 2) return pick(std::integral_constant<uint32_t, 1>());
-    return p.n <= 4 ? pick(std::integral_constant<uint32_t, 2>()) : pick(std::integral_constant<uint32_t, 4>());
+    if (p.n > 2) return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 1, 2>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, 2>);
+    if (two) return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 2, 1>) : go(mx_gemv_kernel<OPURE_MX_FP4, 2, 1>);
+    return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 1, 1>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, 1>);
 }
 
 }  // namespace opure
