@@ -120,21 +120,19 @@ __global__ void __launch_bounds__(kThreads, 2)
                 break;
             }
             const uint32_t kb = kb0 + i;
-            if (one && warp == 0) {
+            if (warp == 0) {
                 // A spreading copy counts the bytes that it reads, not the slots that it fills.
-                mbar_expect_tx(&full[s], kBBytes / 2 + kMxTileBytes * (kSwiglu ? 2 : 1));
-                tc::load_2d(b_tile(s), &wmap, kb * kK, r0, &full[s]);
-                if (kSwiglu) tc::load_2d(b_tile(s) + kBBytes / 2, &wmap, kb * kK, p.half + r0, &full[s]);
+                tc::expect_tx(one, &full[s], kBBytes / 2 + kMxTileBytes * (kSwiglu ? 2 : 1));
+                tc::load_2d(one, b_tile(s), &wmap, kb * kK, r0, &full[s]);
+                if (kSwiglu) tc::load_2d(one, b_tile(s) + kBBytes / 2, &wmap, kb * kK, p.half + r0, &full[s]);
                 const size_t tile = (size_t(r0 / 128) * p.kblocks + kb) * kMxTileBytes;
-                bulk_load(sf_tile(s) + 512, p.ws + tile, kMxTileBytes, &full[s]);
-                if (kSwiglu) bulk_load(sf_tile(s) + 1024, p.us + tile, kMxTileBytes, &full[s]);
+                tc::bulk(one, sf_tile(s) + 512, p.ws + tile, kMxTileBytes, &full[s]);
+                if (kSwiglu) tc::bulk(one, sf_tile(s) + 1024, p.us + tile, kMxTileBytes, &full[s]);
+            } else {
+                tc::expect_tx(one, &full[s], a_bytes * p.x_format / 8 + kMxTileBytes);
+                tc::load_2d(one, a_tile(s), &xmap, kb * kK, m0, &full[s]);
+                tc::bulk(one, sf_tile(s), p.xs + (size_t(m0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
             }
-            if (one && warp == 3) {
-                mbar_expect_tx(&full[s], a_bytes * p.x_format / 8 + kMxTileBytes);
-                tc::load_2d(a_tile(s), &xmap, kb * kK, m0, &full[s]);
-                bulk_load_keep(sf_tile(s), p.xs + (size_t(m0 / 128) * p.kblocks + kb) * kMxTileBytes, kMxTileBytes, &full[s]);
-            }
-            __syncwarp();
             if (++s == p.stages) {
                 s = 0;
                 phase ^= 1;
@@ -160,21 +158,18 @@ __global__ void __launch_bounds__(kThreads, 2)
             const uint32_t sf = tbase + kN + s * kScaleCols;
             const uint64_t ds = tc::desc_scales(smem_addr(sf_tile(s)));
             const uint64_t da = tc::desc_sw128(smem_addr(a_tile(s))), db = tc::desc_sw128(smem_addr(b_tile(s)));
-            if (one) {
-                tc::copy_scales(sf, ds);
-                tc::copy_scales(sf + 4, ds + (512 >> 4));
-                if (kSwiglu) tc::copy_scales(sf + 8, ds + (1024 >> 4));
+            tc::copy_scales(one, sf, ds);
+            tc::copy_scales(one, sf + 4, ds + (512 >> 4));
+            if (kSwiglu) tc::copy_scales(one, sf + 8, ds + (1024 >> 4));
 #pragma unroll
-                for (uint32_t k = 0; k < kK / 32; ++k) {
-                    const uint32_t id = idesc | tc::idesc_block(k), acc = (i | k) != 0;
-                    tc::mma_mxf8f6f4(tbase, da + 2 * k, db + 2 * k, id, sf, sf + 4 + shift, acc);
-                    if (kSwiglu)
-                        tc::mma_mxf8f6f4(tbase + kN / 2, da + 2 * k, db + 2 * k + (kBBytes / 2 >> 4), id, sf, sf + 8 + shift, acc);
-                }
-                tc::commit(&empty[s]);
-                if (i + 1 == nk) tc::commit(&done);
+            for (uint32_t k = 0; k < kK / 32; ++k) {
+                const uint32_t id = idesc | tc::idesc_block(k), acc = (i | k) != 0;
+                tc::mma_mxf8f6f4(one, tbase, da + 2 * k, db + 2 * k, id, sf, sf + 4 + shift, acc);
+                if (kSwiglu)
+                    tc::mma_mxf8f6f4(one, tbase + kN / 2, da + 2 * k, db + 2 * k + (kBBytes / 2 >> 4), id, sf, sf + 8 + shift, acc);
             }
-            __syncwarp();
+            tc::commit(one, &empty[s]);
+            if (i + 1 == nk) tc::commit(one, &done);
             if (++s == p.stages) {
                 s = 0;
                 phase ^= 1;

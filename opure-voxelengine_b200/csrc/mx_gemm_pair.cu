@@ -167,14 +167,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     break;
                 }
                 const uint32_t bar = full0 + s * 8, kb = i * S::kBlocks;
-                if (one) {
-                    if (rank == 0) mbar_expect_tx(&full[s], 2 * S::kTx);
-                    tc::load_2d_pair(a_tile(s), &xmap, i * 128, m0, bar);
-                    tc::load_2d_pair(b_tile(s), &wmap, i * 128, w_row, bar);
-                    tc::load_4d_pair(sf_tile(s), &xsmap, 0, kb, m0 / 128, 0, bar);
-                    tc::load_4d_pair(sf_tile(s) + S::kBlocks * kMxTileBytes, &wsmap, 0, kb, r0 / 128, 0, bar);
-                }
-                __syncwarp();
+                tc::expect_tx(one && rank == 0, &full[s], 2 * S::kTx);
+                tc::load_2d_pair(one, a_tile(s), &xmap, i * 128, m0, bar);
+                tc::load_2d_pair(one, b_tile(s), &wmap, i * 128, w_row, bar);
+                tc::load_4d_pair(one, sf_tile(s), &xsmap, 0, kb, m0 / 128, 0, bar);
+                tc::load_4d_pair(one, sf_tile(s) + S::kBlocks * kMxTileBytes, &wsmap, 0, kb, r0 / 128, 0, bar);
                 if (++s == kStages) {
                     s = 0;
                     phase ^= 1;
@@ -215,26 +212,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     s = 0;
                     phase ^= 1;
                 }
-                if (one) {
 #pragma unroll
-                    for (uint32_t b = 0; b < S::kBlocks; ++b) {
-                        tc::copy_scales_pair(sfa + b * 4, ds + b * kTile16);
-                        tc::copy_scales_pair(sfb + b * 8, ds + (S::kBlocks + b) * kTile16);
-                        tc::copy_scales_pair(sfb + b * 8 + 4, ds + (2 * S::kBlocks + b) * kTile16);
-                    }
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const uint32_t more = (i | k) != 0;
-                        if constexpr (XF == OPURE_MX_FP8)
-                            tc::mma_mxf8f6f4_pair(acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k), sfa, sfb, more);
-                        else if (i * 2 + k / 2 < p.kblocks)
-                            tc::mma_mxf4_pair(acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k % 2 * 2), sfa + k / 2 * 4,
-                                              sfb + k / 2 * 8, more);
-                    }
-                    tc::commit_pair(release);
-                    if (i + 1 == stages) tc::commit_pair(&acc_full[lt & 1u]);
+                for (uint32_t b = 0; b < S::kBlocks; ++b) {
+                    tc::copy_scales_pair(one, sfa + b * 4, ds + b * kTile16);
+                    tc::copy_scales_pair(one, sfb + b * 8, ds + (S::kBlocks + b) * kTile16);
+                    tc::copy_scales_pair(one, sfb + b * 8 + 4, ds + (2 * S::kBlocks + b) * kTile16);
                 }
-                __syncwarp();
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t more = (i | k) != 0;
+                    if constexpr (XF == OPURE_MX_FP8)
+                        tc::mma_mxf8f6f4_pair(one, acc, da + 2 * k, db + 2 * k, idesc | tc::idesc_block(k), sfa, sfb, more);
+                    else
+                        tc::mma_mxf4_pair(one && i * 2 + k / 2 < p.kblocks, acc, da + 2 * k, db + 2 * k,
+                                          idesc | tc::idesc_block(k % 2 * 2), sfa + k / 2 * 4, sfb + k / 2 * 8, more);
+                }
+                tc::commit_pair(one, release);
+                if (i + 1 == stages) tc::commit_pair(one, &acc_full[lt & 1u]);
             }
         }
     } else if (warp >= kEpiWarp) {

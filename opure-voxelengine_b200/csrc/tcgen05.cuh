@@ -9,11 +9,12 @@
 namespace opure {
 namespace tc {
 
-__device__ __forceinline__ void load_2d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint64_t *bar) {
+__device__ __forceinline__ void load_2d(bool one, void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint64_t *bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
+        "{\n .reg .pred e;\n setp.ne.b32 e, %5, 0;\n"
+        " @e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}" ::"r"(
+            smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar)), "r"(uint32_t(one))
         : "memory");
 }
 
@@ -29,10 +30,11 @@ __device__ __forceinline__ void alloc(uint32_t *dst, uint32_t ncols) {
 __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
-// One lane of a converged warp. The loops that issue loads and MMAs run on all lanes, and only
-// the instructions themselves on this one: addresses and descriptors then stay in uniform
-// registers, where the instructions want them (a loop inside "if (lane == 0)" moved each there
-// and took 1,000 cycles for 4 MMAs that execute in 512).
+// One lane of a converged warp. The loops that issue loads and MMAs run on all lanes, and the
+// instructions themselves are predicated on this one (`one`): addresses and descriptors then stay
+// in uniform registers, where the instructions want them, and the warp does not diverge. A loop
+// inside "if (lane == 0)" moved each operand there and took 1,000 cycles for 4 MMAs that execute
+// in 512; a branch around the instructions cost 150 cycles a stage to converge again.
 __device__ __forceinline__ bool elect() {
     uint32_t r;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
@@ -54,8 +56,10 @@ __device__ __forceinline__ uint64_t desc_scales(uint32_t addr) {
 
 // Copies a 512-byte scale tile (128 rows x 4 blocks) to 4 TMEM columns, into all four lane
 // quarters: column j holds rows 32 j .., one block per byte.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(bool one, uint32_t taddr, uint64_t desc) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n @e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(taddr),
+                 "l"(desc), "r"(uint32_t(one))
+                 : "memory");
 }
 
 // Element formats in the instruction descriptor: of kind::mxf8f6f4, and E2M1 of kind::mxf4.
@@ -67,19 +71,22 @@ constexpr __host__ __device__ uint32_t idesc_mx(uint32_t a_format, uint32_t b_fo
 __device__ __forceinline__ uint32_t idesc_block(uint32_t b) { return (b << 4) | (b << 29); }
 
 // D[tmem] (+)= (A scaled) (B scaled)^T over K = 32: one scale per row.
-__device__ __forceinline__ void mma_mxf8f6f4(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+__device__ __forceinline__ void mma_mxf8f6f4(bool one, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                              uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 e, %7, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(uint32_t(one))
         : "memory");
 }
 
 // Arrives on `bar` once every tcgen05 operation this thread issued before has completed.
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+__device__ __forceinline__ void commit(bool one, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_addr(bar)),
+        "r"(uint32_t(one))
+        : "memory");
 }
 
 // 32 neighbouring fp32 columns of this thread's TMEM lane (valid after wait_ld).
@@ -101,19 +108,21 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 // memory holds its 128 rows of A and its half of B's rows, at the same offsets in both.
 
 // A load into this CTA that completes on an mbarrier of either CTA of the pair (a cluster address).
-__device__ __forceinline__ void load_2d_pair(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar) {
+__device__ __forceinline__ void load_2d_pair(bool one, void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        "{\n .reg .pred e;\n setp.ne.b32 e, %5, 0;\n"
+        " @e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];\n}" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(uint32_t(one))
         : "memory");
 }
-__device__ __forceinline__ void load_4d_pair(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t w,
-                                             uint32_t bar) {
+__device__ __forceinline__ void load_4d_pair(bool one, void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z,
+                                             uint32_t w, uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        "{\n .reg .pred e;\n setp.ne.b32 e, %7, 0;\n"
+        " @e cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4, %5}], [%6];\n}" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "r"(uint32_t(one))
         : "memory");
 }
 __device__ __forceinline__ void alloc_pair(uint32_t *dst, uint32_t ncols) {
@@ -125,36 +134,56 @@ __device__ __forceinline__ void dealloc_pair(uint32_t taddr, uint32_t ncols) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 // Scale tile to TMEM in both CTAs, each from its own shared memory.
-__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales_pair(bool one, uint32_t taddr, uint64_t desc) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n @e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}" ::"r"(taddr),
+                 "l"(desc), "r"(uint32_t(one))
+                 : "memory");
 }
 // K = 32 of byte slots, one scale per row.
-__device__ __forceinline__ void mma_mxf8f6f4_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+__device__ __forceinline__ void mma_mxf8f6f4_pair(bool one, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                                   uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 e, %7, 0;\n"
+        " @e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(uint32_t(one))
         : "memory");
 }
 // K = 64 of packed E2M1 on both sides, two scales per row.
-__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+__device__ __forceinline__ void mma_mxf4_pair(bool one, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                               uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 e, %7, 0;\n"
+        " @e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(uint32_t(one))
         : "memory");
 }
 // Arrives on `bar` of both CTAs once every tcgen05 operation this thread issued before has completed.
-__device__ __forceinline__ void commit_pair(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                     smem_addr(bar)),
-                 "h"(uint16_t(3))
-                 : "memory");
+__device__ __forceinline__ void commit_pair(bool one, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n"
+        " @e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}" ::"r"(
+            smem_addr(bar)),
+        "h"(uint16_t(3)), "r"(uint32_t(one))
+        : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void expect_tx(bool one, uint64_t *bar, uint32_t bytes) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(
+            smem_addr(bar)),
+        "r"(bytes), "r"(uint32_t(one))
+        : "memory");
+}
+// bulk_load_keep (tma.cuh) by one lane.
+__device__ __forceinline__ void bulk(bool one, void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %4, 0;\n"
+        " @e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}" ::"r"(smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(bar)), "r"(uint32_t(one))
+        : "memory");
 }
 
 // ---- TMA stores ----------------------------------------------------------------------------
