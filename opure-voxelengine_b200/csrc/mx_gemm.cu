@@ -29,6 +29,7 @@ constexpr uint32_t kK = 128;       // columns per stage: one 128-byte swizzled r
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxStages = 10;
 constexpr uint32_t kMaxSplits = 8;  // portable cluster size
+constexpr uint32_t kPrefetch = 8;   // stages of weights that are asked for ahead
 constexpr uint32_t kBBytes = kN * kK;
 constexpr uint32_t kScaleBytes = 2048;  // per stage: x tile, w (or gate) tile, up tile; keeps 1 KB alignment
 constexpr uint32_t kScaleCols = 12;     // TMEM columns of a stage's scales
@@ -42,7 +43,7 @@ struct GemmParams {
     uint32_t n, rows, kblocks, splits, stages;
     uint32_t a_rows;              // token rows that a stage holds: multiple of 8, at most 128
     uint32_t half;                // SwiGLU: first up row = result columns
-    uint32_t sums_offset;         // of the received sums, past the ring
+    uint32_t sums_offset;         // of the received sums from the ring's start; 0: in its place
     bool vec;                     // rows of y and residual allow accesses of 4 values
     uint32_t x_format;
     void *y;
@@ -79,10 +80,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes; };
     auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
     // Results in units of 4 tokens x 32 columns. Unit u is finished by CTA u % splits, whose
-    // sums[u / splits][split][side] receive every split's part. Not in the ring: a CTA that is
-    // done with its split sends while this one still computes. A token's eight pieces of 16 bytes
-    // stand in an order of its own (piece ^ token % 8), so that 32 tokens' stores spread over all
-    // banks.
+    // sums[u / splits][split][side] receive every split's part: past the ring where there is room,
+    // else in its place, and the splits wait for one another before they send. A token's eight
+    // pieces of 16 bytes stand in an order of its own (piece ^ token % 8), so that 32 tokens'
+    // stores spread over all banks.
     uint8_t *sums = base + p.sums_offset;
     const uint32_t n = min(p.n - m0, kM), units = (n + 3) / 4 * kChunks;
     const uint32_t own_units = (units + p.splits - 1 - split) / p.splits;
@@ -105,7 +106,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = tmem_base;
-    tc::cluster_arrive();  // this CTA's recv is ready
+    // The weights may be asked for before the kernel that this one waits for has ended.
+    if (warp == 0) {
+        const bool one = tc::elect();
+        for (uint32_t i = 0; i < min(nk, kPrefetch); ++i) {
+            tc::prefetch_2d(one, &wmap, (kb0 + i) * kK, r0);
+            if (kSwiglu) tc::prefetch_2d(one, &wmap, (kb0 + i) * kK, p.half + r0);
+        }
+    }
+    if (p.splits > 1 && p.sums_offset) tc::cluster_arrive();  // this CTA can receive
     grid_dependency_wait();
     grid_dependents_launch();
 
@@ -189,7 +198,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     // Accumulators -> the CTAs that finish them. Warps w and w + 4 share TMEM lanes 32 (w % 4) ..
     // (tokens); each takes half of the columns.
-    tc::cluster_wait();
+    if (p.splits > 1) {
+        if (!p.sums_offset) tc::cluster_arrive();
+        tc::cluster_wait();
+    }
     const uint32_t quarter = warp & 3u, part = warp >> 2, token = quarter * 32 + lane;
     if (!failed && quarter * 32 < n) {
 #pragma unroll
@@ -332,21 +344,24 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.splits = std::max(1u, std::min({kMaxSplits, p.kblocks, uint32_t(ctx->sm_count) / std::max(1u, tiles * mtiles)}));
     p.a_rows = std::min(kM, (p.n + 7) & ~7u);
     const uint32_t stage_bytes = kBBytes + kScaleBytes + p.a_rows * kK;
-    // After the ring: the rest of the last stage's 128 rows of A, and the received sums (without a
-    // split they take the ring's place, which is done with by then); before it 1 KB to align it.
+    // Before the ring 1 KB to align it, after it the rest of the last stage's 128 rows of A and the
+    // received sums; these take the ring's place where they would leave it less than 4 stages (or
+    // all that it needs) or there are no splits.
     const uint32_t chunks = swiglu ? kN / 64 : kN / 32, units = ceil_div(std::min(p.n, kM), 4) * chunks;
     const size_t sums = size_t(ceil_div(units, p.splits)) * p.splits * (swiglu ? 2 : 1) * kUnit;
-    const size_t tail = size_t(kM - p.a_rows) * kK, fixed = 1024 + tail + (p.splits > 1 ? sums : 0);
+    const size_t rest = size_t(kM - p.a_rows) * kK;
+    // Two CTAs per SM (TMEM's 512 columns allow it and, above 75 KB each, no third), so that the
+    // next kernel's CTAs set up while this one's work: a chain of 8-token 8192 -> 2048 products
+    // took 5.8 us a call with half of the shared memory each, 9.7 us with all of it.
     auto stages_in = [&](size_t bytes) {
-        return std::min<uint32_t>({kMaxStages, uint32_t((bytes - fixed) / stage_bytes), ceil_div(p.kblocks, p.splits)});
+        return std::min<uint32_t>({kMaxStages, uint32_t((bytes - 1024 - rest) / stage_bytes), ceil_div(p.kblocks, p.splits)});
     };
-    // More CTAs than SMs go two to an SM (TMEM's 512 columns allow it and, above 75 KB each, no
-    // third) where that leaves each a ring of at least 4 stages, or all that it needs.
-    p.stages = stages_in(std::min<size_t>(ctx->smem_optin, 227 * 1024) - 1024);
-    if (tiles * mtiles * p.splits > uint32_t(ctx->sm_count) && stages_in(kHalfSmem) >= std::min(4u, p.stages))
-        p.stages = stages_in(kHalfSmem);
-    p.sums_offset = p.splits > 1 ? p.stages * stage_bytes + uint32_t(tail) : 0;
-    const size_t smem = std::max<size_t>({1024 + p.stages * stage_bytes + tail, 1024 + p.sums_offset + sums, 80 * 1024});
+    p.stages = stages_in(kHalfSmem);
+    if (p.splits > 1 && sums < kHalfSmem / 2 && stages_in(kHalfSmem - sums) >= std::min(4u, p.stages)) {
+        p.stages = stages_in(kHalfSmem - sums);
+        p.sums_offset = p.stages * stage_bytes + uint32_t(rest);
+    }
+    const size_t smem = std::max<size_t>({1024 + p.stages * stage_bytes + rest, 1024 + p.sums_offset + sums, 80 * 1024});
     p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
     if (swiglu) {
         const size_t side = opure_mx_scale_bytes(p.half, a->w.cols);

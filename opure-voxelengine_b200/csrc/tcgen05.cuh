@@ -18,6 +18,20 @@ __device__ __forceinline__ void load_2d(bool one, void *dst, const CUtensorMap *
         : "memory");
 }
 
+// Into L2 only (harmless before a dependency wait: a late write of the predecessor shows there).
+__device__ __forceinline__ void prefetch_2d(bool one, const CUtensorMap *map, uint32_t x, uint32_t y) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %3, 0;\n @e cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n}" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(x), "r"(y), "r"(uint32_t(one))
+        : "memory");
+}
+__device__ __forceinline__ void prefetch(bool one, const void *p, uint32_t bytes) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n @e cp.async.bulk.prefetch.L2.global [%0], %1;\n}" ::"l"(p), "r"(bytes),
+                 "r"(uint32_t(one))
+                 : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -207,6 +221,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // This CTA's shared-memory address as CTA `rank` of the cluster sees its own.
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -219,8 +235,6 @@ __device__ __forceinline__ void st_async_f4(uint32_t addr, uint32_t a, uint32_t 
                  "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 }  // namespace tc
 }  // namespace opure
