@@ -1,4 +1,4 @@
-// mx_gemv.cu -- the product of microscaled matrices for at most 4 tokens: decode's weight
+// mx_gemv.cu -- the product of microscaled matrices for one or two tokens: decode's weight
 // streaming.
 //
 // Bound by memory: a weight is 0.53 bytes and used once per token. At the measured 6.45 TB/s an SM
@@ -26,7 +26,7 @@
 namespace opure {
 namespace {
 
-constexpr uint32_t kMaxTokens = 4;
+constexpr uint32_t kMaxTokens = 2;  // from 3 on mx_gemm.cu is as fast (4 x 2048 x 8192: 5.7 us both) or faster (4 x 49152 x 576: 12.5 and 8.6)
 constexpr uint32_t kMaxWarps = 16;
 
 struct GemvParams {
@@ -62,29 +62,28 @@ struct Weights {
     uint4 w[2 * MT];
     uint16_t s[2 * MT];
 };
-// Two tokens' 128 columns: this lane's block of its token (or zeros), and two blocks' scales.
+// The tokens' 128 columns: this lane's block of its token (or zeros), and two blocks' scales.
 template <uint32_t XF>
 struct Tokens {
     uint4 x[XF / 4];
     uint16_t s;
 };
 
-// MT: tiles of 16 rows per warp. NP: pairs of tokens.
-template <uint32_t XF, uint32_t MT, uint32_t NP>
+// MT: tiles of 16 rows per warp.
+template <uint32_t XF, uint32_t MT>
 __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
-    constexpr uint32_t kAhead = MT == 1 ? 4 : 3;  // pieces of weights in flight
+    constexpr uint32_t kAhead = MT == 1 ? 4 : 3;  // pieces in flight
     constexpr uint32_t kRows = 16 * MT;
-    __shared__ float part[kMaxWarps][kRows][2 * NP + 1];
+    __shared__ float part[kMaxWarps][kRows][kMaxTokens + 1];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t unit = warp / p.splits, split = warp % p.splits;
     const uint32_t pieces = mx_kp(p.cols) / 128;
     const bool swiglu = p.epilogue == OPURE_EPI_SWIGLU;
-    // This warp's rows. In SwiGLU the first 32 / kRows units are gate rows, the others up rows,
-    // whose scale tiles are counted from the first up row.
-    constexpr uint32_t kGate = 32 / kRows;
-    const bool up = swiglu && unit >= kGate;
+    // This warp's rows. In SwiGLU (two tiles a warp) unit 0 is 32 gate rows and unit 1 the up rows
+    // that go with them, whose scale tiles are counted from the first up row.
+    const bool up = swiglu && unit;
     const uint32_t c0 = blockIdx.x * (swiglu ? 32 : p.units * kRows);  // first result column of the CTA
-    const uint32_t local = c0 + (up ? unit - kGate : unit) * kRows + g;
+    const uint32_t local = c0 + (swiglu ? 0 : unit * kRows) + g;
     const uint32_t limit = swiglu ? p.half : p.rows, first = up ? p.half : 0;
     const size_t row_bytes = mx_row_bytes(OPURE_MX_FP4, p.cols);
     const uint8_t *w[2 * MT], *ws[2 * MT];
@@ -102,29 +101,26 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
     grid_dependency_wait();
     grid_dependents_launch();
 
-    // Column g of the MMA is block g % 4 of token g / 4 of the pair: the lanes t = g % 4 hold it.
-    // D's columns 2 t and 2 t + 1 are blocks 2 t % 4 and the next of token t / 2.
-    const uint8_t *x = p.x + t * (4 * XF), *xs = p.xs + t % 2 * 2;
-    const size_t x_bytes = mx_row_bytes(XF, p.cols);
-    auto load_weights = [&](Weights<MT> &in, uint32_t k) {
+    // Column g of the MMA is block g % 4 of token g / 4: the lanes t = g % 4 hold it. D's columns
+    // 2 t and 2 t + 1 are blocks 2 t % 4 and the next of token t / 2.
+    const bool holds = t == g % 4 && g / 4 < p.n;
+    const uint8_t *x = p.x + g / 4 * mx_row_bytes(XF, p.cols) + t * (4 * XF);
+    const uint8_t *xs = p.xs + mx_scale_offset(p.cols, min(t / 2, p.n - 1), 0) + t % 2 * 2;
+    auto load = [&](Weights<MT> &in, Tokens<XF> &tk, uint32_t k) {
 #pragma unroll
         for (uint32_t j = 0; j < 2 * MT; ++j) {
             in.w[j] = ldg_stream(w[j] + size_t(k) * 64);
             in.s[j] = *reinterpret_cast<const uint16_t *>(ws[j] + size_t(k) * kMxTileBytes);
         }
-    };
-    auto load_tokens = [&](Tokens<XF> &in, uint32_t pair, uint32_t k) {
-        const uint32_t token = pair * 2 + g / 4, of = min(pair * 2 + t / 2, p.n - 1);
 #pragma unroll
         for (uint32_t j = 0; j < XF / 4; ++j) {
-            in.x[j] = make_uint4(0, 0, 0, 0);
-            if (t == g % 4 && token < p.n)
-                in.x[j] = *reinterpret_cast<const uint4 *>(x + token * x_bytes + size_t(k) * (16 * XF) + j * 16);
+            tk.x[j] = make_uint4(0, 0, 0, 0);
+            if (holds) tk.x[j] = *reinterpret_cast<const uint4 *>(x + size_t(k) * (16 * XF) + j * 16);
         }
-        in.s = *reinterpret_cast<const uint16_t *>(xs + mx_scale_offset(p.cols, of, 0) + size_t(k) * kMxTileBytes);
+        tk.s = *reinterpret_cast<const uint16_t *>(xs + size_t(k) * kMxTileBytes);
     };
-    float acc[NP][2 * MT] = {};
-    auto compute = [&](const Weights<MT> &wt, const Tokens<XF> &tk, float (&sum)[2 * MT]) {
+    float sum_of[2 * MT] = {};
+    auto compute = [&](const Weights<MT> &wt, const Tokens<XF> &tk) {
         // The tokens' 32 values per lane as fp16 pairs, in the order of the weights' codes.
         uint32_t b[16];
         const uint32_t *c = reinterpret_cast<const uint32_t *>(tk.x);
@@ -159,42 +155,30 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
             for (uint32_t j = 0; j < 2; ++j) {
                 float s0, s1;
                 scale_pair(wt.s[2 * m + j], s0, s1);
-                sum[2 * m + j] = fmaf(d[2 * j] * x0, s0, fmaf(d[2 * j + 1] * x1, s1, sum[2 * m + j]));
+                sum_of[2 * m + j] = fmaf(d[2 * j] * x0, s0, fmaf(d[2 * j + 1] * x1, s1, sum_of[2 * m + j]));
             }
         }
     };
     Weights<MT> in[kAhead];
-    Tokens<XF> tk[kAhead];  // one pair: in flight beside the weights
+    Tokens<XF> tk[kAhead];
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; ++i)
-        if (split + i * p.splits < pieces) {
-            load_weights(in[i], split + i * p.splits);
-            if (NP == 1) load_tokens(tk[i], 0, split + i * p.splits);
-        }
+        if (split + i * p.splits < pieces) load(in[i], tk[i], split + i * p.splits);
     for (uint32_t k0 = split; k0 < pieces; k0 += kAhead * p.splits) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
             const uint32_t k = k0 + i * p.splits, next = k + kAhead * p.splits;
             if (k >= pieces) break;
-#pragma unroll
-            for (uint32_t pair = 0; pair < NP; ++pair) {
-                if (NP > 1) load_tokens(tk[i], pair, k);
-                compute(in[i], tk[i], acc[pair]);
-            }
-            if (next < pieces) {
-                load_weights(in[i], next);
-                if (NP == 1) load_tokens(tk[i], 0, next);
-            }
+            compute(in[i], tk[i]);
+            if (next < pieces) load(in[i], tk[i], next);
         }
     }
     // Lanes t and t ^ 1 hold two blocks each of one token.
 #pragma unroll
-    for (uint32_t pair = 0; pair < NP; ++pair)
-#pragma unroll
-        for (uint32_t j = 0; j < 2 * MT; ++j) {
-            const float v = acc[pair][j] + __shfl_xor_sync(0xffffffffu, acc[pair][j], 1);
-            if (t % 2 == 0) part[warp][g + 8 * j][pair * 2 + t / 2] = v;
-        }
+    for (uint32_t j = 0; j < 2 * MT; ++j) {
+        const float v = sum_of[j] + __shfl_xor_sync(0xffffffffu, sum_of[j], 1);
+        if (t % 2 == 0) part[warp][g + 8 * j][t / 2] = v;
+    }
     __syncthreads();
 
     // Results: a thread takes 4 neighbouring columns of a token.
@@ -287,14 +271,13 @@ opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t 
     const uint32_t pieces = mx_kp(p.cols) / 128, sms = uint32_t(ctx->sm_count);
     const uint32_t row_tiles = swiglu ? mx_kp(p.half) / 32 * 4 : ceil_div(p.rows, 16);
     // Two tiles per warp halve the work on the tokens' side; one where that would leave SMs empty.
-    const bool two = p.n <= 2 && (swiglu || row_tiles >= 2 * sms);
+    const bool two = swiglu || row_tiles >= 2 * sms;
     const uint32_t units_all = two ? (row_tiles + 1) / 2 : row_tiles;
-    choose(p, pieces, units_all, swiglu ? (two ? 2 : 4) : 0, two, sms);
+    choose(p, pieces, units_all, swiglu ? 2 : 0, two, sms);
     const dim3 grid(ceil_div(units_all, p.units)), block(32 * p.units * p.splits);
     auto go = [&](auto kernel) { return launch(ctx, kernel, grid, block, 0, true, p); };
-    if (p.n > 2) return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 1, 2>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, 2>);
-    if (two) return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 2, 1>) : go(mx_gemv_kernel<OPURE_MX_FP4, 2, 1>);
-    return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 1, 1>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1, 1>);
+    if (two) return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 2>) : go(mx_gemv_kernel<OPURE_MX_FP4, 2>);
+    return fp8 ? go(mx_gemv_kernel<OPURE_MX_FP8, 1>) : go(mx_gemv_kernel<OPURE_MX_FP4, 1>);
 }
 
 }  // namespace opure
