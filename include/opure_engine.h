@@ -45,7 +45,17 @@ typedef struct opure_engine_options {
                                  position attends to the last kv_window / page_size - 1 whole
                                  pages and its own; 0: every position up to max_len */
     uint32_t tp_allreduce;    /* tensor parallel: OPURE_TP_* (0: OPURE_TP_AUTO)          */
+    uint32_t weights;         /* OPURE_WEIGHTS_*: how the layer matrices are kept        */
 } opure_engine_options;
+
+enum {
+    OPURE_WEIGHTS_STORED = 0, /* as the model file has them: fp16, or int8 with its scales */
+    OPURE_WEIGHTS_MXFP4 = 1   /* quantised to 4-bit microscaled form on upload (OPURE_MX_FP4):
+                                 0.53 bytes per weight in memory and per step; the linear
+                                 layers then take 8-bit microscaled inputs (opure_mx_gemm).
+                                 Embeddings, norms and the lm_head stay fp16. Per-op kernels
+                                 only; floating-point models on one GPU                     */
+};
 
 enum {
     OPURE_TP_AUTO = 0,        /* the peer kernels (measured faster than NCCL at 2, 4 and
@@ -72,6 +82,7 @@ typedef struct opure_engine_info {
     uint64_t kv_bytes_per_token;  /* fp16 K+V, all layers, one sequence                 */
     uint32_t tp_ranks;            /* tensor-parallel ranks (1 without a communicator)     */
     uint32_t tp_peer;             /* 1: collectives run as NVLink peer kernels, 0: NCCL   */
+    uint32_t weights;             /* OPURE_WEIGHTS_*                                      */
 } opure_engine_info;
 
 typedef struct opure_generate_timing {

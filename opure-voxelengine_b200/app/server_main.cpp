@@ -1,6 +1,6 @@
 // opure_server -- the HTTP front end (GET /health, POST /generate, GET /metrics) over
-// libopure_engine: `opure_server --model <dir> [--port N] [--gpus 0,1,...]`, one engine
-// per listed GPU (the reference's opure_server, src/app/Opure_Server.cpp:470-540, runs one
+// libopure_engine: `opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4]`,
+// one engine per listed GPU (the reference's opure_server, src/app/Opure_Server.cpp:470-540, runs one
 // engine on its one D3D12 device). Runs until SIGINT/SIGTERM.
 #include <csignal>
 #include <cstdio>
@@ -22,6 +22,8 @@ int main(int argc, char **argv) {
     std::string model;
     unsigned port = 8080;
     std::vector<int> gpus{0};
+    opure_engine_options opts{};
+    opts.use_graphs = 1;
     for (int i = 1; i < argc; ++i) {
         const std::string a = argv[i];
         if (a == "--model" && i + 1 < argc) {
@@ -36,8 +38,11 @@ int main(int argc, char **argv) {
                 p = *end == ',' ? end + 1 : end;
                 if (end == p && *p) break;
             }
+        } else if (a == "--weights" && i + 1 < argc && !std::strcmp(argv[i + 1], "mxfp4")) {
+            ++i;
+            opts.weights = OPURE_WEIGHTS_MXFP4;
         } else {
-            std::printf("usage: opure_server --model <dir> [--port N] [--gpus 0,1,...]\n"
+            std::printf("usage: opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4]\n"
                         "routes: GET /health, POST /generate {\"tokens\":[...],\"max_tokens\":64}, GET /metrics\n");
             return a == "--help" || a == "-h" ? 0 : 2;
         }
@@ -48,7 +53,8 @@ int main(int argc, char **argv) {
     }
     opure_server *srv = nullptr;
     const opure_status st =
-        opure_server_start(model.c_str(), gpus.data(), uint32_t(gpus.size()), uint16_t(port), nullptr, &srv);
+        opure_server_start(model.c_str(), gpus.data(), uint32_t(gpus.size()), uint16_t(port),
+                           opts.weights ? &opts : nullptr, &srv);
     if (st != OPURE_OK) {
         std::fprintf(stderr, "opure_server: %s: %s\n", opure_strerror(st), opure_engine_last_error(nullptr));
         return 1;

@@ -70,6 +70,8 @@ opure::engine::EngineOptions ToOptions(const opure_engine_options *o) {
         opts.prefillChunk = o->prefill_chunk;
         opts.kvWindow = o->kv_window;
         opts.tpAllreduce = o->tp_allreduce;
+        OPURE_CHECK(o->weights <= OPURE_WEIGHTS_MXFP4, "unknown weight format");
+        opts.mxWeights = o->weights == OPURE_WEIGHTS_MXFP4;
     }
     return opts;
 }
@@ -237,6 +239,7 @@ void FillInfo(const opure::graph::Graph &g, opure_engine_info *info) {
     info->stream_bytes = g.StreamBytes();
     info->kv_bytes_per_token = c.KvBytesPerToken() / g.Local().tpSize;  // this shard's KV heads
     info->tp_ranks = g.Local().tpSize;
+    info->weights = p.mx ? OPURE_WEIGHTS_MXFP4 : OPURE_WEIGHTS_STORED;
 }
 
 }  // namespace

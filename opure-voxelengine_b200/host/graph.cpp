@@ -110,6 +110,16 @@ bool ModelConfig::Validate(std::string &err) const {
     return true;
 }
 
+// Bytes from a microscaled matrix's codes to its scales.
+static uint64_t MxScalesAt(uint64_t rows, uint64_t cols) {
+    return Align(opure_mx_code_bytes(OPURE_MX_FP4, uint32_t(rows), uint32_t(cols)), 256);
+}
+
+opure_mx_matrix Graph::MxMatrix(void *arena, uint64_t offset, uint64_t rows, uint64_t cols) {
+    auto *codes = static_cast<uint8_t *>(arena) + offset;
+    return {codes, codes + MxScalesAt(rows, cols), uint32_t(rows), uint32_t(cols), OPURE_MX_FP4};
+}
+
 void Graph::Release() {
     stream_.Close();
     loaded_ = false;
@@ -157,15 +167,21 @@ void Graph::PlanLayout(const LayoutOptions &opts) {
             allQ &= t->IsQuantized();
         }
     OPURE_CHECK(!anyQ || allQ, "layer matrices mix int8 and floating point");
+    OPURE_CHECK(!opts.mxWeights || (!anyQ && ts == 1),
+                "microscaled weights need a floating-point model on one device");
+    plan_.mx = opts.mxWeights;
     plan_.wDtype = allQ ? OPURE_W_Q8 : OPURE_W_F16;
     const uint64_t eb = allQ ? 1 : 2;
-    plan_.hasFused = opts.fusedLayouts && ts == 1;
+    plan_.hasFused = opts.fusedLayouts && ts == 1 && !plan_.mx;
 
     uint64_t cur = 0;
     auto place = [&](uint64_t bytes) {
         const uint64_t at = cur;
         cur = Align(cur + bytes, 256);
         return at;
+    };
+    auto matrix = [&](uint64_t rows, uint64_t cols) {
+        return place(plan_.mx ? MxScalesAt(rows, cols) + opure_mx_scale_bytes(uint32_t(rows), uint32_t(cols)) : rows * cols * eb);
     };
     plan_.embedTokens = place(uint64_t(cfg_.vocabSize) * h * 2);  // embeddings stay fp16
     plan_.finalNorm = place(h * 2);
@@ -184,10 +200,10 @@ void Graph::PlanLayout(const LayoutOptions &opts) {
         VramPlan::LayerTensors &t = plan_.layers[l];
         t.inputNorm = place(h * 2);
         t.postAttNorm = place(h * 2);
-        t.wqkv = place(qkv * h * eb);
-        t.wo = place(h * att * eb);
-        t.wgu = place(2 * ff * h * eb);
-        t.wdown = place(h * ff * eb);
+        t.wqkv = matrix(qkv, h);
+        t.wo = matrix(h, att);
+        t.wgu = matrix(2 * ff, h);
+        t.wdown = matrix(h, ff);
         if (plan_.hasFused) {
             t.woBlk = place(h * h * eb);
             t.wdownT = place(h * ff * eb);
@@ -201,8 +217,10 @@ void Graph::PlanLayout(const LayoutOptions &opts) {
 uint64_t Graph::StreamBytes() const {
     const uint64_t eb = plan_.wDtype == OPURE_W_Q8 ? 1 : 2;
     const uint64_t h = cfg_.hiddenSize, ff = local_.inter, hd = cfg_.HeadDim();
-    const uint64_t perLayer = (uint64_t(local_.QkvRows(uint32_t(hd))) * h + h * local_.heads * hd + 3 * ff * h) * eb +
-                              2 * h * 2;
+    const uint64_t qkv = local_.QkvRows(uint32_t(hd)), att = uint64_t(local_.heads) * hd;
+    auto mx = [](uint64_t rows, uint64_t cols) { return rows * (cols / 2 + (cols + 31) / 32); };
+    const uint64_t matrices = plan_.mx ? mx(qkv, h) + mx(h, att) + mx(2 * ff, h) + mx(h, ff) : (qkv * h + h * att + 3 * ff * h) * eb;
+    const uint64_t perLayer = matrices + 2 * h * 2;
     return perLayer * cfg_.numLayers + uint64_t(local_.vocab) * h * (plan_.lmQuantized ? 1 : 2) + h * 2;
 }
 
@@ -227,9 +245,29 @@ void Graph::UploadWeights(opure_ctx *ctx, void *arena) {
             safetensors::NarrowToF16(t.dtype, stream_.Data(t), n, reinterpret_cast<uint16_t *>(out.data()));
         }
     };
-    auto put = [&](uint64_t off, const std::vector<uint8_t> &bytes) {
-        OPURE_CUDA_CHECK(opure_h2d(ctx, base + off, bytes.data(), bytes.size()));
+    auto upload = [&](void *dst, const std::vector<uint8_t> &bytes) {
+        OPURE_CUDA_CHECK(opure_h2d(ctx, dst, bytes.data(), bytes.size()));
         OPURE_CUDA_CHECK(opure_sync(ctx, 600000));  // staging is reused
+    };
+    auto put = [&](uint64_t off, const std::vector<uint8_t> &bytes) { upload(base + off, bytes); };
+    // Microscaled weights: a matrix is gathered as fp16 in device memory, then quantised there.
+    struct DeviceTemp {
+        opure_ctx *ctx;
+        void *p = nullptr;
+        ~DeviceTemp() { opure_free(ctx, p); }
+    } whole{ctx};
+    if (plan_.mx) {
+        const uint64_t qkvRows = local_.QkvRows(hd);
+        OPURE_CUDA_CHECK(opure_alloc(ctx, std::max({qkvRows * h, 2 * ff * h, h * h}) * 2, &whole.p));
+    }
+    // Part of a layer matrix, `within` bytes from its start.
+    auto put_part = [&](uint64_t off, uint64_t within, const std::vector<uint8_t> &bytes) {
+        upload(plan_.mx ? static_cast<uint8_t *>(whole.p) + within : base + off + within, bytes);
+    };
+    auto finish = [&](uint64_t off, uint64_t nrows, uint64_t cols) {
+        if (!plan_.mx) return;
+        const opure_mx_matrix m = MxMatrix(arena, off, nrows, cols);
+        OPURE_CUDA_CHECK(opure_mx_quantize(ctx, whole.p, OPURE_F16, cols, &m));
     };
 
     fetch(spec_.Embed(), stage, false);
@@ -269,17 +307,19 @@ void Graph::UploadWeights(opure_ctx *ctx, void *arena) {
         fetch(b.postAttNorm, stage, false);
         put(t.postAttNorm, stage);
         // q; k; v contiguous, so the three projections run as one GEMV over QkvRows().
-        uint64_t off = t.wqkv;
+        uint64_t off = 0;
         for (const TensorRef *r : {&b.wq, &b.wk, &b.wv}) {
             fetch(*r, stage, q8);
             const uint64_t nr = r == &b.wq ? hq : hk;
             rows(stage, h, uint64_t(tr) * nr, nr);  // this shard's heads
-            put(off, stage);
+            put_part(t.wqkv, off, stage);
             off += stage.size();
         }
+        finish(t.wqkv, hq + 2 * hk, h);
         fetch(b.wo, a, q8);
         cols_of(a, h, h, uint64_t(tr) * hq, hq);  // input columns of this shard's heads
-        put(t.wo, a);
+        put_part(t.wo, 0, a);
+        finish(t.wo, h, hq);
         if (plan_.hasFused) {
             // woBlk[g][o][c] = Wo[o][g*G*hd + c]: each kv head's input columns contiguous.
             const uint64_t gw = uint64_t(G) * hd;
@@ -291,13 +331,15 @@ void Graph::UploadWeights(opure_ctx *ctx, void *arena) {
         }
         fetch(b.gate, stage, q8);
         rows(stage, h, uint64_t(tr) * ffl, ffl);
-        put(t.wgu, stage);
+        put_part(t.wgu, 0, stage);
         fetch(b.up, stage, q8);
         rows(stage, h, uint64_t(tr) * ffl, ffl);
-        put(t.wgu + ffl * h * eb, stage);
+        put_part(t.wgu, ffl * h * eb, stage);
+        finish(t.wgu, 2 * ffl, h);
         fetch(b.down, a, q8);
         cols_of(a, h, ff, uint64_t(tr) * ffl, ffl);
-        put(t.wdown, a);
+        put_part(t.wdown, 0, a);
+        finish(t.wdown, h, ffl);
         if (plan_.hasFused) {
             b2.resize(a.size());
             for (uint64_t o = 0; o < h; ++o)

@@ -49,6 +49,7 @@ struct LayoutOptions {
     // split by rows (whole heads / intermediate rows), o_proj and down_proj by columns (the
     // matching input slice), the lm_head by vocabulary rows; embeddings and norms are whole.
     uint32_t tpSize = 1, tpRank = 0;
+    bool mxWeights = false;  // layer matrices quantised to 4-bit microscaled form on upload
 };
 
 // The part of the model one tensor-parallel shard computes (the whole model at tpSize 1).
@@ -76,6 +77,9 @@ struct VramPlan {
     uint32_t wDtype = OPURE_W_F16;  // matrices: OPURE_W_F16 or OPURE_W_Q8
     bool lmQuantized = false;
     bool hasFused = false;
+    // Layer matrices as MXFP4 (opure_mx_matrix): at each matrix's offset its codes, then, from
+    // the next multiple of 256 bytes, its scales.
+    bool mx = false;
     uint64_t weightBytes = 0;
 };
 
@@ -99,6 +103,8 @@ public:
     const ModelSpec &Spec() const { return spec_; }
     bool IsLoaded() const { return loaded_; }
     bool IsQuantized() const { return plan_.wDtype == OPURE_W_Q8; }
+    // The microscaled matrix at `offset` of the arena (Plan().mx).
+    static opure_mx_matrix MxMatrix(void *arena, uint64_t offset, uint64_t rows, uint64_t cols);
 
 private:
     void PlanLayout(const LayoutOptions &opts);

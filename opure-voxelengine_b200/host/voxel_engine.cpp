@@ -42,7 +42,10 @@ void VoxelEngine::Shutdown() {
                     static_cast<void *>(buf_.sync), static_cast<void *>(buf_.trace),
                     static_cast<void *>(buf_.prefillKeys), static_cast<void *>(buf_.packAttn),
                     static_cast<void *>(buf_.packRes), static_cast<void *>(buf_.packAct),
-                    static_cast<void *>(buf_.sumsq), weights_})
+                    static_cast<void *>(buf_.sumsq), static_cast<void *>(buf_.mxNorm.codes),
+                    static_cast<void *>(buf_.mxNorm.scales), static_cast<void *>(buf_.mxAttn.codes),
+                    static_cast<void *>(buf_.mxAttn.scales), static_cast<void *>(buf_.mxAct.codes),
+                    static_cast<void *>(buf_.mxAct.scales), weights_})
         if (p) opure_free(ctx_, p);
     for (auto &s : attnScratch_) opure_free(ctx_, s.second.first);
     attnScratch_.clear();
@@ -73,6 +76,7 @@ void VoxelEngine::Initialize(const std::string &modelDir, const EngineOptions &o
     }
     graph::LayoutOptions lo;
     lo.fusedLayouts = opts.path != 1;  // grouped o_proj and transposed down_proj
+    lo.mxWeights = opts.mxWeights;
     comm_ = comm;
     if (comm) {
         OPURE_CUDA_CHECK(opure_comm_info(comm, &lo.tpSize, &lo.tpRank));
@@ -135,7 +139,7 @@ bool VoxelEngine::Chained(uint32_t n) const {
     const graph::ModelConfig &c = graph_.Config();
     const graph::VramPlan &p = graph_.Plan();
     const uint32_t att = c.numHeads * c.HeadDim();
-    return !comm_ && p.wDtype == OPURE_W_F16 && !p.lmQuantized && n >= 16 && n <= 256 && n <= maxVec_ &&
+    return !comm_ && !p.mx && p.wDtype == OPURE_W_F16 && !p.lmQuantized && n >= 16 && n <= 256 && n <= maxVec_ &&
            (c.HeadDim() == 64 || c.HeadDim() == 128) &&  // the attention kernel with packed output
            c.hiddenSize % 64 == 0 && c.intermediateSize % 64 == 0 && att % 64 == 0 && c.hiddenSize <= 16384 &&
            c.intermediateSize <= 16384 && att <= 16384 && buf_.packRes != nullptr;
@@ -164,7 +168,23 @@ void VoxelEngine::AllocBuffers() {
     buf_.base1 = Alloc<float>(ctx_, size_t(B) * c.hiddenSize);
     buf_.delta0 = Alloc<long long>(ctx_, size_t(B) * c.hiddenSize);
     buf_.delta1 = Alloc<long long>(ctx_, size_t(B) * c.hiddenSize);
-    if (!comm_ && B >= 16) {
+    if (graph_.Plan().mx) {
+        auto matrix = [&](uint32_t cols) {
+            void *codes = nullptr, *scales = nullptr;
+            OPURE_CUDA_CHECK(opure_alloc(ctx_, opure_mx_code_bytes(OPURE_MX_FP8, B, cols), &codes));
+            opure_mx_matrix m{static_cast<uint8_t *>(codes), nullptr, B, cols, OPURE_MX_FP8};
+            if (opure_alloc(ctx_, opure_mx_scale_bytes(B, cols), &scales) != OPURE_OK) {
+                opure_free(ctx_, codes);
+                ThrowError("out of device memory for the microscaled activations");
+            }
+            m.scales = static_cast<uint8_t *>(scales);
+            return m;
+        };
+        buf_.mxNorm = matrix(c.hiddenSize);
+        buf_.mxAttn = matrix(c.numHeads * c.HeadDim());
+        buf_.mxAct = matrix(c.intermediateSize);
+        buf_.partial = Alloc<float>(ctx_, size_t(B) * c.hiddenSize);
+    } else if (!comm_ && B >= 16) {
         const uint32_t nv = std::min<uint32_t>(B, 256);
         const uint32_t att = c.numHeads * c.HeadDim();
         auto packed = [&](uint32_t len) {
@@ -234,7 +254,79 @@ opure_step_io VoxelEngine::StepIO(uint32_t n) const {
     return io;
 }
 
+// RoPE, the KV append and attention of the step's q;k;v rows; `packed` (or null) also receives
+// the attention output as a chained operand.
+void VoxelEngine::RecordAttention(uint32_t L, uint32_t n, uint32_t qkvRows, uint16_t *packed) {
+    const graph::ModelConfig &c = graph_.Config();
+    const graph::LocalGeometry &lg = graph_.Local();
+    const opure_kv_layout kv = kv_.Layout(L);
+    OPURE_CUDA_CHECK(opure_rope_kv_append(ctx_, buf_.qkv, qkvRows, buf_.q, buf_.seq, buf_.pos, n, lg.heads,
+                                          c.ropeTheta, &kv));
+    opure_attn_args a{};
+    a.q = buf_.q;
+    a.out = buf_.attn;
+    a.seq = buf_.seq;
+    a.seq_len = buf_.seqLen;
+    a.n = n;
+    a.n_q = 1;
+    a.n_heads = lg.heads;
+    a.scale = opts_.attnScale;
+    a.max_ctx = maxLen_;
+    a.split_tokens = 0;
+    a.scratch = AttnScratch(n, &a.scratch_bytes);
+    a.kv = kv;
+    a.out_packed = packed;
+    OPURE_CUDA_CHECK(opure_attention(ctx_, &a));
+}
+
+// A layer over 4-bit microscaled weights: every linear layer takes 8-bit microscaled inputs, which
+// the norm, the SwiGLU product's epilogue or (attention) a quantise call writes. The o_proj's
+// result joins the residual in the norm after it, the down_proj's in its own epilogue.
+void VoxelEngine::RecordLayerMx(uint32_t L, uint32_t n) {
+    const graph::ModelConfig &c = graph_.Config();
+    const graph::VramPlan::LayerTensors &t = graph_.Plan().layers[L];
+    const uint32_t h = c.hiddenSize, ff = c.intermediateSize, qkvRows = c.QkvRows(), att = c.numHeads * c.HeadDim();
+    auto rows = [&](opure_mx_matrix m) {
+        m.rows = n;
+        return m;
+    };
+    const opure_mx_matrix norm = rows(buf_.mxNorm), attn = rows(buf_.mxAttn), act = rows(buf_.mxAct);
+    auto normed = [&](const float *x, uint64_t gain, const float *residual) {
+        opure_mx_norm_args a{};
+        a.x = x;
+        a.x_type = OPURE_F32;
+        a.x_stride = h;
+        a.residual = residual;
+        a.sum = residual ? buf_.x : nullptr;
+        a.gain = reinterpret_cast<const uint16_t *>(At(weights_, gain));
+        a.eps = c.rmsNormEps;
+        a.out = norm;
+        OPURE_CUDA_CHECK(opure_mx_rmsnorm(ctx_, &a));
+    };
+    auto product = [&](uint64_t w, uint32_t outRows, uint32_t cols, const opure_mx_matrix &x, uint32_t epilogue, float *y) {
+        opure_mx_gemm_args a{};
+        a.w = graph::Graph::MxMatrix(weights_, w, outRows, cols);
+        a.x = x;
+        a.epilogue = epilogue;
+        a.y = y;
+        a.y_type = OPURE_F32;
+        a.y_stride = outRows;
+        if (epilogue == OPURE_EPI_ADD) a.residual = y;
+        if (epilogue == OPURE_EPI_SWIGLU) a.out = act;
+        OPURE_CUDA_CHECK(opure_mx_gemm(ctx_, &a));
+    };
+    normed(buf_.x, t.inputNorm, nullptr);
+    product(t.wqkv, qkvRows, h, norm, OPURE_EPI_STORE, buf_.qkv);
+    RecordAttention(L, n, qkvRows, nullptr);
+    OPURE_CUDA_CHECK(opure_mx_quantize(ctx_, buf_.attn, OPURE_F32, att, &attn));
+    product(t.wo, h, att, attn, OPURE_EPI_STORE, buf_.partial);
+    normed(buf_.partial, t.postAttNorm, buf_.x);
+    product(t.wgu, 2 * ff, h, norm, OPURE_EPI_SWIGLU, nullptr);
+    product(t.wdown, h, ff, act, OPURE_EPI_ADD, buf_.x);
+}
+
 void VoxelEngine::RecordLayer(uint32_t L, uint32_t n) {
+    if (graph_.Plan().mx) return RecordLayerMx(L, n);
     const graph::ModelConfig &c = graph_.Config();
     const graph::VramPlan &plan = graph_.Plan();
     const graph::VramPlan::LayerTensors &t = plan.layers[L];
@@ -320,24 +412,7 @@ void VoxelEngine::RecordLayer(uint32_t L, uint32_t n) {
         gemv(At(weights_, t.wqkv + uint64_t(qr + kr) * h * eb), t.sv, t.sv, kr, h, buf_.x, h, buf_.qkv + qr + kr,
              qkvRows, OPURE_PRO_RMSNORM, inNorm, OPURE_EPI_STORE, nullptr);
     }
-    const opure_kv_layout kv = kv_.Layout(L);
-    OPURE_CUDA_CHECK(opure_rope_kv_append(ctx_, buf_.qkv, qkvRows, buf_.q, buf_.seq, buf_.pos, n, lg.heads,
-                                          c.ropeTheta, &kv));
-    opure_attn_args a{};
-    a.q = buf_.q;
-    a.out = buf_.attn;
-    a.seq = buf_.seq;
-    a.seq_len = buf_.seqLen;
-    a.n = n;
-    a.n_q = 1;
-    a.n_heads = lg.heads;
-    a.scale = opts_.attnScale;
-    a.max_ctx = maxLen_;
-    a.split_tokens = 0;
-    a.scratch = AttnScratch(n, &a.scratch_bytes);
-    a.kv = kv;
-    a.out_packed = ch ? buf_.packAttn : nullptr;
-    OPURE_CUDA_CHECK(opure_attention(ctx_, &a));
+    RecordAttention(L, n, qkvRows, ch ? buf_.packAttn : nullptr);
     if (!comm_) {
         // o_proj + residual, in place on the residual stream.
         gemv(At(weights_, t.wo), t.so, t.so, h, h, buf_.attn, h, buf_.x, h, OPURE_PRO_NONE, nullptr, OPURE_EPI_ADD,
@@ -933,6 +1008,11 @@ void VoxelEngine::PoisonBanks(float fill) {
         OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.known, none.data(), B * 4));
         OPURE_CUDA_CHECK(opure_sync(ctx_, 60000));
     }
+    for (const opure_mx_matrix &m : {buf_.mxNorm, buf_.mxAttn, buf_.mxAct})
+        if (m.codes) {  // microscaled activations: NaN codes and scales
+            OPURE_CUDA_CHECK(opure_fill(ctx_, m.codes, 0xff, opure_mx_code_bytes(m.format, m.rows, m.cols)));
+            OPURE_CUDA_CHECK(opure_fill(ctx_, m.scales, 0xff, opure_mx_scale_bytes(m.rows, m.cols)));
+        }
     if (buf_.packRes) {
         // Chained tensor-core operands: fp16 pairs (the fill's fp16 bits) and the sums of squares.
         const uint32_t nv = std::min<uint32_t>(B, 256), att = c.numHeads * c.HeadDim();

@@ -53,6 +53,7 @@ struct EngineOptions {
                                     // ring, and a position attends to the last kvWindow / pageSize - 1
                                     // whole pages and its own
     uint32_t tpAllreduce = 0;       // tensor parallel: 0 auto (peer kernels when mappable), 1 NCCL, 2 peer
+    bool mxWeights = false;         // layer matrices quantised to 4-bit microscaled form on upload
 };
 
 struct GenerateResult {
@@ -186,7 +187,8 @@ public:
         // Fused path: second residual base and the two fixed-point delta buffers.
         float *base1 = nullptr;
         long long *delta0 = nullptr, *delta1 = nullptr;
-        float *partial = nullptr;  // tensor parallelism: [maxBatch][hidden] shard partial sums
+        float *partial = nullptr;  // tensor parallelism: [maxBatch][hidden] shard partial sums;
+                                   // microscaled weights: the o_proj's result
         uint32_t *sync = nullptr;  // grid-barrier words of the persistent decode kernel
         unsigned long long *trace = nullptr;  // its phase timestamps (EngineOptions.phaseTrace)
         unsigned long long *prefillKeys = nullptr;  // [maxBatch] chunked prefill's last-token keys
@@ -196,6 +198,9 @@ public:
         // squares for the consumer's RMSNorm.
         uint16_t *packAttn = nullptr, *packRes = nullptr, *packAct = nullptr;
         float *sumsq = nullptr;
+        // Microscaled weights: the inputs of q;k;v and gate;up (normed residual), of the o_proj
+        // (attention output) and of the down_proj (SwiGLU activation), in 8 bits.
+        opure_mx_matrix mxNorm{}, mxAttn{}, mxAct{};
     };
     // True when steps of n vectors run on opure_decode_fused.
     bool UsesFused(uint32_t n) const;
@@ -207,6 +212,8 @@ private:
     void AllocBuffers();
     void RecordStep(uint32_t n, bool logits);
     void RecordLayer(uint32_t layer, uint32_t n);
+    void RecordLayerMx(uint32_t layer, uint32_t n);
+    void RecordAttention(uint32_t layer, uint32_t n, uint32_t qkvRows, uint16_t *packed);
     void TpGemvAllreduce(const void *w, float scale, uint32_t rows, uint32_t cols, const float *in,
                          uint32_t in_stride, uint32_t n);
     // Split-K attention scratch for batch n (one zeroed buffer per batch size, so its

@@ -17,10 +17,11 @@ class EngineOptions(C.Structure):
     _fields_ = [("max_new_tokens", u32), ("max_batch", u32), ("max_len", u32), ("page_size", u32),
                 ("page_seed", u64), ("use_graphs", u32), ("attn_scale", f32), ("path", u32),
                 ("phase_trace", u32), ("prefill_chunk", u32), ("kv_window", u32),
-                ("tp_allreduce", u32)]
+                ("tp_allreduce", u32), ("weights", u32)]
 
 
 PATH_AUTO, PATH_UNFUSED, PATH_FUSED, PATH_FUSED_LAYERS = 0, 1, 2, 3
+WEIGHTS_STORED, WEIGHTS_MXFP4 = 0, 1
 TP_AUTO, TP_NCCL, TP_PEER = 0, 1, 2
 
 
@@ -29,7 +30,7 @@ class EngineInfo(C.Structure):
                 ("kv_heads", u32), ("head_dim", u32), ("max_pos", u32), ("max_len", u32),
                 ("max_batch", u32), ("page_size", u32), ("w_dtype", u32), ("weight_bytes", u64),
                 ("stream_bytes", u64), ("kv_bytes_per_token", u64), ("tp_ranks", u32),
-                ("tp_peer", u32)]
+                ("tp_peer", u32), ("weights", u32)]
 
 
 class Timing(C.Structure):
@@ -213,16 +214,17 @@ class Engine:
                  attn_scale: float = 1.0, max_new_tokens: int = 256, path: int = PATH_AUTO,
                  share: "Engine | None" = None, comm: "cuda.Comm | None" = None,
                  phase_trace: bool = False, prefill_chunk: int = 0, kv_window: int = 0,
-                 tp_allreduce: int = TP_AUTO):
+                 tp_allreduce: int = TP_AUTO, weights: int = WEIGHTS_STORED):
         """With `share`, the engine runs on that engine's ctx (stream), as the draft of a
         speculative pair must; it keeps a reference so the owner outlives it. With `comm`
         it is that communicator's tensor-parallel shard, on the communicator's ctx, whose
         all-reduces run as NCCL calls (`tp_allreduce` TP_NCCL, and TP_AUTO at 2 ranks) or
         as NVLink peer kernels (TP_PEER, and TP_AUTO at any rank count, when every pair of GPUs
-        can map each other's memory)."""
+        can map each other's memory). `weights` WEIGHTS_MXFP4 quantises the layer matrices to
+        4-bit microscaled form on upload."""
         o = EngineOptions(max_new_tokens, max_batch, max_len, page_size, page_seed,
                           int(use_graphs), attn_scale, path, int(phase_trace), prefill_chunk, kv_window,
-                          tp_allreduce)
+                          tp_allreduce, weights)
         h = C.c_void_p()
         if comm is not None:
             st = lib().opure_engine_create_tp(model_dir.encode(), comm.ctx.h, comm.h, C.byref(o), C.byref(h))
@@ -404,7 +406,8 @@ class Server:
         devs = np.ascontiguousarray(list(devices), np.int32)
         o = EngineOptions(engine_opts.get("max_new_tokens", 256), engine_opts.get("max_batch", 1),
                           engine_opts.get("max_len", 0), engine_opts.get("page_size", 64),
-                          engine_opts.get("page_seed", 3), 1, 1.0, engine_opts.get("path", PATH_AUTO), 0, 0, 0, 0)
+                          engine_opts.get("page_seed", 3), 1, 1.0, engine_opts.get("path", PATH_AUTO), 0, 0, 0, 0,
+                          engine_opts.get("weights", WEIGHTS_STORED))
         h = C.c_void_p()
         _check(lib().opure_server_start(model_dir.encode() if model_dir else None, _p(devs) if devs.size else None,
                                         int(devs.size), port, C.byref(o), C.byref(h)), "opure_server_start")
