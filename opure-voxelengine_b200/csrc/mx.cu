@@ -27,7 +27,7 @@ struct Groups {
     }
 };
 
-template <typename T, uint32_t FMT, bool VEC, uint32_t U>
+template <typename T, uint32_t FMT, uint32_t U>
 __global__ void __launch_bounds__(kThreads)
     mx_quantize_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {
     grid_dependency_wait();
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kThreads)
     for (uint32_t i = 0; i < U; ++i) {
         in[i] = groups.at(first + i * (kThreads / 8), row[i], c[i]);
         const T *p = x + size_t(row[i]) * stride + c[i];
-        if (VEC && in[i] && c[i] + 16 <= cols) {
+        if (in[i] && c[i] + 16 <= cols) {
             load16(p, raw[i]);
         } else {
             T *r = reinterpret_cast<T *>(raw[i]);
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-template <typename T, uint32_t FMT, bool VEC, uint32_t U>
+template <typename T, uint32_t FMT, uint32_t U>
 __global__ void __launch_bounds__(kThreads)
     mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, Groups groups, uint32_t cols) {
     grid_dependency_wait();
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads)
             r[2 * j + 1] = from_f32<T>(f.y * s);
         }
         T *p = y + size_t(row[i]) * stride + c[i];
-        if (VEC && c[i] + 16 <= cols) {
+        if (c[i] + 16 <= cols) {
 #pragma unroll
             for (uint32_t j = 0; j < sizeof(T) / 2; ++j)
                 stg256(reinterpret_cast<uint8_t *>(p) + 32 * j, *reinterpret_cast<const uint32_t(*)[8]>(raw + 8 * j));
@@ -138,6 +138,76 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
+// The same for rows that 32-byte accesses cannot serve (odd strides, unaligned pointers): a warp
+// takes a group, a lane one column of each of its four blocks, so that neighbouring lanes still
+// touch neighbouring values. About twice the instructions per value; reading 16 values a lane one
+// by one took 8 times as long as the bytes.
+constexpr uint32_t kGroupBlocks = 4;
+
+template <uint32_t FMT>
+__device__ __forceinline__ void narrow_store(const float (&v)[kGroupBlocks], uint8_t *codes, uint32_t *scale) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t word = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
+        const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
+        word |= byte << (8 * b);
+        const float f = v[b] * mx_inverse(byte), next = __shfl_down_sync(0xffffffffu, f, 1);
+        const float pair[8] = {f, next};
+        const uint32_t c = byte == 255u ? 0u : FMT == OPURE_MX_FP4 ? mx_pack_fp4(pair) : mx_pack_fp8(f, 0.f, 0.f, 0.f);
+        if (FMT == OPURE_MX_FP8)
+            codes[b * 32 + lane] = uint8_t(c);
+        else if (lane % 2 == 0)
+            codes[b * 16 + lane / 2] = uint8_t(c);
+    }
+    if (lane == 0) *scale = word;
+}
+
+template <typename T, uint32_t FMT>
+__global__ void __launch_bounds__(kThreads)
+    mx_quantize_narrow_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    uint32_t row, c;
+    if (!groups.at((blockIdx.x * kThreads + threadIdx.x) / 32, row, c)) return;
+    c = c / 128 * 128;
+    const T *p = x + size_t(row) * stride;
+    float v[kGroupBlocks];
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
+        const uint32_t col = c + b * 32 + (threadIdx.x & 31u);
+        v[b] = col < cols ? to_f32(p[col]) : 0.f;
+    }
+    narrow_store<FMT>(v, codes + size_t(row) * mx_row_bytes(FMT, cols) + size_t(c) * FMT / 8,
+                      reinterpret_cast<uint32_t *>(scales + mx_scale_offset(cols, row, c / kMxBlock)));
+}
+
+template <typename T, uint32_t FMT>
+__global__ void __launch_bounds__(kThreads)
+    mx_dequantize_narrow_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, Groups groups, uint32_t cols) {
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t row, c;
+    if (!groups.at((blockIdx.x * kThreads + threadIdx.x) / 32, row, c)) return;
+    c = c / 128 * 128;
+    const uint8_t *src = codes + size_t(row) * mx_row_bytes(FMT, cols) + size_t(c) * FMT / 8;
+    const uint32_t word = *reinterpret_cast<const uint32_t *>(scales + mx_scale_offset(cols, row, c / kMxBlock));
+    uint32_t code[kGroupBlocks];
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) code[b] = FMT == OPURE_MX_FP8 ? src[b * 32 + lane] : src[b * 16 + lane / 2] >> (lane % 2 * 4);
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
+        const uint32_t col = c + b * 32 + lane;
+        uint32_t h[4];
+        if constexpr (FMT == OPURE_MX_FP4)
+            mx_unpack_fp4(code[b] & 15u, h);
+        else
+            mx_unpack_fp8(code[b], h[0], h[1]);
+        if (col < cols) y[size_t(row) * stride + col] = from_f32<T>(h2f2(h[0]).x * mx_scale_value(word >> (8 * b) & 255u));
+    }
+}
+
 // ---- norm ---------------------------------------------------------------------------------
 struct NormParams {
     const void *x, *residual;
@@ -146,31 +216,48 @@ struct NormParams {
     const __half *gain;
     float eps;
     uint8_t *codes, *scales;
-    uint32_t cols;
-    bool vec, gain_vec;  // rows of x, residual and sum, and the gain, allow 16-byte accesses
+    uint32_t rows, cols;
+    bool gain_vec;  // the gain allows 16-byte accesses
 };
 
-// One CTA per row. With KEEP a thread holds its (up to KEEP) octets of s between the sum of
-// squares and the codes, so that x and residual are read once; KEEP 0, for rows longer than
-// 16384, reads them twice (the second time from L2).
-template <typename T, uint32_t FMT, uint32_t KEEP>
-__global__ void __launch_bounds__(1024) mx_rmsnorm_kernel(NormParams p) {
+// Sum over a row's threads: a warp's, or a CTA's (part: 32 floats).
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float *part) {
+    v = warp_sum(v);
+    if constexpr (!WARP) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+        for (uint32_t w = 0; w < blockDim.x / 32; ++w) v += part[w];
+    }
+    return v;
+}
+
+// One CTA per row, or (WARP) one warp per row where there are many short ones: 15007 rows of 75
+// took 16 us as that many CTAs. With KEEP a thread holds its (up to KEEP) octets of s between the
+// sum of squares and the codes, so that x and residual are read once; KEEP 0, for rows longer
+// than 16384, reads them twice (the second time from L2).
+template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
+__global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(NormParams p) {
     __shared__ float part[32];
     grid_dependency_wait();
     grid_dependents_launch();
-    const uint32_t row = blockIdx.x, cols = p.cols, kp = mx_kp(cols), step = blockDim.x * 8, c0 = threadIdx.x * 8;
+    const uint32_t width = WARP ? 32 : blockDim.x, place = WARP ? threadIdx.x & 31u : threadIdx.x;
+    const uint32_t row = WARP ? (blockIdx.x * kThreads + threadIdx.x) / 32 : blockIdx.x;
+    if (WARP && row >= p.rows) return;
+    const uint32_t cols = p.cols, kp = mx_kp(cols), step = width * 8, c0 = place * 8;
     const T *x = static_cast<const T *>(p.x) + size_t(row) * p.stride;
     const T *r = p.residual ? static_cast<const T *>(p.residual) + size_t(row) * p.stride : nullptr;
     T *sum = p.sum ? static_cast<T *>(p.sum) + size_t(row) * p.stride : nullptr;
     auto load = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
-        if (p.vec && n == 8)
+        if (n == 8)
             load8(x + c, v);
         else
             load8_part(x + c, n, v);
         if (r) {
             float t[8];
-            if (p.vec && n == 8)
+            if (n == 8)
                 load8(r + c, t);
             else
                 load8_part(r + c, n, t);
@@ -195,11 +282,7 @@ __global__ void __launch_bounds__(1024) mx_rmsnorm_kernel(NormParams p) {
             square(kept[0]);
         }
     }
-    ss = warp_sum(ss);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
-    __syncthreads();
-    ss = 0.f;
-    for (uint32_t w = 0; w < blockDim.x / 32; ++w) ss += part[w];
+    ss = row_sum<WARP>(ss, part);
     const float inv = 1.0f / sqrtf(ss / float(cols) + p.eps);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[8]) {
@@ -207,7 +290,7 @@ __global__ void __launch_bounds__(1024) mx_rmsnorm_kernel(NormParams p) {
         // sum may be x or residual: this thread alone reads and writes these columns, and it
         // has read them for the last time.
         if (sum && n) {
-            if (p.vec && n == 8)
+            if (n == 8)
                 store8(sum + c, v);
             else
                 store8_part(sum + c, n, v);
@@ -240,17 +323,61 @@ __global__ void __launch_bounds__(1024) mx_rmsnorm_kernel(NormParams p) {
     }
 }
 
-// The groups of a matrix, and how many each lane takes: two where that still fills every SM, so
-// that more loads are in flight; one in smaller calls, where latency counts.
-bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
+// Rows that 16-byte accesses cannot serve: one CTA per row, a lane one column of each block, as in
+// the narrow kernels above. x and residual are read twice (the second time from L1 or L2).
+template <typename T, uint32_t FMT>
+__global__ void __launch_bounds__(1024) mx_rmsnorm_narrow_kernel(NormParams p) {
+    __shared__ float part[32];
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const uint32_t row = blockIdx.x, cols = p.cols, kp = mx_kp(cols), lane = threadIdx.x & 31u;
+    const T *x = static_cast<const T *>(p.x) + size_t(row) * p.stride;
+    const T *r = p.residual ? static_cast<const T *>(p.residual) + size_t(row) * p.stride : nullptr;
+    T *sum = p.sum ? static_cast<T *>(p.sum) + size_t(row) * p.stride : nullptr;
+    auto at = [&](uint32_t c) { return c < cols ? to_f32(x[c]) + (r ? to_f32(r[c]) : 0.f) : 0.f; };
+    // A warp's columns: groups of 128, in both passes.
+    float ss = 0.f;
+    for (uint32_t c = threadIdx.x / 32 * 128; c < cols; c += blockDim.x * 4) {
+        float v[kGroupBlocks];
+#pragma unroll
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = at(c + b * 32 + lane);
+#pragma unroll
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) ss = fmaf(v[b], v[b], ss);
+    }
+    ss = row_sum<false>(ss, part);
+    const float inv = 1.0f / sqrtf(ss / float(cols) + p.eps);
+    uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
+    for (uint32_t c = threadIdx.x / 32 * 128; c < kp; c += blockDim.x * 4) {
+        float v[kGroupBlocks];
+#pragma unroll
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = at(c + b * 32 + lane);
+#pragma unroll
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) {
+            const uint32_t col = c + b * 32 + lane;
+            if (col < cols) {
+                // sum may be x or residual: this thread alone reads and writes this column, and it
+                // has read it for the last time.
+                if (sum) sum[col] = from_f32<T>(v[b]);
+                v[b] = v[b] * inv * (p.gain ? __half2float(p.gain[col]) : 1.f);
+            }
+        }
+        narrow_store<FMT>(v, codes + size_t(c) * FMT / 8,
+                          reinterpret_cast<uint32_t *>(p.scales + mx_scale_offset(cols, row, c / kMxBlock)));
+    }
+}
+
+// The groups of a matrix, and how many each lane of the wide kernels takes: two where that still
+// fills every SM, so that more loads are in flight; one in smaller calls, where latency counts.
+bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, bool wide, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
     g.rows = m.rows;
     g.per_row = mx_kp(m.cols) / 128;
     g.magic = g.per_row == 1 ? 0 : uint32_t(0xffffffffu / g.per_row + 1);
     const uint64_t groups = uint64_t(m.rows) * g.per_row;
     if (groups >= (uint64_t(1) << 31) - kThreads) return false;
     per_lane = groups >= uint64_t(ctx->sm_count) * 8 * kThreads / 8 ? 2 : 1;
-    blocks = ceil_div(groups * 8, kThreads * per_lane);
-    return true;
+    const uint64_t grid = wide ? (groups * 8 + kThreads * per_lane - 1) / (kThreads * per_lane) : (groups * 32 + kThreads - 1) / kThreads;
+    blocks = uint32_t(grid);
+    return grid <= 0x7fffffffu / kThreads;  // thread indices are 32-bit
 }
 bool rows_aligned32(const void *p, uint32_t type, size_t stride) {
     return reinterpret_cast<uintptr_t>(p) % 32 == 0 && stride * type_bytes(type) % 32 == 0;
@@ -281,8 +408,8 @@ opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, s
     if (!x) return OPURE_ERR_INVALID_ARG;
     Groups groups;
     uint32_t per_lane, blocks;
-    if (!make_groups(ctx, *out, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
-    const bool vec = rows_aligned32(x, x_type, x_stride);
+    const bool wide = rows_aligned32(x, x_type, x_stride);
+    if (!make_groups(ctx, *out, wide, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
     return with_type(x_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
@@ -291,8 +418,8 @@ opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, s
         };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            if (per_lane == 1) return vec ? go(mx_quantize_kernel<T, F, true, 1>) : go(mx_quantize_kernel<T, F, false, 1>);
-            return vec ? go(mx_quantize_kernel<T, F, true, 2>) : go(mx_quantize_kernel<T, F, false, 2>);
+            if (!wide) return go(mx_quantize_narrow_kernel<T, F>);
+            return per_lane == 1 ? go(mx_quantize_kernel<T, F, 1>) : go(mx_quantize_kernel<T, F, 2>);
         };
         return out->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
                                            : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
@@ -307,8 +434,8 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
     if (!y) return OPURE_ERR_INVALID_ARG;
     Groups groups;
     uint32_t per_lane, blocks;
-    if (!make_groups(ctx, *x, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
-    const bool vec = rows_aligned32(y, y_type, y_stride);
+    const bool wide = rows_aligned32(y, y_type, y_stride);
+    if (!make_groups(ctx, *x, wide, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
     return with_type(y_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
@@ -317,8 +444,8 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
         };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            if (per_lane == 1) return vec ? go(mx_dequantize_kernel<T, F, true, 1>) : go(mx_dequantize_kernel<T, F, false, 1>);
-            return vec ? go(mx_dequantize_kernel<T, F, true, 2>) : go(mx_dequantize_kernel<T, F, false, 2>);
+            if (!wide) return go(mx_dequantize_narrow_kernel<T, F>);
+            return per_lane == 1 ? go(mx_dequantize_kernel<T, F, 1>) : go(mx_dequantize_kernel<T, F, 2>);
         };
         return x->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
                                          : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
@@ -334,20 +461,29 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
     if (a->out.rows == 0) return OPURE_OK;
     if (!a->x) return OPURE_ERR_INVALID_ARG;
     if (a->out.rows > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
-    NormParams p{a->x, a->residual, a->sum, a->x_stride, reinterpret_cast<const __half *>(a->gain), a->eps,
-                 a->out.codes, a->out.scales, a->out.cols,
-                 rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
-                     rows_aligned16(a->sum, a->x_type, a->x_stride),
-                 reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
-    // A thread per 8 values up to 1024 threads, then two octets each.
+    const NormParams p{a->x, a->residual, a->sum, a->x_stride, reinterpret_cast<const __half *>(a->gain), a->eps,
+                       a->out.codes, a->out.scales, a->out.rows, a->out.cols, reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
+    const bool wide = rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
+                      rows_aligned16(a->sum, a->x_type, a->x_stride);
+    // A thread per 8 values up to 1024 threads, then two octets each; narrow rows a lane per 4. Rows
+    // of up to 512 values go one to a warp where they give every SM 8 or more: at 8 rows of 2048 a
+    // whole CTA per row has the shorter chain, and with few rows more loads in flight.
     const uint32_t octets = mx_kp(a->out.cols) / 8, keep = octets <= 1024 ? 1 : octets <= 2048 ? 2 : 0;
-    const uint32_t threads = keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
+    const uint32_t threads = !wide ? std::min(1024u, octets * 2) : keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
+    const bool warps = wide && octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
     return with_type(a->x_type, [&](auto t) {
         using T = decltype(t);
-        auto go = [&](auto kernel) { return launch(ctx, kernel, dim3(a->out.rows), dim3(threads), 0, true, p); };
+        auto go = [&](auto kernel) {
+            return warps ? launch(ctx, kernel, dim3(ceil_div(a->out.rows, kThreads / 32)), dim3(kThreads), 0, true, p)
+                         : launch(ctx, kernel, dim3(a->out.rows), dim3(threads), 0, true, p);
+        };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            return keep == 1 ? go(mx_rmsnorm_kernel<T, F, 1>) : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2>) : go(mx_rmsnorm_kernel<T, F, 0>);
+            if (!wide) return go(mx_rmsnorm_narrow_kernel<T, F>);
+            if (warps) return octets <= 32 ? go(mx_rmsnorm_kernel<T, F, 1, true>) : go(mx_rmsnorm_kernel<T, F, 2, true>);
+            return keep == 1   ? go(mx_rmsnorm_kernel<T, F, 1, false>)
+                   : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2, false>)
+                               : go(mx_rmsnorm_kernel<T, F, 0, false>);
         };
         return a->out.format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
                                              : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
