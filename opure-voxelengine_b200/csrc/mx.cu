@@ -152,16 +152,31 @@ __device__ __forceinline__ void narrow_store(const float (&v)[kGroupBlocks], uin
     for (uint32_t b = 0; b < kGroupBlocks; ++b) {
         const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
         word |= byte << (8 * b);
-        const float f = v[b] * mx_inverse(byte), next = __shfl_down_sync(0xffffffffu, f, 1);
-        const float pair[8] = {f, next};
-        const uint32_t c = byte == 255u ? 0u : FMT == OPURE_MX_FP4 ? mx_pack_fp4(pair) : mx_pack_fp8(f, 0.f, 0.f, 0.f);
-        if (FMT == OPURE_MX_FP8)
-            codes[b * 32 + lane] = uint8_t(c);
-        else if (lane % 2 == 0)
-            codes[b * 16 + lane / 2] = uint8_t(c);
+        const float f = v[b] * mx_inverse(byte);
+        if constexpr (FMT == OPURE_MX_FP8) {
+            const uint32_t c = mx_pack_fp8(f);
+            codes[b * 32 + lane] = uint8_t(byte == 255u ? 0u : c);
+        } else {
+            const uint32_t c = mx_pack_fp4(f, __shfl_down_sync(0xffffffffu, f, 1));
+            if (lane % 2 == 0) codes[b * 16 + lane / 2] = uint8_t(byte == 255u ? 0u : c);
+        }
     }
     if (lane == 0) *scale = word;
 }
+
+// A lane's four columns of a group (p at the lane's first one; `left` columns from there on).
+template <typename T>
+__device__ __forceinline__ void narrow_load(const T *p, uint32_t left, float (&v)[kGroupBlocks]) {
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = b * 32 < left ? to_f32(p[b * 32]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void narrow_write(T *p, uint32_t left, const float (&v)[kGroupBlocks]) {
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b)
+        if (b * 32 < left) p[b * 32] = from_f32<T>(v[b]);
+}
+__device__ __forceinline__ uint32_t columns_left(uint32_t cols, uint32_t first) { return first < cols ? cols - first : 0u; }
 
 template <typename T, uint32_t FMT>
 __global__ void __launch_bounds__(kThreads)
@@ -171,13 +186,9 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t row, c;
     if (!groups.at((blockIdx.x * kThreads + threadIdx.x) / 32, row, c)) return;
     c = c / 128 * 128;
-    const T *p = x + size_t(row) * stride;
+    const uint32_t first = c + (threadIdx.x & 31u);
     float v[kGroupBlocks];
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-        const uint32_t col = c + b * 32 + (threadIdx.x & 31u);
-        v[b] = col < cols ? to_f32(p[col]) : 0.f;
-    }
+    narrow_load(x + size_t(row) * stride + first, columns_left(cols, first), v);
     narrow_store<FMT>(v, codes + size_t(row) * mx_row_bytes(FMT, cols) + size_t(c) * FMT / 8,
                       reinterpret_cast<uint32_t *>(scales + mx_scale_offset(cols, row, c / kMxBlock)));
 }
@@ -196,16 +207,13 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t code[kGroupBlocks];
 #pragma unroll
     for (uint32_t b = 0; b < kGroupBlocks; ++b) code[b] = FMT == OPURE_MX_FP8 ? src[b * 32 + lane] : src[b * 16 + lane / 2] >> (lane % 2 * 4);
+    float v[kGroupBlocks];
 #pragma unroll
     for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-        const uint32_t col = c + b * 32 + lane;
-        uint32_t h[4];
-        if constexpr (FMT == OPURE_MX_FP4)
-            mx_unpack_fp4(code[b] & 15u, h);
-        else
-            mx_unpack_fp8(code[b], h[0], h[1]);
-        if (col < cols) y[size_t(row) * stride + col] = from_f32<T>(h2f2(h[0]).x * mx_scale_value(word >> (8 * b) & 255u));
+        const uint32_t h = FMT == OPURE_MX_FP4 ? mx_unpack_fp4_pair(code[b] & 15u) : mx_unpack_fp8_pair(code[b]);
+        v[b] = h2f2(h).x * mx_scale_value(word >> (8 * b) & 255u);
     }
+    narrow_write(y + size_t(row) * stride + c + lane, columns_left(cols, c + lane), v);
 }
 
 // ---- norm ---------------------------------------------------------------------------------
@@ -323,46 +331,74 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
     }
 }
 
-// Rows that 16-byte accesses cannot serve: one CTA per row, a lane one column of each block, as in
-// the narrow kernels above. x and residual are read twice (the second time from L1 or L2).
-template <typename T, uint32_t FMT>
-__global__ void __launch_bounds__(1024) mx_rmsnorm_narrow_kernel(NormParams p) {
+// Rows that 16-byte accesses cannot serve: a lane one column of each block, as in the narrow
+// kernels above; one CTA per row, or (WARP) one warp. With KEEP a warp holds its (up to KEEP) groups
+// of s; KEEP 0, for rows longer than 16384, reads x and residual twice.
+template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
+__global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kernel(NormParams p) {
     __shared__ float part[32];
     grid_dependency_wait();
     grid_dependents_launch();
-    const uint32_t row = blockIdx.x, cols = p.cols, kp = mx_kp(cols), lane = threadIdx.x & 31u;
-    const T *x = static_cast<const T *>(p.x) + size_t(row) * p.stride;
-    const T *r = p.residual ? static_cast<const T *>(p.residual) + size_t(row) * p.stride : nullptr;
-    T *sum = p.sum ? static_cast<T *>(p.sum) + size_t(row) * p.stride : nullptr;
-    auto at = [&](uint32_t c) { return c < cols ? to_f32(x[c]) + (r ? to_f32(r[c]) : 0.f) : 0.f; };
-    // A warp's columns: groups of 128, in both passes.
-    float ss = 0.f;
-    for (uint32_t c = threadIdx.x / 32 * 128; c < cols; c += blockDim.x * 4) {
-        float v[kGroupBlocks];
+    const uint32_t row = WARP ? (blockIdx.x * kThreads + threadIdx.x) / 32 : blockIdx.x;
+    if (WARP && row >= p.rows) return;
+    const uint32_t cols = p.cols, kp = mx_kp(cols), lane = threadIdx.x & 31u;
+    const uint32_t first = WARP ? 0 : threadIdx.x / 32 * 128, step = WARP ? 128 : blockDim.x * 4;  // a warp's groups
+    const size_t base = size_t(row) * p.stride + lane;
+    const T *x = static_cast<const T *>(p.x) + base, *r = static_cast<const T *>(p.residual) + base;
+    T *sum = static_cast<T *>(p.sum) + base;
+    auto load = [&](uint32_t c, float (&v)[kGroupBlocks]) {
+        const uint32_t left = columns_left(cols, c + lane);
+        narrow_load(x + c, left, v);
+        if (p.residual) {
+            float t[kGroupBlocks];
+            narrow_load(r + c, left, t);
 #pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = at(c + b * 32 + lane);
+            for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] += t[b];
+        }
+    };
+    float ss = 0.f;
+    auto square = [&](const float (&v)[kGroupBlocks]) {
 #pragma unroll
         for (uint32_t b = 0; b < kGroupBlocks; ++b) ss = fmaf(v[b], v[b], ss);
+    };
+    float kept[KEEP ? KEEP : 1][kGroupBlocks];
+    if constexpr (KEEP > 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < KEEP; ++i)
+            if (first + i * step < kp) load(first + i * step, kept[i]);
+#pragma unroll
+        for (uint32_t i = 0; i < KEEP; ++i)
+            if (first + i * step < kp) square(kept[i]);
+    } else {
+        for (uint32_t c = first; c < kp; c += step) {
+            load(c, kept[0]);
+            square(kept[0]);
+        }
     }
-    ss = row_sum<false>(ss, part);
+    ss = row_sum<WARP>(ss, part);
     const float inv = 1.0f / sqrtf(ss / float(cols) + p.eps);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
-    for (uint32_t c = threadIdx.x / 32 * 128; c < kp; c += blockDim.x * 4) {
-        float v[kGroupBlocks];
+    auto finish = [&](uint32_t c, float (&v)[kGroupBlocks]) {
+        const uint32_t left = columns_left(cols, c + lane);
+        // sum may be x or residual: this thread alone reads and writes these columns, and it has
+        // read them for the last time.
+        if (p.sum) narrow_write(sum + c, left, v);
+        float g[kGroupBlocks] = {1.f, 1.f, 1.f, 1.f};
+        if (p.gain) narrow_load(p.gain + c + lane, left, g);
 #pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = at(c + b * 32 + lane);
-#pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-            const uint32_t col = c + b * 32 + lane;
-            if (col < cols) {
-                // sum may be x or residual: this thread alone reads and writes this column, and it
-                // has read it for the last time.
-                if (sum) sum[col] = from_f32<T>(v[b]);
-                v[b] = v[b] * inv * (p.gain ? __half2float(p.gain[col]) : 1.f);
-            }
-        }
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = v[b] * inv * g[b];
         narrow_store<FMT>(v, codes + size_t(c) * FMT / 8,
                           reinterpret_cast<uint32_t *>(p.scales + mx_scale_offset(cols, row, c / kMxBlock)));
+    };
+    if constexpr (KEEP > 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < KEEP; ++i)
+            if (first + i * step < kp) finish(first + i * step, kept[i]);
+    } else {
+        for (uint32_t c = first; c < kp; c += step) {
+            load(c, kept[0]);
+            finish(c, kept[0]);
+        }
     }
 }
 
@@ -465,12 +501,16 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
                        a->out.codes, a->out.scales, a->out.rows, a->out.cols, reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
     const bool wide = rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
                       rows_aligned16(a->sum, a->x_type, a->x_stride);
-    // A thread per 8 values up to 1024 threads, then two octets each; narrow rows a lane per 4. Rows
-    // of up to 512 values go one to a warp where they give every SM 8 or more: at 8 rows of 2048 a
-    // whole CTA per row has the shorter chain, and with few rows more loads in flight.
-    const uint32_t octets = mx_kp(a->out.cols) / 8, keep = octets <= 1024 ? 1 : octets <= 2048 ? 2 : 0;
-    const uint32_t threads = !wide ? std::min(1024u, octets * 2) : keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
-    const bool warps = wide && octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
+    // A thread per 8 values up to 1024 threads, then two octets each; narrow rows a warp per 128
+    // values up to 8 warps, then up to four groups each. Rows of up to 512 values go one to a warp
+    // where that gives every SM 8 or more; fewer or longer ones have a CTA each, for more loads in
+    // flight.
+    const uint32_t octets = mx_kp(a->out.cols) / 8, groups = octets / 16;
+    const uint32_t keep = octets <= 1024 ? 1 : octets <= 2048 ? 2 : 0;
+    const uint32_t threads = !wide  ? 32 * std::min(32u, std::max(std::min(groups, 8u), ceil_div(groups, 4)))
+                             : keep ? (ceil_div(octets, keep) + 31) / 32 * 32
+                                    : 1024;
+    const bool warps = octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
     return with_type(a->x_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
@@ -479,7 +519,10 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
         };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            if (!wide) return go(mx_rmsnorm_narrow_kernel<T, F>);
+            if (!wide)
+                return warps  ? go(mx_rmsnorm_narrow_kernel<T, F, 4, true>)
+                       : keep ? go(mx_rmsnorm_narrow_kernel<T, F, 4, false>)
+                              : go(mx_rmsnorm_narrow_kernel<T, F, 0, false>);
             if (warps) return octets <= 32 ? go(mx_rmsnorm_kernel<T, F, 1, true>) : go(mx_rmsnorm_kernel<T, F, 2, true>);
             return keep == 1   ? go(mx_rmsnorm_kernel<T, F, 1, false>)
                    : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2, false>)
