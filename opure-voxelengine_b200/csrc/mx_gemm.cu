@@ -11,9 +11,12 @@
 //     columns a stage (codes by tiled TMA, scale tiles by bulk copies) into a ring of
 //     shared-memory stages; warp 1 copies the scale tiles to TMEM and issues the MMAs. A K
 //     split is a thread-block cluster whose CTAs share the epilogue: each sends its sums to the
-//     CTAs that finish them (st.async, counted by the receiver's mbarrier; nobody waits for a
-//     reader), which add the splits in rank order, so that results do not depend on timing. In
-//     SwiGLU a tile is 64 gate rows and the 64 up rows that go with them.
+//     CTAs that finish them (counted by the receiver's mbarrier), which add the splits in rank
+//     order, so that results do not depend on timing. Few tokens' sums go from registers
+//     (st.async); many are laid out in shared memory and go as one bulk copy per receiver, which
+//     is several times as fast per byte but needs a cluster barrier before a CTA may leave
+//     (8 splits of 64 tokens: 9.3 us against 11.2; of 3 tokens: 6.9 against 6.1). In SwiGLU a
+//     tile is 64 gate rows and the 64 up rows that go with them.
 // All waits are bounded (1 s); a timeout is reported in the ctx status word.
 #include <algorithm>
 #include <type_traits>
@@ -29,6 +32,7 @@ constexpr uint32_t kK = 128;       // columns per stage: one 128-byte swizzled r
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxStages = 10;
 constexpr uint32_t kMaxSplits = 8;  // portable cluster size
+constexpr uint32_t kDirect = 16;    // tokens whose sums go straight from registers
 constexpr uint32_t kPrefetch = 8;   // stages of weights that are asked for ahead
 constexpr uint32_t kBBytes = kN * kK;
 constexpr uint32_t kScaleBytes = 2048;  // per stage: x tile, w (or gate) tile, up tile; keeps 1 KB alignment
@@ -43,7 +47,8 @@ struct GemmParams {
     uint32_t n, rows, kblocks, splits, stages;
     uint32_t a_rows;              // token rows that a stage holds: multiple of 8, at most 128
     uint32_t half;                // SwiGLU: first up row = result columns
-    uint32_t sums_offset;         // of the received sums from the ring's start; 0: in its place
+    uint32_t sums_offset;         // of the received sums from the ring's start
+    bool apart;                   // they are past the ring
     bool vec;                     // rows of y and residual allow accesses of 4 values
     uint32_t x_format;
     void *y;
@@ -79,14 +84,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto b_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes; };
     auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes; };
     auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
-    // Results in units of 4 tokens x 32 columns. Unit u is finished by CTA u % splits, whose
-    // sums[u / splits][split][side] receive every split's part: past the ring where there is room,
-    // else in its place, and the splits wait for one another before they send. A token's eight
-    // pieces of 16 bytes stand in an order of its own (piece ^ token % 8), so that 32 tokens'
-    // stores spread over all banks.
-    uint8_t *sums = base + p.sums_offset;
+    // Results in units of 4 tokens x 32 columns (and 2 sides in SwiGLU). Unit u is finished by CTA
+    // u % splits, as its unit u / splits. Every CTA lays its sums out by receiver (`mine`, in the
+    // ring's place) and sends each its part, which arrives in that one's `sums`, one part per split:
+    // past the ring where there is room, else after `mine`, and the splits wait for one another
+    // before they send. Without splits sums is mine. A token's eight pieces of 16 bytes stand in an
+    // order of its own (piece ^ token % 8), so that 32 tokens' stores spread over all banks.
+    uint8_t *mine = base, *sums = base + p.sums_offset;
     const uint32_t n = min(p.n - m0, kM), units = (n + 3) / 4 * kChunks;
     const uint32_t own_units = (units + p.splits - 1 - split) / p.splits;
+    const uint32_t part_bytes = (units + p.splits - 1) / p.splits * kSides * kUnit;  // room per split
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < p.stages; ++s) {
@@ -95,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         mbar_init(&done, 1);
         mbar_init(&recv, 1);
-        mbar_expect_tx(&recv, own_units * p.splits * kSides * kUnit);
+        if (p.splits > 1) mbar_expect_tx(&recv, own_units * p.splits * kSides * kUnit);
         fail = 0;
         issued_s[0] = issued_s[1] = consumed_s = 0;
         tc::prefetch_map(&wmap);
@@ -114,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (kSwiglu) tc::prefetch_2d(one, &wmap, (kb0 + i) * kK, p.half + r0);
         }
     }
-    if (p.splits > 1 && p.sums_offset) tc::cluster_arrive();  // this CTA can receive
+    if (p.splits > 1 && p.apart) tc::cluster_arrive();  // this CTA can receive
     grid_dependency_wait();
     grid_dependents_launch();
 
@@ -196,12 +203,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (failed && threadIdx.x == 0)  // leave no copy in flight into this CTA's shared memory
         for (uint32_t i = consumed_s; i < max(issued_s[0], issued_s[1]); ++i) mbar_wait(&full[i % p.stages], (i / p.stages) & 1u);
 
-    // Accumulators -> the CTAs that finish them. Warps w and w + 4 share TMEM lanes 32 (w % 4) ..
+    // Accumulators -> `mine`, or to the receivers. Warps w and w + 4 share TMEM lanes 32 (w % 4) ..
     // (tokens); each takes half of the columns.
-    if (p.splits > 1) {
-        if (!p.sums_offset) tc::cluster_arrive();
-        tc::cluster_wait();
-    }
+    const bool direct = p.splits > 1 && n <= kDirect;
+    if (p.splits > 1 && !p.apart) tc::cluster_arrive();
+    if (direct) tc::cluster_wait();
     const uint32_t quarter = warp & 3u, part = warp >> 2, token = quarter * 32 + lane;
     if (!failed && quarter * 32 < n) {
 #pragma unroll
@@ -210,17 +216,43 @@ __global__ void __launch_bounds__(kThreads, 2)
             tc::ld32(tmem + ((quarter * 32) << 16) + part * (kN / 2) + c * 32, r);
             tc::wait_ld();
             if (token < (n + 3) / 4 * 4) {
-                const uint32_t u = token / 4 * kChunks + (kSwiglu ? c : part * 2 + c);
-                const uint32_t at = ((u / p.splits * p.splits + split) * kSides + (kSwiglu ? part : 0)) * kUnit + token % 4 * 128;
-                const uint32_t dst = tc::map_rank(smem_addr(sums + at), u % p.splits);
-                const uint32_t bar = tc::map_rank(smem_addr(&recv), u % p.splits);
+                const uint32_t u = token / 4 * kChunks + (kSwiglu ? c : part * 2 + c), to = u % p.splits;
+                const uint32_t at = (u / p.splits * kSides + (kSwiglu ? part : 0)) * kUnit + token % 4 * 128;
+                if (direct) {
+                    const uint32_t dst = tc::map_rank(smem_addr(sums + split * part_bytes + at), to), bar = tc::map_rank(smem_addr(&recv), to);
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) tc::st_async_f4(dst + ((j ^ (lane & 7u)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3], bar);
+                    for (uint32_t j = 0; j < 8; ++j)
+                        tc::st_async_f4(dst + ((j ^ (lane & 7u)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3], bar);
+                } else {
+                    uint8_t *dst = mine + to * part_bytes + at;
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j)
+                        *reinterpret_cast<uint4 *>(dst + ((j ^ (lane & 7u)) << 4)) =
+                            make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+                }
             }
         }
     }
-    const bool got = mbar_wait(&recv, 0);
-    if (!got && threadIdx.x == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 83, blockIdx.x);
+    bool got = !failed;
+    if (!direct) {
+        tc::fence_async_shared();
+        __syncthreads();
+    }
+    if (p.splits > 1) {
+        if (!direct) {
+            tc::cluster_wait();
+            if (!failed && threadIdx.x < p.splits) {
+                const uint32_t to = threadIdx.x, bytes = (units + p.splits - 1 - to) / p.splits * kSides * kUnit;
+                if (bytes)
+                    tc::bulk_send(tc::map_rank(smem_addr(sums + split * part_bytes), to), mine + to * part_bytes, bytes,
+                                  tc::map_rank(smem_addr(&recv), to));
+            }
+        }
+        got = mbar_wait(&recv, 0);
+        if (!got && threadIdx.x == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 83, blockIdx.x);
+        got = __all_sync(0xffffffffu, got);
+        if (!direct) tc::cluster_arrive();  // has all that was sent to it
+    }
 
     // Epilogue: a warp takes a unit, a lane 4 columns of a token.
     for (uint32_t l = warp; got && l < own_units; l += kThreads / 32) {
@@ -233,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (q >= p.splits) break;
 #pragma unroll
             for (uint32_t s = 0; s < kSides; ++s) {
-                const float4 f = lds_f4(reinterpret_cast<const float *>(sums + ((l * p.splits + q) * kSides + s) * kUnit + piece));
+                const float4 f = lds_f4(reinterpret_cast<const float *>(sums + q * part_bytes + (l * kSides + s) * kUnit + piece));
                 v[s][0] += f.x; v[s][1] += f.y; v[s][2] += f.z; v[s][3] += f.w;
             }
         }
@@ -254,9 +286,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc::fence_before();
     __syncthreads();
     if (warp == 2) tc::dealloc(tmem, kTmemCols);
-    // Nobody reads another CTA's memory, so a CTA may leave when it has all of its sums. One that
-    // gave up waiting stays until the others have left or gave up too: they may still send.
-    if (!got) tc::cluster_sync();
+    // A CTA leaves when what it sent by bulk copies has arrived (or its receiver gave up). Registers
+    // need no such wait, unless this CTA gave up: then the others may still send to it.
+    if (p.splits > 1 && !direct) tc::cluster_wait();
+    if (direct && !__syncthreads_and(got)) tc::cluster_sync();
 }
 
 // Scale tiles of the two halves of a matrix, each as a matrix of its own, one after the other:
@@ -275,6 +308,24 @@ __global__ void __launch_bounds__(256) mx_split_scales_kernel(const uint8_t *src
 }
 
 // ---- host -------------------------------------------------------------------------------
+// K splits, at most one CTA per SM, by the least estimated time (returned, in ns). Measured on one
+// B200: a stage takes 270 ns (SwiGLU, with twice the MMAs, 400), launch, first loads and a plain
+// epilogue 6 us, SwiGLU's 9; joining splits 1 us and, as all SMs exchange more sums, up to 8 us more
+// for 128 tokens on every SM. CTAs go two to an SM.
+uint64_t choose_splits(GemmParams &p, uint64_t tiles, bool swiglu, uint32_t sms) {
+    const uint64_t waves = (tiles + 2 * sms - 1) / (2 * sms), n = std::min(p.n, kM), stage = swiglu ? 400 : 270;
+    uint64_t best = ~uint64_t(0);
+    for (uint32_t s = 1; s == 1 || (s <= std::min(kMaxSplits, p.kblocks) && s * tiles <= sms); ++s) {
+        const uint64_t ctas = s * tiles, join = s > 1 ? 1000 + n * ctas * ctas * 8000 / (uint64_t(kM) * sms * sms) : 0;
+        const uint64_t ns = 4000 + waves * (ceil_div(p.kblocks, s) * stage + (swiglu ? 5000 : 2000) + join);
+        if (ns < best) {
+            best = ns;
+            p.splits = s;
+        }
+    }
+    return best;
+}
+
 template <int EPI, typename T>
 opure_status launch_gemm(opure_ctx *ctx, const CUtensorMap &wm, const CUtensorMap &xm, const GemmParams &p, uint32_t tiles,
                          size_t smem) {
@@ -340,28 +391,28 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     if (p.n > 65535u * kM) return OPURE_ERR_UNSUPPORTED;
     const uint32_t tiles = swiglu ? mx_kp(p.half) / (kN / 2) : ceil_div(p.rows, kN);
     const uint32_t mtiles = ceil_div(p.n, kM);
-    // As many K splits as fill the SMs once.
-    p.splits = std::max(1u, std::min({kMaxSplits, p.kblocks, uint32_t(ctx->sm_count) / std::max(1u, tiles * mtiles)}));
+    const uint64_t here_ns = choose_splits(p, uint64_t(tiles) * mtiles, swiglu, uint32_t(ctx->sm_count));
     p.a_rows = std::min(kM, (p.n + 7) & ~7u);
     const uint32_t stage_bytes = kBBytes + kScaleBytes + p.a_rows * kK;
-    // Before the ring 1 KB to align it, after it the rest of the last stage's 128 rows of A and the
-    // received sums; these take the ring's place where they would leave it less than 4 stages (or
-    // all that it needs) or there are no splits.
+    // Before the ring 1 KB to align it, after it the rest of the last stage's 128 rows of A and, where
+    // that leaves the ring 4 stages or all that it needs, the received sums; else these and the sums
+    // to send take the ring's place.
     const uint32_t chunks = swiglu ? kN / 64 : kN / 32, units = ceil_div(std::min(p.n, kM), 4) * chunks;
     const size_t sums = size_t(ceil_div(units, p.splits)) * p.splits * (swiglu ? 2 : 1) * kUnit;
     const size_t rest = size_t(kM - p.a_rows) * kK;
     // Two CTAs per SM (TMEM's 512 columns allow it and, above 75 KB each, no third), so that the
     // next kernel's CTAs set up while this one's work: a chain of 8-token 8192 -> 2048 products
-    // took 5.8 us a call with half of the shared memory each, 9.7 us with all of it.
+    // took 5.8 us a call with half of the shared memory each, 9.7 us with all of it. Only the sums
+    // of more than 100 tokens with splits need more than half.
     auto stages_in = [&](size_t bytes) {
         return std::min<uint32_t>({kMaxStages, uint32_t((bytes - 1024 - rest) / stage_bytes), ceil_div(p.kblocks, p.splits)});
     };
     p.stages = stages_in(kHalfSmem);
-    if (p.splits > 1 && sums < kHalfSmem / 2 && stages_in(kHalfSmem - sums) >= std::min(4u, p.stages)) {
-        p.stages = stages_in(kHalfSmem - sums);
-        p.sums_offset = p.stages * stage_bytes + uint32_t(rest);
-    }
-    const size_t smem = std::max<size_t>({1024 + p.stages * stage_bytes + rest, 1024 + p.sums_offset + sums, 80 * 1024});
+    p.apart = p.splits > 1 && sums < kHalfSmem / 2 && stages_in(kHalfSmem - sums) >= std::min(4u, p.stages);
+    if (p.apart) p.stages = stages_in(kHalfSmem - sums);
+    const size_t ring = p.stages * stage_bytes + rest;
+    p.sums_offset = p.splits == 1 ? 0 : uint32_t(p.apart ? std::max(ring, sums) : sums);
+    const size_t smem = std::max<size_t>({1024 + ring, 1024 + p.sums_offset + sums, 80 * 1024});
     p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
     if (swiglu) {
         const size_t side = opure_mx_scale_bytes(p.half, a->w.cols);
@@ -376,7 +427,7 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
         p.us = p.ws + side;
     }
     if (mx_gemv_suits(a)) return mx_gemv(ctx, a, p.ws, p.us);
-    if (mx_gemm_pair_suits(ctx, a)) return mx_gemm_pair(ctx, a, p.ws);
+    if (mx_gemm_pair_ns(ctx, a) < here_ns) return mx_gemm_pair(ctx, a, p.ws);
     CUtensorMap wm, xm;
     if (!make_slot_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_slot_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;
     if (swiglu)

@@ -78,7 +78,7 @@ inline bool make_slot_map(CUtensorMap *m, const opure_mx_matrix &a, uint32_t box
 
 // The product over pairs of SMs, for many tokens (a already validated; w_scales the scale tiles
 // of w, in SwiGLU those of its gate half followed by those of its up half).
-bool mx_gemm_pair_suits(const opure_ctx *ctx, const opure_mx_gemm_args *a);
+uint64_t mx_gemm_pair_ns(const opure_ctx *ctx, const opure_mx_gemm_args *a);  // estimated time
 opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *w_scales);
 
 // The product for one or two tokens, weights streamed through registers (a already validated; ws and us the

@@ -400,10 +400,11 @@ bool make_map(CUtensorMap *m, CUtensorMapDataType type, uint32_t rank, const voi
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool mx_gemm_pair_suits(const opure_ctx *ctx, const opure_mx_gemm_args *a) {
-    const bool swiglu = a->epilogue == OPURE_EPI_SWIGLU;
-    const uint64_t ntiles = swiglu ? mx_kp(a->w.rows / 2) / kHalf : (uint64_t(a->w.rows) + kTile - 1) / kTile;
-    return a->x.rows > kHalf && (uint64_t(a->x.rows) + kTile - 1) / kTile * ntiles * 4 >= uint32_t(ctx->sm_count);
+uint64_t mx_gemm_pair_ns(const opure_ctx *ctx, const opure_mx_gemm_args *a) {
+    const uint64_t ntiles = a->epilogue == OPURE_EPI_SWIGLU ? mx_kp(a->w.rows / 2) / kHalf : (uint64_t(a->w.rows) + kTile - 1) / kTile;
+    const uint64_t tiles = (uint64_t(a->x.rows) + kTile - 1) / kTile * ntiles, pairs = uint64_t(ctx->sm_count) / 2;
+    const uint64_t stages = ceil_div(mx_kp(a->w.cols), a->x.format == OPURE_MX_FP8 ? 128 : 256);
+    return a->x.rows <= kHalf ? ~uint64_t(0) : 4300 + (tiles + pairs - 1) / pairs * (stages * 360 + 1000);
 }
 
 opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *w_scales) {

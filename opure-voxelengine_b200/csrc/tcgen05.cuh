@@ -235,6 +235,13 @@ __device__ __forceinline__ void st_async_f4(uint32_t addr, uint32_t a, uint32_t 
                  "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar)
                  : "memory");
 }
+// Shared memory to a CTA of the cluster (cluster addresses), counted by an mbarrier there. The
+// source has to stay until the receiver has counted it.
+__device__ __forceinline__ void bulk_send(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "r"(smem_addr(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 
 }  // namespace tc
 }  // namespace opure
