@@ -176,8 +176,6 @@ __device__ __forceinline__ void narrow_write(T *p, uint32_t left, const float (&
     for (uint32_t b = 0; b < kGroupBlocks; ++b)
         if (b * 32 < left) p[b * 32] = from_f32<T>(v[b]);
 }
-__device__ __forceinline__ uint32_t columns_left(uint32_t cols, uint32_t first) { return first < cols ? cols - first : 0u; }
-
 template <typename T, uint32_t FMT>
 __global__ void __launch_bounds__(kThreads)
     mx_quantize_narrow_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {

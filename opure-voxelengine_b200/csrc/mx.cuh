@@ -22,6 +22,8 @@ __host__ __device__ __forceinline__ size_t mx_scale_offset(uint32_t cols, uint32
            block % 4;
 }
 
+__device__ __forceinline__ uint32_t columns_left(uint32_t cols, uint32_t first) { return first < cols ? cols - first : 0u; }
+
 // The scale byte of a block from the largest magnitude's bits. Magnitudes compare as
 // integers, so a NaN or infinity in the block is the largest and gives 255.
 template <uint32_t FMT>

@@ -15,8 +15,9 @@
 //            next is computed. TMEM's 512 columns hold two of 256 and 128 of scales by letting
 //            the two overlap by 128 columns, which are read first; then the next tile may begin.
 //
-// Results go through shared memory: whole rows of 128 bytes that TMA stores, or, where y's
-// alignment or the residual forbids it, 32 columns of a row at a time by a warp. In SwiGLU the
+// Results go through shared memory, a slab of 32 tokens x 128 bytes at a time, which TMA stores, or,
+// where y's alignment forbids that, a warp row by row. The residual comes into the slab by the same
+// ways, the first two slabs of a tile while its products still run. In SwiGLU the
 // even CTA holds gate rows and the odd CTA the up rows that go with them; a thread owns a token's
 // 32 columns, which is a block of the MX result.
 #include <cudaTypedefs.h>
@@ -32,15 +33,16 @@ namespace {
 
 constexpr uint32_t kTile = 256;    // tokens and weight rows per tile
 constexpr uint32_t kHalf = 128;    // of each, per CTA
-constexpr uint32_t kStages = 5;
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kEpiWarp = 4, kEpiWarps = 8;
 constexpr uint32_t kOperand = kHalf * 128;  // bytes of a CTA's part of one operand of a stage
-constexpr uint32_t kSlab = 4096;            // result staging per warp: 32 rows of 128 bytes
+constexpr uint32_t kSlab = 4096;            // 32 rows of 128 bytes
 constexpr uint32_t kTmemCols = 512, kAcc1 = 128, kScaleCol = 384;  // accumulator 0 starts at column 0
 
-template <uint32_t XF>
+template <uint32_t XF, int EPI>
 struct Shape {
+    // Slabs per warp (two where residuals are fetched ahead), and the stages that leaves room for.
+    static constexpr uint32_t kSlabs = EPI == OPURE_EPI_ADD ? 2 : 1, kStages = EPI == OPURE_EPI_ADD ? 4 : 5;
     static constexpr uint32_t kBlocks = XF == OPURE_MX_FP8 ? 1 : 2;  // scale tiles (128 columns) per stage
     static constexpr uint32_t kScaleBytes = kBlocks * 3 * kMxTileBytes;
     static constexpr uint32_t kStageBytes = 2 * kOperand + kScaleBytes;
@@ -50,7 +52,8 @@ struct Shape {
     static_assert(kStages * kScaleCols <= kTmemCols - kScaleCol, "TMEM columns");
     // Bytes that arrive per CTA and stage; a copy that spreads codes counts what it reads.
     static constexpr uint32_t kTx = kOperand + (XF == OPURE_MX_FP8 ? kOperand / 2 : kOperand) + kScaleBytes;
-    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStageBytes + kEpiWarps * kSlab;
+    static constexpr size_t kSmem = 1024 + size_t(kStages) * kStageBytes + kEpiWarps * kSlabs * kSlab;
+    static_assert(kSmem <= 226 * 1024, "shared memory");
 };
 
 struct PairParams {
@@ -59,7 +62,7 @@ struct PairParams {
     size_t y_stride;
     const void *residual;
     uint8_t *out, *outs;
-    bool tma_store;
+    bool tma, words;  // rows of y and residual: 16-byte aligned (TMA); 4-byte aligned
     DeviceStatus *st;
 };
 
@@ -107,12 +110,13 @@ template <uint32_t XF, int EPI, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                         const __grid_constant__ CUtensorMap wsmap, const __grid_constant__ CUtensorMap xsmap,
-                        const __grid_constant__ CUtensorMap ymap, PairParams p) {
-    using S = Shape<XF>;
+                        const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap rmap, PairParams p) {
+    using S = Shape<XF, EPI>;
+    constexpr uint32_t kStages = S::kStages;
     constexpr bool kSwiglu = EPI == OPURE_EPI_SWIGLU;
     constexpr uint32_t kResult = kSwiglu ? kHalf : kTile;  // result columns per tile
     extern __shared__ uint8_t dsm[];
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], drained;
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], drained, fetched[kEpiWarps][2];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int fail;
 
@@ -122,7 +126,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto a_tile = [&](uint32_t s) { return base + s * 2 * kOperand; };
     auto b_tile = [&](uint32_t s) { return base + s * 2 * kOperand + kOperand; };
     uint8_t *slabs = base + kStages * 2 * kOperand;
-    auto sf_tile = [&](uint32_t s) { return slabs + kEpiWarps * kSlab + s * S::kScaleBytes; };
+    auto sf_tile = [&](uint32_t s) { return slabs + kEpiWarps * S::kSlabs * kSlab + s * S::kScaleBytes; };
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
@@ -132,6 +136,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         mbar_init(&acc_full[0], 1);
         mbar_init(&acc_full[1], 1);
         mbar_init(&drained, 2 * kEpiWarps);
+        for (uint32_t w = 0; w < kEpiWarps; ++w) {
+            mbar_init(&fetched[w][0], 1);
+            mbar_init(&fetched[w][1], 1);
+        }
         fail = 0;
         tc::prefetch_map(&wmap);
         tc::prefetch_map(&xmap);
@@ -234,13 +242,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else if (warp >= kEpiWarp) {
         const uint32_t quarter = warp & 3u, part = (warp - kEpiWarp) >> 2;  // TMEM lanes, 64 columns of either half
         const uint32_t drain_bar = tc::map_rank(smem_addr(&drained), 0);
-        uint8_t *slab = slabs + (warp - kEpiWarp) * kSlab;
+        uint8_t *slab0 = slabs + (warp - kEpiWarp) * S::kSlabs * kSlab;
+        uint32_t fetch_phase[2] = {0, 0};
         uint32_t lt = 0;
         for (uint32_t t = first; t < tiles; t += pairs, ++lt) {
             const uint32_t b = lt & 1u;
             const uint32_t row0 = t % p.mtiles * kTile + rank * kHalf + quarter * 32, row = row0 + lane;
             const uint32_t r0 = t / p.mtiles * kResult;
             const uint32_t acc = tmem + b * kAcc1 + ((quarter * 32) << 16);
+            const uint32_t shared_side = b ? 0 : kHalf, other_side = kHalf - shared_side, c0 = part * 64;
+            // Without SwiGLU: this warp's 128 columns in steps of a slab, the shared ones first.
+            constexpr uint32_t kCols = kSwiglu ? 64 : 128 / sizeof(T), kSteps = 128 / kCols;
+            auto step_col = [&](uint32_t step) {
+                return (step < kSteps / 2 ? shared_side : other_side) + c0 + step % (kSteps / 2) * kCols;
+            };
+            auto slab_of = [&](uint32_t step) { return slab0 + step % S::kSlabs * kSlab; };
+            auto inside = [&](uint32_t step) { return row0 < p.n && r0 + step_col(step) < p.rows; };
+            // Word l of slab row r: four bytes of 16-byte piece l / 4, which stands at piece ^ r % 8.
+            auto word = [&](uint8_t *slab, uint32_t r) { return slab + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4; };
+            constexpr uint32_t kPer = kSwiglu ? 1 : 4 / sizeof(T);  // columns per word
+            auto fetch = [&](uint32_t step) {
+                if constexpr (EPI == OPURE_EPI_ADD) {
+                    if (!inside(step)) return;
+                    const uint32_t col = r0 + step_col(step);
+                    uint8_t *slab = slab_of(step);
+                    __syncwarp();
+                    if (p.tma) {
+                        if (lane == 0) tc::store_wait_read();  // what was in the slab has left
+                        uint64_t *bar = &fetched[warp - kEpiWarp][step % 2];
+                        tc::expect_tx(lane == 0, bar, kSlab);
+                        tc::load_2d(lane == 0, slab, &rmap, col, row0, bar);
+                    } else {
+                        const T *src = static_cast<const T *>(p.residual) + size_t(row0) * p.y_stride + col + lane * kPer;
+                        const uint32_t left = columns_left(p.rows, col + lane * kPer), rows = min(p.n - row0, 32u);
+#pragma unroll 8
+                        for (uint32_t r = 0; r < rows; ++r, src += p.y_stride) {
+                            uint8_t *dst = word(slab, r);
+                            if (p.words && left >= kPer)
+                                tc::copy4_async(dst, src);
+                            else
+#pragma unroll
+                                for (uint32_t k = 0; k < kPer; ++k)
+                                    if (k < left) reinterpret_cast<T *>(dst)[k] = src[k];
+                        }
+                    }
+                }
+            };
+            if constexpr (!kSwiglu) {
+                fetch(0);
+                fetch(1);
+            }
             if (!warp_wait(&acc_full[b], (lt >> 1) & 1u)) {
                 if (lane == 0 && !fail) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 87, blockIdx.x);
                 fail = 1;
@@ -254,7 +305,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) tc::arrive_cluster(drain_bar);
             };
-            const uint32_t shared_side = b ? 0 : kHalf, other_side = kHalf - shared_side, c0 = part * 64;
             if constexpr (kSwiglu) {
                 // Blocks 2 part and 2 part + 1 of the tile's four: gate columns 32 j, up 128 + 32 j.
                 constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
@@ -300,59 +350,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     tc::ld32(acc + c + 32, v[1]);
                     tc::wait_ld();
                     if (h == 0) release();
-                    const uint32_t col = r0 + c;
-                    if (EPI == OPURE_EPI_STORE && p.tma_store) {
-                        constexpr uint32_t kCols = 128 / sizeof(T);  // columns of a slab row
 #pragma unroll
-                        for (uint32_t q = 0; q < 64 / kCols; ++q) {
-                            if (lane == 0) tc::store_wait_read();
+                    for (uint32_t q = 0; q < kSteps / 2; ++q) {
+                        const uint32_t step = h * (kSteps / 2) + q, col = r0 + step_col(step);
+                        uint8_t *slab = slab_of(step);
+                        if (inside(step)) {
+                            if constexpr (EPI == OPURE_EPI_ADD) {
+                                if (p.tma) {
+                                    if (!mbar_wait(&fetched[warp - kEpiWarp][step % 2], fetch_phase[step % 2]))
+                                        report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 88, blockIdx.x);
+                                    fetch_phase[step % 2] ^= 1;
+                                } else {
+                                    tc::copy_async_wait();
+                                }
+                            } else if (p.tma && lane == 0) {
+                                tc::store_wait_read();
+                            }
                             __syncwarp();
 #pragma unroll
                             for (uint32_t e = 0; e < 8; ++e) {  // 16 bytes each
-                                uint4 u;
+                                uint4 *at = reinterpret_cast<uint4 *>(slab + lane * 128 + ((e ^ (lane & 7u)) << 4));
+                                uint4 u = {};
+                                if constexpr (EPI == OPURE_EPI_ADD) u = *at;
                                 T *h8 = reinterpret_cast<T *>(&u);
 #pragma unroll
                                 for (uint32_t k = 0; k < 16 / sizeof(T); ++k) {
-                                    const uint32_t at = q * kCols + e * (16 / sizeof(T)) + k;
-                                    h8[k] = from_f32<T>(__uint_as_float(v[at / 32][at % 32]));
+                                    const uint32_t i = q * kCols + e * (16 / sizeof(T)) + k;
+                                    float f = __uint_as_float(v[i / 32][i % 32]);
+                                    if constexpr (EPI == OPURE_EPI_ADD) f += to_f32(h8[k]);
+                                    h8[k] = from_f32<T>(f);
                                 }
-                                *reinterpret_cast<uint4 *>(slab + lane * 128 + ((e ^ (lane & 7u)) << 4)) = u;
+                                *at = u;
                             }
-                            tc::fence_async_shared();
-                            __syncwarp();
-                            if (lane == 0 && row0 < p.n && col + q * kCols < p.rows) tc::store_2d(&ymap, col + q * kCols, row0, slab);
-                        }
-                    } else {
-                        float *f = reinterpret_cast<float *>(slab);
+                            if (p.tma) {
+                                tc::fence_async_shared();
+                                __syncwarp();
+                                if (lane == 0) tc::store_2d(&ymap, col, row0, slab);
+                            } else {
+                                __syncwarp();
+                                T *dst = static_cast<T *>(p.y) + size_t(row0) * p.y_stride + col + lane * kPer;
+                                const uint32_t left = columns_left(p.rows, col + lane * kPer), rows = min(p.n - row0, 32u);
+#pragma unroll 8
+                                for (uint32_t r = 0; r < rows; ++r, dst += p.y_stride) {
+                                    const uint32_t w = *reinterpret_cast<const uint32_t *>(word(slab, r));
+                                    if (p.words && left >= kPer)
+                                        *reinterpret_cast<uint32_t *>(dst) = w;
+                                    else
 #pragma unroll
-                        for (uint32_t q = 0; q < 2; ++q) {
-                            __syncwarp();
-#pragma unroll
-                            for (uint32_t k = 0; k < 32; ++k) f[lane * 32 + (k ^ lane)] = __uint_as_float(v[q][k]);
-                            __syncwarp();
-                            const uint32_t cc = col + q * 32 + lane;
-                            if (cc < p.rows) {
-                                for (uint32_t r = 0; r < 32; r += 8) {
-                                    float res[8];
-#pragma unroll
-                                    for (uint32_t k = 0; k < 8; ++k) {
-                                        res[k] = 0.f;
-                                        if (EPI == OPURE_EPI_ADD && row0 + r + k < p.n)
-                                            res[k] = to_f32(static_cast<const T *>(p.residual)[(row0 + r + k) * p.y_stride + cc]);
-                                    }
-#pragma unroll
-                                    for (uint32_t k = 0; k < 8; ++k)
-                                        if (row0 + r + k < p.n)
-                                            static_cast<T *>(p.y)[(row0 + r + k) * p.y_stride + cc] =
-                                                from_f32<T>(f[(r + k) * 32 + (lane ^ (r + k))] + res[k]);
+                                        for (uint32_t k = 0; k < kPer; ++k)
+                                            if (k < left) dst[k] = reinterpret_cast<const T *>(&w)[k];
                                 }
+                                __syncwarp();
                             }
                         }
+                        if (step + 2 < kSteps) fetch(step + 2);
                     }
                 }
             }
         }
-        if (EPI == OPURE_EPI_STORE && p.tma_store && lane == 0) tc::store_wait();
+        if (!kSwiglu && p.tma && lane == 0) tc::store_wait();
         __syncwarp();
     }
     tc::fence_before();
@@ -378,13 +434,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 template <uint32_t XF, int EPI, typename T>
-opure_status launch_pair(opure_ctx *ctx, const CUtensorMap (&m)[5], const PairParams &p) {
+opure_status launch_pair(opure_ctx *ctx, const CUtensorMap (&m)[6], const PairParams &p) {
     auto *kernel = mx_gemm_pair_kernel<XF, EPI, T>;
     const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<XF>::kSmem));
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(Shape<XF, EPI>::kSmem));
     if (e != cudaSuccess) return cuda_status(e);
     const uint32_t pairs = std::min(uint32_t(ctx->sm_count) / 2, p.mtiles * p.ntiles);
-    return launch(ctx, kernel, dim3(2 * pairs), dim3(kThreads), Shape<XF>::kSmem, true, m[0], m[1], m[2], m[3], m[4], p);
+    return launch(ctx, kernel, dim3(2 * pairs), dim3(kThreads), Shape<XF, EPI>::kSmem, true, m[0], m[1], m[2], m[3], m[4], m[5], p);
 }
 
 }  // namespace
@@ -422,8 +478,8 @@ opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uin
     p.out = a->out.codes;
     p.outs = a->out.scales;
     p.st = ctx->status;
-    // Maps: w, x, their scale tiles, y.
-    CUtensorMap m[5] = {};
+    // Maps: w, x, their scale tiles, y, residual.
+    CUtensorMap m[6] = {};
     auto codes = [&](CUtensorMap *t, const opure_mx_matrix &q) {
         if (fp8) return make_slot_map(t, q, kHalf);
         const size_t bytes = mx_row_bytes(q.format, q.cols);
@@ -441,13 +497,21 @@ opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uin
     if (!codes(&m[0], a->w) || !codes(&m[1], a->x) || !scales(&m[2], w_scales, swiglu ? p.half : p.rows, swiglu ? 2 : 1, swiglu ? 1 : 2) ||
         !scales(&m[3], a->x.scales, p.n, 1, 1))
         return OPURE_ERR_UNSUPPORTED;
-    m[4] = m[3];
-    if (a->epilogue == OPURE_EPI_STORE && rows_aligned16(a->y, a->y_type, a->y_stride)) {
+    m[4] = m[5] = m[3];
+    if (!swiglu) {
+        const bool add = a->epilogue == OPURE_EPI_ADD;
         const uint32_t size = type_bytes(a->y_type);
         const CUtensorMapDataType type = a->y_type == OPURE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                          : a->y_type == OPURE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        p.tma_store = make_map(&m[4], type, a->y, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        auto rows = [&](CUtensorMap *t, const void *ptr) {
+            // A store that ends inside 16 bytes wrote all of them: rows have to be whole pieces.
+            return rows_aligned16(ptr, a->y_type, a->y_stride) && size_t(p.rows) * size % 16 == 0 &&
+                   make_map(t, type, ptr, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        };
+        p.tma = rows(&m[4], a->y) && (!add || rows(&m[5], a->residual));
+        p.words = a->y_stride * size % 4 == 0 && reinterpret_cast<uintptr_t>(a->y) % 4 == 0 &&
+                  (!add || reinterpret_cast<uintptr_t>(a->residual) % 4 == 0);
     }
     auto go = [&](auto t, auto epi) {
         using T = decltype(t);

@@ -208,6 +208,11 @@ __device__ __forceinline__ void store_2d(const CUtensorMap *map, uint32_t x, uin
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// 4 bytes to shared memory, asynchronously.
+__device__ __forceinline__ void copy4_async(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
