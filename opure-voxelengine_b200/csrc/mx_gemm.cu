@@ -256,9 +256,29 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     // Epilogue: a warp takes a unit, a lane 4 columns of a token.
     for (uint32_t l = warp; got && l < own_units; l += kThreads / 32) {
-        const uint32_t u = l * p.splits + split, i = m0 + u / kChunks * 4 + lane / 8;
-        const uint32_t col = r0 + u % kChunks * 32 + lane % 8 * 4;
-        const uint32_t piece = lane / 8 * 128 + ((lane ^ (u / kChunks * 4 + lane / 8)) & 7u) * 16;
+        const uint32_t u = l * p.splits + split, token0 = u / kChunks * 4, col0 = r0 + u % kChunks * 32;
+        if constexpr (!kSwiglu) {
+            if (!p.vec) {
+                // Unaligned rows: a lane one column of each token, so that neighbouring lanes touch
+                // neighbouring values.
+                const uint32_t col = col0 + lane;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t i = m0 + token0 + k;
+                    const float *src = reinterpret_cast<const float *>(sums + l * kUnit + k * 128 + (((lane >> 2) ^ ((token0 + k) & 7u)) << 4)) + (lane & 3u);
+                    float v = 0.f;
+                    for (uint32_t q = 0; q < p.splits; ++q) v += *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(src) + q * part_bytes);
+                    if (i < p.n && col < p.rows) {
+                        const size_t at = i * p.y_stride + col;
+                        if constexpr (EPI == OPURE_EPI_ADD) v += to_f32(static_cast<const T *>(p.residual)[at]);
+                        static_cast<T *>(p.y)[at] = from_f32<T>(v);
+                    }
+                }
+                continue;
+            }
+        }
+        const uint32_t i = m0 + token0 + lane / 8, col = col0 + lane % 8 * 4;
+        const uint32_t piece = lane / 8 * 128 + ((lane ^ (token0 + lane / 8)) & 7u) * 16;
         float v[kSides][4] = {};
 #pragma unroll
         for (uint32_t q = 0; q < kMaxSplits; ++q) {
@@ -274,13 +294,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
                 v[0][j] = col + j < p.half ? silu(v[0][j]) * v[1][j] : 0.f;  // gate rows past the half are up rows
-            const uint32_t block = col / 32 * 32;
-            store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(block) * kF / 8,
-                            p.outs + mx_scale_offset(p.half, i, block / 32), i < p.n && block < mx_kp(p.half));
+            store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(col0) * kF / 8,
+                            p.outs + mx_scale_offset(p.half, i, col0 / 32), i < p.n && col0 < mx_kp(p.half));
         } else if (i < p.n) {
             const size_t at = i * p.y_stride + col;
-            store_quad<EPI>(v[0], static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at,
-                            col < p.rows ? min(p.rows - col, 4u) : 0u, p.vec);
+            store_quad<EPI>(v[0], static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at, columns_left(p.rows, col));
         }
     }
     tc::fence_before();
@@ -309,11 +327,12 @@ __global__ void __launch_bounds__(256) mx_split_scales_kernel(const uint8_t *src
 
 // ---- host -------------------------------------------------------------------------------
 // K splits, at most one CTA per SM, by the least estimated time (returned, in ns). Measured on one
-// B200: a stage takes 270 ns (SwiGLU, with twice the MMAs, 400), launch, first loads and a plain
-// epilogue 6 us, SwiGLU's 9; joining splits 1 us and, as all SMs exchange more sums, up to 8 us more
-// for 128 tokens on every SM. CTAs go two to an SM.
+// B200: a stage takes 270 ns (SwiGLU, with twice the MMAs, 400), with two CTAs on an SM 670 for
+// both; launch, first loads and a plain epilogue 6 us, SwiGLU's 9; joining splits 1 us and, as all
+// SMs exchange more sums, up to 8 us more for 128 tokens on every SM.
 uint64_t choose_splits(GemmParams &p, uint64_t tiles, bool swiglu, uint32_t sms) {
-    const uint64_t waves = (tiles + 2 * sms - 1) / (2 * sms), n = std::min(p.n, kM), stage = swiglu ? 400 : 270;
+    const uint64_t waves = (tiles + 2 * sms - 1) / (2 * sms), n = std::min(p.n, kM);
+    const uint64_t stage = tiles > sms ? (swiglu ? 1000 : 670) : swiglu ? 400 : 270;
     uint64_t best = ~uint64_t(0);
     for (uint32_t s = 1; s == 1 || (s <= std::min(kMaxSplits, p.kblocks) && s * tiles <= sms); ++s) {
         const uint64_t ctas = s * tiles, join = s > 1 ? 1000 + n * ctas * ctas * 8000 / (uint64_t(kM) * sms * sms) : 0;

@@ -31,11 +31,11 @@ __device__ __forceinline__ void store_block(const float (&v)[4], uint8_t *codes,
     if (lane == 0) *scale = uint8_t(byte);
 }
 
-// Stores (EPI: adds the residual to) the first m of 4 neighbouring results; with `vec` all four at
-// once where m is 4.
+// Stores (EPI: adds the residual to) the first `left` of 4 neighbouring results; all four at once
+// where there are as many (y and res aligned for that).
 template <int EPI, typename T>
-__device__ __forceinline__ void store_quad(float (&v)[4], T *y, const T *res, uint32_t m, bool vec) {
-    if (vec && m == 4) {
+__device__ __forceinline__ void store_quad(float (&v)[4], T *y, const T *res, uint32_t left) {
+    if (left >= 4) {
         struct alignas(4 * sizeof(T)) Quad {
             T v[4];
         } o;
@@ -50,7 +50,7 @@ __device__ __forceinline__ void store_quad(float (&v)[4], T *y, const T *res, ui
     } else {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            if (j >= m) break;
+            if (j >= left) break;
             if constexpr (EPI == OPURE_EPI_ADD) v[j] += to_f32(res[j]);
             y[j] = from_f32<T>(v[j]);
         }

@@ -205,13 +205,20 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
                 store_block<OPURE_MX_FP8>(v, p.out + token * mx_row_bytes(OPURE_MX_FP8, p.half) + c0, scale, real);
         } else if (real) {
             const size_t at = token * p.y_stride + col;
-            const uint32_t m = col < p.rows ? min(p.rows - col, 4u) : 0u;
+            const uint32_t left = columns_left(p.rows, col);
             auto store = [&](auto type) {
                 using T = decltype(type);
-                if (p.epilogue == OPURE_EPI_ADD)
-                    store_quad<OPURE_EPI_ADD>(v, static_cast<T *>(p.y) + at, static_cast<const T *>(p.residual) + at, m, p.vec);
-                else
-                    store_quad<OPURE_EPI_STORE>(v, static_cast<T *>(p.y) + at, static_cast<const T *>(nullptr), m, p.vec);
+                T *y = static_cast<T *>(p.y) + at;
+                const T *res = static_cast<const T *>(p.residual) + at;
+                // One or two tokens: unaligned values one at a time cost nothing that shows.
+                for (uint32_t j = 0; j < 4; j += p.vec ? 4 : 1) {
+                    if (j >= left) break;
+                    if (p.vec) {
+                        p.epilogue == OPURE_EPI_ADD ? store_quad<OPURE_EPI_ADD>(v, y, res, left) : store_quad<OPURE_EPI_STORE>(v, y, res, left);
+                    } else {
+                        y[j] = from_f32<T>(p.epilogue == OPURE_EPI_ADD ? v[j] + to_f32(res[j]) : v[j]);
+                    }
+                }
             };
             if (p.y_type == OPURE_F32)
                 store(float());
