@@ -262,17 +262,19 @@ __global__ void __launch_bounds__(kThreads, 2)
                 // Unaligned rows: a lane one column of each token, so that neighbouring lanes touch
                 // neighbouring values.
                 const uint32_t col = col0 + lane;
+                const size_t at = (m0 + token0) * p.y_stride + col;
+                const uint32_t tokens = col < p.rows ? columns_left(n, token0) : 0;
+                float res[4] = {};
+                if constexpr (EPI == OPURE_EPI_ADD)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        if (k < tokens) res[k] = to_f32(static_cast<const T *>(p.residual)[at + k * p.y_stride]);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k) {
-                    const uint32_t i = m0 + token0 + k;
-                    const float *src = reinterpret_cast<const float *>(sums + l * kUnit + k * 128 + (((lane >> 2) ^ ((token0 + k) & 7u)) << 4)) + (lane & 3u);
+                    const uint8_t *src = sums + l * kUnit + k * 128 + (((lane >> 2) ^ ((token0 + k) & 7u)) << 4) + (lane & 3u) * 4;
                     float v = 0.f;
-                    for (uint32_t q = 0; q < p.splits; ++q) v += *reinterpret_cast<const float *>(reinterpret_cast<const uint8_t *>(src) + q * part_bytes);
-                    if (i < p.n && col < p.rows) {
-                        const size_t at = i * p.y_stride + col;
-                        if constexpr (EPI == OPURE_EPI_ADD) v += to_f32(static_cast<const T *>(p.residual)[at]);
-                        static_cast<T *>(p.y)[at] = from_f32<T>(v);
-                    }
+                    for (uint32_t q = 0; q < p.splits; ++q) v += *reinterpret_cast<const float *>(src + q * part_bytes);
+                    if (k < tokens) static_cast<T *>(p.y)[at + k * p.y_stride] = from_f32<T>(v + res[k]);
                 }
                 continue;
             }
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-                v[0][j] = col + j < p.half ? silu(v[0][j]) * v[1][j] : 0.f;  // gate rows past the half are up rows
+                v[0][j] = col + j < p.half ? swiglu(v[0][j], v[1][j]) : 0.f;  // gate rows past the half are up rows
             store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(col0) * kF / 8,
                             p.outs + mx_scale_offset(p.half, i, col0 / 32), i < p.n && col0 < mx_kp(p.half));
         } else if (i < p.n) {

@@ -96,11 +96,6 @@ __device__ __forceinline__ uint32_t quantize_block(float (&v)[32], uint8_t *dst,
     return byte;
 }
 
-// silu(g) u with the hardware's exp2 and reciprocal, each within 2 units of fp32's last place
-// (exp's argument times log2 e adds |g| 2^-24): far below a step of the 8-bit result, and a
-// third of the instructions of expf and a rounded division.
-__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
-
 // The results' warps stop together when one of their lanes gives up.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase) {
     return __all_sync(0xffffffffu, mbar_wait(bar, phase));

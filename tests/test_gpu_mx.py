@@ -205,7 +205,8 @@ def check_quantized(got, y, cols, fmt, rel, most_flips):
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows,cols,stride,shift", [
     (1, 1, None, 0), (1, 576, None, 0), (3, 33, 48, 0), (130, 577, None, 0), (64, 2048, None, 0), (5, 2048, 2056, 1),
-    (2, 4104, None, 0), (3, 8192, None, 0), (2, 16385, 16392, 0), (2, 20000, None, 0)])
+    (2, 4104, None, 0), (3, 8192, None, 0), (2, 16385, 16392, 0), (2, 20000, None, 0), (1300, 64, None, 0), (1201, 300, 304, 8),
+    (1211, 75, None, 0), (1190, 512, 513, 1), (3, 9001, None, 0), (2, 17001, 17003, 1)])
 def test_rmsnorm(ctx, t, fmt, rows, cols, stride, shift):
     rng = np.random.default_rng(cols + rows)
     X, R, S = (Rows(ctx, rows, cols, t, stride, shift) for _ in range(3))
@@ -330,6 +331,57 @@ def test_gemm_swiglu(ctx, fmt, out_fmt, n, ff, cols):
     assert (np.abs(v - y) <= bound).all()
     assert np.mean(code != want_code) <= 2e-3 + 2.0 / code.size
     assert np.mean(byte != want_byte) <= 2e-3 + 1.0 / byte.size
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n,rows,cols,stride,shift", [
+    (2, 100, 200, 103, 1), (40, 300, 260, 304, 8), (64, 129, 1000, 131, 1), (300, 1000, 384, 1008, 0), (300, 1003, 384, 1008, 8),
+    (260, 1001, 130, 1003, 3)])
+def test_gemm_store_strided(ctx, t, fmt, n, rows, cols, stride, shift):
+    """Rows with room between them, which stays as it was, at every alignment."""
+    rng = np.random.default_rng(n + rows + cols)
+    X, x = random_mx(ctx, rng, n, cols, fmt)
+    W, w = random_mx(ctx, rng, rows, cols, cu.MX_FP4, 0.02)
+    y = x @ w.T
+    Y = Rows(ctx, n, rows, t, stride, shift)
+    ctx.mx_gemm(cu.MxGemmArgs(w=W.m, x=X.m, y=Y.ptr, y_type=cu.VALUE_TYPES[t], y_stride=stride))
+    assert (np.abs(Y.get() - y) <= product_bound(x, w, y, t)).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("epi,t", [(cu.EPI_STORE, "f32"), (cu.EPI_STORE, "bf16"), (cu.EPI_ADD, "f32"), (cu.EPI_ADD, "f16"),
+                                   (cu.EPI_SWIGLU, "f32")])
+def test_gemm_many_tiles(ctx, fmt, epi, t):
+    """More 256 x 256 tiles than pairs of SMs, so that a pair goes from one accumulator to the other
+    and back, with an end inside the last tiles."""
+    rng = np.random.default_rng(6)
+    n, rows, cols = 2000, 5100 if epi == cu.EPI_SWIGLU else 5000, 640
+    X, x = random_mx(ctx, rng, n, cols, fmt)
+    W, w = random_mx(ctx, rng, rows, cols, cu.MX_FP4, 0.02)
+    y = x @ w.T
+    if epi == cu.EPI_SWIGLU:
+        out = Mx(ctx, n, rows // 2, cu.MX_FP8)
+        ctx.mx_gemm(cu.MxGemmArgs(w=W.m, x=X.m, epilogue=epi, out=out.m))
+        g, u = y[:, :rows // 2], y[:, rows // 2:]
+        want = g / (1 + np.exp(-g)) * u
+        code, byte = out.get()
+        v = mx.values(code, byte, rows // 2, cu.MX_FP8)
+        s = np.repeat(np.exp2(byte.astype(np.float64) - 127), 32, 1)[:, :rows // 2]
+        # Half a step of E4M3, the product's error as in test_gemm_swiglu, and the limit of 448.
+        err = 1.1 * product_bound(x, w[:rows // 2], g, "f32") * np.abs(u) + 1.1 * product_bound(x, w[rows // 2:], u, "f32") * np.abs(g)
+        bound = np.maximum(np.abs(want) * 2.0 ** -4, 2.0 ** -10 * s) * (1 + 2.0 ** -20) + 2 * err
+        assert (np.abs(v - want) <= bound + np.where(np.abs(want) + err > 448 * s, 64 * s, 0)).all()
+        assert np.mean(code != mx.quantize(want, cu.MX_FP8)[0]) <= 2e-3
+        return
+    Y, R = Rows(ctx, n, rows, t), Rows(ctx, n, rows, t)
+    a = cu.MxGemmArgs(w=W.m, x=X.m, epilogue=epi, y=Y.ptr, y_type=cu.VALUE_TYPES[t], y_stride=rows)
+    if epi == cu.EPI_ADD:
+        r = R.put(rng.standard_normal((n, rows)))
+        a.residual = R.ptr
+        y = y + r
+    ctx.mx_gemm(a)
+    assert (np.abs(Y.get() - y) <= product_bound(x, w, y, t) + 2.0 ** -22 * np.abs(y)).all()
 
 
 @pytest.mark.parametrize("n,rows,cols", [(1, 130, 576), (20, 200, 300), (300, 520, 300)])
