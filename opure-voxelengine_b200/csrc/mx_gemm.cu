@@ -409,7 +409,8 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.out = a->out.codes;
     p.outs = a->out.scales;
     p.st = ctx->status;
-    if (p.n > 65535u * kM) return OPURE_ERR_UNSUPPORTED;
+    // Grid dimensions and TMA's 32-bit signed coordinates.
+    if (p.n > 65535u * kM || p.rows > (1u << 30) || a->w.cols > (1u << 30)) return OPURE_ERR_UNSUPPORTED;
     const uint32_t tiles = swiglu ? mx_kp(p.half) / (kN / 2) : ceil_div(p.rows, kN);
     const uint32_t mtiles = ceil_div(p.n, kM);
     const uint64_t here_ns = choose_splits(p, uint64_t(tiles) * mtiles, swiglu, uint32_t(ctx->sm_count));

@@ -62,7 +62,8 @@ struct PairParams {
     size_t y_stride;
     const void *residual;
     uint8_t *out, *outs;
-    bool tma, words;  // rows of y and residual: 16-byte aligned (TMA); 4-byte aligned
+    bool tma;        // rows of y and residual are whole, aligned 16-byte pieces
+    uint32_t grain;  // without tma: bytes that a lane moves at once, 8, 4 or (0) a value
     DeviceStatus *st;
 };
 
@@ -253,9 +254,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             auto slab_of = [&](uint32_t step) { return slab0 + step % S::kSlabs * kSlab; };
             auto inside = [&](uint32_t step) { return row0 < p.n && r0 + step_col(step) < p.rows; };
-            // Word l of slab row r: four bytes of 16-byte piece l / 4, which stands at piece ^ r % 8.
-            auto word = [&](uint8_t *slab, uint32_t r) { return slab + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4; };
-            constexpr uint32_t kPer = kSwiglu ? 1 : 4 / sizeof(T);  // columns per word
+            // Without TMA: slab rows to and from memory, `grain` bytes a lane, so that one or two rows
+            // go at a time. move(slab place, row's place in memory, whole grain, values of it inside).
+            auto by_rows = [&](auto grain, uint32_t col, uint8_t *slab, auto move) {
+                constexpr uint32_t G = decltype(grain)::value, kLanes = 128 / G, kValues = G / sizeof(T);
+                const uint32_t l = lane % kLanes, at = l * G, rows = min(p.n - row0, 32u);
+                const uint32_t left = columns_left(p.rows, col + l * kValues);
+                size_t place = size_t(row0 + lane / kLanes) * p.y_stride + col + l * kValues;
+#pragma unroll 8
+                for (uint32_t r = lane / kLanes; r < rows; r += 32 / kLanes, place += 32 / kLanes * p.y_stride)
+                    move(slab + r * 128 + (((at >> 4) ^ (r & 7u)) << 4) + (at & 15u), place, left >= kValues, left);
+            };
+            auto with_grain = [&](auto f) {
+                if (p.grain == 8)
+                    f(std::integral_constant<uint32_t, 8>(), true);
+                else
+                    f(std::integral_constant<uint32_t, 4>(), p.grain == 4);
+            };
             auto fetch = [&](uint32_t step) {
                 if constexpr (EPI == OPURE_EPI_ADD) {
                     if (!inside(step)) return;
@@ -268,18 +283,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         tc::expect_tx(lane == 0, bar, kSlab);
                         tc::load_2d(lane == 0, slab, &rmap, col, row0, bar);
                     } else {
-                        const T *src = static_cast<const T *>(p.residual) + size_t(row0) * p.y_stride + col + lane * kPer;
-                        const uint32_t left = columns_left(p.rows, col + lane * kPer), rows = min(p.n - row0, 32u);
-#pragma unroll 8
-                        for (uint32_t r = 0; r < rows; ++r, src += p.y_stride) {
-                            uint8_t *dst = word(slab, r);
-                            if (p.words && left >= kPer)
-                                tc::copy4_async(dst, src);
-                            else
+                        with_grain([&](auto grain, bool whole) {
+                            constexpr uint32_t G = decltype(grain)::value;
+                            by_rows(grain, col, slab, [&](uint8_t *dst, size_t place, bool all, uint32_t left) {
+                                const T *src = static_cast<const T *>(p.residual) + place;
+                                if (whole && all)
+                                    tc::copy_async<G>(dst, src);
+                                else
 #pragma unroll
-                                for (uint32_t k = 0; k < kPer; ++k)
-                                    if (k < left) reinterpret_cast<T *>(dst)[k] = src[k];
-                        }
+                                    for (uint32_t k = 0; k < G / sizeof(T); ++k)
+                                        if (k < left) reinterpret_cast<T *>(dst)[k] = src[k];
+                            });
+                        });
                     }
                 }
             };
@@ -383,18 +398,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 if (lane == 0) tc::store_2d(&ymap, col, row0, slab);
                             } else {
                                 __syncwarp();
-                                T *dst = static_cast<T *>(p.y) + size_t(row0) * p.y_stride + col + lane * kPer;
-                                const uint32_t left = columns_left(p.rows, col + lane * kPer), rows = min(p.n - row0, 32u);
-#pragma unroll 8
-                                for (uint32_t r = 0; r < rows; ++r, dst += p.y_stride) {
-                                    const uint32_t w = *reinterpret_cast<const uint32_t *>(word(slab, r));
-                                    if (p.words && left >= kPer)
-                                        *reinterpret_cast<uint32_t *>(dst) = w;
-                                    else
+                                with_grain([&](auto grain, bool whole) {
+                                    using Word = std::conditional_t<decltype(grain)::value == 8, uint2, uint32_t>;
+                                    by_rows(grain, col, slab, [&](uint8_t *src, size_t place, bool all, uint32_t left) {
+                                        const Word w = *reinterpret_cast<const Word *>(src);
+                                        T *dst = static_cast<T *>(p.y) + place;
+                                        if (whole && all)
+                                            *reinterpret_cast<Word *>(dst) = w;
+                                        else
 #pragma unroll
-                                        for (uint32_t k = 0; k < kPer; ++k)
-                                            if (k < left) dst[k] = reinterpret_cast<const T *>(&w)[k];
-                                }
+                                            for (uint32_t k = 0; k < sizeof(Word) / sizeof(T); ++k)
+                                                if (k < left) dst[k] = reinterpret_cast<const T *>(&w)[k];
+                                    });
+                                });
                                 __syncwarp();
                             }
                         }
@@ -505,8 +521,9 @@ opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uin
                    make_map(t, type, ptr, p.rows, p.n, a->y_stride * size, 128 / size, 32, CU_TENSOR_MAP_SWIZZLE_128B);
         };
         p.tma = rows(&m[4], a->y) && (!add || rows(&m[5], a->residual));
-        p.words = a->y_stride * size % 4 == 0 && reinterpret_cast<uintptr_t>(a->y) % 4 == 0 &&
-                  (!add || reinterpret_cast<uintptr_t>(a->residual) % 4 == 0);
+        for (uint32_t grain : {8u, 4u})
+            if (!p.grain && (a->y_stride * size | reinterpret_cast<uintptr_t>(a->y) | (add ? reinterpret_cast<uintptr_t>(a->residual) : 0)) % grain == 0)
+                p.grain = grain;
     }
     auto go = [&](auto t, auto epi) {
         using T = decltype(t);

@@ -208,9 +208,10 @@ __device__ __forceinline__ void store_2d(const CUtensorMap *map, uint32_t x, uin
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// 4 bytes to shared memory, asynchronously.
-__device__ __forceinline__ void copy4_async(void *dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+// 4 or 8 bytes to shared memory, asynchronously.
+template <uint32_t BYTES>
+__device__ __forceinline__ void copy_async(void *dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(dst)), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }

@@ -473,6 +473,34 @@ def test_calls_in_a_graph_and_back_to_back(ctx):
     g.free()
 
 
+def test_calls_allocate_nothing(ctx):
+    rng = np.random.default_rng(1)
+    n, d, ff = 150, 576, 1500
+    X, Y = Rows(ctx, n, d, "f32"), Rows(ctx, n, d, "f32")
+    X.put(rng.standard_normal((n, d)))
+    W1, _ = random_mx(ctx, rng, 2 * ff, d, cu.MX_FP4, 0.02)
+    W2, _ = random_mx(ctx, rng, d, ff, cu.MX_FP4, 0.02)
+    a, h = Mx(ctx, n, d, cu.MX_FP8), Mx(ctx, n, ff, cu.MX_FP8)
+
+    def layer():
+        for rows in (1, 20, n):
+            for m in (a.m, h.m):
+                m.rows = rows
+            ctx.mx_quantize(X.ptr, cu.F32, d, a.m)
+            ctx.mx_rmsnorm(cu.MxNormArgs(x=X.ptr, x_type=cu.F32, x_stride=d, eps=1e-5, out=a.m))
+            ctx.mx_gemm(cu.MxGemmArgs(w=W1.m, x=a.m, epilogue=cu.EPI_SWIGLU, out=h.m))
+            ctx.mx_gemm(cu.MxGemmArgs(w=W2.m, x=h.m, y=Y.ptr, y_type=cu.F32, y_stride=d))
+            ctx.mx_dequantize(a.m, Y.ptr, cu.F32, d)
+
+    layer()
+    ctx.sync()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(5):
+        layer()
+    ctx.sync()
+    assert torch.cuda.mem_get_info()[0] == free
+
+
 # ---- nothing to do, and refusals -------------------------------------------------------------
 def test_empty(ctx):
     e4, e8 = cu.MxMatrix(0, 0, 0, 64, cu.MX_FP4), cu.MxMatrix(0, 0, 0, 64, cu.MX_FP8)
