@@ -226,17 +226,39 @@ struct NormParams {
     bool gain_vec;  // the gain allows 16-byte accesses
 };
 
-// Sum over a row's threads: a warp's, or a CTA's (part: 32 floats).
+// Sum over a row's threads: a warp's, or a CTA's (part: 32 values).
 template <bool WARP>
-__device__ __forceinline__ float row_sum(float v, float *part) {
-    v = warp_sum(v);
+__device__ __forceinline__ double row_sum(double v, double *part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (!WARP) {
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = 0.f;
+        v = 0.0;
         for (uint32_t w = 0; w < blockDim.x / 32; ++w) v += part[w];
     }
     return v;
+}
+
+// A result that lies on the other side of a rounding boundary of its code is a whole step off, so
+// the norm's own rounding is kept out of the way: squares are summed in 64 bits, the inverse root
+// is a pair of floats (one Newton step from rsqrt, with the products' rest by fma), and so is each
+// product until it is rounded to fp32 once. Six more fp32 instructions per value, which the memory
+// hides.
+struct Inverse {
+    float hi, lo;
+};
+__device__ __forceinline__ Inverse inverse_rms(double sum_of_squares, uint32_t cols, float eps) {
+    const double m = sum_of_squares / double(cols) + double(eps);
+    const float mh = float(m), ml = float(m - double(mh)), y = rsqrtf(mh);
+    const float p = mh * y, rest = fmaf(-p, y, 1.0f) - fmaf(mh, y, -p) * y - ml * y * y;  // 1 - m y^2
+    const float lo = 0.5f * y * rest;
+    return {y, isfinite(lo) ? lo : 0.f};  // m of 0 or beyond fp32: the root alone
+}
+__device__ __forceinline__ float normed(float v, Inverse inv, float gain) {
+    const float p = v * inv.hi, rest = fmaf(v, inv.hi, -p) + v * inv.lo, q = p * gain;
+    const float low = fmaf(p, gain, -q) + rest * gain;
+    return isfinite(low) ? q + low : q;
 }
 
 // One CTA per row, or (WARP) one warp per row where there are many short ones: 15007 rows of 75
@@ -245,7 +267,7 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
 // than 16384, reads them twice (the second time from L2).
 template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
 __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(NormParams p) {
-    __shared__ float part[32];
+    __shared__ double part[32];
     grid_dependency_wait();
     grid_dependents_launch();
     const uint32_t width = WARP ? 32 : blockDim.x, place = WARP ? threadIdx.x & 31u : threadIdx.x;
@@ -271,10 +293,10 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
             for (int j = 0; j < 8; ++j) v[j] += t[j];
         }
     };
-    float ss = 0.f;
+    double ss = 0.0;
     auto square = [&](const float (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        for (int j = 0; j < 8; ++j) ss = fma(double(v[j]), double(v[j]), ss);
     };
     float kept[KEEP ? KEEP : 1][8];
     if constexpr (KEEP > 0) {
@@ -289,7 +311,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
         }
     }
     ss = row_sum<WARP>(ss, part);
-    const float inv = 1.0f / sqrtf(ss / float(cols) + p.eps);
+    const Inverse inv = inverse_rms(ss, cols, p.eps);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
@@ -308,10 +330,10 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
             else
                 load8_part(p.gain + c, n, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = v[j] * inv * g[j];
+            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], inv, g[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= inv;
+            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], inv, 1.f);
         }
         const uint32_t byte = mx_store_octet<FMT>(v, codes, c / 8, c < kp);
         const uint32_t word = mx_scale_word(byte);
@@ -334,7 +356,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
 // of s; KEEP 0, for rows longer than 16384, reads x and residual twice.
 template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
 __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kernel(NormParams p) {
-    __shared__ float part[32];
+    __shared__ double part[32];
     grid_dependency_wait();
     grid_dependents_launch();
     const uint32_t row = WARP ? (blockIdx.x * kThreads + threadIdx.x) / 32 : blockIdx.x;
@@ -354,10 +376,10 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kern
             for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] += t[b];
         }
     };
-    float ss = 0.f;
+    double ss = 0.0;
     auto square = [&](const float (&v)[kGroupBlocks]) {
 #pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) ss = fmaf(v[b], v[b], ss);
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) ss = fma(double(v[b]), double(v[b]), ss);
     };
     float kept[KEEP ? KEEP : 1][kGroupBlocks];
     if constexpr (KEEP > 0) {
@@ -374,7 +396,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kern
         }
     }
     ss = row_sum<WARP>(ss, part);
-    const float inv = 1.0f / sqrtf(ss / float(cols) + p.eps);
+    const Inverse inv = inverse_rms(ss, cols, p.eps);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[kGroupBlocks]) {
         const uint32_t left = columns_left(cols, c + lane);
@@ -384,7 +406,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kern
         float g[kGroupBlocks] = {1.f, 1.f, 1.f, 1.f};
         if (p.gain) narrow_load(p.gain + c + lane, left, g);
 #pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = v[b] * inv * g[b];
+        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = normed(v[b], inv, g[b]);
         narrow_store<FMT>(v, codes + size_t(c) * FMT / 8,
                           reinterpret_cast<uint32_t *>(p.scales + mx_scale_offset(cols, row, c / kMxBlock)));
     };
