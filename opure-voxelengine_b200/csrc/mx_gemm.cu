@@ -18,6 +18,10 @@
 //     (8 splits of 64 tokens: 9.3 us against 11.2; of 3 tokens: 6.9 against 6.1). In SwiGLU a
 //     tile is 64 gate rows and the 64 up rows that go with them.
 // All waits are bounded (1 s); a timeout is reported in the ctx status word.
+//
+// Bound by latency: the first data is there 1,500 clocks after the launch, a stage takes its single
+// issuing warp about 270 ns, the epilogue 1,300 clocks. Measured: 64 x 6144 x 2048 to fp32 7.5 us,
+// 37 x 1003 x 1100 with 4-bit tokens to bf16 5.4 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -1,9 +1,9 @@
 // mx_gemv.cu -- the product of microscaled matrices for one or two tokens: decode's weight
 // streaming.
 //
-// Bound by memory: a weight is 0.53 bytes and used once per token. At the measured 6.45 TB/s an SM
-// gets 23 bytes, 43 weights, a clock, so that about 3 lane instructions per weight is all that its
-// 128 lanes have. mma.sync m16n8k16 (fp16 in, fp32 out) takes the multiplications; the codes'
+// Its floor is memory: a weight is 0.53 bytes and used once per token. At the measured 6.45 TB/s an
+// SM gets 23 bytes, 43 weights, a clock, so that about 3 lane instructions per weight is all that
+// its 128 lanes have. mma.sync m16n8k16 (fp16 in, fp32 out) takes the multiplications; the codes'
 // values are exact in fp16, and a block's sum is scaled by both scales in fp32. The tensor-core
 // kernels' fixed costs (TMEM, tensor maps, a single issuing thread) are what this kernel avoids.
 //
@@ -19,6 +19,10 @@
 // A CTA is units x splits warps: a unit is 16 MT rows (in SwiGLU the CTA's units are 32 gate rows
 // and the 32 up rows that go with them), shared by `splits` warps that take every splits'th 128
 // columns and are added in order through shared memory.
+//
+// Measured: 1 x 49152 x 576 6.0 us (2.5 TB/s; its 15 MB are 2.4 us of memory), 1 x 2048 x 8192 4.5
+// us, 1 x 576 x 576 2.2 us. At these sizes latency bounds it: launch, first loads, and one or two
+// more rounds of loads by the 11 to 16 warps that fit an SM.
 #include <algorithm>
 
 #include "mx_gemm.cuh"
