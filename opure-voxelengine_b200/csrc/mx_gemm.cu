@@ -82,12 +82,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t nk = uint32_t(uint64_t(p.kblocks) * (split + 1) / p.splits) - kb0;
     const uint32_t a_bytes = p.a_rows * kK, stage_bytes = kBBytes + kScaleBytes + a_bytes;
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dsm) + 1023) & ~uintptr_t(1023));
-    // Stage: [B 16 KB][scales 2 KB][A]. The MMA reads 128 rows of A whatever a_rows is; rows past
-    // a_rows are other bytes of this allocation (the launch adds room after the last stage) and
-    // only reach accumulator lanes of tokens that are not there.
-    auto b_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes; };
-    auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes; };
-    auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + kBBytes + kScaleBytes; };
+    // Stage: [A][B 16 KB][scales 2 KB]. The MMA reads 128 rows of A whatever a_rows is; rows past
+    // a_rows are the stage's B and only reach accumulator lanes of tokens that are not there.
+    auto a_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes; };
+    auto b_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + a_bytes; };
+    auto sf_tile = [&](uint32_t s) { return base + size_t(s) * stage_bytes + a_bytes + kBBytes; };
     // Results in units of 4 tokens x 32 columns (and 2 sides in SwiGLU). Unit u is finished by CTA
     // u % splits, as its unit u / splits. Every CTA lays its sums out by receiver (`mine`, in the
     // ring's place) and sends each its part, which arrives in that one's `sums`, one part per split:
@@ -425,18 +424,17 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     // to send take the ring's place.
     const uint32_t chunks = swiglu ? kN / 64 : kN / 32, units = ceil_div(std::min(p.n, kM), 4) * chunks;
     const size_t sums = size_t(ceil_div(units, p.splits)) * p.splits * (swiglu ? 2 : 1) * kUnit;
-    const size_t rest = size_t(kM - p.a_rows) * kK;
     // Two CTAs per SM (TMEM's 512 columns allow it and, above 75 KB each, no third), so that the
     // next kernel's CTAs set up while this one's work: a chain of 8-token 8192 -> 2048 products
     // took 5.8 us a call with half of the shared memory each, 9.7 us with all of it. Only the sums
     // of more than 100 tokens with splits need more than half.
     auto stages_in = [&](size_t bytes) {
-        return std::min<uint32_t>({kMaxStages, uint32_t((bytes - 1024 - rest) / stage_bytes), ceil_div(p.kblocks, p.splits)});
+        return std::min<uint32_t>({kMaxStages, uint32_t((bytes - 1024) / stage_bytes), ceil_div(p.kblocks, p.splits)});
     };
     p.stages = stages_in(kHalfSmem);
     p.apart = p.splits > 1 && sums < kHalfSmem / 2 && stages_in(kHalfSmem - sums) >= std::min(4u, p.stages);
     if (p.apart) p.stages = stages_in(kHalfSmem - sums);
-    const size_t ring = p.stages * stage_bytes + rest;
+    const size_t ring = size_t(p.stages) * stage_bytes;
     p.sums_offset = p.splits == 1 ? 0 : uint32_t(p.apart ? std::max(ring, sums) : sums);
     const size_t smem = std::max<size_t>({1024 + ring, 1024 + p.sums_offset + sums, 80 * 1024});
     p.vec = rows_aligned16(a->y, a->y_type, a->y_stride) && rows_aligned16(a->residual, a->y_type, a->y_stride);
