@@ -29,21 +29,108 @@ struct Groups {
     }
 };
 
-template <typename T, uint32_t FMT, uint32_t U>
+// Rows that 32-byte accesses cannot serve (odd strides, unaligned pointers) are read and written
+// in the aligned 16-byte words that hold a lane's values, and the values shifted into their places
+// in registers. 10432 x 3109 fp16 to 4 bits and back: 39 us; with a warp per group and a lane per
+// column of each block, whose shuffles and small accesses the SMs cannot issue fast enough, 92 us.
+//
+// 16 values of w from `bytes` (whole values, up to 15 bytes) on.
+template <typename T>
+__device__ __forceinline__ void shift_words(const uint32_t (&w)[4 * sizeof(T) + 4], uint32_t bytes, uint32_t (&out)[4 * sizeof(T)]) {
+    constexpr uint32_t N = 4 * sizeof(T);
+    uint32_t t[N + 2], u[N + 1];
+#pragma unroll
+    for (uint32_t i = 0; i < N + 2; ++i) t[i] = bytes & 8u ? w[i + 2] : w[i];
+#pragma unroll
+    for (uint32_t i = 0; i < N + 1; ++i) u[i] = bytes & 4u ? t[i + 1] : t[i];
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) out[i] = sizeof(T) == 4 ? u[i] : __funnelshift_r(u[i], u[i + 1], (bytes & 3u) * 8u);
+}
+
+// The words that hold the 16 values at p, of a matrix in [begin, end); returns how many bytes of
+// them come before p.
+template <typename T>
+__device__ __forceinline__ uint32_t load16_any(const T *p, const T *begin, const T *end, uint32_t (&w)[4 * sizeof(T) + 4]) {
+    constexpr uint32_t kWords = sizeof(T);  // of 16 bytes
+    const uint32_t before = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p) - before;
+    if (first < reinterpret_cast<uintptr_t>(begin) || first + 16 * (kWords + (before != 0)) > reinterpret_cast<uintptr_t>(end)) {
+        T *r = reinterpret_cast<T *>(w);
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) r[j] = p[j];
+        return 0;
+    }
+    const uint4 *words = reinterpret_cast<const uint4 *>(first);
+    uint4 q[kWords + 1];
+#pragma unroll
+    for (uint32_t k = 0; k < kWords; ++k) q[k] = words[k];
+    q[kWords] = before ? words[kWords] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (uint32_t k = 0; k <= kWords; ++k) {
+        w[4 * k] = q[k].x;
+        w[4 * k + 1] = q[k].y;
+        w[4 * k + 2] = q[k].z;
+        w[4 * k + 3] = q[k].w;
+    }
+    return before;
+}
+
+// 16 values to any address: words across two lanes are written by the later lane, if it holds all
+// of its values (full) and the lane before it the same row's (follows). All lanes of the warp call.
+template <typename T>
+__device__ __forceinline__ void store16_any(T *p, bool full, bool follows, const uint32_t (&raw)[4 * sizeof(T)]) {
+    constexpr uint32_t kWords = sizeof(T);
+    const uint32_t lane = threadIdx.x & 31u, before = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const bool joins = full && follows && lane != 0;
+    const bool joined = __shfl_down_sync(0xffffffffu, joins, 1) && lane != 31;
+    uint32_t w[4 * kWords + 4], out[4 * kWords];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xffffffffu, raw[4 * kWords - 4 + i], 1);
+#pragma unroll
+    for (uint32_t i = 0; i < 4 * kWords; ++i) w[4 + i] = raw[i];
+    if (!full) return;
+    const T *r = reinterpret_cast<const T *>(raw);
+    uint4 *words = reinterpret_cast<uint4 *>(reinterpret_cast<uintptr_t>(p) - before);
+    if (before == 0) {
+#pragma unroll
+        for (uint32_t k = 0; k < kWords; ++k) words[k] = make_uint4(raw[4 * k], raw[4 * k + 1], raw[4 * k + 2], raw[4 * k + 3]);
+        return;
+    }
+    shift_words<T>(w, 16 - before, out);
+#pragma unroll
+    for (uint32_t k = 0; k < kWords; ++k)
+        if (k || joins) words[k] = make_uint4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+    constexpr uint32_t kPer = 16 / sizeof(T);  // values per word
+    const uint32_t later = before / sizeof(T);  // of them after a word's beginning
+    if (!joins)
+#pragma unroll
+        for (uint32_t j = 0; j < kPer - 1; ++j)
+            if (j + later < kPer) p[j] = r[j];
+    if (!joined)
+#pragma unroll
+        for (uint32_t j = 17 - kPer; j < 16; ++j)
+            if (j + later >= 16) p[j] = r[j];
+}
+
+template <typename T, uint32_t FMT, uint32_t U, bool ANY>
 __global__ void __launch_bounds__(kThreads)
     mx_quantize_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {
     grid_dependency_wait();
     grid_dependents_launch();
     const uint32_t first = (blockIdx.x * U * kThreads + threadIdx.x) / 8;
-    uint32_t raw[U][4 * sizeof(T)];
-    uint32_t row[U], c[U];
+    uint32_t raw[U][4 * sizeof(T) + (ANY ? 4 : 0)];
+    uint32_t row[U], c[U], before[U];
     bool in[U];
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
         in[i] = groups.at(first + i * (kThreads / 8), row[i], c[i]);
         const T *p = x + size_t(row[i]) * stride + c[i];
+        before[i] = 0;
         if (in[i] && c[i] + 16 <= cols) {
-            load16(p, raw[i]);
+            if constexpr (ANY)
+                before[i] = load16_any(p, x, x + size_t(groups.rows - 1) * stride + cols, raw[i]);
+            else
+                load16(p, raw[i]);
         } else {
             T *r = reinterpret_cast<T *>(raw[i]);
 #pragma unroll
@@ -53,8 +140,15 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
         float v[16];
+        if constexpr (ANY) {
+            uint32_t place[4 * sizeof(T)];
+            shift_words<T>(raw[i], before[i], place);
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) v[j] = to_f32(reinterpret_cast<const T *>(raw[i])[j]);
+            for (uint32_t j = 0; j < 16; ++j) v[j] = to_f32(reinterpret_cast<const T *>(place)[j]);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) v[j] = to_f32(reinterpret_cast<const T *>(raw[i])[j]);
+        }
         float f = max_abs3(v[0], v[1], 0.f);
 #pragma unroll
         for (uint32_t j = 2; j < 16; j += 2) f = max_abs3(f, v[j], v[j + 1]);
@@ -82,7 +176,7 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-template <typename T, uint32_t FMT, uint32_t U>
+template <typename T, uint32_t FMT, uint32_t U, bool ANY>
 __global__ void __launch_bounds__(kThreads)
     mx_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, Groups groups, uint32_t cols) {
     grid_dependency_wait();
@@ -103,7 +197,12 @@ __global__ void __launch_bounds__(kThreads)
     }
 #pragma unroll
     for (uint32_t i = 0; i < U; ++i) {
-        if (!in[i]) continue;
+        if constexpr (ANY) {
+            if (!__any_sync(0xffffffffu, in[i])) continue;
+            if (!in[i]) code[i] = Word{}, scale[i] = 0;
+        } else if (!in[i]) {
+            continue;
+        }
         const float s = mx_scale_value(scale[i]);
         uint32_t h[8];
         const uint32_t *w = reinterpret_cast<const uint32_t *>(&code[i]);
@@ -128,11 +227,16 @@ __global__ void __launch_bounds__(kThreads)
             r[2 * j + 1] = from_f32<T>(f.y * s);
         }
         T *p = y + size_t(row[i]) * stride + c[i];
-        if (c[i] + 16 <= cols) {
+        const bool full = c[i] + 16 <= cols;
+        if constexpr (ANY) {
+            // The lane before holds the columns before, unless a row begins here.
+            store16_any(p, in[i] && full, c[i] != 0, raw);
+        } else if (full) {
 #pragma unroll
             for (uint32_t j = 0; j < sizeof(T) / 2; ++j)
                 stg256(reinterpret_cast<uint8_t *>(p) + 32 * j, *reinterpret_cast<const uint32_t(*)[8]>(raw + 8 * j));
-        } else {
+        }
+        if (in[i] && !full) {
 #pragma unroll
             for (uint32_t j = 0; j < 16; ++j)
                 if (c[i] + j < cols) p[j] = r[j];
@@ -140,81 +244,6 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// The same for rows that 32-byte accesses cannot serve (odd strides, unaligned pointers): a warp
-// takes a group, a lane one column of each of its four blocks, so that neighbouring lanes still
-// touch neighbouring values. About twice the instructions per value; reading 16 values a lane one
-// by one took 8 times as long as the bytes.
-constexpr uint32_t kGroupBlocks = 4;
-
-template <uint32_t FMT>
-__device__ __forceinline__ void narrow_store(const float (&v)[kGroupBlocks], uint8_t *codes, uint32_t *scale) {
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t word = 0;
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-        const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
-        word |= byte << (8 * b);
-        const float f = v[b] * mx_inverse(byte);
-        if constexpr (FMT == OPURE_MX_FP8) {
-            const uint32_t c = mx_pack_fp8(f);
-            codes[b * 32 + lane] = uint8_t(byte == 255u ? 0u : c);
-        } else {
-            const uint32_t c = mx_pack_fp4(f, __shfl_down_sync(0xffffffffu, f, 1));
-            if (lane % 2 == 0) codes[b * 16 + lane / 2] = uint8_t(byte == 255u ? 0u : c);
-        }
-    }
-    if (lane == 0) *scale = word;
-}
-
-// A lane's four columns of a group (p at the lane's first one; `left` columns from there on).
-template <typename T>
-__device__ __forceinline__ void narrow_load(const T *p, uint32_t left, float (&v)[kGroupBlocks]) {
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = b * 32 < left ? to_f32(p[b * 32]) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void narrow_write(T *p, uint32_t left, const float (&v)[kGroupBlocks]) {
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b)
-        if (b * 32 < left) p[b * 32] = from_f32<T>(v[b]);
-}
-template <typename T, uint32_t FMT>
-__global__ void __launch_bounds__(kThreads)
-    mx_quantize_narrow_kernel(const T *x, size_t stride, uint8_t *codes, uint8_t *scales, Groups groups, uint32_t cols) {
-    grid_dependency_wait();
-    grid_dependents_launch();
-    uint32_t row, c;
-    if (!groups.at((blockIdx.x * kThreads + threadIdx.x) / 32, row, c)) return;
-    c = c / 128 * 128;
-    const uint32_t first = c + (threadIdx.x & 31u);
-    float v[kGroupBlocks];
-    narrow_load(x + size_t(row) * stride + first, columns_left(cols, first), v);
-    narrow_store<FMT>(v, codes + size_t(row) * mx_row_bytes(FMT, cols) + size_t(c) * FMT / 8,
-                      reinterpret_cast<uint32_t *>(scales + mx_scale_offset(cols, row, c / kMxBlock)));
-}
-
-template <typename T, uint32_t FMT>
-__global__ void __launch_bounds__(kThreads)
-    mx_dequantize_narrow_kernel(const uint8_t *codes, const uint8_t *scales, T *y, size_t stride, Groups groups, uint32_t cols) {
-    grid_dependency_wait();
-    grid_dependents_launch();
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t row, c;
-    if (!groups.at((blockIdx.x * kThreads + threadIdx.x) / 32, row, c)) return;
-    c = c / 128 * 128;
-    const uint8_t *src = codes + size_t(row) * mx_row_bytes(FMT, cols) + size_t(c) * FMT / 8;
-    const uint32_t word = *reinterpret_cast<const uint32_t *>(scales + mx_scale_offset(cols, row, c / kMxBlock));
-    uint32_t code[kGroupBlocks];
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) code[b] = FMT == OPURE_MX_FP8 ? src[b * 32 + lane] : src[b * 16 + lane / 2] >> (lane % 2 * 4);
-    float v[kGroupBlocks];
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-        const uint32_t h = FMT == OPURE_MX_FP4 ? mx_unpack_fp4_pair(code[b] & 15u) : mx_unpack_fp8_pair(code[b]);
-        v[b] = h2f2(h).x * mx_scale_value(word >> (8 * b) & 255u);
-    }
-    narrow_write(y + size_t(row) * stride + c + lane, columns_left(cols, c + lane), v);
-}
 
 // ---- norm ---------------------------------------------------------------------------------
 struct NormParams {
@@ -353,8 +382,43 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
     }
 }
 
-// Rows that 16-byte accesses cannot serve: a lane one column of each block, as in the narrow
-// kernels above; one CTA per row, or (WARP) one warp. With KEEP a warp holds its (up to KEEP) groups
+// For rows that 16-byte accesses cannot serve a warp takes a group, a lane one column of each of its
+// four blocks, so that neighbouring lanes still touch neighbouring values.
+constexpr uint32_t kGroupBlocks = 4;
+
+template <uint32_t FMT>
+__device__ __forceinline__ void narrow_store(const float (&v)[kGroupBlocks], uint8_t *codes, uint32_t *scale) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t word = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
+        const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
+        word |= byte << (8 * b);
+        const float f = v[b] * mx_inverse(byte);
+        if constexpr (FMT == OPURE_MX_FP8) {
+            const uint32_t c = mx_pack_fp8(f);
+            codes[b * 32 + lane] = uint8_t(byte == 255u ? 0u : c);
+        } else {
+            const uint32_t c = mx_pack_fp4(f, __shfl_down_sync(0xffffffffu, f, 1));
+            if (lane % 2 == 0) codes[b * 16 + lane / 2] = uint8_t(byte == 255u ? 0u : c);
+        }
+    }
+    if (lane == 0) *scale = word;
+}
+
+// A lane's four columns of a group (p at the lane's first one; `left` columns from there on).
+template <typename T>
+__device__ __forceinline__ void narrow_load(const T *p, uint32_t left, float (&v)[kGroupBlocks]) {
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = b * 32 < left ? to_f32(p[b * 32]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void narrow_write(T *p, uint32_t left, const float (&v)[kGroupBlocks]) {
+#pragma unroll
+    for (uint32_t b = 0; b < kGroupBlocks; ++b)
+        if (b * 32 < left) p[b * 32] = from_f32<T>(v[b]);
+}
+// Rows that 16-byte accesses cannot serve: one CTA per row, or (WARP) one warp. With KEEP a warp holds its (up to KEEP) groups
 // of s; KEEP 0, for rows longer than 16384, reads x and residual twice.
 template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
 __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kernel(NormParams p) {
@@ -426,14 +490,14 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kern
 
 // The groups of a matrix, and how many each lane of the wide kernels takes: two where that still
 // fills every SM, so that more loads are in flight; one in smaller calls, where latency counts.
-bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, bool wide, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
+bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
     g.rows = m.rows;
     g.per_row = mx_kp(m.cols) / 128;
     g.magic = g.per_row == 1 ? 0 : uint32_t(0xffffffffu / g.per_row + 1);
     const uint64_t groups = uint64_t(m.rows) * g.per_row;
     if (groups >= (uint64_t(1) << 31) - kThreads) return false;
     per_lane = groups >= uint64_t(ctx->sm_count) * 8 * kThreads / 8 ? 2 : 1;
-    const uint64_t grid = wide ? (groups * 8 + kThreads * per_lane - 1) / (kThreads * per_lane) : (groups * 32 + kThreads - 1) / kThreads;
+    const uint64_t grid = (groups * 8 + kThreads * per_lane - 1) / (kThreads * per_lane);
     blocks = uint32_t(grid);
     return grid <= 0x7fffffffu / kThreads;  // thread indices are 32-bit
 }
@@ -467,7 +531,7 @@ opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, s
     Groups groups;
     uint32_t per_lane, blocks;
     const bool wide = rows_aligned32(x, x_type, x_stride);
-    if (!make_groups(ctx, *out, wide, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
+    if (!make_groups(ctx, *out, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
     return with_type(x_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
@@ -476,8 +540,8 @@ opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, s
         };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            if (!wide) return go(mx_quantize_narrow_kernel<T, F>);
-            return per_lane == 1 ? go(mx_quantize_kernel<T, F, 1>) : go(mx_quantize_kernel<T, F, 2>);
+            if (!wide) return per_lane == 1 ? go(mx_quantize_kernel<T, F, 1, true>) : go(mx_quantize_kernel<T, F, 2, true>);
+            return per_lane == 1 ? go(mx_quantize_kernel<T, F, 1, false>) : go(mx_quantize_kernel<T, F, 2, false>);
         };
         return out->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
                                            : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
@@ -493,7 +557,7 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
     Groups groups;
     uint32_t per_lane, blocks;
     const bool wide = rows_aligned32(y, y_type, y_stride);
-    if (!make_groups(ctx, *x, wide, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
+    if (!make_groups(ctx, *x, groups, per_lane, blocks)) return OPURE_ERR_UNSUPPORTED;
     return with_type(y_type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto kernel) {
@@ -502,8 +566,8 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
         };
         auto pick = [&](auto format) {
             constexpr uint32_t F = decltype(format)::value;
-            if (!wide) return go(mx_dequantize_narrow_kernel<T, F>);
-            return per_lane == 1 ? go(mx_dequantize_kernel<T, F, 1>) : go(mx_dequantize_kernel<T, F, 2>);
+            if (!wide) return per_lane == 1 ? go(mx_dequantize_kernel<T, F, 1, true>) : go(mx_dequantize_kernel<T, F, 2, true>);
+            return per_lane == 1 ? go(mx_dequantize_kernel<T, F, 1, false>) : go(mx_dequantize_kernel<T, F, 2, false>);
         };
         return x->format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
                                          : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());

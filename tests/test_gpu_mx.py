@@ -126,6 +126,37 @@ def test_quantize(ctx, t, fmt, rows, cols, stride, shift):
     assert np.array_equal(code, want_code)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shift", range(8))
+def test_quantize_and_back_from_any_address(ctx, t, shift):
+    """Every offset from a 16-byte boundary that a 2-byte type can have, and rows that end anywhere."""
+    rng = np.random.default_rng(shift)
+    for rows, cols, stride in [(3, 1100 + shift, None), (9, 16, 17), (5, 145, 149), (2, 15, None)]:
+        src, y, out = Rows(ctx, rows, cols, t, stride, shift), Rows(ctx, rows, cols, t, stride, shift), Mx(ctx, rows, cols, mx.FP8)
+        x = src.put(rng.standard_normal((rows, cols)))
+        ctx.mx_quantize(src.ptr, cu.VALUE_TYPES[t], src.stride, out.m)
+        code, byte = out.get()
+        want_code, want_byte = mx.quantize(x, mx.FP8)
+        assert np.array_equal(byte, want_byte) and np.array_equal(code, want_code)
+        ctx.mx_dequantize(out.m, y.ptr, cu.VALUE_TYPES[t], y.stride)
+        assert np.array_equal(y.get(), encode(mx.values(want_code, want_byte, cols, mx.FP8), t)[1])
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_and_back_many_unaligned_rows(ctx, t, fmt):
+    rng = np.random.default_rng(7)
+    rows, cols = 3001, 1611
+    src, y, out = Rows(ctx, rows, cols, t, None, 1), Rows(ctx, rows, cols, t, 1613, 3), Mx(ctx, rows, cols, fmt)
+    x = src.put(rng.standard_normal((rows, cols)))
+    ctx.mx_quantize(src.ptr, cu.VALUE_TYPES[t], src.stride, out.m)
+    code, byte = out.get()
+    want_code, want_byte = mx.quantize(x, fmt)
+    assert np.array_equal(byte, want_byte) and np.array_equal(code, want_code)
+    ctx.mx_dequantize(out.m, y.ptr, cu.VALUE_TYPES[t], y.stride)
+    assert np.array_equal(y.get(), encode(mx.values(want_code, want_byte, cols, fmt), t)[1])
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_quantize_special_values(ctx, fmt):
     """Empty blocks, ties, the limits of fp32, subnormals, infinities and NaN, one per block."""
