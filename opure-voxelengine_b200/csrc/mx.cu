@@ -5,6 +5,7 @@
 // 2048 fp16 to 4 bits and back 81.5 us (6,250 GB/s), the norm of 8192 x 2048 fp32 with residual and
 // sum 34.4 us (6,360 GB/s); copies run at 6,451 GB/s.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "mx.cuh"
@@ -34,10 +35,13 @@ struct Groups {
 // in registers. 10432 x 3109 fp16 to 4 bits and back: 39 us; with a warp per group and a lane per
 // column of each block, whose shuffles and small accesses the SMs cannot issue fast enough, 92 us.
 //
-// 16 values of w from `bytes` (whole values, up to 15 bytes) on.
-template <typename T>
-__device__ __forceinline__ void shift_words(const uint32_t (&w)[4 * sizeof(T) + 4], uint32_t bytes, uint32_t (&out)[4 * sizeof(T)]) {
-    constexpr uint32_t N = 4 * sizeof(T);
+template <typename T, uint32_t V>
+constexpr uint32_t kRegs = V * sizeof(T) / 4;  // of V values
+
+// V values of w, from `bytes` (whole values, at most 15 bytes) on.
+template <typename T, uint32_t V>
+__device__ __forceinline__ void shift_words(const uint32_t (&w)[kRegs<T, V> + 4], uint32_t bytes, uint32_t (&out)[kRegs<T, V>]) {
+    constexpr uint32_t N = kRegs<T, V>;
     uint32_t t[N + 2], u[N + 1];
 #pragma unroll
     for (uint32_t i = 0; i < N + 2; ++i) t[i] = bytes & 8u ? w[i + 2] : w[i];
@@ -47,17 +51,17 @@ __device__ __forceinline__ void shift_words(const uint32_t (&w)[4 * sizeof(T) + 
     for (uint32_t i = 0; i < N; ++i) out[i] = sizeof(T) == 4 ? u[i] : __funnelshift_r(u[i], u[i + 1], (bytes & 3u) * 8u);
 }
 
-// The words that hold the 16 values at p, of a matrix in [begin, end); returns how many bytes of
+// The words that hold the V values at p, of a matrix in [begin, end); returns how many bytes of
 // them come before p.
-template <typename T>
-__device__ __forceinline__ uint32_t load16_any(const T *p, const T *begin, const T *end, uint32_t (&w)[4 * sizeof(T) + 4]) {
-    constexpr uint32_t kWords = sizeof(T);  // of 16 bytes
+template <typename T, uint32_t V>
+__device__ __forceinline__ uint32_t load_any(const T *p, const T *begin, const T *end, uint32_t (&w)[kRegs<T, V> + 4]) {
+    constexpr uint32_t kWords = kRegs<T, V> / 4;  // of 16 bytes
     const uint32_t before = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
     const uintptr_t first = reinterpret_cast<uintptr_t>(p) - before;
     if (first < reinterpret_cast<uintptr_t>(begin) || first + 16 * (kWords + (before != 0)) > reinterpret_cast<uintptr_t>(end)) {
         T *r = reinterpret_cast<T *>(w);
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) r[j] = p[j];
+        for (uint32_t j = 0; j < V; ++j) r[j] = p[j];
         return 0;
     }
     const uint4 *words = reinterpret_cast<const uint4 *>(first);
@@ -75,11 +79,11 @@ __device__ __forceinline__ uint32_t load16_any(const T *p, const T *begin, const
     return before;
 }
 
-// 16 values to any address: words across two lanes are written by the later lane, if it holds all
+// V values to any address: words across two lanes are written by the later lane, if it holds all
 // of its values (full) and the lane before it the same row's (follows). All lanes of the warp call.
-template <typename T>
-__device__ __forceinline__ void store16_any(T *p, bool full, bool follows, const uint32_t (&raw)[4 * sizeof(T)]) {
-    constexpr uint32_t kWords = sizeof(T);
+template <typename T, uint32_t V>
+__device__ __forceinline__ void store_any(T *p, bool full, bool follows, const uint32_t (&raw)[kRegs<T, V>]) {
+    constexpr uint32_t kWords = kRegs<T, V> / 4;
     const uint32_t lane = threadIdx.x & 31u, before = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
     const bool joins = full && follows && lane != 0;
     const bool joined = __shfl_down_sync(0xffffffffu, joins, 1) && lane != 31;
@@ -96,7 +100,7 @@ __device__ __forceinline__ void store16_any(T *p, bool full, bool follows, const
         for (uint32_t k = 0; k < kWords; ++k) words[k] = make_uint4(raw[4 * k], raw[4 * k + 1], raw[4 * k + 2], raw[4 * k + 3]);
         return;
     }
-    shift_words<T>(w, 16 - before, out);
+    shift_words<T, V>(w, 16 - before, out);
 #pragma unroll
     for (uint32_t k = 0; k < kWords; ++k)
         if (k || joins) words[k] = make_uint4(out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
@@ -108,8 +112,8 @@ __device__ __forceinline__ void store16_any(T *p, bool full, bool follows, const
             if (j + later < kPer) p[j] = r[j];
     if (!joined)
 #pragma unroll
-        for (uint32_t j = 17 - kPer; j < 16; ++j)
-            if (j + later >= 16) p[j] = r[j];
+        for (uint32_t j = V + 1 - kPer; j < V; ++j)
+            if (j + later >= V) p[j] = r[j];
 }
 
 template <typename T, uint32_t FMT, uint32_t U, bool ANY>
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(kThreads)
         before[i] = 0;
         if (in[i] && c[i] + 16 <= cols) {
             if constexpr (ANY)
-                before[i] = load16_any(p, x, x + size_t(groups.rows - 1) * stride + cols, raw[i]);
+                before[i] = load_any<T, 16>(p, x, x + size_t(groups.rows - 1) * stride + cols, raw[i]);
             else
                 load16(p, raw[i]);
         } else {
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kThreads)
         float v[16];
         if constexpr (ANY) {
             uint32_t place[4 * sizeof(T)];
-            shift_words<T>(raw[i], before[i], place);
+            shift_words<T, 16>(raw[i], before[i], place);
 #pragma unroll
             for (uint32_t j = 0; j < 16; ++j) v[j] = to_f32(reinterpret_cast<const T *>(place)[j]);
         } else {
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(kThreads)
         const bool full = c[i] + 16 <= cols;
         if constexpr (ANY) {
             // The lane before holds the columns before, unless a row begins here.
-            store16_any(p, in[i] && full, c[i] != 0, raw);
+            store_any<T, 16>(p, in[i] && full, c[i] != 0, raw);
         } else if (full) {
 #pragma unroll
             for (uint32_t j = 0; j < sizeof(T) / 2; ++j)
@@ -272,10 +276,10 @@ __device__ __forceinline__ double row_sum(double v, double *part) {
 }
 
 // A result that lies on the other side of a rounding boundary of its code is a whole step off, so
-// the norm's own rounding is kept out of the way: squares are summed in 64 bits, the inverse root
-// is a pair of floats (one Newton step from rsqrt, with the products' rest by fma), and so is each
-// product until it is rounded to fp32 once. Six more fp32 instructions per value, which the memory
-// hides.
+// the norm's own rounding is kept out of the way: a lane's 8 squares are added in fp32, whose
+// errors even out over a row, and those sums in 64 bits; the inverse root is a pair of floats (one
+// Newton step from rsqrt, with the products' rest by fma), and so is its product with the gain, so
+// that a result is rounded once. Each square in 64 bits cost YYY.
 struct Inverse {
     float hi, lo;
 };
@@ -286,17 +290,18 @@ __device__ __forceinline__ Inverse inverse_rms(double sum_of_squares, uint32_t c
     const float lo = 0.5f * y * rest;
     return {y, isfinite(lo) ? lo : 0.f};  // m of 0 or beyond fp32: the root alone
 }
-__device__ __forceinline__ float normed(float v, Inverse inv, float gain) {
-    const float p = v * inv.hi, rest = fmaf(v, inv.hi, -p) + v * inv.lo, q = p * gain;
-    const float low = fmaf(p, gain, -q) + rest * gain;
-    return isfinite(low) ? q + low : q;
+// Inf and NaN may come out as NaN: either makes the block's scale NaN.
+__device__ __forceinline__ float normed(float v, Inverse inv) { return fmaf(v, inv.hi, v * inv.lo); }
+__device__ __forceinline__ Inverse gained(Inverse inv, float gain) {
+    const float hi = inv.hi * gain;
+    return {hi, fmaf(inv.lo, gain, fmaf(inv.hi, gain, -hi))};
 }
 
 // One CTA per row, or (WARP) one warp per row where there are many short ones: 15007 rows of 75
 // took 16 us as that many CTAs. With KEEP a thread holds its (up to KEEP) octets of s between the
 // sum of squares and the codes, so that x and residual are read once; KEEP 0, for rows longer
 // than 16384, reads them twice (the second time from L2).
-template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
+template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP, bool ANY>
 __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(NormParams p) {
     __shared__ double part[32];
     grid_dependency_wait();
@@ -310,24 +315,42 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
     T *sum = p.sum ? static_cast<T *>(p.sum) + size_t(row) * p.stride : nullptr;
     auto load = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
-        if (n == 8)
-            load8(x + c, v);
-        else
+        float t[8];
+        if (n < 8) {
             load8_part(x + c, n, v);
+            if (r) load8_part(r + c, n, t);
+        } else if constexpr (ANY) {
+            const size_t size = size_t(p.rows - 1) * p.stride + cols;
+            const T *px = static_cast<const T *>(p.x), *pr = static_cast<const T *>(p.residual);
+            uint32_t wx[kRegs<T, 8> + 4], wr[kRegs<T, 8> + 4], place[kRegs<T, 8>];
+            const uint32_t bx = load_any<T, 8>(x + c, px, px + size, wx), br = r ? load_any<T, 8>(r + c, pr, pr + size, wr) : 0u;
+            shift_words<T, 8>(wx, bx, place);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_f32(reinterpret_cast<const T *>(place)[j]);
+            if (r) {
+                shift_words<T, 8>(wr, br, place);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = to_f32(reinterpret_cast<const T *>(place)[j]);
+            }
+        } else {
+            load8(x + c, v);
+            if (r) load8(r + c, t);
+        }
         if (r) {
-            float t[8];
-            if (n == 8)
-                load8(r + c, t);
-            else
-                load8_part(r + c, n, t);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += t[j];
         }
     };
     double ss = 0.0;
     auto square = [&](const float (&v)[8]) {
+        float q = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fma(double(v[j]), double(v[j]), ss);
+        for (int j = 0; j < 8; ++j) q = fmaf(v[j], v[j], q);
+        if (q >= 0x1p-100f && q <= FLT_MAX) {
+            ss += double(q);
+        } else {  // squares that fp32 has no room for, zeros, NaN
+            for (int j = 0; j < 8; ++j) ss = fma(double(v[j]), double(v[j]), ss);
+        }
     };
     float kept[KEEP ? KEEP : 1][8];
     if constexpr (KEEP > 0) {
@@ -346,13 +369,18 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
-        // sum may be x or residual: this thread alone reads and writes these columns, and it
-        // has read them for the last time.
-        if (sum && n) {
-            if (n == 8)
+        // sum may be x or residual: this thread alone uses these columns' values and has read them
+        // for the last time; what the next lane writes of them comes from this one.
+        if (sum) {
+            if constexpr (ANY) {
+                uint32_t raw[kRegs<T, 8>];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) reinterpret_cast<T *>(raw)[j] = from_f32<T>(v[j]);
+                store_any<T, 8>(sum + c, n == 8, c != 0, raw);
+            } else if (n == 8) {
                 store8(sum + c, v);
-            else
-                store8_part(sum + c, n, v);
+            }
+            if (n < 8) store8_part(sum + c, n, v);
         }
         if (p.gain && n) {
             float g[8];
@@ -361,10 +389,10 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
             else
                 load8_part(p.gain + c, n, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], inv, g[j]);
+            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], gained(inv, g[j]));
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], inv, 1.f);
+            for (int j = 0; j < 8; ++j) v[j] = normed(v[j], inv);
         }
         const uint32_t byte = mx_store_octet<FMT>(v, codes, c / 8, c < kp);
         const uint32_t word = mx_scale_word(byte);
@@ -378,112 +406,6 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
         for (uint32_t b = 0; b < kp; b += step) {
             load(b + c0, kept[0]);
             finish(b + c0, kept[0]);
-        }
-    }
-}
-
-// For rows that 16-byte accesses cannot serve a warp takes a group, a lane one column of each of its
-// four blocks, so that neighbouring lanes still touch neighbouring values.
-constexpr uint32_t kGroupBlocks = 4;
-
-template <uint32_t FMT>
-__device__ __forceinline__ void narrow_store(const float (&v)[kGroupBlocks], uint8_t *codes, uint32_t *scale) {
-    const uint32_t lane = threadIdx.x & 31u;
-    uint32_t word = 0;
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) {
-        const uint32_t byte = mx_scale_byte<FMT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[b]) & 0x7fffffffu));
-        word |= byte << (8 * b);
-        const float f = v[b] * mx_inverse(byte);
-        if constexpr (FMT == OPURE_MX_FP8) {
-            const uint32_t c = mx_pack_fp8(f);
-            codes[b * 32 + lane] = uint8_t(byte == 255u ? 0u : c);
-        } else {
-            const uint32_t c = mx_pack_fp4(f, __shfl_down_sync(0xffffffffu, f, 1));
-            if (lane % 2 == 0) codes[b * 16 + lane / 2] = uint8_t(byte == 255u ? 0u : c);
-        }
-    }
-    if (lane == 0) *scale = word;
-}
-
-// A lane's four columns of a group (p at the lane's first one; `left` columns from there on).
-template <typename T>
-__device__ __forceinline__ void narrow_load(const T *p, uint32_t left, float (&v)[kGroupBlocks]) {
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = b * 32 < left ? to_f32(p[b * 32]) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void narrow_write(T *p, uint32_t left, const float (&v)[kGroupBlocks]) {
-#pragma unroll
-    for (uint32_t b = 0; b < kGroupBlocks; ++b)
-        if (b * 32 < left) p[b * 32] = from_f32<T>(v[b]);
-}
-// Rows that 16-byte accesses cannot serve: one CTA per row, or (WARP) one warp. With KEEP a warp holds its (up to KEEP) groups
-// of s; KEEP 0, for rows longer than 16384, reads x and residual twice.
-template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP>
-__global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_narrow_kernel(NormParams p) {
-    __shared__ double part[32];
-    grid_dependency_wait();
-    grid_dependents_launch();
-    const uint32_t row = WARP ? (blockIdx.x * kThreads + threadIdx.x) / 32 : blockIdx.x;
-    if (WARP && row >= p.rows) return;
-    const uint32_t cols = p.cols, kp = mx_kp(cols), lane = threadIdx.x & 31u;
-    const uint32_t first = WARP ? 0 : threadIdx.x / 32 * 128, step = WARP ? 128 : blockDim.x * 4;  // a warp's groups
-    const size_t base = size_t(row) * p.stride + lane;
-    const T *x = static_cast<const T *>(p.x) + base, *r = static_cast<const T *>(p.residual) + base;
-    T *sum = static_cast<T *>(p.sum) + base;
-    auto load = [&](uint32_t c, float (&v)[kGroupBlocks]) {
-        const uint32_t left = columns_left(cols, c + lane);
-        narrow_load(x + c, left, v);
-        if (p.residual) {
-            float t[kGroupBlocks];
-            narrow_load(r + c, left, t);
-#pragma unroll
-            for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] += t[b];
-        }
-    };
-    double ss = 0.0;
-    auto square = [&](const float (&v)[kGroupBlocks]) {
-#pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) ss = fma(double(v[b]), double(v[b]), ss);
-    };
-    float kept[KEEP ? KEEP : 1][kGroupBlocks];
-    if constexpr (KEEP > 0) {
-#pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)
-            if (first + i * step < kp) load(first + i * step, kept[i]);
-#pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)
-            if (first + i * step < kp) square(kept[i]);
-    } else {
-        for (uint32_t c = first; c < kp; c += step) {
-            load(c, kept[0]);
-            square(kept[0]);
-        }
-    }
-    ss = row_sum<WARP>(ss, part);
-    const Inverse inv = inverse_rms(ss, cols, p.eps);
-    uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
-    auto finish = [&](uint32_t c, float (&v)[kGroupBlocks]) {
-        const uint32_t left = columns_left(cols, c + lane);
-        // sum may be x or residual: this thread alone reads and writes these columns, and it has
-        // read them for the last time.
-        if (p.sum) narrow_write(sum + c, left, v);
-        float g[kGroupBlocks] = {1.f, 1.f, 1.f, 1.f};
-        if (p.gain) narrow_load(p.gain + c + lane, left, g);
-#pragma unroll
-        for (uint32_t b = 0; b < kGroupBlocks; ++b) v[b] = normed(v[b], inv, g[b]);
-        narrow_store<FMT>(v, codes + size_t(c) * FMT / 8,
-                          reinterpret_cast<uint32_t *>(p.scales + mx_scale_offset(cols, row, c / kMxBlock)));
-    };
-    if constexpr (KEEP > 0) {
-#pragma unroll
-        for (uint32_t i = 0; i < KEEP; ++i)
-            if (first + i * step < kp) finish(first + i * step, kept[i]);
-    } else {
-        for (uint32_t c = first; c < kp; c += step) {
-            load(c, kept[0]);
-            finish(c, kept[0]);
         }
     }
 }
@@ -587,15 +509,12 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
                        a->out.codes, a->out.scales, a->out.rows, a->out.cols, reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
     const bool wide = rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
                       rows_aligned16(a->sum, a->x_type, a->x_stride);
-    // A thread per 8 values up to 1024 threads, then two octets each; narrow rows a warp per 128
-    // values up to 8 warps, then up to four groups each. Rows of up to 512 values go one to a warp
-    // where that gives every SM 8 or more; fewer or longer ones have a CTA each, for more loads in
-    // flight.
-    const uint32_t octets = mx_kp(a->out.cols) / 8, groups = octets / 16;
+    // A thread per 8 values up to 1024 threads, then two octets each. Rows of up to 512 values go
+    // one to a warp where that gives every SM 8 or more; fewer or longer ones have a CTA each, for
+    // more loads in flight.
+    const uint32_t octets = mx_kp(a->out.cols) / 8;
     const uint32_t keep = octets <= 1024 ? 1 : octets <= 2048 ? 2 : 0;
-    const uint32_t threads = !wide  ? 32 * std::min(32u, std::max(std::min(groups, 8u), ceil_div(groups, 4)))
-                             : keep ? (ceil_div(octets, keep) + 31) / 32 * 32
-                                    : 1024;
+    const uint32_t threads = keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
     const bool warps = octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
     return with_type(a->x_type, [&](auto t) {
         using T = decltype(t);
@@ -603,19 +522,19 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
             return warps ? launch(ctx, kernel, dim3(ceil_div(a->out.rows, kThreads / 32)), dim3(kThreads), 0, true, p)
                          : launch(ctx, kernel, dim3(a->out.rows), dim3(threads), 0, true, p);
         };
-        auto pick = [&](auto format) {
+        auto pick = [&](auto format, auto any) {
             constexpr uint32_t F = decltype(format)::value;
-            if (!wide)
-                return warps  ? go(mx_rmsnorm_narrow_kernel<T, F, 4, true>)
-                       : keep ? go(mx_rmsnorm_narrow_kernel<T, F, 4, false>)
-                              : go(mx_rmsnorm_narrow_kernel<T, F, 0, false>);
-            if (warps) return octets <= 32 ? go(mx_rmsnorm_kernel<T, F, 1, true>) : go(mx_rmsnorm_kernel<T, F, 2, true>);
-            return keep == 1   ? go(mx_rmsnorm_kernel<T, F, 1, false>)
-                   : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2, false>)
-                               : go(mx_rmsnorm_kernel<T, F, 0, false>);
+            constexpr bool A = decltype(any)::value;
+            if (warps) return octets <= 32 ? go(mx_rmsnorm_kernel<T, F, 1, true, A>) : go(mx_rmsnorm_kernel<T, F, 2, true, A>);
+            return keep == 1   ? go(mx_rmsnorm_kernel<T, F, 1, false, A>)
+                   : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2, false, A>)
+                               : go(mx_rmsnorm_kernel<T, F, 0, false, A>);
         };
-        return a->out.format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>())
-                                             : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>());
+        auto pick_format = [&](auto any) {
+            return a->out.format == OPURE_MX_FP4 ? pick(std::integral_constant<uint32_t, OPURE_MX_FP4>(), any)
+                                                 : pick(std::integral_constant<uint32_t, OPURE_MX_FP8>(), any);
+        };
+        return wide ? pick_format(std::false_type()) : pick_format(std::true_type());
     });
 }
 

@@ -61,27 +61,6 @@ __device__ __forceinline__ uint32_t mx_pack_fp8(float v0, float v1, float v2, fl
         : "f"(v0), "f"(v1), "f"(v2), "f"(v3));
     return r;
 }
-// One code, and two (the first in the low half).
-__device__ __forceinline__ uint32_t mx_pack_fp8(float v) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
-    return r;
-}
-__device__ __forceinline__ uint32_t mx_pack_fp4(float lo, float hi) {
-    uint32_t r;
-    asm("{\n .reg .b8 a;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n mov.b32 %0, {a, a, a, a};\n}" : "=r"(r) : "f"(lo), "f"(hi));
-    return r & 0xffu;
-}
-__device__ __forceinline__ uint32_t mx_unpack_fp4_pair(uint32_t byte) {
-    uint32_t h;
-    asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %1;\n cvt.rn.f16x2.e2m1x2 %0, a;\n}" : "=r"(h) : "r"(byte));
-    return h;
-}
-__device__ __forceinline__ uint32_t mx_unpack_fp8_pair(uint32_t codes) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(codes)));
-    return h;
-}
 // 8 E2M1 codes -> 4 fp16 pairs (exact).
 __device__ __forceinline__ void mx_unpack_fp4(uint32_t w, uint32_t (&h)[4]) {
     asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"

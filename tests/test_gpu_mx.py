@@ -255,6 +255,24 @@ def test_rmsnorm(ctx, t, fmt, rows, cols, stride, shift):
     check_quantized(out.get(), y, cols, fmt, 2.0 ** -18, 2.0 ** -12)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shift", range(8))
+def test_rmsnorm_in_place_at_any_address(ctx, t, shift):
+    """x and the residual at different offsets from a 16-byte boundary, the sum over either: values
+    that share a word with other lanes' or rows' stay what they are."""
+    rng = np.random.default_rng(shift)
+    for rows, cols, stride in [(5, 1100 + shift, None), (3, 8, 9), (4, 145, 149), (1200, 75, None), (2, 9001, None), (2, 17001, None)]:
+        X, R = Rows(ctx, rows, cols, t, stride, shift), Rows(ctx, rows, cols, t, stride, (shift * 3 + 1) % 8)
+        x, r = X.put(rng.standard_normal((rows, cols))), R.put(rng.standard_normal((rows, cols)))
+        S, other, kept = (X, R, r) if shift % 2 else (R, X, x)
+        out = Mx(ctx, rows, cols, mx.FP8)
+        ctx.mx_rmsnorm(cu.MxNormArgs(x=X.ptr, x_type=cu.VALUE_TYPES[t], x_stride=X.stride, residual=R.ptr, sum=S.ptr, eps=1e-5, out=out.m))
+        s = x + r
+        assert (np.abs(S.get() - s) <= np.abs(s) * (2.0 ** -24 + HALF_ULP[t]) * 1.001 + TINY[t]).all()
+        assert np.array_equal(other.get(), kept)
+        check_quantized(out.get(), s / np.sqrt((s * s).mean(1, keepdims=True) + 1e-5), cols, mx.FP8, 2.0 ** -18, 2.0 ** -12)
+
+
 def test_rmsnorm_options(ctx):
     """No residual, no gain, no sum; sum over x; sum over the residual; a zero row; a NaN row."""
     rng = np.random.default_rng(5)
