@@ -255,7 +255,7 @@ struct NormParams {
     void *sum;
     size_t stride;
     const __half *gain;
-    float eps;
+    double per_col, eps;  // per_col: 1 / cols
     uint8_t *codes, *scales;
     uint32_t rows, cols;
     bool gain_vec;  // the gain allows 16-byte accesses
@@ -269,8 +269,9 @@ __device__ __forceinline__ double row_sum(double v, double *part) {
     if constexpr (!WARP) {
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = 0.0;
-        for (uint32_t w = 0; w < blockDim.x / 32; ++w) v += part[w];
+        v = (threadIdx.x & 31) < blockDim.x / 32 ? part[threadIdx.x & 31] : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     return v;
 }
@@ -279,14 +280,15 @@ __device__ __forceinline__ double row_sum(double v, double *part) {
 // the norm's own rounding is kept out of the way: a lane's 8 squares are added in fp32, whose
 // errors even out over a row, and those sums in 64 bits; the inverse root is a pair of floats (one
 // Newton step from rsqrt, with the products' rest by fma), and so is its product with the gain, so
-// that a result is rounded once. Each square in 64 bits cost YYY.
+// that a result is rounded once. Each square in 64 bits
+// cost 1831 x 7528 fp16 37 us instead of 31.
 struct Inverse {
     float hi, lo;
 };
-__device__ __forceinline__ Inverse inverse_rms(double sum_of_squares, uint32_t cols, float eps) {
-    const double m = sum_of_squares / double(cols) + double(eps);
+__device__ __forceinline__ Inverse inverse_rms(double sum_of_squares, const NormParams &p) {
+    const double m = fma(sum_of_squares, p.per_col, p.eps);
     const float mh = float(m), ml = float(m - double(mh)), y = rsqrtf(mh);
-    const float p = mh * y, rest = fmaf(-p, y, 1.0f) - fmaf(mh, y, -p) * y - ml * y * y;  // 1 - m y^2
+    const float q = mh * y, rest = fmaf(-q, y, 1.0f) - fmaf(mh, y, -q) * y - ml * y * y;  // 1 - m y^2
     const float lo = 0.5f * y * rest;
     return {y, isfinite(lo) ? lo : 0.f};  // m of 0 or beyond fp32: the root alone
 }
@@ -302,7 +304,7 @@ __device__ __forceinline__ Inverse gained(Inverse inv, float gain) {
 // sum of squares and the codes, so that x and residual are read once; KEEP 0, for rows longer
 // than 16384, reads them twice (the second time from L2).
 template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP, bool ANY>
-__global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(NormParams p) {
+__global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_rmsnorm_kernel(NormParams p) {
     __shared__ double part[32];
     grid_dependency_wait();
     grid_dependents_launch();
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : 1024) mx_rmsnorm_kernel(Norm
         }
     }
     ss = row_sum<WARP>(ss, part);
-    const Inverse inv = inverse_rms(ss, cols, p.eps);
+    const Inverse inv = inverse_rms(ss, p);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
@@ -505,15 +507,19 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
     if (a->out.rows == 0) return OPURE_OK;
     if (!a->x) return OPURE_ERR_INVALID_ARG;
     if (a->out.rows > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
-    const NormParams p{a->x, a->residual, a->sum, a->x_stride, reinterpret_cast<const __half *>(a->gain), a->eps,
+    const NormParams p{a->x, a->residual, a->sum, a->x_stride, reinterpret_cast<const __half *>(a->gain), 1.0 / a->out.cols, a->eps,
                        a->out.codes, a->out.scales, a->out.rows, a->out.cols, reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
     const bool wide = rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
                       rows_aligned16(a->sum, a->x_type, a->x_stride);
-    // A thread per 8 values up to 1024 threads, then two octets each. Rows of up to 512 values go
-    // one to a warp where that gives every SM 8 or more; fewer or longer ones have a CTA each, for
-    // more loads in flight.
+    // A thread per octet up to 1024 threads, then two octets each. Where that is more threads than
+    // the SMs hold at once, octets of 2-byte types, whose loads are half as long, go two (four) to a
+    // thread for more bytes in flight: 1831 x 7524 fp16 36 us instead of 51, 512 x 16384 bf16 18 us
+    // instead of 22; but fp32 39 us instead of 37 and, with fewer rows, 600 x 577 bf16 3.9 us
+    // instead of 3.2. Rows of up to 512 values go one to a warp where that gives every SM 8 or more;
+    // fewer or longer ones have a CTA each.
     const uint32_t octets = mx_kp(a->out.cols) / 8;
-    const uint32_t keep = octets <= 1024 ? 1 : octets <= 2048 ? 2 : 0;
+    const bool twice = type_bytes(a->x_type) == 2 && uint64_t(a->out.rows) * octets > uint64_t(ctx->sm_count) * 2048;
+    const uint32_t keep = octets > 2048 ? 0 : (octets <= 1024 ? 1 : 2) * (twice ? 2 : 1);
     const uint32_t threads = keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
     const bool warps = octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
     return with_type(a->x_type, [&](auto t) {
@@ -526,6 +532,8 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
             constexpr uint32_t F = decltype(format)::value;
             constexpr bool A = decltype(any)::value;
             if (warps) return octets <= 32 ? go(mx_rmsnorm_kernel<T, F, 1, true, A>) : go(mx_rmsnorm_kernel<T, F, 2, true, A>);
+            if constexpr (sizeof(T) == 2)
+                if (keep == 4) return go(mx_rmsnorm_kernel<T, F, 4, false, A>);
             return keep == 1   ? go(mx_rmsnorm_kernel<T, F, 1, false, A>)
                    : keep == 2 ? go(mx_rmsnorm_kernel<T, F, 2, false, A>)
                                : go(mx_rmsnorm_kernel<T, F, 0, false, A>);

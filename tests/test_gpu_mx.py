@@ -273,6 +273,30 @@ def test_rmsnorm_in_place_at_any_address(ctx, t, shift):
         check_quantized(out.get(), s / np.sqrt((s * s).mean(1, keepdims=True) + 1e-5), cols, mx.FP8, 2.0 ** -18, 2.0 ** -12)
 
 
+@pytest.mark.parametrize("t,rows,cols,stride", [
+    ("f16", 2500, 1024, None), ("bf16", 2501, 1001, None), ("f16", 330, 7524, None), ("bf16", 160, 16384, None), ("f16", 161, 16000, 16003)])
+def test_rmsnorm_more_octets_than_threads(ctx, t, rows, cols, stride):
+    rng = np.random.default_rng(rows)
+    X, R = Rows(ctx, rows, cols, t, stride), Rows(ctx, rows, cols, t, stride)
+    x, r = X.put(rng.standard_normal((rows, cols))), R.put(rng.standard_normal((rows, cols)))
+    out = Mx(ctx, rows, cols, mx.FP8)
+    ctx.mx_rmsnorm(cu.MxNormArgs(x=X.ptr, x_type=cu.VALUE_TYPES[t], x_stride=X.stride, residual=R.ptr, sum=X.ptr, eps=1e-5, out=out.m))
+    s = x + r
+    assert (np.abs(X.get() - s) <= np.abs(s) * (2.0 ** -24 + HALF_ULP[t]) * 1.001 + TINY[t]).all()
+    check_quantized(out.get(), s / np.sqrt((s * s).mean(1, keepdims=True) + 1e-5), cols, mx.FP8, 2.0 ** -18, 2.0 ** -12)
+
+
+def test_rmsnorm_of_values_whose_squares_fp32_cannot_hold(ctx):
+    """Sums of 8 squares that overflow, and squares near the last subnormal; the mean is a float."""
+    rng = np.random.default_rng(3)
+    rows, cols = 2, 640
+    X = Rows(ctx, rows, cols, "f32")
+    x = X.put(rng.standard_normal((rows, cols)) * np.array([[1e19], [1e-17]]))
+    out = Mx(ctx, rows, cols, mx.FP8)
+    ctx.mx_rmsnorm(cu.MxNormArgs(x=X.ptr, x_type=cu.F32, x_stride=cols, eps=0.0, out=out.m))
+    check_quantized(out.get(), x / np.sqrt((x * x).mean(1, keepdims=True)), cols, mx.FP8, 2.0 ** -18, 2.0 ** -12)
+
+
 def test_rmsnorm_options(ctx):
     """No residual, no gain, no sum; sum over x; sum over the residual; a zero row; a NaN row."""
     rng = np.random.default_rng(5)
