@@ -35,7 +35,6 @@ struct Groups {
 // in the aligned 16-byte words that hold a lane's values, and the values shifted into their places
 // in registers. 10432 x 3109 fp16 to 4 bits and back: 39 us; with a warp per group and a lane per
 // column of each block, whose shuffles and small accesses the SMs cannot issue fast enough, 92 us.
-//
 template <typename T, uint32_t V>
 constexpr uint32_t kRegs = V * sizeof(T) / 4;  // of V values
 
@@ -303,7 +302,8 @@ __device__ __forceinline__ Inverse gained(Inverse inv, float gain) {
 // One CTA per row, or (WARP) one warp per row where there are many short ones: 15007 rows of 75
 // took 16 us as that many CTAs. With KEEP a thread holds its (up to KEEP) octets of s between the
 // sum of squares and the codes, so that x and residual are read once; KEEP 0, for rows longer
-// than 16384, reads them twice (the second time from L2).
+// than 16384, reads them twice (the second time from L2). ANY: rows that 16-byte accesses cannot
+// serve.
 template <typename T, uint32_t FMT, uint32_t KEEP, bool WARP, bool ANY>
 __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_rmsnorm_kernel(NormParams p) {
     __shared__ double part[32];
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_r
     }
 }
 
-// The groups of a matrix, and how many each lane of the wide kernels takes: two where that still
+// The groups of a matrix, and how many each lane of its kernels takes: two where that still
 // fills every SM, so that more loads are in flight; one in smaller calls, where latency counts.
 bool make_groups(const opure_ctx *ctx, const opure_mx_matrix &m, Groups &g, uint32_t &per_lane, uint32_t &blocks) {
     g.rows = m.rows;
