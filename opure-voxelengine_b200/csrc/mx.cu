@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_r
     grid_dependency_wait();
     grid_dependents_launch();
     const uint32_t width = WARP ? 32 : blockDim.x, place = WARP ? threadIdx.x & 31u : threadIdx.x;
-    const uint32_t row = WARP ? (blockIdx.x * kThreads + threadIdx.x) / 32 : blockIdx.x;
+    const uint32_t row = WARP ? mx_warp_row(blockIdx.x, threadIdx.x, kThreads) : blockIdx.x;
     if (WARP && row >= p.rows) return;
     const uint32_t cols = p.cols, kp = mx_kp(cols), step = width * 8, c0 = place * 8;
     const T *x = static_cast<const T *>(p.x) + size_t(row) * p.stride;

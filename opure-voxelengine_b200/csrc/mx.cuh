@@ -21,6 +21,11 @@ __host__ __device__ __forceinline__ size_t mx_scale_offset(uint32_t cols, uint32
     return (size_t(row / 128) * (mx_kp(cols) / 128) + block / 4) * kMxTileBytes + row % 32 * 16 + row / 32 % 4 * 4 +
            block % 4;
 }
+// The row of a warp in a grid with a warp per row: no larger than the rows are, where the index of
+// the thread would pass 32 bits from 2^27 rows on.
+__host__ __device__ __forceinline__ uint32_t mx_warp_row(uint32_t block, uint32_t thread, uint32_t threads) {
+    return block * (threads / 32) + thread / 32;
+}
 
 __device__ __forceinline__ uint32_t columns_left(uint32_t cols, uint32_t first) { return first < cols ? cols - first : 0u; }
 
