@@ -326,7 +326,8 @@ opure_status opure_mx_dequantize(opure_ctx *ctx, const opure_mx_matrix *x, void 
 
 /* s = x + residual;  out = MX(s / sqrt(mean(s^2) + eps) * gain), per row, s in fp32: the
  * residual add (Opure_AddRes.usf:29-43) and RMSNorm (Opure_RMSNorm.usf:31-79) before a
- * linear layer in one pass. residual and sum share x's type and stride. */
+ * linear layer in one pass. residual and sum share x's type and stride. More than 2^31 - 1 rows
+ * or 2^32 - 8192 columns are refused (OPURE_ERR_UNSUPPORTED). */
 typedef struct opure_mx_norm_args {
     const void *x;             /* [out.rows][x_stride]                            */
     uint32_t x_type;           /* opure_type                                      */

@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_r
     const uint32_t width = WARP ? 32 : blockDim.x, place = WARP ? threadIdx.x & 31u : threadIdx.x;
     const uint32_t row = WARP ? mx_warp_row(blockIdx.x, threadIdx.x, kThreads) : blockIdx.x;
     if (WARP && row >= p.rows) return;
-    const uint32_t cols = p.cols, kp = mx_kp(cols), step = width * 8, c0 = place * 8;
+    const uint32_t cols = p.cols, kp = mx_kp(cols), step = width * 8, c0 = place * 8;  // no sum of these passes 2^32
     const T *x = static_cast<const T *>(p.x) + size_t(row) * p.stride;
     const T *r = p.residual ? static_cast<const T *>(p.residual) + size_t(row) * p.stride : nullptr;
     T *sum = p.sum ? static_cast<T *>(p.sum) + size_t(row) * p.stride : nullptr;
@@ -507,7 +507,7 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
         return OPURE_ERR_INVALID_ARG;
     if (a->out.rows == 0) return OPURE_OK;
     if (!a->x) return OPURE_ERR_INVALID_ARG;
-    if (a->out.rows > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
+    if (!mx_norm_takes(a->out.rows, a->out.cols)) return OPURE_ERR_UNSUPPORTED;
     const NormParams p{a->x, a->residual, a->sum, a->x_stride, reinterpret_cast<const __half *>(a->gain), 1.0 / a->out.cols, a->eps,
                        a->out.codes, a->out.scales, a->out.rows, a->out.cols, reinterpret_cast<uintptr_t>(a->gain) % 16 == 0};
     const bool wide = rows_aligned16(a->x, a->x_type, a->x_stride) && rows_aligned16(a->residual, a->x_type, a->x_stride) &&
@@ -521,7 +521,7 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a) {
     const uint32_t octets = mx_kp(a->out.cols) / 8;
     const bool twice = type_bytes(a->x_type) == 2 && uint64_t(a->out.rows) * octets > uint64_t(ctx->sm_count) * 2048;
     const uint32_t keep = octets > 2048 ? 0 : (octets <= 1024 ? 1 : 2) * (twice ? 2 : 1);
-    const uint32_t threads = keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : 1024;
+    const uint32_t threads = keep ? (ceil_div(octets, keep) + 31) / 32 * 32 : kMxNormStep / 8;
     const bool warps = octets <= 64 && a->out.rows >= uint32_t(ctx->sm_count) * 8;
     return with_type(a->x_type, [&](auto t) {
         using T = decltype(t);

@@ -195,6 +195,11 @@ __device__ __forceinline__ uint32_t mx_scale_word(uint32_t byte) {
     return s;
 }
 
+// The norm goes over a row longer than 16384 columns this many at a time, counted in 32 bits, which
+// the last step must not pass; and over rows with a 31-bit grid.
+constexpr uint32_t kMxNormStep = 8192;
+inline bool mx_norm_takes(uint32_t rows, uint32_t cols) { return rows <= 0x7fffffffu && cols <= 0u - kMxNormStep; }
+
 // ---- host checks -------------------------------------------------------------------------
 inline bool mx_valid(const opure_mx_matrix &m) {
     return (m.format == OPURE_MX_FP4 || m.format == OPURE_MX_FP8) && m.cols != 0 && m.cols <= 0xffffff80u &&

@@ -35,3 +35,16 @@ def test_rmsnorm_of_2_to_27_rows(ctx):
         tail = scales.download(np.uint8, cu.mx_scale_bytes(at + seen - first, cols), first // 128 * 512)
         assert np.array_equal(mx.untile(tail, at + seen - first, cols)[at - first:], byte)
     assert (codes.download(np.uint8, 64, (rows // 2) * 64) == 0).all()
+
+
+def test_rmsnorm_refuses_what_it_cannot_count(ctx):
+    """Sizes alone: refused before anything is launched, so no memory of that size is needed."""
+    x = ctx.buffer(1024)
+
+    def norm(rows, cols):
+        ctx.mx_rmsnorm(cu.MxNormArgs(x=x.ptr, x_type=cu.F16, x_stride=1 << 32, eps=1.0, out=cu.MxMatrix(x.ptr, x.ptr, rows, cols, mx.FP8)))
+
+    for rows, cols in [(1, 2 ** 32 - 8191), (1, 0xffffff80), (2 ** 31, 1)]:
+        with pytest.raises(cu.OpureError) as e:
+            norm(rows, cols)
+        assert e.value.status == cu.ERR_UNSUPPORTED
