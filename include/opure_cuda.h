@@ -346,7 +346,8 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a);
  *   OPURE_EPI_ADD     y = residual + acc (residual may be y; same type and stride)
  *   OPURE_EPI_SWIGLU  w is [gate; up] (w.rows even): out = MX(silu(gate) * up), the next
  *                     product's x, out.cols = w.rows / 2; y is not used
- * Any number of rows, from one token to a long prompt. */
+ * A result is finite where every block's two scales multiply to at most 2^127 and no sum of its
+ * blocks passes fp32. Any number of rows, from one token to a long prompt. */
 typedef struct opure_mx_gemm_args {
     opure_mx_matrix w;         /* [rows][cols]                                    */
     opure_mx_matrix x;         /* [tokens][cols]                                  */

@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
             for (uint32_t j = 0; j < 2; ++j) {
                 float s0, s1;
                 scale_pair(wt.s[2 * m + j], s0, s1);
-                sum_of[2 * m + j] = fmaf(d[2 * j] * x0, s0, fmaf(d[2 * j + 1] * x1, s1, sum_of[2 * m + j]));
+                // The scales first: d times one of them can pass fp32 where the other would bring it back.
+                sum_of[2 * m + j] = fmaf(d[2 * j], x0 * s0, fmaf(d[2 * j + 1], x1 * s1, sum_of[2 * m + j]));
             }
         }
     };
