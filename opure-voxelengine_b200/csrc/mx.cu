@@ -282,21 +282,36 @@ __device__ __forceinline__ double row_sum(double v, double *part) {
 // Newton step from rsqrt, with the products' rest by fma), and so is its product with the gain, so
 // that a result is rounded once. Each square in 64 bits
 // cost 1831 x 7528 fp16 37 us instead of 31.
+//
+// Where the mean square m leaves the middle of fp32's range, values are first multiplied by a power
+// of two (`pre`) that brings it back, and the root is taken of m pre^2: every finite row has a norm,
+// from subnormals to the largest values (8192 x 2048 bf16 28.3 us; without the test 27.9).
 struct Inverse {
-    float hi, lo;
+    float hi, lo, pre;
 };
+// WIDE: T has such values (fp16 has not).
+template <bool WIDE>
 __device__ __forceinline__ Inverse inverse_rms(double sum_of_squares, const NormParams &p) {
-    const double m = fma(sum_of_squares, p.per_col, p.eps);
-    const float mh = float(m), ml = float(m - double(mh)), y = rsqrtf(mh);
+    double m = fma(sum_of_squares, p.per_col, p.eps);
+    float mh = float(m), pre = 1.f;
+    if (WIDE && __builtin_expect(!(mh >= 0x1p-100f && mh <= 0x1p100f), 0)) {
+        const int e = int(uint32_t(__double2hiint(m)) >> 20 & 0x7ffu) - 1023;  // |m| is 2^e or more, 0 2^-1023
+        const int half = min(max(e / 2, -120), 120);
+        pre = __uint_as_float(uint32_t(127 - half) << 23);
+        m *= __hiloint2double((1023 - 2 * half) << 20, 0);
+        mh = float(m);
+        asm volatile("");  // a branch, not predicated instructions for every row
+    }
+    const float ml = float(m - double(mh)), y = rsqrtf(mh);
     const float q = mh * y, rest = fmaf(-q, y, 1.0f) - fmaf(mh, y, -q) * y - ml * y * y;  // 1 - m y^2
     const float lo = 0.5f * y * rest;
-    return {y, isfinite(lo) ? lo : 0.f};  // m of 0 or beyond fp32: the root alone
+    return {y, isfinite(lo) ? lo : 0.f, pre};  // m of 0, infinity or NaN: the root alone
 }
 // Inf and NaN may come out as NaN: either makes the block's scale NaN.
 __device__ __forceinline__ float normed(float v, Inverse inv) { return fmaf(v, inv.hi, v * inv.lo); }
 __device__ __forceinline__ Inverse gained(Inverse inv, float gain) {
     const float hi = inv.hi * gain;
-    return {hi, fmaf(inv.lo, gain, fmaf(inv.hi, gain, -hi))};
+    return {hi, fmaf(inv.lo, gain, fmaf(inv.hi, gain, -hi)), 1.f};
 }
 
 // One CTA per row, or (WARP) one warp per row where there are many short ones: 15007 rows of 75
@@ -368,7 +383,8 @@ __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_r
         }
     }
     ss = row_sum<WARP>(ss, part);
-    const Inverse inv = inverse_rms(ss, p);
+    constexpr bool kWide = !std::is_same_v<T, __half>;
+    const Inverse inv = inverse_rms<kWide>(ss, p);
     uint8_t *codes = p.codes + size_t(row) * mx_row_bytes(FMT, cols);
     auto finish = [&](uint32_t c, float (&v)[8]) {
         const uint32_t n = c < cols ? min(cols - c, 8u) : 0u;
@@ -385,6 +401,9 @@ __global__ void __launch_bounds__(WARP ? kThreads : KEEP == 4 ? 512 : 1024) mx_r
             }
             if (n < 8) store8_part(sum + c, n, v);
         }
+        if (kWide && inv.pre != 1.f)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= inv.pre;
         if (p.gain && n) {
             float g[8];
             if (p.gain_vec && n == 8)
