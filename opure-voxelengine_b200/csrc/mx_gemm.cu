@@ -298,8 +298,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         if constexpr (kSwiglu) {
             constexpr uint32_t kF = sizeof(T) == 1 ? OPURE_MX_FP8 : OPURE_MX_FP4;
 #pragma unroll
+            for (uint32_t j = 0; j < 4; j += 2) swiglu2(v[0][j], v[0][j + 1], v[1][j], v[1][j + 1]);
+#pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-                v[0][j] = col + j < p.half ? swiglu(v[0][j], v[1][j]) : 0.f;  // gate rows past the half are up rows
+                if (col + j >= p.half) v[0][j] = 0.f;  // gate rows past the half are up rows
             store_block<kF>(v[0], p.out + i * mx_row_bytes(kF, p.half) + size_t(col0) * kF / 8,
                             p.outs + mx_scale_offset(p.half, i, col0 / 32), i < p.n && col0 < mx_kp(p.half));
         } else if (i < p.n) {

@@ -341,10 +341,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     float v[32];
                     if (b) {
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) v[q] = swiglu(__uint_as_float(pre[j][q]), __uint_as_float(cur[q]));
+                        for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(pre[j][q]);
+#pragma unroll
+                        for (int q = 0; q < 32; q += 2) swiglu2(v[q], v[q + 1], __uint_as_float(cur[q]), __uint_as_float(cur[q + 1]));
                     } else {
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) v[q] = swiglu(__uint_as_float(cur[q]), __uint_as_float(pre[j][q]));
+                        for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(cur[q]);
+#pragma unroll
+                        for (int q = 0; q < 32; q += 2) swiglu2(v[q], v[q + 1], __uint_as_float(pre[j][q]), __uint_as_float(pre[j][q + 1]));
                     }
                     if (col + 32 > p.half) {
 #pragma unroll

@@ -202,7 +202,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
         for (uint32_t j = 0; j < 4; ++j) v[j] = sum(c + j, token);
         if (swiglu) {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) v[j] = col + j < p.half ? silu(v[j]) * sum(32 + c + j, token) : 0.f;
+            for (uint32_t j = 0; j < 4; j += 2) swiglu2(v[j], v[j + 1], sum(32 + c + j, token), sum(33 + c + j, token));
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (col + j >= p.half) v[j] = 0.f;  // gate rows past the half repeat the last one
             uint8_t *scale = p.outs + mx_scale_offset(p.half, token, c0 / 32);
             if (p.out_format == OPURE_MX_FP4)
                 store_block<OPURE_MX_FP4>(v, p.out + token * mx_row_bytes(OPURE_MX_FP4, p.half) + size_t(c0) / 2, scale, real);
