@@ -347,7 +347,13 @@ opure_status opure_mx_rmsnorm(opure_ctx *ctx, const opure_mx_norm_args *a);
  *   OPURE_EPI_SWIGLU  w is [gate; up] (w.rows even): out = MX(silu(gate) * up), the next
  *                     product's x, out.cols = w.rows / 2; y is not used
  * A result is finite where every block's two scales multiply to at most 2^127 and no sum of its
- * blocks passes fp32. Any number of rows, from one token to a long prompt. */
+ * blocks passes fp32.
+ * From one token to 65535 * 128, up to 2^30 rows and columns of w; more is refused
+ * (OPURE_ERR_UNSUPPORTED). So is OPURE_EPI_SWIGLU with three or more tokens where w.rows / 2 is no
+ * multiple of 128 and w has more than half a billion values: the call then sorts the scales of both
+ * halves into tiles of their own, and the ctx's workspace holds 16 MiB of them. A gate half padded
+ * with zero rows to a multiple of 128 (and the up half likewise) needs no sorting; out's padding to
+ * 128 columns takes the results of those rows. */
 typedef struct opure_mx_gemm_args {
     opure_mx_matrix w;         /* [rows][cols]                                    */
     opure_mx_matrix x;         /* [tokens][cols]                                  */

@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // Scale tiles of the two halves of a matrix, each as a matrix of its own, one after the other:
-// what SwiGLU needs when the second half does not start on a tile. One thread per (row, 128
+// what SwiGLU on the tensor cores needs when the second half does not start on a tile. One thread per (row, 128
 // columns).
 __global__ void __launch_bounds__(256) mx_split_scales_kernel(const uint8_t *src, uint8_t *dst, uint32_t half, uint32_t kblocks) {
     grid_dependency_wait();
@@ -417,6 +417,7 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     p.st = ctx->status;
     // Grid dimensions and TMA's 32-bit signed coordinates.
     if (p.n > 65535u * kM || p.rows > (1u << 30) || a->w.cols > (1u << 30)) return OPURE_ERR_UNSUPPORTED;
+    if (mx_gemv_suits(a)) return mx_gemv(ctx, a);
     const uint32_t tiles = swiglu ? mx_kp(p.half) / (kN / 2) : ceil_div(p.rows, kN);
     const uint32_t mtiles = ceil_div(p.n, kM);
     const uint64_t here_ns = choose_splits(p, uint64_t(tiles) * mtiles, swiglu, uint32_t(ctx->sm_count));
@@ -453,7 +454,6 @@ opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a) {
         }
         p.us = p.ws + side;
     }
-    if (mx_gemv_suits(a)) return mx_gemv(ctx, a, p.ws, p.us);
     if (mx_gemm_pair_ns(ctx, a) < here_ns) return mx_gemm_pair(ctx, a, p.ws);
     CUtensorMap wm, xm;
     if (!make_slot_map(&wm, a->w, swiglu ? kN / 2 : kN) || !make_slot_map(&xm, a->x, p.a_rows)) return OPURE_ERR_UNSUPPORTED;

@@ -126,9 +126,8 @@ inline bool make_slot_map(CUtensorMap *m, const opure_mx_matrix &a, uint32_t box
 uint64_t mx_gemm_pair_ns(const opure_ctx *ctx, const opure_mx_gemm_args *a);  // estimated time
 opure_status mx_gemm_pair(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *w_scales);
 
-// The product for one or two tokens, weights streamed through registers (a already validated; ws and us the
-// scale tiles of w, or in SwiGLU of its gate and its up half).
+// The product for one or two tokens, weights streamed through registers (a already validated).
 bool mx_gemv_suits(const opure_mx_gemm_args *a);
-opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *ws, const uint8_t *us);
+opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a);
 
 }  // namespace opure

@@ -34,7 +34,7 @@ constexpr uint32_t kMaxTokens = 2;  // from 3 on mx_gemm.cu is as fast (4 x 2048
 constexpr uint32_t kMaxWarps = 16;
 
 struct GemvParams {
-    const uint8_t *w, *ws, *us, *x, *xs;
+    const uint8_t *w, *ws, *x, *xs;
     uint32_t n, rows, cols, half, units, splits;
     uint32_t epilogue, y_type, out_format;
     void *y;
@@ -84,18 +84,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32) mx_gemv_kernel(GemvParams p) {
     const uint32_t pieces = mx_kp(p.cols) / 128;
     const bool swiglu = p.epilogue == OPURE_EPI_SWIGLU;
     // This warp's rows. In SwiGLU (two tiles a warp) unit 0 is 32 gate rows and unit 1 the up rows
-    // that go with them, whose scale tiles are counted from the first up row.
-    const bool up = swiglu && unit;
+    // that go with them.
     const uint32_t c0 = blockIdx.x * (swiglu ? 32 : p.units * kRows);  // first result column of the CTA
     const uint32_t local = c0 + (swiglu ? 0 : unit * kRows) + g;
-    const uint32_t limit = swiglu ? p.half : p.rows, first = up ? p.half : 0;
+    const uint32_t limit = swiglu ? p.half : p.rows, first = swiglu && unit ? p.half : 0;
     const size_t row_bytes = mx_row_bytes(OPURE_MX_FP4, p.cols);
     const uint8_t *w[2 * MT], *ws[2 * MT];
 #pragma unroll
     for (uint32_t j = 0; j < 2 * MT; ++j) {
         const uint32_t r = min(local + 8 * j, limit - 1);  // rows past the end repeat the last one
         w[j] = p.w + (first + r) * row_bytes + t * 16;
-        ws[j] = (up ? p.us : p.ws) + mx_scale_offset(p.cols, r, 0) + t % 2 * 2;
+        ws[j] = p.ws + mx_scale_offset(p.cols, first + r, 0) + t % 2 * 2;
     }
     // The weights may be asked for before the kernel that this one waits for has ended, into L2
     // only, where a late write of its would show.
@@ -262,12 +261,11 @@ void choose(GemvParams &p, uint32_t pieces, uint32_t units_all, uint32_t cta_uni
 
 bool mx_gemv_suits(const opure_mx_gemm_args *a) { return a->x.rows <= kMaxTokens; }
 
-opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a, const uint8_t *ws, const uint8_t *us) {
+opure_status mx_gemv(opure_ctx *ctx, const opure_mx_gemm_args *a) {
     const bool swiglu = a->epilogue == OPURE_EPI_SWIGLU, fp8 = a->x.format == OPURE_MX_FP8;
     GemvParams p{};
     p.w = a->w.codes;
-    p.ws = ws;
-    p.us = us;
+    p.ws = a->w.scales;
     p.x = a->x.codes;
     p.xs = a->x.scales;
     p.n = a->x.rows;
