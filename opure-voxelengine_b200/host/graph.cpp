@@ -180,6 +180,7 @@ void Graph::PlanLayout(const LayoutOptions &opts) {
         cur = Align(cur + bytes, 256);
         return at;
     };
+    plan_.gateRows = plan_.mx ? uint32_t(Align(ff, 128)) : uint32_t(ff);
     auto matrix = [&](uint64_t rows, uint64_t cols) {
         return place(plan_.mx ? MxScalesAt(rows, cols) + opure_mx_scale_bytes(uint32_t(rows), uint32_t(cols)) : rows * cols * eb);
     };
@@ -202,7 +203,7 @@ void Graph::PlanLayout(const LayoutOptions &opts) {
         t.postAttNorm = place(h * 2);
         t.wqkv = matrix(qkv, h);
         t.wo = matrix(h, att);
-        t.wgu = matrix(2 * ff, h);
+        t.wgu = matrix(2 * uint64_t(plan_.gateRows), h);
         t.wdown = matrix(h, ff);
         if (plan_.hasFused) {
             t.woBlk = place(h * h * eb);
@@ -219,7 +220,8 @@ uint64_t Graph::StreamBytes() const {
     const uint64_t h = cfg_.hiddenSize, ff = local_.inter, hd = cfg_.HeadDim();
     const uint64_t qkv = local_.QkvRows(uint32_t(hd)), att = uint64_t(local_.heads) * hd;
     auto mx = [](uint64_t rows, uint64_t cols) { return rows * (cols / 2 + (cols + 31) / 32); };
-    const uint64_t matrices = plan_.mx ? mx(qkv, h) + mx(h, att) + mx(2 * ff, h) + mx(h, ff) : (qkv * h + h * att + 3 * ff * h) * eb;
+    const uint64_t matrices = plan_.mx ? mx(qkv, h) + mx(h, att) + mx(2 * uint64_t(plan_.gateRows), h) + mx(h, ff)
+                                       : (qkv * h + h * att + 3 * ff * h) * eb;
     const uint64_t perLayer = matrices + 2 * h * 2;
     return perLayer * cfg_.numLayers + uint64_t(local_.vocab) * h * (plan_.lmQuantized ? 1 : 2) + h * 2;
 }
@@ -256,9 +258,10 @@ void Graph::UploadWeights(opure_ctx *ctx, void *arena) {
         void *p = nullptr;
         ~DeviceTemp() { opure_free(ctx, p); }
     } whole{ctx};
+    const uint64_t gateRows = plan_.gateRows;
     if (plan_.mx) {
         const uint64_t qkvRows = local_.QkvRows(hd);
-        OPURE_CUDA_CHECK(opure_alloc(ctx, std::max({qkvRows * h, 2 * ff * h, h * h}) * 2, &whole.p));
+        OPURE_CUDA_CHECK(opure_alloc(ctx, std::max({qkvRows * h, 2 * gateRows * h, h * h}) * 2, &whole.p));
     }
     // Part of a layer matrix, `within` bytes from its start.
     auto put_part = [&](uint64_t off, uint64_t within, const std::vector<uint8_t> &bytes) {
@@ -332,10 +335,12 @@ void Graph::UploadWeights(opure_ctx *ctx, void *arena) {
         fetch(b.gate, stage, q8);
         rows(stage, h, uint64_t(tr) * ffl, ffl);
         put_part(t.wgu, 0, stage);
+        if (gateRows != ffl)  // zeros, of which the up rows then leave the padding
+            OPURE_CUDA_CHECK(opure_fill(ctx, static_cast<uint8_t *>(whole.p) + ffl * h * eb, 0, (2 * gateRows - ffl) * h * eb));
         fetch(b.up, stage, q8);
         rows(stage, h, uint64_t(tr) * ffl, ffl);
-        put_part(t.wgu, ffl * h * eb, stage);
-        finish(t.wgu, 2 * ffl, h);
+        put_part(t.wgu, gateRows * h * eb, stage);
+        finish(t.wgu, 2 * gateRows, h);
         fetch(b.down, a, q8);
         cols_of(a, h, ff, uint64_t(tr) * ffl, ffl);
         put_part(t.wdown, 0, a);

@@ -80,6 +80,9 @@ struct VramPlan {
     // Layer matrices as MXFP4 (opure_mx_matrix): at each matrix's offset its codes, then, from
     // the next multiple of 256 bytes, its scales.
     bool mx = false;
+    // Rows of the gate and of the up half of wgu as they are placed: with microscaled weights a multiple
+    // of 128, zeros past the model's, so that either half begins on a tile of scales.
+    uint32_t gateRows = 0;
     uint64_t weightBytes = 0;
 };
 

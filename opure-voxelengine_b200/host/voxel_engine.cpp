@@ -286,6 +286,7 @@ void VoxelEngine::RecordLayerMx(uint32_t L, uint32_t n) {
     const graph::ModelConfig &c = graph_.Config();
     const graph::VramPlan::LayerTensors &t = graph_.Plan().layers[L];
     const uint32_t h = c.hiddenSize, ff = c.intermediateSize, qkvRows = c.QkvRows(), att = c.numHeads * c.HeadDim();
+    const uint32_t gateRows = graph_.Plan().gateRows;  // ff up to a multiple of 128
     auto rows = [&](opure_mx_matrix m) {
         m.rows = n;
         return m;
@@ -312,7 +313,10 @@ void VoxelEngine::RecordLayerMx(uint32_t L, uint32_t n) {
         a.y_type = OPURE_F32;
         a.y_stride = outRows;
         if (epilogue == OPURE_EPI_ADD) a.residual = y;
-        if (epilogue == OPURE_EPI_SWIGLU) a.out = act;
+        if (epilogue == OPURE_EPI_SWIGLU) {
+            a.out = act;  // the padding rows' results are the padding that act has anyway
+            a.out.cols = gateRows;
+        }
         OPURE_CUDA_CHECK(opure_mx_gemm(ctx_, &a));
     };
     normed(buf_.x, t.inputNorm, nullptr);
@@ -321,7 +325,7 @@ void VoxelEngine::RecordLayerMx(uint32_t L, uint32_t n) {
     OPURE_CUDA_CHECK(opure_mx_quantize(ctx_, buf_.attn, OPURE_F32, att, &attn));
     product(t.wo, h, att, attn, OPURE_EPI_STORE, buf_.partial);
     normed(buf_.partial, t.postAttNorm, buf_.x);
-    product(t.wgu, 2 * ff, h, norm, OPURE_EPI_SWIGLU, nullptr);
+    product(t.wgu, 2 * gateRows, h, norm, OPURE_EPI_SWIGLU, nullptr);
     product(t.wdown, h, ff, act, OPURE_EPI_ADD, buf_.x);
 }
 
