@@ -199,7 +199,7 @@ void VoxelEngine::AllocBuffers() {
         buf_.packAct = packed(c.intermediateSize);
         buf_.sumsq = Alloc<float>(ctx_, size_t((c.hiddenSize + 127) / 128) * nv);
     }
-    if (comm_) buf_.partial = Alloc<float>(ctx_, size_t(B) * c.hiddenSize);
+    if (comm_ && !buf_.partial) buf_.partial = Alloc<float>(ctx_, size_t(B) * c.hiddenSize);
     buf_.sync = Alloc<uint32_t>(ctx_, 3 * size_t(c.numLayers) + 1);
     if (opts_.phaseTrace) {
         opure_device_info di{};

@@ -1,6 +1,8 @@
 """The engine over 4-bit microscaled weights: what it keeps, and the ways to it."""
 import pytest
+import torch
 
+from voxelengine import cuda as cu
 from voxelengine import engine as ve
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +21,20 @@ def test_gate_and_up_begin_on_tiles(model, tmp_path):
     with ve.Engine(model, max_len=64, weights=ve.WEIGHTS_MXFP4) as a, ve.Engine(whole, max_len=64, weights=ve.WEIGHTS_MXFP4) as b:
         assert a.info.inter == 336 and b.info.inter == 384
         assert a.info.weight_bytes == b.info.weight_bytes
+
+
+def test_one_rank_of_tensor_parallelism(model):
+    """A communicator of one rank holds the whole model: the same tokens, and all memory comes back."""
+    prompt = [int(t) for t in ve.prompt(2, SPEC["vocab"], 7)]
+    with ve.Engine(model, max_len=64, weights=ve.WEIGHTS_MXFP4) as eng:
+        want = eng.generate([prompt], 6)[0][0]
+    with cu.Ctx(0) as ctx:
+        comm = cu.Comm(ctx, 1, 0, cu.comm_unique_id())
+        free = []
+        for _ in range(5):
+            with ve.Engine(model, max_len=64, max_batch=8192, weights=ve.WEIGHTS_MXFP4, comm=comm) as eng:
+                assert [int(t) for t in eng.generate([prompt], 6)[0][0]] == [int(t) for t in want]
+            ctx.sync()
+            free.append(torch.cuda.mem_get_info()[0])
+        comm.close()
+    assert free[1:] == free[:-1], free  # 8192 rows of 192 values are 6 MB
