@@ -1,7 +1,12 @@
 """The engine over 4-bit microscaled weights: what it keeps, and the ways to it."""
+import http.client
+import json
+
+import numpy as np
 import pytest
 import torch
 
+from test_gpu_mx_engine import Forward
 from voxelengine import cuda as cu
 from voxelengine import engine as ve
 
@@ -38,3 +43,57 @@ def test_one_rank_of_tensor_parallelism(model):
             free.append(torch.cuda.mem_get_info()[0])
         comm.close()
     assert free[1:] == free[:-1], free  # 8192 rows of 192 values are 6 MB
+
+
+def test_server_over_microscaled_weights(model):
+    """POST /generate gives the microscaled engine's tokens, which are not the stored weights'."""
+    prompt = [int(t) for t in ve.prompt(3, SPEC["vocab"], 9)]
+    with ve.Engine(model, max_len=64, weights=ve.WEIGHTS_MXFP4) as eng:
+        want = [int(t) for t in eng.generate([prompt], 12)[0][0]]
+    with ve.Server(model, devices=[0], max_len=64, weights=ve.WEIGHTS_MXFP4) as s:
+        c = http.client.HTTPConnection("127.0.0.1", s.port, timeout=60)
+        c.request("POST", "/generate", json.dumps({"tokens": prompt, "max_tokens": 12}))
+        r = c.getresponse()
+        got = json.loads(r.read())
+        c.close()
+    assert r.status == 200 and got["tokens"] == want
+
+
+def test_after_work_of_another_stream(model):
+    """Memory that another stream (here torch's) writes and reads: ordered on the device, in both
+    directions, through the stream that opure_stream gives."""
+    n, cols = 4096, 4096
+    with cu.Ctx(0) as ctx:
+        own = torch.cuda.ExternalStream(cu.lib().opure_stream(ctx.h))
+        side = torch.cuda.Stream()
+        q = ctx.mx_matrix(n, cols, cu.MX_FP8)
+        x, y = torch.zeros(n, cols, device="cuda"), torch.zeros(n, cols, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for k in range(5):
+                big = torch.full((n, cols), float(k), device="cuda")
+                for _ in range(20):
+                    big = big * 1.0
+                x.copy_(big)              # not there yet when the next lines run
+                own.wait_stream(side)
+                ctx.mx_quantize(x.data_ptr(), cu.F32, cols, q)
+                ctx.mx_dequantize(q, y.data_ptr(), cu.F32, cols)
+                side.wait_stream(own)
+                got = y.clone()
+                y.zero_()
+                assert bool((got == float(k)).all())
+        torch.cuda.synchronize()
+
+
+def test_logits_are_those_of_the_definition(model):
+    """Against the 64-bit forward. What differs: an 8-bit operand whose value lies within fp32's error of
+    a rounding boundary is a step off (16,000 operands for 9 positions, a chance of 2^-15 each: under
+    0.5 expected, each 2^-3.5 of one of 192 inputs, 0.6% of a layer's share), and a few fp16 keys and
+    values likewise (6e-5 each). So most prompts agree to 1e-3 of the logits' spread, all to 2e-2."""
+    forward, errors = Forward(model), []
+    with ve.Engine(model, max_len=64, weights=ve.WEIGHTS_MXFP4) as eng:
+        for seed in range(11):
+            prompt = [int(t) for t in ve.prompt(50 + seed, SPEC["vocab"], 9)]
+            want = forward.logits(prompt)[-1]
+            errors.append(np.sqrt(np.mean((eng.forward_logits(prompt) - want) ** 2)) / want.std())
+    assert np.median(errors) <= 1e-3 and max(errors) <= 2e-2, errors
