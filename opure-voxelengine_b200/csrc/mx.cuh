@@ -37,8 +37,8 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
     if (amax_bits >= 0x7f800000u) return 255u;
     return uint32_t(max(int(amax_bits >> 23) - kEmax, 0));
 }
-// 2^(127 - byte): what a block's values are multiplied by. Exact for every byte below 255
-// (the quantiser's are at most 252); 0 for 255, whose codes are 0.
+// 2^(127 - byte): what a block's values are multiplied by. Exact for bytes up to 253 (those of finite
+// blocks are at most 252); 0 for 255, whose codes are 0.
 __device__ __forceinline__ float mx_inverse(uint32_t byte) {
     return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
 }

@@ -26,11 +26,6 @@ __device__ __forceinline__ void prefetch_2d(bool one, const CUtensorMap *map, ui
         "r"(x), "r"(y), "r"(uint32_t(one))
         : "memory");
 }
-__device__ __forceinline__ void prefetch(bool one, const void *p, uint32_t bytes) {
-    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %2, 0;\n @e cp.async.bulk.prefetch.L2.global [%0], %1;\n}" ::"l"(p), "r"(bytes),
-                 "r"(uint32_t(one))
-                 : "memory");
-}
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
