@@ -54,7 +54,10 @@ enum {
                                  0.53 bytes per weight in memory and per step; the linear
                                  layers then take 8-bit microscaled inputs (opure_mx_gemm).
                                  Embeddings, norms and the lm_head stay fp16. Per-op kernels
-                                 only; floating-point models on one GPU                     */
+                                 only, so that a small model at batch 1 is faster with stored
+                                 weights and their persistent step (135M shape: 2,233 against
+                                 1,245 tokens/s; 1.7B shape: 525 against 1,054);
+                                 floating-point models on one GPU                           */
 };
 
 enum {

@@ -3,8 +3,8 @@
 //
 // All three are bound by memory: a value is read once and its code written once. Measured: 49152 x
 // 2048 fp16 to 4 bits and back 81.5 us (6,250 GB/s), the norm of 8192 x 2048 fp32 with residual and
-// sum 34.4 us (6,360 GB/s); copies run at 6,451 GB/s. The norm of 2-byte types is bound by instructions
-// (8192 x 2048 fp16 26.7 us, 18.3 us for the bytes): 8 values a lane share a scale's work.
+// sum 34.3 us (6,370 GB/s); copies run at 6,451 GB/s. The norm of 2-byte types is bound by instructions
+// (8192 x 2048 fp16 26.5 us, bf16 28.3 us, 18.3 us for the bytes): 8 values a lane share a scale's work.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>

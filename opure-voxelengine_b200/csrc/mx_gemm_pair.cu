@@ -21,10 +21,10 @@
 // even CTA holds gate rows and the odd CTA the up rows that go with them; a thread owns a token's
 // 32 columns, which is a block of the MX result.
 //
-// Measured in short bursts (and back to back, where the power limit lowers the clock): 4096 x 16384
-// x 2048 with 8-bit tokens and SwiGLU 98 (112) us, 2.8 (2.4) PFLOP/s; 8192 x 16384 x 2048 with
-// 4-bit tokens to fp16 124 (138) us, 4.4 (4.0) PFLOP/s. Of a tile's 11,200 clocks with 8-bit tokens
-// the tensor cores need 8,192; 2,300 go where the next tile waits for the shared columns.
+// Measured back to back, where the power limit lowers the clock: 4096 x 16384 x 2048 with 8-bit tokens
+// and SwiGLU 118 us (102 to 107 us on another B200), 2.3 PFLOP/s; 8192 x 16384 x 2048 with 4-bit
+// tokens to fp16 141 us, 3.9 PFLOP/s. Of a tile's clocks with 8-bit tokens the tensor cores need 8,192;
+// 2,300 go where the next tile waits for the shared columns.
 #include <cudaTypedefs.h>
 
 #include <algorithm>

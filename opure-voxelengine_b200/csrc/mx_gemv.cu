@@ -20,8 +20,8 @@
 // and the 32 up rows that go with them), shared by `splits` warps that take every splits'th 128
 // columns and are added in order through shared memory.
 //
-// Measured: 1 x 49152 x 576 6.0 us (2.5 TB/s; its 15 MB are 2.4 us of memory), 1 x 2048 x 8192 4.5
-// us, 1 x 576 x 576 2.2 us. At these sizes latency bounds it: launch, first loads, and one or two
+// Measured: 1 x 49152 x 576 6.0 us (2.5 TB/s; its 15 MB are 2.4 us of memory), 1 x 2048 x 8192 4.6
+// us, 1 x 576 x 576 2.0 us, SwiGLU of 1 x 16384 x 2048 7.4 us (2.8 for its bytes). At these sizes latency bounds it: launch, first loads, and one or two
 // more rounds of loads by the 11 to 16 warps that fit an SM.
 #include <algorithm>
 
