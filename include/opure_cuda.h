@@ -317,7 +317,9 @@ size_t opure_mx_code_bytes(uint32_t format, uint32_t rows, uint32_t cols);
 size_t opure_mx_scale_bytes(uint32_t rows, uint32_t cols);
 
 /* x [out->rows][x_stride] of an opure_type, x_stride >= out->cols, to MX. What lies between x's
- * rows may be read along with them, here and in opure_mx_rmsnorm, but is not used. */
+ * rows may be read along with them, here and in opure_mx_rmsnorm, but is not used. More than
+ * 2^29 - 64 groups of 128 columns (rows times cols / 128, rounded up) are refused, here and in
+ * opure_mx_dequantize (OPURE_ERR_UNSUPPORTED). */
 opure_status opure_mx_quantize(opure_ctx *ctx, const void *x, uint32_t x_type, size_t x_stride,
                                const opure_mx_matrix *out);
 /* The values that an MX matrix stands for, rounded to an opure_type: y [x->rows][y_stride]. */

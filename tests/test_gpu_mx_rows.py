@@ -48,3 +48,13 @@ def test_rmsnorm_refuses_what_it_cannot_count(ctx):
         with pytest.raises(cu.OpureError) as e:
             norm(rows, cols)
         assert e.value.status == cu.ERR_UNSUPPORTED
+
+
+def test_quantize_and_dequantize_refuse_what_they_cannot_count(ctx):
+    x = ctx.buffer(1024)
+    for rows, cols in [(2 ** 29 - 63, 1), (2 ** 28, 129), (2 ** 32 - 1, 1)]:
+        m = cu.MxMatrix(x.ptr, x.ptr, rows, cols, mx.FP4)
+        for call in (lambda: ctx.mx_quantize(x.ptr, cu.F16, 1 << 32, m), lambda: ctx.mx_dequantize(m, x.ptr, cu.F16, 1 << 32)):
+            with pytest.raises(cu.OpureError) as e:
+                call()
+            assert e.value.status == cu.ERR_UNSUPPORTED
