@@ -368,6 +368,135 @@ typedef struct opure_mx_gemm_args {
 } opure_mx_gemm_args;
 opure_status opure_mx_gemm(opure_ctx *ctx, const opure_mx_gemm_args *a);
 
+/* ---- 4-bit paged KV cache -----------------------------------------------------------------
+ * Keys and values at 0.5625 bytes each (fp16: 2; the reference's contiguous region has fp32 words,
+ * Opure_Graph.cpp:396-400): E2M1 codes, two per byte, and one E4M3 scale for each 16 columns of a
+ * row, beside one power of two for all keys and one for all values. An addition: the reference has
+ * neither pages nor a quantised cache.
+ *
+ * A block of 16 columns with largest magnitude m has the scale s = m / (6 t) rounded to the nearest
+ * E4M3 value (ties to even, at most 448), t = k_scale or v_scale; its codes are the values divided
+ * by s t, rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives (ties to the even
+ * code, at most 6); where s is 0 they are 0. So t = 1 covers magnitudes up to 2688. A block that holds
+ * an infinity or NaN gets the scale NaN and codes 0: all of it reads as NaN.
+ *
+ * Layout. pool [page][n_kv] of page_size / 16 groups of 16 positions; a group takes 18 head_dim
+ * bytes: 8 head_dim of key codes, 8 head_dim of value codes, head_dim of key scales, head_dim of
+ * value scales. Each part is cut into panels of 64 columns; within a panel, columns counted from 0,
+ * positions of the group 0 .. 15, the even column of a byte in its low half:
+ *   key codes     [8 g][4 c][2 u] x 8 bytes   position 8 u + g, columns 16 c .. 16 c + 15
+ *   value codes   [8 g][4 c][4 t] x 4 bytes   position 2 c + t % 2 + 8 (t / 2), columns 8 g .. 8 g + 7
+ *   key scales    [8 g][4 c][2 u]             position 8 u + g, columns 16 c .. 16 c + 15
+ *   value scales  [4 b][4 c][4 t]             position 2 c + t % 2 + 8 (t / 2), columns 16 b .. 16 b + 15
+ * (the order in which the lanes of a warp hold an operand of mma.m16n8k16). */
+typedef struct opure_kv4_layout {
+    uint8_t *pool;             /* n_pages * opure_kv4_page_bytes(), 16-byte aligned   */
+    const int32_t *page_table; /* [n_seq][max_pages], as opure_kv_layout              */
+    uint32_t n_pages, max_pages;
+    uint32_t page_size;        /* 16, 32, 64 or 128                               */
+    uint32_t n_kv;
+    uint32_t head_dim;         /* 64 or 128                                       */
+    uint32_t ring;             /* sliding window, as opure_kv_layout (0: off)         */
+    float k_scale, v_scale;    /* powers of two from 2^-60 to 2^60; 0 stands for 1   */
+} opure_kv4_layout;
+/* Bytes of one page of a layer (0 for a page_size or head_dim that is not supported). */
+size_t opure_kv4_page_bytes(uint32_t n_kv, uint32_t head_dim, uint32_t page_size);
+
+/* RoPE + append in 4 bits for n token vectors: opure_rope_kv_append for this cache, with values of
+ * any opure_type. Row i of qkv holds [q | k | v]; q and k are rotated to position pos[i] (interleaved
+ * pairs, in double; theta 0: not rotated), the rotated q goes to row i of q_out, and the rotated k
+ * and v are quantised into the cache of sequence seq[i] at that position. The keys are quantised
+ * from their exact rotated values, not from values rounded to the type. A vector with seq[i] < 0 is
+ * padding: nothing of it is read or written. A row of the cache (a position of a sequence, or of its
+ * ring) may be written once per call. */
+typedef struct opure_kv4_append_args {
+    const void *qkv;           /* [n][stride] of type                             */
+    uint32_t type;             /* opure_type of qkv and q_out                       */
+    size_t stride;             /* >= (n_heads + 2 kv.n_kv) * head_dim               */
+    void *q_out;               /* [n][q_stride], or NULL. May be qkv with q_stride = stride */
+    size_t q_stride;           /* >= n_heads * head_dim                             */
+    const int32_t *seq, *pos;  /* [n]                                             */
+    uint32_t n, n_heads;
+    double theta;
+    opure_kv4_layout kv;
+} opure_kv4_append_args;
+opure_status opure_kv4_append(opure_ctx *ctx, const opure_kv4_append_args *a);
+
+/* The values that the cache stands for at position pos[i] of sequence seq[i], rounded to a type:
+ * row i of k and v is [n_kv * head_dim]. Rows with seq[i] < 0 are left as they are. */
+typedef struct opure_kv4_read_args {
+    void *k, *v;               /* [n][stride] of type; either may be NULL           */
+    uint32_t type;
+    size_t stride;             /* >= kv.n_kv * head_dim                             */
+    const int32_t *seq, *pos;  /* [n]                                             */
+    uint32_t n;
+    opure_kv4_layout kv;
+} opure_kv4_read_args;
+opure_status opure_kv4_read(opure_ctx *ctx, const opure_kv4_read_args *a);
+
+/* opure_attention over the 4-bit cache: single tokens, a few tokens per sequence, or prompts.
+ * Entry i is sequence seq[i] with queries of consecutive positions; its query j attends to keys
+ * [0, seq_len[i] + j), or the window's part of them with a ring. The entry's queries are rows
+ * q_begin[i] .. q_begin[i + 1] - 1 of q, at most n_q (more are reported as OPURE_ERR_DEVICE_BOUNDS
+ * and left out); q_begin NULL: n_q rows each. Rows from q_begin[n] on are not touched. A query
+ * without keys (seq[i] < 0, or seq_len[i] + j <= 0) gets zeros. Query head h reads kv head
+ * h / (n_heads / n_kv). Sums and the softmax are fp32; queries and probabilities are split into
+ * fp16 pairs, so that products keep 22 bits, except that with 16-bit types the probabilities of
+ * entries with more than 8 (query, head) rows per kv head may be rounded to fp16 once.
+ *
+ * scratch: opure_kv4_attention_scratch_bytes(...) bytes, 16-byte aligned, caller-owned. Zero before
+ * the first call (opure_fill); every call leaves its counters zero. Calls that may run at the same
+ * time need scratch of their own. */
+typedef struct opure_kv4_attn_args {
+    const void *q;             /* [n_rows][q_stride] of type, rows [n_heads][head_dim] */
+    void *out;                 /* [n_rows][out_stride] of type, apart from q           */
+    uint32_t type;             /* opure_type                                      */
+    size_t q_stride, out_stride; /* >= n_heads * head_dim                           */
+    const int32_t *seq, *seq_len; /* [n]                                          */
+    const int32_t *q_begin;    /* [n + 1], not decreasing, or NULL                   */
+    uint32_t n;                /* entries                                         */
+    uint32_t n_rows;           /* rows of q and out (q_begin NULL: n * n_q)            */
+    uint32_t n_q;              /* most queries of an entry                          */
+    uint32_t n_heads;
+    float scale;
+    uint32_t max_ctx;          /* upper bound of seq_len[i] + queries of i - 1          */
+    uint32_t split_tokens;     /* keys per split; 0 = choose                         */
+    void *scratch;
+    size_t scratch_bytes;
+    opure_kv4_layout kv;
+    uint16_t *out_packed;      /* NULL, or a packed operand of the n_rows output vectors
+                                  (see opure_gemv_args), written besides out            */
+} opure_kv4_attn_args;
+size_t opure_kv4_attention_scratch_bytes(uint32_t n, uint32_t n_rows, uint32_t n_q, uint32_t n_heads, uint32_t n_kv,
+                                         uint32_t head_dim, uint32_t max_ctx, uint32_t split_tokens);
+opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn_args *a);
+
+/* ---- scores of given tokens -------------------------------------------------------------
+ * Per row of logits: the log probability of a given token and its rank (how many tokens come before
+ * it in the order of larger logits first, equal ones by their index), the entropy of the softmax in
+ * nats, the log-sum-exp, and the `top` first tokens of that order with their log probabilities. One
+ * pass over the logits. NaN is never among the first tokens (fewer than `top` others: index -1, log
+ * probability -inf after them) and makes the row's other results NaN; so does +inf, or a row of -inf
+ * alone. -inf is a token of probability 0. A negative token asks for none: its log probability and
+ * rank are 0. A token past the vocabulary is reported (OPURE_ERR_DEVICE_BOUNDS), its log probability
+ * NaN and its rank 0. The rank of a token whose logit is NaN is 0. The reference reads logits back
+ * to the host for its statistics (RefreshLogitStats, Opure_VoxelEngine.cpp:832-876). */
+#define OPURE_SCORE_MAX_TOP 32u
+typedef struct opure_score_args {
+    const void *logits;        /* [rows][stride] of type                          */
+    uint32_t type;             /* opure_type                                      */
+    uint32_t vocab, rows;
+    size_t stride;             /* >= vocab                                        */
+    const int32_t *tokens;     /* [rows], or NULL: logprob and rank are not written    */
+    float *logprob;            /* [rows] or NULL                                  */
+    int32_t *rank;             /* [rows] or NULL                                  */
+    float *entropy, *lse;      /* [rows] or NULL                                  */
+    uint32_t top;              /* 0 .. OPURE_SCORE_MAX_TOP, at most vocab             */
+    int32_t *top_tokens;       /* [rows][top]                                     */
+    float *top_logprobs;       /* [rows][top]                                     */
+} opure_score_args;
+opure_status opure_token_scores(opure_ctx *ctx, const opure_score_args *a);
+
 /* ---- decode-step bookkeeping ----------------------------------------------------
  * A decode step computes one token vector per entry. opure_step_begin / opure_step_end
  * bracket the per-layer kernels of a step so that a captured step graph replays with no

@@ -88,6 +88,34 @@ class MxGemmArgs(C.Structure):
                 ("y_stride", sz), ("residual", P), ("out", MxMatrix)]
 
 
+class Kv4Layout(C.Structure):
+    """A layer of the 4-bit paged KV cache (opure_kv4_layout)."""
+    _fields_ = [("pool", P), ("page_table", P), ("n_pages", u32), ("max_pages", u32), ("page_size", u32),
+                ("n_kv", u32), ("head_dim", u32), ("ring", u32), ("k_scale", f32), ("v_scale", f32)]
+
+
+class Kv4AppendArgs(C.Structure):
+    _fields_ = [("qkv", P), ("type", u32), ("stride", sz), ("q_out", P), ("q_stride", sz), ("seq", P), ("pos", P),
+                ("n", u32), ("n_heads", u32), ("theta", C.c_double), ("kv", Kv4Layout)]
+
+
+class Kv4ReadArgs(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("type", u32), ("stride", sz), ("seq", P), ("pos", P), ("n", u32), ("kv", Kv4Layout)]
+
+
+class Kv4AttnArgs(C.Structure):
+    _fields_ = [("q", P), ("out", P), ("type", u32), ("q_stride", sz), ("out_stride", sz), ("seq", P), ("seq_len", P),
+                ("q_begin", P), ("n", u32), ("n_rows", u32), ("n_q", u32), ("n_heads", u32), ("scale", f32),
+                ("max_ctx", u32), ("split_tokens", u32), ("scratch", P), ("scratch_bytes", sz), ("kv", Kv4Layout),
+                ("out_packed", P)]
+
+
+class ScoreArgs(C.Structure):
+    """opure_score_args: log probabilities, ranks, entropies and the most likely tokens of rows of logits."""
+    _fields_ = [("logits", P), ("type", u32), ("vocab", u32), ("rows", u32), ("stride", sz), ("tokens", P), ("logprob", P),
+                ("rank", P), ("entropy", P), ("lse", P), ("top", u32), ("top_tokens", P), ("top_logprobs", P)]
+
+
 class DeviceInfo(C.Structure):
     _fields_ = [("device", i32), ("sm_count", i32), ("cc_major", i32), ("cc_minor", i32),
                 ("hbm_bytes", u64), ("l2_bytes", u64), ("smem_per_block_optin", u32),
@@ -129,6 +157,8 @@ _SIGS = {
     "opure_peer_argmax": [P, P, P, u32, u32],
     "opure_mx_quantize": [P, P, u32, sz, P], "opure_mx_dequantize": [P, P, P, u32, sz],
     "opure_mx_rmsnorm": [P, P], "opure_mx_gemm": [P, P],
+    "opure_kv4_append": [P, P], "opure_kv4_read": [P, P], "opure_kv4_attention": [P, P],
+    "opure_token_scores": [P, P],
 }
 
 
@@ -157,6 +187,10 @@ def lib() -> C.CDLL:
         L.opure_mx_code_bytes.restype = sz
         L.opure_mx_scale_bytes.argtypes = [u32, u32]
         L.opure_mx_scale_bytes.restype = sz
+        L.opure_kv4_page_bytes.argtypes = [u32, u32, u32]
+        L.opure_kv4_page_bytes.restype = sz
+        L.opure_kv4_attention_scratch_bytes.argtypes = [u32] * 8
+        L.opure_kv4_attention_scratch_bytes.restype = sz
         _lib = L
     return _lib
 
@@ -202,6 +236,15 @@ def mx_code_bytes(fmt: int, rows: int, cols: int) -> int:
 def mx_scale_bytes(rows: int, cols: int) -> int:
     """Bytes of its scales (tiles of 128 rows x 128 columns, 512 bytes each)."""
     return int(lib().opure_mx_scale_bytes(rows, cols))
+
+
+def kv4_page_bytes(n_kv: int, head_dim: int, page_size: int) -> int:
+    """Bytes of one page of a layer of the 4-bit KV cache."""
+    return int(lib().opure_kv4_page_bytes(n_kv, head_dim, page_size))
+
+
+def kv4_attention_scratch_bytes(n, n_rows, n_q, n_heads, n_kv, head_dim, max_ctx, split_tokens=0) -> int:
+    return int(lib().opure_kv4_attention_scratch_bytes(n, n_rows, n_q, n_heads, n_kv, head_dim, max_ctx, split_tokens))
 
 
 class DeviceBuffer:
@@ -315,6 +358,18 @@ class Ctx:
 
     def mx_gemm(self, args: MxGemmArgs):
         check(lib().opure_mx_gemm(self.h, C.byref(args)), "opure_mx_gemm")
+
+    def kv4_append(self, args: Kv4AppendArgs):
+        check(lib().opure_kv4_append(self.h, C.byref(args)), "opure_kv4_append")
+
+    def kv4_read(self, args: Kv4ReadArgs):
+        check(lib().opure_kv4_read(self.h, C.byref(args)), "opure_kv4_read")
+
+    def kv4_attention(self, args: Kv4AttnArgs):
+        check(lib().opure_kv4_attention(self.h, C.byref(args)), "opure_kv4_attention")
+
+    def token_scores(self, args: ScoreArgs):
+        check(lib().opure_token_scores(self.h, C.byref(args)), "opure_token_scores")
 
     def call(self, name: str, *args):
         check(getattr(lib(), name)(self.h, *args), name)
