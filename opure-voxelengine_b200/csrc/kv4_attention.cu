@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
         row_begin[nt] = window_begin(len0 + int32_t(j) - 1, P, p.kv.ring);
     }
 
-    float acc[HD / 16][NT][4] = {};
+    float acc[HD / 16][NT][2] = {};
     float m_run[NT], l_run[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -291,9 +291,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
 #pragma unroll
                     for (uint32_t i = 0; i < HD / 16; ++i)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[i][nt][v] *= f;
+                        for (int v = 0; v < 2; ++v) acc[i][nt][v] *= f;
                 }
             }
+            // The tensor cores cut sums off where fp32 would round them: 32 positions' sums start from 0
+            // and join the others here (left to run on, their bias was 3 times all other errors).
+            float part[HD / 16][NT][4] = {};
             uint32_t pf[2][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -343,9 +346,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
                                 for (uint32_t b = 0; b < kKv4Group; ++b) sees = sees || (bad >> b & 1u && t0 + b >= row_begin[nt] && t0 + b < row_end[nt]);
                                 if (sees)
 #pragma unroll
-                                    for (uint32_t i = 0; i < 4; ++i)
-#pragma unroll
-                                        for (int v = 0; v < 4; ++v) acc[pn * 4 + i][nt][v] = NAN;
+                                    for (uint32_t i = 0; i < 4; ++i) acc[pn * 4 + i][nt][0] = acc[pn * 4 + i][nt][1] = NAN;
                             }
                         }
                     }
@@ -361,9 +362,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
                     for (uint32_t i = 0; i < 4; ++i) {
                         const uint32_t a[4] = {hmul2(e01[i], s01), hmul2(o01[i], s01), hmul2(e23[i], s23), hmul2(o23[i], s23)};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(acc[pn * 4 + i][nt], a, pf[u][nt][0], pf[u][nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma16816(part[pn * 4 + i][nt], a, pf[u][nt][0], pf[u][nt][1]);
                     }
                 }
+#pragma unroll
+            for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) acc[i][nt][v] += fmaf(part[i][nt][2 * v + 1], 0x1p-11f, part[i][nt][2 * v]);
         }
         __syncwarp();
         fill(k + S, next_page, lane < 4);
@@ -387,8 +394,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
 #pragma unroll
         for (uint32_t i = 0; i < HD / 16; ++i) {
             float *o = state + r * HD + i / 4 * 64 + 8 * g + i % 4 * 2;
-            o[0] = fmaf(acc[i][nt][1], 0x1p-11f, acc[i][nt][0]);
-            o[1] = fmaf(acc[i][nt][3], 0x1p-11f, acc[i][nt][2]);
+            o[0] = acc[i][nt][0];
+            o[1] = acc[i][nt][1];
         }
         if (g == 0) {
             state[kRows * HD + r] = m_run[nt];
