@@ -16,9 +16,7 @@
 // raised only when a score passes it by 2^8 (probabilities stay below 2^8, the sums in fp32).
 #include <algorithm>
 
-#include "attn_core.cuh"
-#include "kv4.cuh"
-#include "tma.cuh"
+#include "kv4_attention.cuh"
 
 namespace opure {
 namespace {
@@ -35,24 +33,6 @@ constexpr uint32_t kRowsSmem = kWarps * kStages<HD> * kStageBytes<HD>;
 template <int HD>
 constexpr int kCtasPerSm = HD == 64 ? 3 : 2;  // what the stages leave room for
 constexpr float kRaise = 8.f;        // log2 units by which a score may pass the running maximum
-
-struct RowsParams {
-    const void *q;
-    void *out;
-    size_t q_stride, out_stride;
-    const int32_t *seq, *seq_len, *q_begin;
-    uint32_t n, n_rows, n_q, n_heads, group;
-    uint32_t row_tiles;
-    float factor;            // scale * log2(e) * k_scale
-    float v_scale;
-    uint32_t split_tokens, n_splits;
-    float *partials;         // [unit][split][row of the tile][HD + 2]
-    uint32_t *counters;      // [unit]
-    opure_kv4_layout kv;
-    DeviceStatus *st;
-    __half *out_packed;
-    uint32_t pk_npad;
-};
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -87,14 +67,8 @@ __device__ __forceinline__ uint32_t lds16_at(uint32_t a) {
     return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_result(const RowsParams &p, uint32_t row, uint32_t i, float v) {
-    static_cast<T *>(p.out)[size_t(row) * p.out_stride + i] = from_f32<T>(v);
-    if (p.out_packed) store_packed(p.out_packed, p.pk_npad, p.n_heads * p.kv.head_dim, row, i, v, p.st, 95);
-}
-
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsParams p) {
+__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4AttnParams p) {
     constexpr uint32_t kRows = 4 * NT, kPanels = HD / 64, S = kStages<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kWarps][S];
@@ -408,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
     float *parts_out = p.partials + (size_t(unit) * p.n_splits + split) * kRows * (HD + 2);
     auto finish = [&](uint32_t r, uint32_t d, float a, float l) {
         const uint32_t q = first + r;
-        store_result<T>(p, row0 + q / p.group, (head * p.group + q % p.group) * HD + d, a / fmaxf(l, 1e-30f) * p.v_scale);
+        kv4_store<T>(p, row0 + q / p.group, (head * p.group + q % p.group) * HD + d, a / fmaxf(l, 1e-30f) * p.v_scale);
     };
     for (uint32_t i = threadIdx.x; i < rows * HD; i += kWarps * 32) {
         const uint32_t r = i / HD, d = i % HD;
@@ -467,25 +441,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(RowsP
 
 // What a call's shape comes to: tiles of rows, units of work without the key split, and the split.
 struct Plan {
+    bool prompt;
     uint32_t tile_rows, row_tiles, split_tokens, n_splits;
     uint64_t units;
-    size_t partial_bytes, counters_off, bytes;
+    size_t counters_off, bytes;
 };
-Plan plan_rows(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t split_tokens, int sms) {
+// More than kFewRows (query, head) rows per kv head go to the kernel for prompts.
+constexpr uint32_t kFewRows = 16;
+Plan make_plan(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t split_tokens, int sms) {
     Plan p{};
     const uint64_t rows = uint64_t(n_q) * group;
-    p.tile_rows = rows <= 4 ? 4 : 8;
+    p.prompt = rows > kFewRows;
+    p.tile_rows = p.prompt ? kKv4PromptRows : rows <= 4 ? 4 : 8;
     p.row_tiles = ceil_div(rows, p.tile_rows);
     p.units = uint64_t(n) * p.row_tiles * n_kv;
-    const uint64_t unit = 2 * kChunk, ctx = std::max(max_ctx, 1u), slots = uint64_t(sms) * (hd == 64 ? 3 : 2);
+    const uint64_t unit = 128, ctx = std::max(max_ctx, 1u), most = p.prompt ? 16 : 64;
+    static_assert(128 % kChunk == 0 && 128 % kKv4PromptKeys == 0, "whole chunks and tiles to a split");
+    const uint64_t slots = p.prompt ? uint64_t(sms) : uint64_t(sms) * (hd == 64 ? 3 : 2) * 4;
     uint64_t want = split_tokens ? (ctx + split_tokens - 1) / split_tokens
-                                 : std::min<uint64_t>(64, std::max<uint64_t>(1, (4 * slots + p.units - 1) / p.units));
+                                 : std::min<uint64_t>(most, std::max<uint64_t>(1, (slots + p.units - 1) / p.units));
     want = std::min<uint64_t>(want, (ctx + unit - 1) / unit);
     const uint64_t per = split_tokens ? split_tokens : (ctx + want - 1) / want;
     p.split_tokens = uint32_t(std::min<uint64_t>((per + unit - 1) / unit * unit, 0xffffff80u));
     p.n_splits = ceil_div(ctx, p.split_tokens);
-    p.partial_bytes = p.n_splits > 1 ? size_t(p.units) * p.n_splits * p.tile_rows * (hd + 2) * sizeof(float) : 0;
-    p.counters_off = (p.partial_bytes + 255) & ~size_t(255);
+    const size_t partials = p.n_splits > 1 ? size_t(p.units) * p.n_splits * p.tile_rows * (hd + 2) * sizeof(float) : 0;
+    p.counters_off = (partials + 255) & ~size_t(255);
     p.bytes = p.counters_off + (p.n_splits > 1 ? size_t(p.units) * sizeof(uint32_t) : 0);
     return p;
 }
@@ -500,7 +480,7 @@ extern "C" size_t opure_kv4_attention_scratch_bytes(uint32_t n, uint32_t n_rows,
     if (!n || !n_rows || !n_q || !n_heads || !kv4_shape(n_kv, hd, 64) || n_heads % n_kv) return 0;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return std::max<size_t>(16, plan_rows(n, n_q, n_heads / n_kv, n_kv, hd, max_ctx, split_tokens, sms).bytes);
+    return std::max<size_t>(16, make_plan(n, n_q, n_heads / n_kv, n_kv, hd, max_ctx, split_tokens, sms).bytes);
 }
 
 extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn_args *a) {
@@ -516,10 +496,10 @@ extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn
         return OPURE_ERR_INVALID_ARG;
     if (!a->q_begin && uint64_t(a->n) * a->n_q != a->n_rows) return OPURE_ERR_INVALID_ARG;
     if (cols > 0x7fffffffu || a->n_rows > 0x7fffffffu || a->max_ctx > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
-    const Plan pl = plan_rows(a->n, a->n_q, a->n_heads / a->kv.n_kv, a->kv.n_kv, hd, a->max_ctx, a->split_tokens, ctx->sm_count);
+    const Plan pl = make_plan(a->n, a->n_q, a->n_heads / a->kv.n_kv, a->kv.n_kv, hd, a->max_ctx, a->split_tokens, ctx->sm_count);
     if (a->scratch_bytes < pl.bytes || reinterpret_cast<uintptr_t>(a->scratch) % 16) return OPURE_ERR_INVALID_ARG;
     if (pl.units > 0x7fffffffu || pl.n_splits > 65535) return OPURE_ERR_UNSUPPORTED;
-    RowsParams p{};
+    Kv4AttnParams p{};
     p.q = a->q;
     p.out = a->out;
     p.q_stride = a->q_stride;
@@ -543,6 +523,7 @@ extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn
     p.st = ctx->status;
     p.out_packed = reinterpret_cast<__half *>(a->out_packed);
     p.pk_npad = (a->n_rows + 15) & ~15u;
+    if (pl.prompt) return kv4_prompt_launch(ctx, p, a->type, uint32_t(pl.units));
     return with_type(a->type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto k, uint32_t smem) -> opure_status {

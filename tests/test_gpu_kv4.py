@@ -320,6 +320,43 @@ def test_attention_several_queries(ctx, t, heads, n_kv, hd, page, lens, queries)
     check(ctx, t, heads, n_kv, hd, page, lens, queries, 0.2, tail=2)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,n_kv,hd,page,lens,queries", [
+    (1, 1, 64, 64, [0], [17]),
+    (2, 2, 64, 64, [0], [128]),
+    (1, 1, 64, 16, [0], [300]),
+    (6, 2, 64, 32, [100, 0, 30], [150, 0, 33]),
+    (4, 1, 64, 128, [257], [65]),
+    (2, 1, 128, 64, [0], [260]),
+    (8, 4, 128, 16, [70, 1], [40, 129]),
+    (5, 1, 128, 128, [63], [26]),
+])
+def test_attention_prompt(ctx, t, heads, n_kv, hd, page, lens, queries):
+    check(ctx, t, heads, n_kv, hd, page, lens, queries, hd ** -0.5, tail=3)
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,page,ring,lens,queries,split", [
+    (2, 2, 64, 128, 3, [520], [100], 0),
+    (3, 1, 64, 64, 5, [120, 0], [200, 130], 0),
+    (2, 1, 128, 128, 2, [300], [80], 128),
+])
+def test_attention_prompt_window(ctx, heads, n_kv, hd, page, ring, lens, queries, split):
+    """Queries of one page, or of a sequence that fits the ring: later positions of a call would overwrite
+    pages that its earlier queries see."""
+    check(ctx, "f32", heads, n_kv, hd, page, lens, queries, 0.125, split=split, ring=ring)
+
+
+@pytest.mark.parametrize("t,hd,split,scale", [("f32", 64, 128, 0.125), ("f32", 128, 256, -0.1), ("f16", 64, 384, 0.3), ("bf16", 128, 128, 0.0)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_attention_prompt_splits(ctx, t, hd, split, scale, graph):
+    check(ctx, t, 4, 2, hd, 64, [500, 0], [90, 140], scale, split=split, graph=graph)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_attention_prompt_strides(ctx, t):
+    check(ctx, t, 6, 2, 64, 16, [70, 10], [30, 20], 0.125, shift=1, stride=5)
+
+
 @pytest.mark.parametrize("heads,n_kv,hd,page,ring,lens,queries,split", [
     (9, 3, 64, 16, 3, [100, 20, 47], [1, 1, 1], 0),
     (4, 2, 128, 64, 2, [300, 64], [5, 5], 128),
@@ -351,7 +388,7 @@ def test_attention_long(ctx):
 
 
 def simple(rng, n_kv=1, hd=64, page=16, length=40):
-    table = np.array([rng.permutation(4)[: (length + page - 1) // page]], np.int32)
+    table = np.array([rng.permutation(4)[: (length + page - 1) // page]], np.int32)  # of 4 pages
     cache = ref.Cache(4, n_kv, hd, page, table)
     fill_cache(cache, rng, [length])
     return cache
@@ -392,6 +429,41 @@ def test_attention_nan_reaches_only_who_sees_it(ctx):
         assert (np.abs(out[:2].reshape(2, 1, 64) - want) <= bound("f32", want, size, top, 64, 24)).all()
         assert np.isnan(out[2:4, 16:32]).all() and np.isfinite(out[2:4, :16]).all() and np.isfinite(out[2:4, 32:]).all()
         assert np.isnan(out[4]).all()
+
+
+def test_attention_prompt_nan_reaches_only_who_sees_it(ctx):
+    """NaN values and keys in the middle of a prompt, and queries that have no keys at its start."""
+    rng = np.random.default_rng(12)
+    n = 200
+    cache = simple(rng, page=128, length=n)
+    k, v = rng.standard_normal((1, 64)), rng.standard_normal((1, 64))
+    v[0, 50] = np.nan
+    cache.put(0, 150, k, v)
+    k2 = k.copy()
+    k2[0, 3] = np.nan
+    cache.put(0, 180, k2, np.ones((1, 64)))
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, n + 5, 64, "f32")
+    x = q.put(rng.standard_normal((n + 5, 64)))
+    out = attend(ctx, dev, q, [0], [-4], [0, n + 5], n + 5, 1, 0.125, n).get()
+    kk, vv = cache.get(0, n)
+    assert (out[:5] == 0).all()
+    want, size, top = ref.attention(x[5:155].reshape(150, 1, 64), kk, vv, [(0, i + 1) for i in range(150)], 0.125)
+    assert (np.abs(out[5:155].reshape(150, 1, 64) - want) <= bound("f32", want, size, top, 64, n)).all()
+    assert np.isnan(out[155:185, 48:64]).all() and np.isfinite(out[155:185, :48]).all() and np.isnan(out[185:]).all()
+
+
+def test_attention_prompt_packed_operand(ctx):
+    rng = np.random.default_rng(13)
+    cache = simple(rng, n_kv=2, length=40)
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, 38, 4 * 64, "f32")
+    q.put(rng.standard_normal((38, 256)))
+    for split in (0, 128):
+        out, pk = attend(ctx, dev, q, [0], [2], [0, 38], 38, 4, 0.125, 256 if split else 40, split, packed=True)
+        half = pk.download(np.float16, (2, 48, 256)).astype(np.float64)
+        got = out.get()
+        assert (np.abs(half[0, :38] + half[1, :38] / 2048 - got) <= 2.0 ** -21 * np.abs(got) + 2.0 ** -30).all() and (half[:, 38:] == 0).all()
 
 
 def test_attention_queries_of_any_size(ctx):
