@@ -2,21 +2,24 @@
 // tcgen05.
 //
 // One CTA owns (entry, 256 rows, kv head, key split); a row is a (query, query head of the group)
-// pair, so all rows share the kv head's keys and values. Per tile of 128 keys (64 with head_dim 128):
+// pair, so all rows share the kv head's keys and values. Per tile of 64 keys:
 //   warps 8-11   convert the tile's codes from memory to fp16 operands in shared memory (scales
 //                included, exact): K rows as they are, V transposed, both in 128-byte swizzled rows; the
 //                codes of the next tile are loaded meanwhile
-//   warp 12      issues S = Q K^T for the two halves of 128 rows, and P V once a half's P is there
+//   warp 12      issues S = Q K^T for the two halves of 128 rows, two tiles ahead of P V
 //   warps 0-3,   a thread per row: maximum, exponentials, row sum; P goes back to tensor memory over S, and
-//   warps 4-7    the tile's P V is added to the row's sums in registers (left to run on in the tensor
-//                cores, whose additions cut off, the sums drift)
-// While one half's threads work on P the tensor cores run the other half's products. With fp32 queries Q
-// and P are pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit
-// types Q is exact in fp16 and P is rounded to it once. A row's queries are scaled by a power of two to
-// [1, 2) first. The maximum is raised only when a score passes it by 2^8.
+//   warps 4-7    the P V of the tile before is added to the row's sums in registers (left to run on in
+//                the tensor cores, whose additions cut off, the sums drift)
+// S has two buffers a half, so a row's thread finds the next scores ready when it is done with a tile, and
+// the other half's thread keeps the exponentials going while it adds. With fp32 queries Q and P are
+// pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit types Q is exact in
+// fp16 and P is rounded to it once. A row's queries are scaled by a power of two to [1, 2) first. The
+// maximum is raised only when a score passes it by 2^8.
 //
-// What bounds it: 16,384 exponentials a half and tile at 16 a clock, as long as the tensor cores need
-// for fp32 (two MMAs for one), twice as long as for 16-bit types.
+// What bounds it: 16,384 exponentials a tile of 64 keys and 256 rows at 16 a clock, 1,024 clocks; the
+// tensor cores need as long for fp32 (two MMAs for one), half for 16-bit types.
+#include <type_traits>
+
 #include "kv4_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -25,22 +28,30 @@ namespace {
 
 constexpr uint32_t kSoftmaxWarps = 8, kThreads = 512, kHalf = 128;
 constexpr uint32_t kMmaWarp = 12;
-constexpr uint32_t kStages = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRaise = 8.f;
+constexpr uint32_t KT = 64;          // keys of a tile
+constexpr uint32_t kGroups = KT / kKv4Group;  // of 16 positions, one to each converting warp
 
 template <typename T, int HD>
 struct Shape {
-    static constexpr bool kPair = sizeof(T) == 4;      // queries and probabilities as fp16 pairs
-    static constexpr uint32_t kKeys = HD == 64 ? 128 : 64;
+    static constexpr bool kPair = sizeof(T) == 4;       // queries and probabilities as fp16 pairs
     static constexpr uint32_t kPanels = HD / 64;
-    static constexpr uint32_t kGroups = kKeys / kKv4Group, kGroupsPerWarp = kGroups / 4;
+    // Q as the A operand: with head_dim 64 in tensor memory (from shared memory, an MMA of 64 columns
+    // would read three bytes of operands for two that the tensor cores can take), else in shared.
+    static constexpr bool kQTmem = HD == 64;
     static constexpr uint32_t kQPart = kHalf * HD * 2;  // bytes of one half's Q, hi or lo
-    static constexpr uint32_t kQBytes = 2 * kQPart * (kPair ? 2 : 1);
-    static constexpr uint32_t kTile = kKeys * HD * 2;   // bytes of K, or of V
+    static constexpr uint32_t kQBytes = kQTmem ? 0 : 2 * kQPart * (kPair ? 2 : 1);
+    static constexpr uint32_t kTile = KT * HD * 2;      // bytes of K, or of V
+    static constexpr uint32_t kStages = HD == 128 && kPair ? 3 : 4;
     static constexpr uint32_t kSmem = kQBytes + kStages * 2 * kTile + 1024;
-    static constexpr uint32_t kChunk = HD == 64 ? 32 : 16;  // columns that a thread works on at a time
-    static constexpr uint32_t kSCol = 0, kOCol = 2 * kKeys;  // TMEM: S of both halves, then O
+    // Registers of a row's thread, and 256 less these for the others (65536 in all). With head_dim 64
+    // they hold a tile's scores between the maximum and the exponentials; with 128 these are read twice.
+    static constexpr int kSoftmaxRegs = HD == 64 ? 200 : 192;
+    static constexpr uint32_t kChunk = HD == 64 ? 64 : 16;  // scores that a thread holds
+    // Tensor memory: S [half][buffer], O [half], Q [half][hi, lo].
+    static constexpr uint32_t kOCol = 4 * KT, kQCol = kOCol + 2 * HD;
+    static_assert(kOCol + 2 * HD + (kQTmem ? 2 * HD : 0) <= kTmemCols, "tensor memory");
 };
 
 __device__ __forceinline__ void mma_ss(bool one, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
@@ -58,7 +69,10 @@ __device__ __forceinline__ void mma_ts(bool one, uint32_t d, uint32_t a, uint64_
         "r"(a), "l"(db), "r"(idesc), "r"(accumulate), "r"(uint32_t(one))
         : "memory");
 }
-__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tc::ld32(taddr, r); }
+__device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[64]) {
+    tc::ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
+    tc::ld32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+}
 __device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -95,11 +109,11 @@ __host__ __device__ constexpr uint32_t column_of(uint32_t d) { return d / 64 * 6
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
     using S = Shape<T, HD>;
-    constexpr uint32_t KT = S::kKeys, kPanels = S::kPanels, CH = S::kChunk;
+    constexpr uint32_t kPanels = S::kPanels, kStages = S::kStages;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], done;
+    __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_full[2], o_full[2], done;
     __shared__ uint32_t tmem_base;
-    __shared__ __align__(16) uint16_t bad_values[kStages][HD / 16][S::kGroups];  // positions whose block is NaN, 16 to a group
+    __shared__ __align__(16) uint16_t bad_values[kStages][HD / 16][kGroups];  // positions whose block is NaN, 16 to a group
     __shared__ uint32_t ticket;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -176,14 +190,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
             mbar_init(&v_empty[s], 1);
         }
         for (uint32_t t = 0; t < 2; ++t) {
-            mbar_init(&s_full[t], 1);
+            mbar_init(&s_full[t][0], 1);
+            mbar_init(&s_full[t][1], 1);
+            mbar_init(&o_full[t], 1);
             mbar_init(&p_full[t], kHalf);
         }
         mbar_init(&done, 1);
     }
     if (warp == kMmaWarp) tc::alloc(&tmem_base, kTmemCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
 
-    // Queries to shared memory: a thread per row.
+    // Queries to tensor or shared memory: a thread per row.
     float factor = 0.f;
     if (warp < kSoftmaxWarps) {
         const uint32_t half = warp / 4, r = threadIdx.x % kHalf;
@@ -211,34 +231,46 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
         const float down = (normal ? __uint_as_float((254u - e) << 23) : 1.f) * (p.factor < 0.f ? -1.f : 1.f);
         factor = (normal ? __uint_as_float(e << 23) : 1.f) * fabsf(p.factor);
         uint8_t *dst = q_smem + half * (S::kQBytes / 2) + r * 128;
-#pragma unroll 4
-        for (uint32_t d = 0; d < HD; d += 8) {
-            uint32_t hi[4], lo[4];
-            float v[8];
-            load(d, v);
+        const uint32_t q_col = tmem + ((warp % 4 * 32) << 16) + S::kQCol + half * HD;
+#pragma unroll 2
+        for (uint32_t d = 0; d < HD; d += 16) {
+            uint32_t hi[8], lo[8];
+            float v[16];
+            load(d, *reinterpret_cast<float(*)[8]>(v));
+            load(d + 8, *reinterpret_cast<float(*)[8]>(v + 8));
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
+            for (uint32_t j = 0; j < 8; ++j) {
                 const float a = v[2 * j] * down, b = v[2 * j + 1] * down;
                 hi[j] = pack_half2(a, b);
                 const float2 h = h2f2(hi[j]);
                 lo[j] = pack_half2(a - h.x, b - h.y);
             }
-            uint8_t *at = dst + d / 64 * (kHalf * 128) + ((d % 64 / 8) ^ (r & 7u)) * 16;
-            *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (S::kPair) *reinterpret_cast<uint4 *>(at + S::kQPart) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if constexpr (S::kQTmem) {
+                st_cols(q_col + d / 2, hi);
+                if (S::kPair) st_cols(q_col + HD / 2 + d / 2, lo);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 2; ++j) {
+                    uint8_t *at = dst + d / 64 * (kHalf * 128) + ((d % 64 / 8 + j) ^ (r & 7u)) * 16;
+                    *reinterpret_cast<uint4 *>(at) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+                    if (S::kPair) *reinterpret_cast<uint4 *>(at + S::kQPart) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+                }
+            }
         }
-        tc::fence_async_shared();
+        if constexpr (S::kQTmem)
+            wait_st();
+        else
+            tc::fence_async_shared();
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = tmem_base;
 
     if (warp < kSoftmaxWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
         const uint32_t half = warp / 4, r = threadIdx.x % kHalf;
         const uint32_t lanes = (warp % 4 * 32) << 16;
-        const uint32_t s_col = tmem + lanes + S::kSCol + half * KT, o_col = tmem + lanes + S::kOCol + half * HD;
+        const uint32_t s_base = tmem + lanes + half * 2 * KT, o_col = tmem + lanes + S::kOCol + half * HD;
         const bool live = r < (half ? half_rows[1] : half_rows[0]);
         const uint32_t j = query_of(half * kHalf + (live ? r : 0u));
         const uint32_t see0 = max(keys_begin(j), k_begin), see1 = live ? min(keys_end(j), k_end) : 0u;
@@ -248,79 +280,105 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
         float m = -INFINITY, l = 0.f;
         uint32_t nan_blocks = 0;  // blocks of 16 dimensions with a NaN among the values that this row sees
         bool ok = true;
-        auto add_products = [&]() {
+        auto add_products = [&](float by) {
+            constexpr uint32_t kOut = HD == 64 ? 64 : 16;
 #pragma unroll
-            for (uint32_t d = 0; d < HD; d += 32) {
-                uint32_t o[32];
-                tc::ld32(o_col + d, o);
+            for (uint32_t d = 0; d < HD; d += kOut) {
+                uint32_t o[kOut];
+                ld_cols(o_col + d, o);
                 tc::wait_ld();
 #pragma unroll
-                for (uint32_t q = 0; q < 32; ++q) acc[d + q] += __uint_as_float(o[q]);
+                for (uint32_t q = 0; q < kOut; q += 2) {
+                    const float2 a = __ffma2_rn(make_float2(__uint_as_float(o[q]), __uint_as_float(o[q + 1])), make_float2(by, by),
+                                                make_float2(acc[d + q], acc[d + q + 1]));
+                    acc[d + q] = a.x;
+                    acc[d + q + 1] = a.y;
+                }
             }
         };
         const uint32_t from_mine = half ? from[1] : from[0], n_mine = (half ? upto[1] : upto[0]) - from_mine;
         for (uint32_t n = 0; n < n_mine; ++n) {
             const uint32_t i = from_mine + n, t0 = (tile0 + i) * KT, st = i % kStages;
-            if (!mbar_wait(&s_full[half], n & 1u)) {
+            const uint32_t s_col = s_base + (n & 1u) * KT;
+            if (!mbar_wait(&s_full[half][n & 1u], n / 2 & 1u)) {
                 if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 100, blockIdx.x);
                 ok = false;
                 break;
             }
             tc::fence_after();
-            if (n) add_products();
-            const bool whole = half_sees(half, i);
-            float top = -INFINITY;
-#pragma unroll
-            for (uint32_t c = 0; c < KT; c += CH) {
+            float raised = 1.f;  // what the sums so far are multiplied by
+            auto step = [&](auto masked) {
+                constexpr bool kMasked = decltype(masked)::value;
+                constexpr uint32_t CH = S::kChunk, PC = CH < 32 ? CH : 32;  // scores held; of one store of P
+                auto seen = [&](uint32_t k) { return t0 + k >= see0 && t0 + k < see1; };
                 uint32_t s[CH];
-                ld_cols(s_col + c, s);
-                tc::wait_ld();
-                if (!whole) {
+                float top = -INFINITY;
+#pragma unroll 1
+                for (uint32_t c = 0; c < KT; c += CH) {
+                    ld_cols(s_col + c, s);
+                    tc::wait_ld();
+                    if (kMasked) {
 #pragma unroll
-                    for (uint32_t q = 0; q < CH; ++q) s[q] = t0 + c + q >= see0 && t0 + c + q < see1 ? s[q] : 0xff800000u;
-                }
-#pragma unroll
-                for (uint32_t q = 0; q < CH; q += 2)
-                    asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(__uint_as_float(s[q])), "f"(__uint_as_float(s[q + 1])));
-            }
-            top = top == -INFINITY ? top : top * factor;
-            if (__any_sync(0xffffffffu, top > m + kRaise)) {
-                const float up = fmaxf(m, top), f = up == -INFINITY ? 1.f : fast_exp2(m - up);
-                m = up;
-                l *= f;
-#pragma unroll
-                for (uint32_t d = 0; d < HD; ++d) acc[d] *= f;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (uint32_t c = 0; c < KT; c += CH) {
-                uint32_t s[CH];
-                ld_cols(s_col + c, s);
-                tc::wait_ld();
-                uint32_t hi[CH / 2], lo[CH / 2];
-                float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-                for (uint32_t q = 0; q < CH; q += 2) {
-                    float2 x = __ffma2_rn(make_float2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), make_float2(factor, factor),
-                                          make_float2(-base, -base));
-                    if (!whole) {
-                        x.x = t0 + c + q >= see0 && t0 + c + q < see1 ? x.x : -INFINITY;
-                        x.y = t0 + c + q + 1 >= see0 && t0 + c + q + 1 < see1 ? x.y : -INFINITY;
+                        for (uint32_t q = 0; q < CH; ++q) s[q] = seen(c + q) ? s[q] : 0xff800000u;
                     }
-                    const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                    sum = __fadd2_rn(sum, e);
-                    hi[q / 2] = pack_half2(e.x, e.y);
-                    if (S::kPair) {
-                        const float2 h = h2f2(hi[q / 2]);
-                        const float2 d = __fadd2_rn(e, make_float2(-h.x, -h.y));
-                        lo[q / 2] = pack_half2(d.x, d.y);
-                    }
+                    float high[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (uint32_t q = 0; q < CH; q += 2)
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(high[q / 2 % 2]) : "f"(__uint_as_float(s[q])), "f"(__uint_as_float(s[q + 1])));
+                    top = fmaxf(top, fmaxf(high[0], high[1]));
                 }
-                l += sum.x + sum.y;
-                // Over the scores that were read: columns c .. c + CH / 2 - 1 hi, then lo.
-                st_cols(s_col + c, hi);
-                if (S::kPair) st_cols(s_col + c + CH / 2, lo);
-            }
+                top = top == -INFINITY ? top : top * factor;
+                if (__any_sync(0xffffffffu, top > m + kRaise)) {
+                    const float up = fmaxf(m, top);
+                    raised = up == -INFINITY ? 1.f : fast_exp2(m - up);
+                    m = up;
+                    l *= raised;
+#pragma unroll
+                    for (uint32_t d = 0; d < HD; ++d) acc[d] *= raised;
+                }
+                const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                for (uint32_t c = 0; c < KT; c += CH) {
+                    if (CH < KT) {
+                        ld_cols(s_col + c, s);
+                        tc::wait_ld();
+                        if (kMasked) {
+#pragma unroll
+                            for (uint32_t q = 0; q < CH; ++q) s[q] = seen(c + q) ? s[q] : 0xff800000u;
+                        }
+                    }
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (uint32_t c2 = 0; c2 < CH; c2 += PC) {
+                        uint32_t hi[PC / 2], lo[PC / 2];
+#pragma unroll
+                        for (uint32_t q = 0; q < PC; q += 2) {
+                            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c2 + q]), __uint_as_float(s[c2 + q + 1])), make_float2(factor, factor),
+                                                  make_float2(-base, -base));
+                            if (kMasked) {  // a factor of 0 has made NaN of -inf
+                                x.x = s[c2 + q] == 0xff800000u ? -INFINITY : x.x;
+                                x.y = s[c2 + q + 1] == 0xff800000u ? -INFINITY : x.y;
+                            }
+                            const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                            sum = __fadd2_rn(sum, e);
+                            hi[q / 2] = pack_half2(e.x, e.y);
+                            if (S::kPair) {
+                                const float2 h = h2f2(hi[q / 2]);
+                                const float2 d = __fadd2_rn(e, make_float2(-h.x, -h.y));
+                                lo[q / 2] = pack_half2(d.x, d.y);
+                            }
+                        }
+                        // Over the scores that were read: of each PC columns the first half hi, then lo.
+                        st_cols(s_col + c + c2, hi);
+                        if (S::kPair) st_cols(s_col + c + c2 + PC / 2, lo);
+                    }
+                    l += sum.x + sum.y;
+                }
+            };
+            if (half_sees(half, i))
+                step(std::false_type());
+            else
+                step(std::true_type());
             wait_st();
             if (!all_see(i)) {
                 // NaN values were left out of V where not all rows see them.
@@ -337,13 +395,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                         for (uint32_t k = 0; k < KT; ++k)
                             if (bad_values[st][b][k / 16] >> (k % 16) & 1u && t0 + k >= see0 && t0 + k < see1) nan_blocks |= 1u << b;
             }
+            if (n) {
+                if (!mbar_wait(&o_full[half], (n - 1) & 1u)) {
+                    if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 105, blockIdx.x);
+                    ok = false;
+                    break;
+                }
+                tc::fence_after();
+                add_products(raised);
+            }
             tc::fence_before();
             arrive(&p_full[half]);
         }
         if (ok && n_mine) {
-            if (mbar_wait(&s_full[half], n_mine & 1u)) {
+            if (mbar_wait(&o_full[half], (n_mine - 1) & 1u)) {
                 tc::fence_after();
-                add_products();
+                add_products(1.f);
             } else if (lane == 0) {
                 report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 102, blockIdx.x);
             }
@@ -379,10 +446,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - S::kSoftmaxRegs));
         if (warp < kMmaWarp) {
-            // Codes to operands. Groups of 16 positions, kGroupsPerWarp to a warp and tile.
-            constexpr uint32_t G = S::kGroupsPerWarp;
+            // Codes to operands, 16 positions a warp and tile.
             const uint32_t w = warp - kSoftmaxWarps, c = lane & 3u, g = lane >> 2;
             const int32_t *table = p.kv.page_table + size_t(max(seq, 0)) * p.kv.max_pages;
             const uint32_t groups_per_page = P / kKv4Group;
@@ -390,17 +456,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                 uint4 k[kPanels], v[kPanels];
                 uint32_t ks[kPanels], vs[kPanels];
             };
-            auto position = [&](uint32_t i, uint32_t k) { return (tile0 + i) * KT + (w * G + k) * kKv4Group; };
-            auto page_of = [&](uint32_t i, uint32_t k) -> int32_t {
-                const uint32_t t = position(i, k);
+            auto position = [&](uint32_t i) { return (tile0 + i) * KT + w * kKv4Group; };
+            auto page_of = [&](uint32_t i) -> int32_t {
+                const uint32_t t = position(i);
                 if (i >= n_tiles || t >= k_end || t + kKv4Group <= k_begin) return -2;
                 const uint32_t lp = ring_slot(t / P, p.kv.ring);
                 return lp < p.kv.max_pages ? table[lp] : -1;
             };
-            auto load = [&](uint32_t i, uint32_t k, int32_t page, Raw &raw) {
+            auto load = [&](uint32_t i, int32_t page, Raw &raw) {
                 const bool good = page >= 0 && uint32_t(page) < p.kv.n_pages;
                 if (!good && page != -2 && lane == 0) report(p.st, OPURE_ERR_DEVICE_BOUNDS, 94, uint32_t(page));
-                const uint8_t *group = p.kv.pool + ((size_t(good ? page : 0) * p.kv.n_kv + head) * groups_per_page + position(i, k) % P / kKv4Group) * kv4_group_bytes(HD);
+                const uint8_t *group = p.kv.pool + ((size_t(good ? page : 0) * p.kv.n_kv + head) * groups_per_page + position(i) % P / kKv4Group) * kv4_group_bytes(HD);
 #pragma unroll
                 for (uint32_t pn = 0; pn < kPanels; ++pn) {
                     raw.k[pn] = raw.v[pn] = make_uint4(0, 0, 0, 0);
@@ -413,13 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     }
                 }
             };
-            Raw raw[G];
-            int32_t page_next[G];
-#pragma unroll
-            for (uint32_t k = 0; k < G; ++k) {
-                load(0, k, page_of(0, k), raw[k]);
-                page_next[k] = page_of(1, k);
-            }
+            Raw raw;
+            load(0, page_of(0), raw);
+            int32_t page_next = page_of(1);
             bool ok = true;
             for (uint32_t i = 0; i < n_tiles; ++i) {
                 const uint32_t st = i % kStages;
@@ -428,19 +490,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                 if (i >= kStages && !mbar_wait(&k_empty[st], (i / kStages - 1) & 1u)) ok = false;
                 if (ok) {
 #pragma unroll
-                    for (uint32_t k = 0; k < G; ++k)
-#pragma unroll
                         for (uint32_t pn = 0; pn < kPanels; ++pn) {
-                            const uint32_t sp = kv4_scale_pair(raw[k].ks[pn]);
+                            const uint32_t sp = kv4_scale_pair(raw.ks[pn]);
 #pragma unroll
                             for (uint32_t u = 0; u < 2; ++u) {
                                 const uint32_t s = u ? __byte_perm(sp, sp, 0x3232) : __byte_perm(sp, sp, 0x1010);
                                 uint32_t h[8];
-                                mx_unpack_fp4(u ? raw[k].k[pn].z : raw[k].k[pn].x, *reinterpret_cast<uint32_t(*)[4]>(h));
-                                mx_unpack_fp4(u ? raw[k].k[pn].w : raw[k].k[pn].y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
+                                mx_unpack_fp4(u ? raw.k[pn].z : raw.k[pn].x, *reinterpret_cast<uint32_t(*)[4]>(h));
+                                mx_unpack_fp4(u ? raw.k[pn].w : raw.k[pn].y, *reinterpret_cast<uint32_t(*)[4]>(h + 4));
 #pragma unroll
                                 for (uint32_t q = 0; q < 8; ++q) h[q] = hmul2(h[q], s);
-                                uint8_t *row = ktile + pn * (KT * 128) + ((w * G + k) * 16 + u * 8 + g) * 128;
+                                uint8_t *row = ktile + pn * (KT * 128) + (w * 16 + u * 8 + g) * 128;
                                 *reinterpret_cast<uint4 *>(row + ((2 * c) ^ g) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
                                 *reinterpret_cast<uint4 *>(row + ((2 * c + 1) ^ g) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
                             }
@@ -454,13 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     break;
                 }
 #pragma unroll
-                for (uint32_t k = 0; k < G; ++k)
-#pragma unroll
                     for (uint32_t pn = 0; pn < kPanels; ++pn) {
-                        uint32_t sv = raw[k].vs[pn];
+                        uint32_t sv = raw.vs[pn];
                         if (!whole) {
                             // Positions that no row sees may hold anything; NaN blocks are named to the rows.
-                            const uint32_t t = position(i, k) + 2 * c;
+                            const uint32_t t = position(i) + 2 * c;
                             uint32_t bad = 0;
 #pragma unroll
                             for (uint32_t b = 0; b < 4; ++b) {
@@ -472,13 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                             }
                             bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
                             bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-                            if (c == 0 && g % 2 == 0) bad_values[st][pn * 4 + g / 2][w * G + k] = uint16_t(bad);
+                            if (c == 0 && g % 2 == 0) bad_values[st][pn * 4 + g / 2][w] = uint16_t(bad);
                         }
                         const uint32_t s01 = kv4_scale_pair(sv), s23 = kv4_scale_pair(sv >> 16), low = 0x0f0f0f0fu;
-                        const uint4 v = raw[k].v[pn];
+                        const uint4 v = raw.v[pn];
                         // A row per dimension, 8 (d % 8) + d / 8; two positions a word.
-                        const uint32_t chunk = (w * G + k) % 4 * 2;
-                        uint8_t *base = vtile + (w * G + k) / 4 * (HD * 128) + (pn * 64 + g) * 128 + c * 4;
+                        const uint32_t chunk = w * 2;
+                        uint8_t *base = vtile + (pn * 64 + g) * 128 + c * 4;
                         auto put = [&](uint32_t word, uint32_t odd, uint32_t s, uint32_t ch) {
                             uint32_t h[4];
                             mx_unpack_fp4(word, h);
@@ -493,11 +551,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     }
                 tc::fence_async_shared();
                 arrive(&v_full[st]);
-#pragma unroll
-                for (uint32_t k = 0; k < G; ++k) {
-                    load(i + 1, k, page_next[k], raw[k]);
-                    page_next[k] = page_of(i + 2, k);
-                }
+                load(i + 1, page_next, raw);
+                page_next = page_of(i + 2);
             }
         } else if (warp == kMmaWarp) {
             const bool one = tc::elect();
@@ -510,46 +565,51 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     ok = false;
                 }
             };
-            for (uint32_t i = 0; i <= n_tiles && ok; ++i) {
+            // Tile i's scores, and the products of tile i - 2, over whose P the scores go.
+            for (uint32_t i = 0; i < n_tiles + 2 && ok; ++i) {
 #pragma unroll
                 for (uint32_t t = 0; t < 2; ++t) {
-                    const bool before = active[t] && i > from[t] && i <= upto[t], now = active[t] && i >= from[t] && i < upto[t];
-                    if (before) {
-                        // P V of the tile before, lo first: its sums are too small to cut much off.
-                        const uint32_t st = (i - 1) % kStages, v = smem_addr(kv_smem + st * 2 * S::kTile + S::kTile);
-                        wait(&p_full[t], (i - 1 - from[t]) & 1u);
-                        wait(&v_full[st], (i - 1) / kStages & 1u);
+                    const uint32_t s_col = tmem + (t * 2 + ((i - from[t]) & 1u)) * KT;
+                    if (i >= from[t] + 2 && i < upto[t] + 2 && active[t]) {
+                        const uint32_t st = (i - 2) % kStages, v = smem_addr(kv_smem + st * 2 * S::kTile + S::kTile);
+                        wait(&p_full[t], (i - from[t]) & 1u);
+                        wait(&v_full[st], (i - 2) / kStages & 1u);
                         if (!ok) break;
                         tc::fence_after();
-                        const uint32_t a = tmem + S::kSCol + t * KT, d = tmem + S::kOCol + t * HD;
+                        constexpr uint32_t PC = S::kChunk < 32 ? S::kChunk : 32;
+                        // lo first: its sums are too small to cut much off.
 #pragma unroll
                         for (uint32_t part = S::kPair ? 0 : 1; part < 2; ++part)
 #pragma unroll
                             for (uint32_t k = 0; k < KT / 16; ++k) {
-                                const uint32_t col = k * 16 / CH * CH + k * 16 % CH / 2 + (part == 0 ? CH / 2 : 0u);
-                                const uint64_t db = tc::desc_sw128(v + k / 4 * (HD * 128) + k % 4 * 32);
-                                mma_ts(one, d, a + col, db, idesc_o, part != (S::kPair ? 0 : 1) || k != 0);
+                                const uint32_t col = k * 16 / PC * PC + k * 16 % PC / 2 + (part == 0 ? PC / 2 : 0u);
+                                mma_ts(one, tmem + S::kOCol + t * HD, s_col + col, tc::desc_sw128(v + k * 32), idesc_o, part != (S::kPair ? 0 : 1) || k != 0);
                             }
+                        tc::commit(one, &o_full[t]);
                     }
-                    if (now) {
+                    if (i >= from[t] && i < upto[t]) {
                         const uint32_t st = i % kStages, kt = smem_addr(kv_smem + st * 2 * S::kTile);
                         wait(&k_full[st], i / kStages & 1u);
                         if (!ok) break;
                         tc::fence_after();
-                        const uint32_t d = tmem + S::kSCol + t * KT;
 #pragma unroll
                         for (uint32_t part = 0; part < (S::kPair ? 2 : 1); ++part) {
-                            const uint32_t q = smem_addr(q_smem + t * (S::kQBytes / 2) + (S::kPair ? 1 - part : 0) * S::kQPart);
+                            const uint32_t which = S::kPair ? 1 - part : 0;
 #pragma unroll
-                            for (uint32_t k = 0; k < HD / 16; ++k)
-                                mma_ss(one, d, tc::desc_sw128(q + k / 4 * (kHalf * 128) + k % 4 * 32),
-                                       tc::desc_sw128(kt + k / 4 * (KT * 128) + k % 4 * 32), idesc_s, part != 0 || k != 0);
+                            for (uint32_t k = 0; k < HD / 16; ++k) {
+                                const uint64_t db = tc::desc_sw128(kt + k / 4 * (KT * 128) + k % 4 * 32);
+                                if constexpr (S::kQTmem)
+                                    mma_ts(one, s_col, tmem + S::kQCol + t * HD + which * (HD / 2) + k * 8, db, idesc_s, part != 0 || k != 0);
+                                else
+                                    mma_ss(one, s_col, tc::desc_sw128(smem_addr(q_smem) + t * (S::kQBytes / 2) + which * S::kQPart + k / 4 * (kHalf * 128) + k % 4 * 32),
+                                           db, idesc_s, part != 0 || k != 0);
+                            }
                         }
+                        tc::commit(one, &s_full[t][(i - from[t]) & 1u]);
                     }
-                    if (before || now) tc::commit(one, &s_full[t]);
                 }
                 if (!ok) break;
-                if (i > 0) tc::commit(one, &v_empty[(i - 1) % kStages]);
+                if (i >= 2) tc::commit(one, &v_empty[(i - 2) % kStages]);
                 if (i < n_tiles) tc::commit(one, &k_empty[i % kStages]);
             }
             // Nothing may be in flight when the tensor memory is given back.
