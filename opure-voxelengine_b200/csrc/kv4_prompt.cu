@@ -6,10 +6,10 @@
 //   warps 8-11   convert the tile's codes from memory to fp16 operands in shared memory (scales
 //                included, exact): K rows as they are, V transposed, both in 128-byte swizzled rows; the
 //                codes of the next tile are loaded meanwhile
-//   warp 12      issues S = Q K^T for the two halves of 128 rows, two tiles ahead of P V
+//   warps 12, 13 issue S = Q K^T for the two halves of 128 rows, two tiles ahead of P V
 //   warps 0-3,   a thread per row: maximum, exponentials, row sum; P goes back to tensor memory over S, and
-//   warps 4-7    the P V of the tile before is added to the row's sums in registers (left to run on in
-//                the tensor cores, whose additions cut off, the sums drift)
+//   warps 4-7    every few tiles their P V is added to the row's sums in registers (left to run on in the
+//                tensor cores, whose additions cut off, the sums drift)
 // S has two buffers a half, so a row's thread finds the next scores ready when it is done with a tile, and
 // the other half's thread keeps the exponentials going while it adds. With fp32 queries Q and P are
 // pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit types Q is exact in
@@ -49,6 +49,9 @@ struct Shape {
     // they hold a tile's scores between the maximum and the exponentials; with 128 these are read twice.
     static constexpr int kSoftmaxRegs = HD == 64 ? 200 : 192;
     static constexpr uint32_t kChunk = HD == 64 ? 64 : 16;  // scores that a thread holds
+    // Tiles whose products add up in tensor memory: a sum of 8 steps of 16 keys is cut off by 2^-22 of
+    // itself at most, of 32 steps by 2^-20, less than one of fp16's roundings of P.
+    static constexpr uint32_t kRun = kPair ? 2 : 8;
     // Tensor memory: S [half][buffer], O [half], Q [half][hi, lo].
     static constexpr uint32_t kOCol = 4 * KT, kQCol = kOCol + 2 * HD;
     static_assert(kOCol + 2 * HD + (kQTmem ? 2 * HD : 0) <= kTmemCols, "tensor memory");
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
     using S = Shape<T, HD>;
     constexpr uint32_t kPanels = S::kPanels, kStages = S::kStages;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_full[2], o_full[2], done;
+    __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_full[2][2], o_full[2][2], done;
     __shared__ uint32_t tmem_base;
     __shared__ __align__(16) uint16_t bad_values[kStages][HD / 16][kGroups];  // positions whose block is NaN, 16 to a group
     __shared__ uint32_t ticket;
@@ -169,7 +172,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
             }
         }
     }
-    const bool active[2] = {upto[0] > from[0], upto[1] > from[1]};
     // Whether every row that works on tile i sees all of it, in one half or in both.
     auto half_sees = [&](uint32_t t, uint32_t i) {
         const uint32_t t0 = (tile0 + i) * KT;
@@ -185,17 +187,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
             mbar_init(&k_full[s], 128);
-            mbar_init(&k_empty[s], 1);
+            mbar_init(&k_empty[s], 2);
             mbar_init(&v_full[s], 128);
-            mbar_init(&v_empty[s], 1);
+            mbar_init(&v_empty[s], 2);
         }
         for (uint32_t t = 0; t < 2; ++t) {
             mbar_init(&s_full[t][0], 1);
             mbar_init(&s_full[t][1], 1);
-            mbar_init(&o_full[t], 1);
-            mbar_init(&p_full[t], kHalf);
+            mbar_init(&o_full[t][0], 1);
+            mbar_init(&o_full[t][1], 1);
+            mbar_init(&p_full[t][0], kHalf);
+            mbar_init(&p_full[t][1], kHalf);
         }
-        mbar_init(&done, 1);
+        mbar_init(&done, 2);
     }
     if (warp == kMmaWarp) tc::alloc(&tmem_base, kTmemCols);
     tc::fence_before();
@@ -296,6 +300,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                 }
             }
         };
+        auto rescale_products = [&](float by) {
+#pragma unroll 1
+            for (uint32_t d = 0; d < HD; d += 16) {
+                uint32_t o[16];
+                ld_cols(o_col + d, o);
+                tc::wait_ld();
+#pragma unroll
+                for (uint32_t q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * by);
+                st_cols(o_col + d, o);
+            }
+            wait_st();
+        };
         const uint32_t from_mine = half ? from[1] : from[0], n_mine = (half ? upto[1] : upto[0]) - from_mine;
         for (uint32_t n = 0; n < n_mine; ++n) {
             const uint32_t i = from_mine + n, t0 = (tile0 + i) * KT, st = i % kStages;
@@ -307,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
             }
             tc::fence_after();
             float raised = 1.f;  // what the sums so far are multiplied by
+            bool rescale = false;  // those in tensor memory too
             auto step = [&](auto masked) {
                 constexpr bool kMasked = decltype(masked)::value;
                 constexpr uint32_t CH = S::kChunk, PC = CH < 32 ? CH : 32;  // scores held; of one store of P
@@ -321,11 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
 #pragma unroll
                         for (uint32_t q = 0; q < CH; ++q) s[q] = seen(c + q) ? s[q] : 0xff800000u;
                     }
-                    float high[2] = {-INFINITY, -INFINITY};
+                    float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (uint32_t q = 0; q < CH; q += 2)
-                        asm("max.f32 %0, %0, %1, %2;" : "+f"(high[q / 2 % 2]) : "f"(__uint_as_float(s[q])), "f"(__uint_as_float(s[q + 1])));
-                    top = fmaxf(top, fmaxf(high[0], high[1]));
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(high[q / 2 % 4]) : "f"(__uint_as_float(s[q])), "f"(__uint_as_float(s[q + 1])));
+                    top = fmaxf(fmaxf(top, high[0]), fmaxf(fmaxf(high[1], high[2]), high[3]));
                 }
                 top = top == -INFINITY ? top : top * factor;
                 if (__any_sync(0xffffffffu, top > m + kRaise)) {
@@ -335,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     l *= raised;
 #pragma unroll
                     for (uint32_t d = 0; d < HD; ++d) acc[d] *= raised;
+                    rescale = true;
                 }
                 const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
@@ -395,20 +413,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                         for (uint32_t k = 0; k < KT; ++k)
                             if (bad_values[st][b][k / 16] >> (k % 16) & 1u && t0 + k >= see0 && t0 + k < see1) nan_blocks |= 1u << b;
             }
-            if (n) {
-                if (!mbar_wait(&o_full[half], (n - 1) & 1u)) {
+            // The products so far are needed where a run of tiles ends, or the maximum was raised. (Two
+            // barriers in turn: the products of tile n - 3 are done, as the scores of tile n - 1 came after them, so
+            // that a wait for tile n - 1 cannot take another of its barrier's phases for it.)
+            const bool run_ends = n % S::kRun == 0;
+            if (n && (run_ends || rescale)) {
+                if (!mbar_wait(&o_full[half][(n - 1) & 1u], (n - 1) / 2 & 1u)) {
                     if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 105, blockIdx.x);
                     ok = false;
                     break;
                 }
                 tc::fence_after();
-                add_products(raised);
+                if (run_ends)
+                    add_products(raised);
+                else
+                    rescale_products(raised);
             }
             tc::fence_before();
-            arrive(&p_full[half]);
+            arrive(&p_full[half][n & 1u]);
         }
         if (ok && n_mine) {
-            if (mbar_wait(&o_full[half], (n_mine - 1) & 1u)) {
+            if (mbar_wait(&o_full[half][(n_mine - 1) & 1u], (n_mine - 1) / 2 & 1u)) {
                 tc::fence_after();
                 add_products(1.f);
             } else if (lane == 0) {
@@ -554,7 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                 load(i + 1, page_next, raw);
                 page_next = page_of(i + 2);
             }
-        } else if (warp == kMmaWarp) {
+        } else if (warp < kMmaWarp + 2) {
+            const uint32_t t = warp - kMmaWarp;  // the half
+            const uint32_t from_t = t ? from[1] : from[0], upto_t = t ? upto[1] : upto[0];
             const bool one = tc::elect();
             constexpr uint32_t idesc_s = (1u << 4) | ((KT >> 3) << 17) | ((kHalf >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t(HD) >> 3) << 17) | ((kHalf >> 4) << 24);
@@ -566,50 +593,48 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                 }
             };
             // Tile i's scores, and the products of tile i - 2, over whose P the scores go.
-            for (uint32_t i = 0; i < n_tiles + 2 && ok; ++i) {
+            for (uint32_t i = 0; i < n_tiles + 2; ++i) {
+                const uint32_t n = i - from_t;
+                const uint32_t s_col = tmem + (t * 2 + (n & 1u)) * KT;
+                if (i >= from_t + 2 && i < upto_t + 2 && upto_t > from_t) {
+                    const uint32_t st = (i - 2) % kStages, v = smem_addr(kv_smem + st * 2 * S::kTile + S::kTile);
+                    wait(&v_full[st], (i - 2) / kStages & 1u);
+                    wait(&p_full[t][n & 1u], (n - 2) / 2 & 1u);
+                    if (!ok) break;
+                    tc::fence_after();
+                    constexpr uint32_t PC = S::kChunk < 32 ? S::kChunk : 32;
+                    // lo first: its sums are too small to cut much off.
 #pragma unroll
-                for (uint32_t t = 0; t < 2; ++t) {
-                    const uint32_t s_col = tmem + (t * 2 + ((i - from[t]) & 1u)) * KT;
-                    if (i >= from[t] + 2 && i < upto[t] + 2 && active[t]) {
-                        const uint32_t st = (i - 2) % kStages, v = smem_addr(kv_smem + st * 2 * S::kTile + S::kTile);
-                        wait(&p_full[t], (i - from[t]) & 1u);
-                        wait(&v_full[st], (i - 2) / kStages & 1u);
-                        if (!ok) break;
-                        tc::fence_after();
-                        constexpr uint32_t PC = S::kChunk < 32 ? S::kChunk : 32;
-                        // lo first: its sums are too small to cut much off.
+                    for (uint32_t part = S::kPair ? 0 : 1; part < 2; ++part)
 #pragma unroll
-                        for (uint32_t part = S::kPair ? 0 : 1; part < 2; ++part)
-#pragma unroll
-                            for (uint32_t k = 0; k < KT / 16; ++k) {
-                                const uint32_t col = k * 16 / PC * PC + k * 16 % PC / 2 + (part == 0 ? PC / 2 : 0u);
-                                mma_ts(one, tmem + S::kOCol + t * HD, s_col + col, tc::desc_sw128(v + k * 32), idesc_o, part != (S::kPair ? 0 : 1) || k != 0);
-                            }
-                        tc::commit(one, &o_full[t]);
-                    }
-                    if (i >= from[t] && i < upto[t]) {
-                        const uint32_t st = i % kStages, kt = smem_addr(kv_smem + st * 2 * S::kTile);
-                        wait(&k_full[st], i / kStages & 1u);
-                        if (!ok) break;
-                        tc::fence_after();
-#pragma unroll
-                        for (uint32_t part = 0; part < (S::kPair ? 2 : 1); ++part) {
-                            const uint32_t which = S::kPair ? 1 - part : 0;
-#pragma unroll
-                            for (uint32_t k = 0; k < HD / 16; ++k) {
-                                const uint64_t db = tc::desc_sw128(kt + k / 4 * (KT * 128) + k % 4 * 32);
-                                if constexpr (S::kQTmem)
-                                    mma_ts(one, s_col, tmem + S::kQCol + t * HD + which * (HD / 2) + k * 8, db, idesc_s, part != 0 || k != 0);
-                                else
-                                    mma_ss(one, s_col, tc::desc_sw128(smem_addr(q_smem) + t * (S::kQBytes / 2) + which * S::kQPart + k / 4 * (kHalf * 128) + k % 4 * 32),
-                                           db, idesc_s, part != 0 || k != 0);
-                            }
+                        for (uint32_t k = 0; k < KT / 16; ++k) {
+                            const uint32_t col = k * 16 / PC * PC + k * 16 % PC / 2 + (part == 0 ? PC / 2 : 0u);
+                            mma_ts(one, tmem + S::kOCol + t * HD, s_col + col, tc::desc_sw128(v + k * 32), idesc_o,
+                                   part != (S::kPair ? 0 : 1) || k != 0 || (n - 2) % S::kRun != 0);
                         }
-                        tc::commit(one, &s_full[t][(i - from[t]) & 1u]);
-                    }
+                    tc::commit(one, &o_full[t][n & 1u]);
                 }
-                if (!ok) break;
                 if (i >= 2) tc::commit(one, &v_empty[(i - 2) % kStages]);
+                if (i >= from_t && i < upto_t) {
+                    const uint32_t st = i % kStages, kt = smem_addr(kv_smem + st * 2 * S::kTile);
+                    wait(&k_full[st], i / kStages & 1u);
+                    if (!ok) break;
+                    tc::fence_after();
+#pragma unroll
+                    for (uint32_t part = 0; part < (S::kPair ? 2 : 1); ++part) {
+                        const uint32_t which = S::kPair ? 1 - part : 0;
+#pragma unroll
+                        for (uint32_t k = 0; k < HD / 16; ++k) {
+                            const uint64_t db = tc::desc_sw128(kt + k / 4 * (KT * 128) + k % 4 * 32);
+                            if constexpr (S::kQTmem)
+                                mma_ts(one, s_col, tmem + S::kQCol + t * HD + which * (HD / 2) + k * 8, db, idesc_s, part != 0 || k != 0);
+                            else
+                                mma_ss(one, s_col, tc::desc_sw128(smem_addr(q_smem) + t * (S::kQBytes / 2) + which * S::kQPart + k / 4 * (kHalf * 128) + k % 4 * 32),
+                                       db, idesc_s, part != 0 || k != 0);
+                        }
+                    }
+                    tc::commit(one, &s_full[t][n & 1u]);
+                }
                 if (i < n_tiles) tc::commit(one, &k_empty[i % kStages]);
             }
             // Nothing may be in flight when the tensor memory is given back.
