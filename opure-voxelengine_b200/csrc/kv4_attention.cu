@@ -11,9 +11,9 @@
 // (exact in fp16). Score tiles come out with positions across lanes; movmatrix turns the
 // probabilities into the second product's operand.
 //
-// Each warp streams its own chunks of 64 positions through a ring of shared-memory stages filled by
-// bulk copies: no barrier between warps until they merge their states. The running maximum is
-// raised only when a score passes it by 2^8 (probabilities stay below 2^8, the sums in fp32).
+// Four warps take chunks of 64 positions in turn from rings of shared-memory stages, one for each,
+// that a fifth fills by bulk copies: no barrier between warps until they merge their states. The running
+// maximum is raised only when a score passes it by 2^8 (probabilities stay below 2^8, the sums in fp32).
 #include <algorithm>
 
 #include "kv4_attention.cuh"
@@ -24,14 +24,17 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kChunk = 64;      // positions per stage
 constexpr uint32_t kChunkGroups = kChunk / kKv4Group;
-template <int HD>
-constexpr uint32_t kStages = HD == 64 ? 4 : 3;
+constexpr uint32_t kThreads = (kWarps + 1) * 32;
+// Stages of a warp's ring and CTAs of an SM: as many of these as registers allow, the rest of shared
+// memory in stages (about 200 KB of copies under way in an SM).
+template <int HD, int NT>
+constexpr int kCtasPerSm = HD == 64 && NT == 1 ? 4 : HD == 64 ? 3 : 2;
+template <int HD, int NT>
+constexpr uint32_t kStages = HD == 64 && NT == 1 ? 3 : HD == 64 ? 4 : 3;
 template <int HD>
 constexpr uint32_t kStageBytes = kChunkGroups * kv4_group_bytes(HD);
-template <int HD>
-constexpr uint32_t kRowsSmem = kWarps * kStages<HD> * kStageBytes<HD>;
-template <int HD>
-constexpr int kCtasPerSm = HD == 64 ? 3 : 2;  // what the stages leave room for
+template <int HD, int NT>
+constexpr uint32_t kRowsSmem = kWarps * kStages<HD, NT> * kStageBytes<HD>;
 constexpr float kRaise = 8.f;        // log2 units by which a score may pass the running maximum
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -39,6 +42,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // from 0
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -68,15 +77,19 @@ __device__ __forceinline__ uint32_t lds16_at(uint32_t a) {
 }
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4AttnParams p) {
-    constexpr uint32_t kRows = 4 * NT, kPanels = HD / 64, S = kStages<HD>;
+__global__ void __launch_bounds__(kThreads, kCtasPerSm<HD, NT>) rows_kernel(Kv4AttnParams p) {
+    constexpr uint32_t kRows = 4 * NT, kPanels = HD / 64, S = kStages<HD, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t full[kWarps][S];
+    __shared__ __align__(8) uint64_t full[kWarps][S], empty[kWarps][S];
     __shared__ uint32_t have[kWarps][S];  // groups of the stage that hold positions of this split
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, c = lane & 3u, g = lane >> 2;
     const uint32_t unit = blockIdx.x, head = unit % p.kv.n_kv, tile = unit / p.kv.n_kv % p.row_tiles,
                    entry = unit / p.kv.n_kv / p.row_tiles;
-    if (lane < S) mbar_init(&full[warp][lane], 1);
+    if (warp < kWarps && lane < S) {
+        mbar_init(&full[warp][lane], 1);
+        mbar_init(&empty[warp][lane], 1);
+    }
+    __syncthreads();
     grid_dependency_wait();
     grid_dependents_launch();
 
@@ -105,53 +118,63 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
     if (end > begin ? split < s_first || split > s_last : split != 0u) return;
     const uint32_t t_begin = max(begin, split * p.split_tokens), t_end = min(end, (split + 1) * p.split_tokens);
     const uint32_t chunk0 = t_begin / kChunk * kChunk, n_chunks = t_end > t_begin ? (t_end - chunk0 + kChunk - 1) / kChunk : 0u;
-    const uint32_t mine = n_chunks > warp ? (n_chunks - warp + kWarps - 1) / kWarps : 0u;  // chunks warp, warp + kWarps, ..
+    auto share = [&](uint32_t w) { return n_chunks > w ? (n_chunks - w + kWarps - 1) / kWarps : 0u; };  // chunks w, w + kWarps, ..
 
-    // Copies. Four lanes fill a stage, each the groups of its part of the chunk (a page, or as much of
-    // one as the chunk covers); `k` counts this warp's chunks.
-    uint8_t *ring = smem + size_t(warp) * S * kStageBytes<HD>;
-    const uint32_t part = lane & 3u, span = min(P, kChunk), parts = kChunk / span;
-    const int32_t *table = p.kv.page_table + size_t(max(seq, 0)) * p.kv.max_pages;
-    auto page_of = [&](uint32_t k) -> int32_t {
-        const uint32_t t = chunk0 + (warp + k * kWarps) * kChunk + part * span;
-        if (k >= mine || part >= parts || t >= t_end || t + span <= t_begin) return -2;  // nothing to copy
-        const uint32_t lp = ring_slot(t / P, p.kv.ring);
-        return lp < p.kv.max_pages ? table[lp] : -1;
-    };
-    auto fill = [&](uint32_t k, int32_t page, bool active) {  // all lanes; `active` lanes are four of one k
-        const uint32_t stage = k % S, t = chunk0 + (warp + k * kWarps) * kChunk + part * span;
-        uint32_t g0 = 0, g1 = 0;
-        if (active && page != -2) {
-            if (page < 0 || uint32_t(page) >= p.kv.n_pages) {
-                report(p.st, OPURE_ERR_DEVICE_BOUNDS, 94, uint32_t(page));
-            } else {
-                g0 = t < t_begin ? (t_begin - t) / kKv4Group : 0u;
-                g1 = min(span, t_end - t + kKv4Group - 1) / kKv4Group;
+    if (warp == kWarps) {
+        // Copies: four lanes fill a warp's stage, each the groups of its part of the chunk (a page, or as
+        // much of one as the chunk covers); `k` counts each warp's chunks.
+        const uint32_t w = lane / 4 % kWarps, part = lane & 3u, span = min(P, kChunk), parts = kChunk / span, mine = share(w);
+        const bool active = lane < 4 * kWarps && part < parts;
+        const int32_t *table = p.kv.page_table + size_t(max(seq, 0)) * p.kv.max_pages;
+        auto page_of = [&](uint32_t k) -> int32_t {
+            const uint32_t t = chunk0 + (w + k * kWarps) * kChunk + part * span;
+            if (!active || k >= mine || t >= t_end || t + span <= t_begin) return -2;  // nothing to copy
+            const uint32_t lp = ring_slot(t / P, p.kv.ring);
+            return lp < p.kv.max_pages ? table[lp] : -1;
+        };
+        int32_t page = page_of(0);
+        const uint32_t rounds = share(0);
+        bool ok = true;
+        for (uint32_t k = 0; k < rounds && ok; ++k) {
+            const int32_t next_page = page_of(k + 1);
+            const uint32_t stage = k % S, t = chunk0 + (w + k * kWarps) * kChunk + part * span;
+            uint32_t g0 = 0, g1 = 0;
+            if (page != -2) {
+                if (page < 0 || uint32_t(page) >= p.kv.n_pages) {
+                    report(p.st, OPURE_ERR_DEVICE_BOUNDS, 94, uint32_t(page));
+                } else {
+                    g0 = t < t_begin ? (t_begin - t) / kKv4Group : 0u;
+                    g1 = min(span, t_end - t + kKv4Group - 1) / kKv4Group;
+                }
             }
+            const uint32_t bytes = (g1 - g0) * kv4_group_bytes(HD);
+            uint32_t sum = bytes, bits = ((1u << g1) - (1u << g0)) << (part * (span / kKv4Group));
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
+            bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
+            const bool there = lane < 4 * kWarps && k < mine;
+            if (k >= S) ok = __all_sync(0xffffffffu, !there || mbar_wait(&empty[w][stage], (k / S - 1) & 1u));
+            if (!ok) {
+                if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 106, blockIdx.x);
+                break;
+            }
+            if (there && part == 0) {
+                have[w][stage] = bits;
+                mbar_expect_tx(&full[w][stage], sum);
+            }
+            __syncwarp();
+            if (there && bytes) {
+                const uint8_t *src = p.kv.pool + ((size_t(page) * p.kv.n_kv + head) * (P / kKv4Group) + t % P / kKv4Group + g0) * kv4_group_bytes(HD);
+                bulk_load_keep(smem + (w * S + stage) * kStageBytes<HD> + (part * (span / kKv4Group) + g0) * kv4_group_bytes(HD), src, bytes, &full[w][stage]);
+            }
+            page = next_page;
         }
-        uint32_t bytes = (g1 - g0) * kv4_group_bytes(HD), sum = bytes;
-        uint32_t bits = ((1u << g1) - (1u << g0)) << (part * (span / kKv4Group));
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
-        bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
-        if (active && part == 0 && k < mine) {
-            have[warp][stage] = bits;
-            mbar_expect_tx(&full[warp][stage], sum);
-        }
-        __syncwarp();
-        if (bytes) {
-            const uint8_t *src = p.kv.pool + ((size_t(page) * p.kv.n_kv + head) * (P / kKv4Group) + t % P / kKv4Group + g0) * kv4_group_bytes(HD);
-            bulk_load_keep(ring + stage * kStageBytes<HD> + (part * (span / kKv4Group) + g0) * kv4_group_bytes(HD), src, bytes, &full[warp][stage]);
-        }
-    };
-    __syncwarp();
-    {
-        const uint32_t k = lane / 4;
-        fill(k, k < S ? page_of(k) : -2, k < S);
     }
-    int32_t next_page = page_of(S);  // asked for a chunk ahead of its copies
+    const uint32_t mine = warp < kWarps ? share(warp) : 0u;
+    uint8_t *ring = smem + size_t(warp) * S * kStageBytes<HD>;
 
+    if (warp < kWarps) {
     // Queries: row r of this lane's column. Each row is scaled by a power of two to [1, 2).
     uint32_t qf[HD / 16][NT][2];
     float factor[NT];
@@ -207,11 +230,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
         }
         const uint32_t groups = have[warp][stage], tok0 = chunk0 + (warp + k * kWarps) * kChunk;
         const bool whole = groups == (1u << kChunkGroups) - 1 && tok0 >= max(all_begin, t_begin) && tok0 + kChunk <= min(all_end, t_end);
+        // The tensor cores cut sums off where fp32 would round them: a chunk's sums start from 0 and join
+        // the others at its end (left to run on, their bias was 3 times all other errors).
+        float part[HD / 16][NT][4];
+        bool started = false;
 #pragma unroll 1
         for (uint32_t h = 0; h < kChunkGroups / 2; ++h) {
             if (!(groups >> (2 * h) & 3u)) continue;
             const uint32_t base = ring_addr + stage * kStageBytes<HD> + 2 * h * kv4_group_bytes(HD);
-            float s[2][NT][4] = {};
+            float s[2][NT][4];
 #pragma unroll
             for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
@@ -229,7 +256,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
                     for (uint32_t st = 0; st < 4; ++st) {
                         const uint32_t a[4] = {hmul2(k0[2 * st], s0), hmul2(k1[2 * st], s1), hmul2(k0[2 * st + 1], s0), hmul2(k1[2 * st + 1], s1)};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(s[u][nt], a, qf[pn * 4 + st][nt][0], qf[pn * 4 + st][nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (pn == 0 && st == 0)
+                                mma16816_first(s[u][nt], a, qf[0][nt][0], qf[0][nt][1]);
+                            else
+                                mma16816(s[u][nt], a, qf[pn * 4 + st][nt][0], qf[pn * 4 + st][nt][1]);
+                        }
                     }
                 }
             // Scores in log2 units: [u][position g, g + 8].
@@ -266,11 +298,21 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
                     for (uint32_t i = 0; i < HD / 16; ++i)
 #pragma unroll
                         for (int v = 0; v < 2; ++v) acc[i][nt][v] *= f;
+                    if (started)
+#pragma unroll
+                        for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) part[i][nt][v] *= f;
                 }
             }
-            // The tensor cores cut sums off where fp32 would round them: 32 positions' sums start from 0
-            // and join the others here (left to run on, their bias was 3 times all other errors).
-            float part[HD / 16][NT][4] = {};
+            if (!started)
+#pragma unroll
+                for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) part[i][nt][v] = 0.f;
+            started = true;
             uint32_t pf[2][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -339,16 +381,16 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
                         for (int nt = 0; nt < NT; ++nt) mma16816(part[pn * 4 + i][nt], a, pf[u][nt][0], pf[u][nt][1]);
                     }
                 }
+        }
+        if (started)
 #pragma unroll
             for (uint32_t i = 0; i < HD / 16; ++i)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int v = 0; v < 2; ++v) acc[i][nt][v] += fmaf(part[i][nt][2 * v + 1], 0x1p-11f, part[i][nt][2 * v]);
-        }
         __syncwarp();
-        fill(k + S, next_page, lane < 4);
-        next_page = page_of(k + S + 1);
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[warp][stage])) : "memory");
     }
     // No copy may still be landing when the stages are used again below: after a wait that gave up,
     // the later ones are waited for too (bounded).
@@ -376,6 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
             state[kRows * HD + kRows + r] = l;
         }
     }
+    }
     __syncthreads();
     auto warp_state = [&](uint32_t w) { return reinterpret_cast<const float *>(smem + size_t(w) * S * kStageBytes<HD>); };
     const uint32_t splits = end > begin ? s_last - s_first + 1 : 1u;
@@ -384,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
         const uint32_t q = first + r;
         kv4_store<T>(p, row0 + q / p.group, (head * p.group + q % p.group) * HD + d, a / fmaxf(l, 1e-30f) * p.v_scale);
     };
-    for (uint32_t i = threadIdx.x; i < rows * HD; i += kWarps * 32) {
+    for (uint32_t i = threadIdx.x; i < rows * HD; i += kThreads) {
         const uint32_t r = i / HD, d = i % HD;
         float m = -INFINITY;
 #pragma unroll
@@ -420,7 +463,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm<HD>) rows_kernel(Kv4At
     if (ticket != splits - 1) return;
     __threadfence();
     const float *parts_in = p.partials + (size_t(unit) * p.n_splits + s_first) * kRows * (HD + 2);
-    for (uint32_t i = threadIdx.x; i < rows * HD; i += kWarps * 32) {
+    for (uint32_t i = threadIdx.x; i < rows * HD; i += kThreads) {
         const uint32_t r = i / HD, d = i % HD;
         float m = -INFINITY;
 #pragma unroll 8
@@ -528,9 +571,9 @@ extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn
         using T = decltype(t);
         auto go = [&](auto k, uint32_t smem) -> opure_status {
             OPURE_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-            return launch(ctx, k, dim3(uint32_t(pl.units), pl.n_splits), dim3(kWarps * 32), smem, true, p);
+            return launch(ctx, k, dim3(uint32_t(pl.units), pl.n_splits), dim3(kThreads), smem, true, p);
         };
-        if (hd == 64) return pl.tile_rows == 4 ? go(rows_kernel<T, 64, 1>, kRowsSmem<64>) : go(rows_kernel<T, 64, 2>, kRowsSmem<64>);
-        return pl.tile_rows == 4 ? go(rows_kernel<T, 128, 1>, kRowsSmem<128>) : go(rows_kernel<T, 128, 2>, kRowsSmem<128>);
+        if (hd == 64) return pl.tile_rows == 4 ? go(rows_kernel<T, 64, 1>, kRowsSmem<64, 1>) : go(rows_kernel<T, 64, 2>, kRowsSmem<64, 2>);
+        return pl.tile_rows == 4 ? go(rows_kernel<T, 128, 1>, kRowsSmem<128, 1>) : go(rows_kernel<T, 128, 2>, kRowsSmem<128, 2>);
     });
 }
