@@ -28,13 +28,14 @@ constexpr uint32_t kThreads = (kWarps + 1) * 32;
 // Stages of a warp's ring and CTAs of an SM: as many of these as registers allow, the rest of shared
 // memory in stages (about 200 KB of copies under way in an SM).
 template <int HD, int NT>
-constexpr int kCtasPerSm = HD == 64 && NT == 1 ? 4 : HD == 64 ? 3 : 2;
+constexpr int kCtasPerSm = HD == 64 && NT == 1 ? 4 : 2;
 template <int HD, int NT>
-constexpr uint32_t kStages = HD == 64 && NT == 1 ? 3 : HD == 64 ? 4 : 3;
+constexpr uint32_t kStages = HD == 64 && NT == 2 ? 6 : 3;
 template <int HD>
 constexpr uint32_t kStageBytes = kChunkGroups * kv4_group_bytes(HD);
 template <int HD, int NT>
 constexpr uint32_t kRowsSmem = kWarps * kStages<HD, NT> * kStageBytes<HD>;
+constexpr uint32_t kMaxSplits = 64;
 constexpr float kRaise = 8.f;        // log2 units by which a score may pass the running maximum
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -175,249 +176,249 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<HD, NT>) rows_kernel(Kv4A
     uint8_t *ring = smem + size_t(warp) * S * kStageBytes<HD>;
 
     if (warp < kWarps) {
-    // Queries: row r of this lane's column. Each row is scaled by a power of two to [1, 2).
-    uint32_t qf[HD / 16][NT][2];
-    float factor[NT];
-    uint32_t row_end[NT], row_begin[NT];
+        // Queries: row r of this lane's column. Each row is scaled by a power of two to [1, 2).
+        uint32_t qf[HD / 16][NT][2];
+        float factor[NT];
+        uint32_t row_end[NT], row_begin[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t col_row = 4 * nt + g / 2;  // the row whose hi (g even) or lo this lane's B column holds
-        const bool live = col_row < rows;
-        const uint32_t q = first + (live ? col_row : 0u);
-        const T *qp = static_cast<const T *>(p.q) + size_t(row0 + q / p.group) * p.q_stride + (size_t(head) * p.group + q % p.group) * HD;
-        float v[HD / 4], m = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t col_row = 4 * nt + g / 2;  // the row whose hi (g even) or lo this lane's B column holds
+            const bool live = col_row < rows;
+            const uint32_t q = first + (live ? col_row : 0u);
+            const T *qp = static_cast<const T *>(p.q) + size_t(row0 + q / p.group) * p.q_stride + (size_t(head) * p.group + q % p.group) * HD;
+            float v[HD / 4], m = 0.f;
 #pragma unroll
-        for (uint32_t k = 0; k < HD / 4; ++k) {  // columns 64 panel + 16 c + ..
-            v[k] = live ? to_f32(qp[k / 16 * 64 + 16 * c + k % 16]) : 0.f;
-            m = fmaxf(m, fabsf(v[k]));
+            for (uint32_t k = 0; k < HD / 4; ++k) {  // columns 64 panel + 16 c + ..
+                v[k] = live ? to_f32(qp[k / 16 * 64 + 16 * c + k % 16]) : 0.f;
+                m = fmaxf(m, fabsf(v[k]));
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            // 2^-floor(log2 m), and back in the factor (m 0, infinite or subnormal: 1).
+            const uint32_t e = __float_as_uint(m) >> 23;
+            const bool normal = e > 0 && e < 253;
+            const float down = normal ? __uint_as_float((254u - e) << 23) : 1.f, up = normal ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+            for (uint32_t k = 0; k < HD / 4; k += 2) {
+                uint32_t pair[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) pair[u] = split_pair(v[k + u] * down);
+                qf[k / 4][nt][k / 2 % 2] = __byte_perm(pair[0], pair[1], g & 1u ? 0x7632 : 0x5410);
+            }
+            // Scores of this lane's accumulators belong to row 4 nt + c, whose columns lanes 8 c .. hold.
+            factor[nt] = __shfl_sync(0xffffffffu, up, 8 * c) * p.factor;
+            const uint32_t r = first + min(4u * nt + c, rows - 1), j = r / p.group;
+            row_end[nt] = uint32_t(max(len0 + int32_t(j), 0));
+            row_begin[nt] = window_begin(len0 + int32_t(j) - 1, P, p.kv.ring);
         }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        // 2^-floor(log2 m), and back in the factor (m 0, infinite or subnormal: 1).
-        const uint32_t e = __float_as_uint(m) >> 23;
-        const bool normal = e > 0 && e < 253;
-        const float down = normal ? __uint_as_float((254u - e) << 23) : 1.f, up = normal ? __uint_as_float(e << 23) : 1.f;
-#pragma unroll
-        for (uint32_t k = 0; k < HD / 4; k += 2) {
-            uint32_t pair[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) pair[u] = split_pair(v[k + u] * down);
-            qf[k / 4][nt][k / 2 % 2] = __byte_perm(pair[0], pair[1], g & 1u ? 0x7632 : 0x5410);
-        }
-        // Scores of this lane's accumulators belong to row 4 nt + c, whose columns lanes 8 c .. hold.
-        factor[nt] = __shfl_sync(0xffffffffu, up, 8 * c) * p.factor;
-        const uint32_t r = first + min(4u * nt + c, rows - 1), j = r / p.group;
-        row_end[nt] = uint32_t(max(len0 + int32_t(j), 0));
-        row_begin[nt] = window_begin(len0 + int32_t(j) - 1, P, p.kv.ring);
-    }
 
-    float acc[HD / 16][NT][2] = {};
-    float m_run[NT], l_run[NT];
+        float acc[HD / 16][NT][2] = {};
+        float m_run[NT], l_run[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        m_run[nt] = -INFINITY;
-        l_run[nt] = 0.f;
-    }
-    const uint32_t ring_addr = smem_addr(ring);
-    bool ok = true;
-    uint32_t k = 0;
-    for (; k < mine; ++k) {
-        const uint32_t stage = k % S;
-        if (!mbar_wait(&full[warp][stage], k / S & 1u)) {
-            if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 96, blockIdx.x);
-            ok = false;
-            break;
+        for (int nt = 0; nt < NT; ++nt) {
+            m_run[nt] = -INFINITY;
+            l_run[nt] = 0.f;
         }
-        const uint32_t groups = have[warp][stage], tok0 = chunk0 + (warp + k * kWarps) * kChunk;
-        const bool whole = groups == (1u << kChunkGroups) - 1 && tok0 >= max(all_begin, t_begin) && tok0 + kChunk <= min(all_end, t_end);
-        // The tensor cores cut sums off where fp32 would round them: a chunk's sums start from 0 and join
-        // the others at its end (left to run on, their bias was 3 times all other errors).
-        float part[HD / 16][NT][4];
-        bool started = false;
+        const uint32_t ring_addr = smem_addr(ring);
+        bool ok = true;
+        uint32_t k = 0;
+        for (; k < mine; ++k) {
+            const uint32_t stage = k % S;
+            if (!mbar_wait(&full[warp][stage], k / S & 1u)) {
+                if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 96, blockIdx.x);
+                ok = false;
+                break;
+            }
+            const uint32_t groups = have[warp][stage], tok0 = chunk0 + (warp + k * kWarps) * kChunk;
+            const bool whole = groups == (1u << kChunkGroups) - 1 && tok0 >= max(all_begin, t_begin) && tok0 + kChunk <= min(all_end, t_end);
+            // The tensor cores cut sums off where fp32 would round them: a chunk's sums start from 0 and join
+            // the others at its end (left to run on, their bias was 3 times all other errors).
+            float part[HD / 16][NT][4];
+            bool started = false;
 #pragma unroll 1
-        for (uint32_t h = 0; h < kChunkGroups / 2; ++h) {
-            if (!(groups >> (2 * h) & 3u)) continue;
-            const uint32_t base = ring_addr + stage * kStageBytes<HD> + 2 * h * kv4_group_bytes(HD);
-            float s[2][NT][4];
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                for (uint32_t pn = 0; pn < kPanels; ++pn) {
-                    const uint32_t at = base + u * kv4_group_bytes(HD);
-                    const uint4 w = lds128_at(at + pn * 512 + lane * 16);
-                    const uint32_t sp = kv4_scale_pair(lds16_at(at + 16 * HD + pn * 64 + lane * 2));
-                    const uint32_t s0 = __byte_perm(sp, sp, 0x1010), s1 = __byte_perm(sp, sp, 0x3232);
-                    uint32_t k0[8], k1[8];
-                    mx_unpack_fp4(w.x, *reinterpret_cast<uint32_t(*)[4]>(k0));
-                    mx_unpack_fp4(w.y, *reinterpret_cast<uint32_t(*)[4]>(k0 + 4));
-                    mx_unpack_fp4(w.z, *reinterpret_cast<uint32_t(*)[4]>(k1));
-                    mx_unpack_fp4(w.w, *reinterpret_cast<uint32_t(*)[4]>(k1 + 4));
-#pragma unroll
-                    for (uint32_t st = 0; st < 4; ++st) {
-                        const uint32_t a[4] = {hmul2(k0[2 * st], s0), hmul2(k1[2 * st], s1), hmul2(k0[2 * st + 1], s0), hmul2(k1[2 * st + 1], s1)};
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            if (pn == 0 && st == 0)
-                                mma16816_first(s[u][nt], a, qf[0][nt][0], qf[0][nt][1]);
-                            else
-                                mma16816(s[u][nt], a, qf[pn * 4 + st][nt][0], qf[pn * 4 + st][nt][1]);
-                        }
-                    }
-                }
-            // Scores in log2 units: [u][position g, g + 8].
-            float x[2][NT][2], top[NT];
-            bool raise = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (uint32_t h = 0; h < kChunkGroups / 2; ++h) {
+                if (!(groups >> (2 * h) & 3u)) continue;
+                const uint32_t base = ring_addr + stage * kStageBytes<HD> + 2 * h * kv4_group_bytes(HD);
+                float s[2][NT][4];
 #pragma unroll
                 for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
-                    for (uint32_t v = 0; v < 2; ++v) {
-                        x[u][nt][v] = fmaf(s[u][nt][2 * v + 1], 0x1p-11f, s[u][nt][2 * v]) * factor[nt];
-                        if (!whole) {
-                            const uint32_t t = tok0 + (2 * h + u) * kKv4Group + v * 8 + g;
-                            const bool seen = t >= max(row_begin[nt], t_begin) && t < min(row_end[nt], t_end) && (groups >> (2 * h + u) & 1u);
-                            x[u][nt][v] = seen ? x[u][nt][v] : -INFINITY;
+                    for (uint32_t pn = 0; pn < kPanels; ++pn) {
+                        const uint32_t at = base + u * kv4_group_bytes(HD);
+                        const uint4 w = lds128_at(at + pn * 512 + lane * 16);
+                        const uint32_t sp = kv4_scale_pair(lds16_at(at + 16 * HD + pn * 64 + lane * 2));
+                        const uint32_t s0 = __byte_perm(sp, sp, 0x1010), s1 = __byte_perm(sp, sp, 0x3232);
+                        uint32_t k0[8], k1[8];
+                        mx_unpack_fp4(w.x, *reinterpret_cast<uint32_t(*)[4]>(k0));
+                        mx_unpack_fp4(w.y, *reinterpret_cast<uint32_t(*)[4]>(k0 + 4));
+                        mx_unpack_fp4(w.z, *reinterpret_cast<uint32_t(*)[4]>(k1));
+                        mx_unpack_fp4(w.w, *reinterpret_cast<uint32_t(*)[4]>(k1 + 4));
+#pragma unroll
+                        for (uint32_t st = 0; st < 4; ++st) {
+                            const uint32_t a[4] = {hmul2(k0[2 * st], s0), hmul2(k1[2 * st], s1), hmul2(k0[2 * st + 1], s0), hmul2(k1[2 * st + 1], s1)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if (pn == 0 && st == 0)
+                                    mma16816_first(s[u][nt], a, qf[0][nt][0], qf[0][nt][1]);
+                                else
+                                    mma16816(s[u][nt], a, qf[pn * 4 + st][nt][0], qf[pn * 4 + st][nt][1]);
+                            }
                         }
                     }
-                top[nt] = fmaxf(fmaxf(x[0][nt][0], x[0][nt][1]), fmaxf(x[1][nt][0], x[1][nt][1]));
-                raise = raise || top[nt] > m_run[nt] + kRaise;
-            }
-            if (__any_sync(0xffffffffu, raise)) {
+                // Scores in log2 units: [u][position g, g + 8].
+                float x[2][NT][2], top[NT];
+                bool raise = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float m = top[nt];  // over the 8 lanes that share this lane's row
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(m, m_run[nt]);
-                    const float f = m == -INFINITY ? 1.f : fast_exp2(m_run[nt] - m);
-                    m_run[nt] = m;
-                    l_run[nt] *= f;
 #pragma unroll
-                    for (uint32_t i = 0; i < HD / 16; ++i)
+                    for (uint32_t u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int v = 0; v < 2; ++v) acc[i][nt][v] *= f;
-                    if (started)
+                        for (uint32_t v = 0; v < 2; ++v) {
+                            x[u][nt][v] = fmaf(s[u][nt][2 * v + 1], 0x1p-11f, s[u][nt][2 * v]) * factor[nt];
+                            if (!whole) {
+                                const uint32_t t = tok0 + (2 * h + u) * kKv4Group + v * 8 + g;
+                                const bool seen = t >= max(row_begin[nt], t_begin) && t < min(row_end[nt], t_end) && (groups >> (2 * h + u) & 1u);
+                                x[u][nt][v] = seen ? x[u][nt][v] : -INFINITY;
+                            }
+                        }
+                    top[nt] = fmaxf(fmaxf(x[0][nt][0], x[0][nt][1]), fmaxf(x[1][nt][0], x[1][nt][1]));
+                    raise = raise || top[nt] > m_run[nt] + kRaise;
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float m = top[nt];  // over the 8 lanes that share this lane's row
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        m = fmaxf(m, m_run[nt]);
+                        const float f = m == -INFINITY ? 1.f : fast_exp2(m_run[nt] - m);
+                        m_run[nt] = m;
+                        l_run[nt] *= f;
 #pragma unroll
                         for (uint32_t i = 0; i < HD / 16; ++i)
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) part[i][nt][v] *= f;
+                            for (int v = 0; v < 2; ++v) acc[i][nt][v] *= f;
+                        if (started)
+#pragma unroll
+                            for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) part[i][nt][v] *= f;
+                    }
                 }
+                if (!started)
+#pragma unroll
+                    for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) part[i][nt][v] = 0.f;
+                started = true;
+                uint32_t pf[2][NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float m = m_run[nt] == -INFINITY ? 0.f : m_run[nt];
+#pragma unroll
+                    for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                        for (uint32_t v = 0; v < 2; ++v) {
+                            const float e = fast_exp2(x[u][nt][v] - m);
+                            l_run[nt] += e;
+                            pf[u][nt][v] = transpose8x8(split_pair(e));
+                        }
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 2; ++u)
+#pragma unroll
+                    for (uint32_t pn = 0; pn < kPanels; ++pn) {
+                        const uint32_t at = base + u * kv4_group_bytes(HD);
+                        uint4 w = lds128_at(at + 8 * HD + pn * 512 + lane * 16);
+                        uint32_t sv = lds32_at(at + 17 * HD + pn * 64 + (g / 2 * 4 + c) * 4);
+                        if (!whole) {
+                            // Positions outside the split, of which anything may lie here: scale 0.
+                            const uint32_t t = tok0 + (2 * h + u) * kKv4Group + 2 * c;
+                            uint32_t keep = 0;
+#pragma unroll
+                            for (uint32_t b = 0; b < 4; ++b) {
+                                const uint32_t tt = t + b % 2 + 8 * (b / 2);
+                                keep |= (tt >= t_begin && tt < t_end ? 0xffu : 0u) << (8 * b);
+                            }
+                            sv &= groups >> (2 * h + u) & 1u ? keep : 0u;
+                            // A value that is NaN reaches the rows that see its position only: its scale
+                            // becomes 0, and those rows' sums NaN (0 times NaN would reach the others).
+                            uint32_t bad = 0;
+#pragma unroll
+                            for (uint32_t b = 0; b < 4; ++b)
+                                if ((sv >> (8 * b) & 0x7fu) == 0x7fu) {
+                                    bad |= 1u << (2 * c + b % 2 + 8 * (b / 2));
+                                    sv &= ~(0xffu << (8 * b));
+                                }
+                            bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+                            bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+                            if (bad) {
+                                const uint32_t t0 = tok0 + (2 * h + u) * kKv4Group;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    bool sees = false;
+                                    for (uint32_t b = 0; b < kKv4Group; ++b) sees = sees || (bad >> b & 1u && t0 + b >= row_begin[nt] && t0 + b < row_end[nt]);
+                                    if (sees)
+#pragma unroll
+                                        for (uint32_t i = 0; i < 4; ++i) acc[pn * 4 + i][nt][0] = acc[pn * 4 + i][nt][1] = NAN;
+                                }
+                            }
+                        }
+                        const uint32_t s01 = kv4_scale_pair(sv), s23 = kv4_scale_pair(sv >> 16);
+                        // Bytes of one column of two positions each, even and odd columns.
+                        const uint32_t lo = 0x0f0f0f0fu;
+                        uint32_t e01[4], o01[4], e23[4], o23[4];
+                        mx_unpack_fp4((w.x & lo) | (w.y << 4 & ~lo), e01);
+                        mx_unpack_fp4((w.x >> 4 & lo) | (w.y & ~lo), o01);
+                        mx_unpack_fp4((w.z & lo) | (w.w << 4 & ~lo), e23);
+                        mx_unpack_fp4((w.z >> 4 & lo) | (w.w & ~lo), o23);
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t a[4] = {hmul2(e01[i], s01), hmul2(o01[i], s01), hmul2(e23[i], s23), hmul2(o23[i], s23)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma16816(part[pn * 4 + i][nt], a, pf[u][nt][0], pf[u][nt][1]);
+                        }
+                    }
             }
-            if (!started)
+            if (started)
 #pragma unroll
                 for (uint32_t i = 0; i < HD / 16; ++i)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) part[i][nt][v] = 0.f;
-            started = true;
-            uint32_t pf[2][NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float m = m_run[nt] == -INFINITY ? 0.f : m_run[nt];
-#pragma unroll
-                for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                    for (uint32_t v = 0; v < 2; ++v) {
-                        const float e = fast_exp2(x[u][nt][v] - m);
-                        l_run[nt] += e;
-                        pf[u][nt][v] = transpose8x8(split_pair(e));
-                    }
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < 2; ++u)
-#pragma unroll
-                for (uint32_t pn = 0; pn < kPanels; ++pn) {
-                    const uint32_t at = base + u * kv4_group_bytes(HD);
-                    uint4 w = lds128_at(at + 8 * HD + pn * 512 + lane * 16);
-                    uint32_t sv = lds32_at(at + 17 * HD + pn * 64 + (g / 2 * 4 + c) * 4);
-                    if (!whole) {
-                        // Positions outside the split, of which anything may lie here: scale 0.
-                        const uint32_t t = tok0 + (2 * h + u) * kKv4Group + 2 * c;
-                        uint32_t keep = 0;
-#pragma unroll
-                        for (uint32_t b = 0; b < 4; ++b) {
-                            const uint32_t tt = t + b % 2 + 8 * (b / 2);
-                            keep |= (tt >= t_begin && tt < t_end ? 0xffu : 0u) << (8 * b);
-                        }
-                        sv &= groups >> (2 * h + u) & 1u ? keep : 0u;
-                        // A value that is NaN reaches the rows that see its position only: its scale
-                        // becomes 0, and those rows' sums NaN (0 times NaN would reach the others).
-                        uint32_t bad = 0;
-#pragma unroll
-                        for (uint32_t b = 0; b < 4; ++b)
-                            if ((sv >> (8 * b) & 0x7fu) == 0x7fu) {
-                                bad |= 1u << (2 * c + b % 2 + 8 * (b / 2));
-                                sv &= ~(0xffu << (8 * b));
-                            }
-                        bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-                        bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-                        if (bad) {
-                            const uint32_t t0 = tok0 + (2 * h + u) * kKv4Group;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                bool sees = false;
-                                for (uint32_t b = 0; b < kKv4Group; ++b) sees = sees || (bad >> b & 1u && t0 + b >= row_begin[nt] && t0 + b < row_end[nt]);
-                                if (sees)
-#pragma unroll
-                                    for (uint32_t i = 0; i < 4; ++i) acc[pn * 4 + i][nt][0] = acc[pn * 4 + i][nt][1] = NAN;
-                            }
-                        }
-                    }
-                    const uint32_t s01 = kv4_scale_pair(sv), s23 = kv4_scale_pair(sv >> 16);
-                    // Bytes of one column of two positions each, even and odd columns.
-                    const uint32_t lo = 0x0f0f0f0fu;
-                    uint32_t e01[4], o01[4], e23[4], o23[4];
-                    mx_unpack_fp4((w.x & lo) | (w.y << 4 & ~lo), e01);
-                    mx_unpack_fp4((w.x >> 4 & lo) | (w.y & ~lo), o01);
-                    mx_unpack_fp4((w.z & lo) | (w.w << 4 & ~lo), e23);
-                    mx_unpack_fp4((w.z >> 4 & lo) | (w.w & ~lo), o23);
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t a[4] = {hmul2(e01[i], s01), hmul2(o01[i], s01), hmul2(e23[i], s23), hmul2(o23[i], s23)};
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(part[pn * 4 + i][nt], a, pf[u][nt][0], pf[u][nt][1]);
-                    }
-                }
+                        for (int v = 0; v < 2; ++v) acc[i][nt][v] += fmaf(part[i][nt][2 * v + 1], 0x1p-11f, part[i][nt][2 * v]);
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[warp][stage])) : "memory");
         }
-        if (started)
-#pragma unroll
-            for (uint32_t i = 0; i < HD / 16; ++i)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) acc[i][nt][v] += fmaf(part[i][nt][2 * v + 1], 0x1p-11f, part[i][nt][2 * v]);
-        __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[warp][stage])) : "memory");
-    }
-    // No copy may still be landing when the stages are used again below: after a wait that gave up,
-    // the later ones are waited for too (bounded).
-    if (!ok)
-        for (uint32_t r = k; r < min(mine, k + S); ++r) (void)mbar_wait(&full[warp][r % S], r / S & 1u);
+        // No copy may still be landing when the stages are used again below: after a wait that gave up,
+        // the later ones are waited for too (bounded).
+        if (!ok)
+            for (uint32_t r = k; r < min(mine, k + S); ++r) (void)mbar_wait(&full[warp][r % S], r / S & 1u);
 
-    // This warp's state to its own stages: [rows][HD] sums, then maxima and denominators.
-    float *state = reinterpret_cast<float *>(ring);
+        // This warp's state to its own stages: [rows][HD] sums, then maxima and denominators.
+        float *state = reinterpret_cast<float *>(ring);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float l = l_run[nt];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        const uint32_t r = 4 * nt + c;
-        __syncwarp();
+        for (int nt = 0; nt < NT; ++nt) {
+            float l = l_run[nt];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const uint32_t r = 4 * nt + c;
+            __syncwarp();
 #pragma unroll
-        for (uint32_t i = 0; i < HD / 16; ++i) {
-            float *o = state + r * HD + i / 4 * 64 + 8 * g + i % 4 * 2;
-            o[0] = acc[i][nt][0];
-            o[1] = acc[i][nt][1];
+            for (uint32_t i = 0; i < HD / 16; ++i) {
+                float *o = state + r * HD + i / 4 * 64 + 8 * g + i % 4 * 2;
+                o[0] = acc[i][nt][0];
+                o[1] = acc[i][nt][1];
+            }
+            if (g == 0) {
+                state[kRows * HD + r] = m_run[nt];
+                state[kRows * HD + kRows + r] = l;
+            }
         }
-        if (g == 0) {
-            state[kRows * HD + r] = m_run[nt];
-            state[kRows * HD + kRows + r] = l;
-        }
-    }
     }
     __syncthreads();
     auto warp_state = [&](uint32_t w) { return reinterpret_cast<const float *>(smem + size_t(w) * S * kStageBytes<HD>); };
@@ -462,19 +463,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<HD, NT>) rows_kernel(Kv4A
     __syncthreads();
     if (ticket != splits - 1) return;
     __threadfence();
+    // The splits' maxima and denominators first, all at once, in the warps' stages.
+    static_assert(2 * kMaxSplits * kRows * sizeof(float) <= kRowsSmem<HD, NT>, "room for them");
     const float *parts_in = p.partials + (size_t(unit) * p.n_splits + s_first) * kRows * (HD + 2);
+    float *maxima = reinterpret_cast<float *>(smem), *sums = maxima + kMaxSplits * kRows;
+    for (uint32_t i = threadIdx.x; i < splits * rows; i += kThreads) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(parts_in + (size_t(i / rows) * kRows + i % rows) * (HD + 2) + HD));
+        maxima[i] = ml.x;
+        sums[i] = ml.y;
+    }
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < rows * HD; i += kThreads) {
         const uint32_t r = i / HD, d = i % HD;
         float m = -INFINITY;
-#pragma unroll 8
-        for (uint32_t sp = 0; sp < splits; ++sp) m = fmaxf(m, __ldcg(parts_in + (size_t(sp) * kRows + r) * (HD + 2) + HD));
+        for (uint32_t sp = 0; sp < splits; ++sp) m = fmaxf(m, maxima[sp * rows + r]);
         float a = 0.f, l = 0.f;
-#pragma unroll 8
+#pragma unroll 16  // independent loads
         for (uint32_t sp = 0; sp < splits; ++sp) {
-            const float *pp = parts_in + (size_t(sp) * kRows + r) * (HD + 2);
-            const float ms = __ldcg(pp + HD), f = ms == -INFINITY ? 1.f : fast_exp2(ms - m);
-            a += __ldcg(pp + d) * f;
-            l += __ldcg(pp + HD + 1) * f;
+            const float ms = maxima[sp * rows + r], f = ms == -INFINITY ? 1.f : fast_exp2(ms - m);
+            a += __ldcg(parts_in + (size_t(sp) * kRows + r) * (HD + 2) + d) * f;
+            l += sums[sp * rows + r] * f;
         }
         finish(r, d, a, l);
     }
@@ -498,13 +506,22 @@ Plan make_plan(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t
     p.tile_rows = p.prompt ? kKv4PromptRows : rows <= 4 ? 4 : 8;
     p.row_tiles = ceil_div(rows, p.tile_rows);
     p.units = uint64_t(n) * p.row_tiles * n_kv;
-    const uint64_t unit = 128, ctx = std::max(max_ctx, 1u), most = p.prompt ? 16 : 64;
-    static_assert(128 % kChunk == 0 && 128 % kKv4PromptKeys == 0, "whole chunks and tiles to a split");
-    const uint64_t slots = p.prompt ? uint64_t(sms) : uint64_t(sms) * (hd == 64 ? 3 : 2) * 4;
-    uint64_t want = split_tokens ? (ctx + split_tokens - 1) / split_tokens
-                                 : std::min<uint64_t>(most, std::max<uint64_t>(1, (slots + p.units - 1) / p.units));
-    want = std::min<uint64_t>(want, (ctx + unit - 1) / unit);
-    const uint64_t per = split_tokens ? split_tokens : (ctx + want - 1) / want;
+    // Splits in steps of a chunk for each warp, or of prompts' tiles.
+    const uint64_t unit = p.prompt ? kKv4PromptKeys : kWarps * kChunk, ctx = std::max(max_ctx, 1u);
+    uint64_t want;
+    if (p.prompt) {
+        want = std::min<uint64_t>(16, (uint64_t(sms) + p.units - 1) / p.units);
+    } else {
+        // As many CTAs as the SMs hold, in splits of 256 keys or more; three times as many where
+        // that leaves 2048 keys to a split, so that the last ones to run are short. Measured: 1 x 4001 keys x 3 kv
+        // heads 12.0 us in splits of 128, 9.4 in 256; 16 x 5 queries x 2000 35 us in 128, 20 in 512 and
+        // 1024; 64 x 32768 x 3 141 us in 4 splits, 122 in 10, 129 in 16; 64 x 4096 x 32 151 us in one, 183 in two.
+        const uint64_t slots = uint64_t(sms) * (hd == 64 ? (p.tile_rows == 4 ? kCtasPerSm<64, 1> : kCtasPerSm<64, 2>) : kCtasPerSm<128, 1>);
+        want = std::min<uint64_t>((slots + p.units - 1) / p.units, (ctx + unit - 1) / unit);
+        want = std::max<uint64_t>(want, std::min<uint64_t>((slots * 3 + p.units - 1) / p.units, ctx / 2048));
+    }
+    want = std::min<uint64_t>(std::max<uint64_t>(want, 1), std::min<uint64_t>(kMaxSplits, (ctx + unit - 1) / unit));
+    const uint64_t per = split_tokens ? std::max<uint64_t>(split_tokens, (ctx + kMaxSplits - 1) / kMaxSplits) : (ctx + want - 1) / want;
     p.split_tokens = uint32_t(std::min<uint64_t>((per + unit - 1) / unit * unit, 0xffffff80u));
     p.n_splits = ceil_div(ctx, p.split_tokens);
     const size_t partials = p.n_splits > 1 ? size_t(p.units) * p.n_splits * p.tile_rows * (hd + 2) * sizeof(float) : 0;
