@@ -46,7 +46,17 @@ typedef struct opure_engine_options {
                                  pages and its own; 0: every position up to max_len */
     uint32_t tp_allreduce;    /* tensor parallel: OPURE_TP_* (0: OPURE_TP_AUTO)          */
     uint32_t weights;         /* OPURE_WEIGHTS_*: how the layer matrices are kept        */
+    uint32_t kv;              /* OPURE_KV_*: how keys and values are cached              */
 } opure_engine_options;
+
+enum {
+    OPURE_KV_FP16 = 0,
+    OPURE_KV_FP4 = 1          /* 4 bits with a scale for each 16 columns (opure_kv4_layout): 0.5625
+                                 bytes a value instead of 2. Appended to and attended over by
+                                 opure_kv4_append and opure_kv4_attention, several queries of a
+                                 sequence at once in chunked prefill and verify steps; per-op kernels
+                                 only, head_dim 64 or 128, on one GPU                       */
+};
 
 enum {
     OPURE_WEIGHTS_STORED = 0, /* as the model file has them: fp16, or int8 with its scales */
@@ -82,10 +92,11 @@ typedef struct opure_engine_info {
     uint32_t max_len, max_batch, page_size, w_dtype;
     uint64_t weight_bytes;        /* resident weight arena                              */
     uint64_t stream_bytes;        /* weight bytes one decode step reads                 */
-    uint64_t kv_bytes_per_token;  /* fp16 K+V, all layers, one sequence                 */
+    uint64_t kv_bytes_per_token;  /* K+V as cached, all layers, one sequence             */
     uint32_t tp_ranks;            /* tensor-parallel ranks (1 without a communicator)     */
     uint32_t tp_peer;             /* 1: collectives run as NVLink peer kernels, 0: NCCL   */
     uint32_t weights;             /* OPURE_WEIGHTS_*                                      */
+    uint32_t kv;                  /* OPURE_KV_*                                           */
 } opure_engine_info;
 
 typedef struct opure_generate_timing {
@@ -248,6 +259,18 @@ opure_status opure_engine_sample_generate(opure_engine *e, const int32_t *prompt
                                           uint32_t budget, const opure_sample_options *o, int32_t *out_tokens,
                                           float *stats, float *logits);
 
+/* Scores of given tokens: for each of n_seq sequences (concatenated in `tokens`, of lens[s] tokens) the
+ * log probability of every token after those before it, its rank, and the entropy (nats) and the `top`
+ * most likely tokens of the distribution it was taken from, as opure_token_scores defines them. Results
+ * are aligned with the tokens; a sequence's first token has none: log probability, rank and entropy 0,
+ * top tokens -1 with log probability -inf. The sequences run as steps of prefill_chunk token vectors
+ * (without one, of max_batch), so that perplexities, or what a 4-bit cache or 4-bit weights cost, come
+ * at the rate of a prefill. logprobs [sum of lens]; ranks, entropies (the same) and top_tokens,
+ * top_logprobs [sum of lens][top] may be NULL, the latter two with top 0. n_seq <= max_batch, lens <= max_len,
+ * one GPU. With a KV window a sequence has to fit it, as for chunked prefill. */
+opure_status opure_engine_score(opure_engine *e, const int32_t *tokens, const uint32_t *lens, uint32_t n_seq, uint32_t top,
+                                float *logprobs, int32_t *ranks, float *entropies, int32_t *top_tokens, float *top_logprobs);
+
 /* Parses config.json, maps model.safetensors, resolves tensor roles and plans the device
  * layout without touching a GPU (the reference's opure_inspect tool, Opure_Inspect.cpp).
  * On failure the reason is copied to err (err_len bytes, may be NULL). */
@@ -260,8 +283,11 @@ opure_status opure_model_inspect(const char *model_dir, opure_engine_info *info,
  * (clamped to 1..2048), "temperature": t (> 0: sampled), "seed": s} and answers
  * {"tokens": [...], "prompt_tokens", "generated_tokens", "ms_per_token", "total_ms",
  * "hit_stop", "engine"}; there is no tokenizer, so a text "prompt" is refused with 400.
+ * POST /score takes {"tokens": [ids], "top": k (0..32)} and answers opure_engine_score's results,
+ * {"logprobs": [...], "ranks": [...], "entropies": [...], "top": [{"tokens", "logprobs"}, ...],
+ * "total_logprob", "engine"}, the first token's null.
  * Bodies over 1 MiB: 413; unknown routes 404; wrong methods 405; chunked bodies 400;
- * /generate with no engine (n_devices 0): 503. */
+ * /generate and /score with no engine (n_devices 0): 503. */
 typedef struct opure_server opure_server;
 opure_status opure_server_start(const char *model_dir, const int *devices, uint32_t n_devices, uint16_t port,
                                 const opure_engine_options *opts, opure_server **out);

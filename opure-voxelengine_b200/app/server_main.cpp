@@ -1,5 +1,5 @@
-// opure_server -- the HTTP front end (GET /health, POST /generate, GET /metrics) over
-// libopure_engine: `opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4]`,
+// opure_server -- the HTTP front end (GET /health, POST /generate, POST /score, GET /metrics) over
+// libopure_engine: `opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4] [--kv fp4]`,
 // one engine per listed GPU (the reference's opure_server, src/app/Opure_Server.cpp:470-540, runs one
 // engine on its one D3D12 device). Runs until SIGINT/SIGTERM.
 #include <csignal>
@@ -41,9 +41,13 @@ int main(int argc, char **argv) {
         } else if (a == "--weights" && i + 1 < argc && !std::strcmp(argv[i + 1], "mxfp4")) {
             ++i;
             opts.weights = OPURE_WEIGHTS_MXFP4;
+        } else if (a == "--kv" && i + 1 < argc && !std::strcmp(argv[i + 1], "fp4")) {
+            ++i;
+            opts.kv = OPURE_KV_FP4;
         } else {
-            std::printf("usage: opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4]\n"
-                        "routes: GET /health, POST /generate {\"tokens\":[...],\"max_tokens\":64}, GET /metrics\n");
+            std::printf("usage: opure_server --model <dir> [--port N] [--gpus 0,1,...] [--weights mxfp4] [--kv fp4]\n"
+                        "routes: GET /health, POST /generate {\"tokens\":[...],\"max_tokens\":64}, "
+                        "POST /score {\"tokens\":[...],\"top\":5}, GET /metrics\n");
             return a == "--help" || a == "-h" ? 0 : 2;
         }
     }
@@ -54,7 +58,7 @@ int main(int argc, char **argv) {
     opure_server *srv = nullptr;
     const opure_status st =
         opure_server_start(model.c_str(), gpus.data(), uint32_t(gpus.size()), uint16_t(port),
-                           opts.weights ? &opts : nullptr, &srv);
+                           opts.weights || opts.kv ? &opts : nullptr, &srv);
     if (st != OPURE_OK) {
         std::fprintf(stderr, "opure_server: %s: %s\n", opure_strerror(st), opure_engine_last_error(nullptr));
         return 1;

@@ -72,6 +72,8 @@ opure::engine::EngineOptions ToOptions(const opure_engine_options *o) {
         opts.tpAllreduce = o->tp_allreduce;
         OPURE_CHECK(o->weights <= OPURE_WEIGHTS_MXFP4, "unknown weight format");
         opts.mxWeights = o->weights == OPURE_WEIGHTS_MXFP4;
+        OPURE_CHECK(o->kv <= OPURE_KV_FP4, "unknown KV cache format");
+        opts.kvFp4 = o->kv == OPURE_KV_FP4;
     }
     return opts;
 }
@@ -210,6 +212,26 @@ opure_status opure_engine_sample_generate(opure_engine *e, const int32_t *prompt
     });
 }
 
+opure_status opure_engine_score(opure_engine *e, const int32_t *tokens, const uint32_t *lens, uint32_t n_seq, uint32_t top,
+                                float *logprobs, int32_t *ranks, float *entropies, int32_t *top_tokens, float *top_logprobs) {
+    if (!e || !tokens || !lens || n_seq == 0 || !logprobs || (top && (!top_tokens || !top_logprobs))) return OPURE_ERR_INVALID_ARG;
+    return Guard(e, [&] {
+        std::vector<std::vector<uint32_t>> seqs(n_seq);
+        for (uint32_t s = 0; s < n_seq; tokens += lens[s++]) seqs[s] = ToU32(tokens, lens[s]);
+        size_t at = 0;
+        for (const auto &r : e->eng.Score(seqs, top)) {
+            std::copy(r.logprobs.begin(), r.logprobs.end(), logprobs + at);
+            if (ranks) std::copy(r.ranks.begin(), r.ranks.end(), ranks + at);
+            if (entropies) std::copy(r.entropies.begin(), r.entropies.end(), entropies + at);
+            if (top) {
+                std::copy(r.topTokens.begin(), r.topTokens.end(), top_tokens + at * top);
+                std::copy(r.topLogprobs.begin(), r.topLogprobs.end(), top_logprobs + at * top);
+            }
+            at += r.logprobs.size();
+        }
+    });
+}
+
 opure_status opure_engine_destroy(opure_engine *e) {
     if (!e) return OPURE_ERR_INVALID_ARG;
     delete e;
@@ -252,6 +274,10 @@ opure_status opure_engine_get_info(opure_engine *e, opure_engine_info *info) {
         info->max_batch = e->eng.Options().maxBatch;
         info->page_size = e->eng.Options().pageSize;
         info->tp_peer = e->eng.UsesPeer() ? 1 : 0;
+        if (e->eng.Options().kvFp4) {
+            info->kv = OPURE_KV_FP4;
+            info->kv_bytes_per_token = uint64_t(info->layers) * opure_kv4_page_bytes(info->kv_heads, info->head_dim, info->page_size) / info->page_size;
+        }
     });
 }
 

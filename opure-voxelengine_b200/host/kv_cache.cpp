@@ -12,7 +12,7 @@ PagedKvCache::~PagedKvCache() { Destroy(); }
 
 void PagedKvCache::Create(opure_ctx *ctx, const graph::ModelConfig &cfg, uint32_t page_size,
                           uint32_t n_pages, uint32_t max_seqs, uint32_t max_pages_per_seq,
-                          uint64_t shuffle_seed, uint32_t ring) {
+                          uint64_t shuffle_seed, uint32_t ring, bool fp4) {
     Destroy();
     OPURE_CHECK(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128,
                 "KV page size must be 16, 32, 64 or 128 tokens");
@@ -27,7 +27,10 @@ void PagedKvCache::Create(opure_ctx *ctx, const graph::ModelConfig &cfg, uint32_
     maxSeqs_ = max_seqs;
     maxPages_ = max_pages_per_seq;
     ring_ = ring;
-    poolBytes_ = uint64_t(n_pages) * 2 * nKv_ * page_size * headDim_ * 2;
+    fp4_ = fp4;
+    OPURE_CHECK(!fp4 || opure_kv4_page_bytes(nKv_, headDim_, page_size), "a 4-bit KV cache needs head_dim 64 or 128");
+    poolBytes_ = fp4 ? uint64_t(n_pages) * opure_kv4_page_bytes(nKv_, headDim_, page_size)
+                     : uint64_t(n_pages) * 2 * nKv_ * page_size * headDim_ * 2;
     OPURE_CUDA_CHECK(opure_alloc(ctx_, poolBytes_ * layers_, &pools_));
     OPURE_CUDA_CHECK(opure_fill(ctx_, pools_, 0, poolBytes_ * layers_));
     void *t = nullptr;
@@ -110,6 +113,19 @@ uint16_t *PagedKvCache::Pool(uint32_t layer) const {
 opure_kv_layout PagedKvCache::Layout(uint32_t layer) const {
     opure_kv_layout l{};
     l.pool = Pool(layer);
+    l.page_table = dTable_;
+    l.n_pages = nPages_;
+    l.max_pages = maxPages_;
+    l.page_size = pageSize_;
+    l.n_kv = nKv_;
+    l.head_dim = headDim_;
+    l.ring = ring_;
+    return l;
+}
+
+opure_kv4_layout PagedKvCache::Layout4(uint32_t layer) const {
+    opure_kv4_layout l{};
+    l.pool = static_cast<uint8_t *>(pools_) + poolBytes_ * layer;
     l.page_table = dTable_;
     l.n_pages = nPages_;
     l.max_pages = maxPages_;

@@ -15,6 +15,8 @@
 // overwrites its own oldest page in place instead of mapping a new one. This replaces the
 // reference's eviction, which shifts the whole cache by one position with a memmove
 // dispatch per layer (EvictOldestKV, Opure_VoxelEngine.cpp:721-763; Opure_Memmove.usf).
+//
+// With fp4 the pools hold the 4-bit form (opure_kv4_layout); pages, table and ring are the same.
 #pragma once
 
 #include <cstdint>
@@ -33,7 +35,7 @@ public:
     PagedKvCache &operator=(const PagedKvCache &) = delete;
 
     void Create(opure_ctx *ctx, const graph::ModelConfig &cfg, uint32_t page_size, uint32_t n_pages,
-                uint32_t max_seqs, uint32_t max_pages_per_seq, uint64_t shuffle_seed, uint32_t ring = 0);
+                uint32_t max_seqs, uint32_t max_pages_per_seq, uint64_t shuffle_seed, uint32_t ring = 0, bool fp4 = false);
     void Destroy();
 
     // Maps pages for positions [0, tokens) of `seq` (with a window: at most `ring` pages,
@@ -48,6 +50,8 @@ public:
     void SyncTable();                              // upload the table when it changed
 
     opure_kv_layout Layout(uint32_t layer) const;
+    opure_kv4_layout Layout4(uint32_t layer) const;
+    bool Fp4() const { return fp4_; }
     uint16_t *Pool(uint32_t layer) const;
     const int32_t *DeviceTable() const { return dTable_; }
     uint32_t PageSize() const { return pageSize_; }
@@ -63,6 +67,7 @@ private:
     uint32_t layers_ = 0, nKv_ = 0, headDim_ = 0;
     uint32_t pageSize_ = 0, nPages_ = 0, maxSeqs_ = 0, maxPages_ = 0, ring_ = 0;
     uint64_t poolBytes_ = 0;
+    bool fp4_ = false;
     void *pools_ = nullptr;            // layers_ * poolBytes_
     int32_t *dTable_ = nullptr;        // [maxSeqs_][maxPages_]
     std::vector<int32_t> table_;       // host mirror, -1 = unmapped

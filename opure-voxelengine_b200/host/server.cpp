@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cctype>
 #include <chrono>
+#include <cmath>
 #include <cstdlib>
 #include <cstdio>
 #include <cstring>
@@ -145,15 +146,10 @@ std::string JsonString(std::string_view s) {
     return out + "\"";
 }
 
-bool ParseGenerate(std::string_view body, uint32_t vocab, GenerateRequest &out, std::string &err) {
-    out = GenerateRequest{};
-    json::Value v;
-    try {
-        v = json::ParseObject(body, "/generate");
-    } catch (const std::exception &e) {
-        err = e.what();
-        return false;
-    }
+namespace {
+
+// The body's "tokens".
+bool ParseTokens(const json::Value &v, uint32_t vocab, std::vector<uint32_t> &out, std::string &err) {
     const json::Value *toks = v.Find("tokens");
     if (!toks) {
         err = v.Find("prompt") ? "this server loads no tokenizer: send the prompt as token ids in \"tokens\""
@@ -169,8 +165,49 @@ bool ParseGenerate(std::string_view body, uint32_t vocab, GenerateRequest &out, 
             err = "\"tokens\" holds an entry that is not a token id of this model";
             return false;
         }
-        out.tokens.push_back(uint32_t(t.inum));
+        out.push_back(uint32_t(t.inum));
     }
+    return true;
+}
+
+bool ParseBody(std::string_view body, const char *route, json::Value &v, std::string &err) {
+    try {
+        v = json::ParseObject(body, route);
+    } catch (const std::exception &e) {
+        err = e.what();
+        return false;
+    }
+    return true;
+}
+
+// A number that JSON has: NaN and infinities as null.
+std::string Number(float x) {
+    if (!std::isfinite(x)) return "null";
+    char b[32];
+    std::snprintf(b, sizeof(b), "%.7g", double(x));
+    return b;
+}
+
+}  // namespace
+
+bool ParseScore(std::string_view body, uint32_t vocab, ScoreRequest &out, std::string &err) {
+    out = ScoreRequest{};
+    json::Value v;
+    if (!ParseBody(body, "/score", v, err) || !ParseTokens(v, vocab, out.tokens, err)) return false;
+    if (const json::Value *t = v.Find("top")) {
+        if (!t->IsNumber() || !t->integral || t->inum < 0 || t->inum > int64_t(OPURE_SCORE_MAX_TOP)) {
+            err = "\"top\" must be a whole number from 0 to " + std::to_string(OPURE_SCORE_MAX_TOP);
+            return false;
+        }
+        out.top = uint32_t(t->inum);
+    }
+    return true;
+}
+
+bool ParseGenerate(std::string_view body, uint32_t vocab, GenerateRequest &out, std::string &err) {
+    out = GenerateRequest{};
+    json::Value v;
+    if (!ParseBody(body, "/generate", v, err) || !ParseTokens(v, vocab, out.tokens, err)) return false;
     if (const json::Value *m = v.Find("max_tokens")) {
         if (!m->IsNumber()) {
             err = "\"max_tokens\" must be a number";
@@ -312,7 +349,15 @@ Response Server::Handle(std::string_view raw, int slot) {
             return {400, "{\"error\":" + JsonString(err) + "}"};
         return Generate(req, slot);
     }
-    if (route == "/health" || route == "/metrics" || route == "/generate")
+    if (route == "/score" && method == "POST") {
+        if (slot < 0) return {503, R"({"error":"no engine is loaded"})"};
+        ScoreRequest req;
+        std::string err;
+        if (!ParseScore(body, engines_[size_t(slot)]->Model().vocabSize, req, err))
+            return {400, "{\"error\":" + JsonString(err) + "}"};
+        return Score(req, slot);
+    }
+    if (route == "/health" || route == "/metrics" || route == "/generate" || route == "/score")
         return {405, R"({"error":"method not allowed"})"};
     return {404, R"({"error":"no such route"})"};
 }
@@ -354,6 +399,41 @@ Response Server::Generate(const GenerateRequest &req, int slot) {
     std::snprintf(perf, sizeof(perf), ",\"ms_per_token\":%.4f,\"total_ms\":%.4f,\"hit_stop\":%s,\"engine\":%d}",
                   r.msPerToken, total_ms, r.hitStop ? "true" : "false", slot);
     return {200, j + perf};
+}
+
+Response Server::Score(const ScoreRequest &req, int slot) {
+    engine::SequenceScores r;
+    try {
+        r = engines_[size_t(slot)]->Score({req.tokens}, req.top).front();
+    } catch (const std::exception &e) {
+        return {200, "{\"error\":" + JsonString(e.what()) + "}"};  // as /generate
+    }
+    {
+        std::lock_guard<std::mutex> lk(metricsMu_);
+        ++served_;
+    }
+    const size_t n = req.tokens.size();
+    auto list = [&](auto &&item) {  // null for the first token, which nothing precedes
+        std::string j = "[null";
+        for (size_t i = 1; i < n; ++i) j += "," + item(i);
+        return j + "]";
+    };
+    double total = 0.0;
+    for (size_t i = 1; i < n; ++i) total += r.logprobs[i];
+    std::string j = "{\"logprobs\":" + list([&](size_t i) { return Number(r.logprobs[i]); });
+    j += ",\"ranks\":" + list([&](size_t i) { return std::to_string(r.ranks[i]); });
+    j += ",\"entropies\":" + list([&](size_t i) { return Number(r.entropies[i]); });
+    if (req.top)
+        j += ",\"top\":" + list([&](size_t i) {
+            std::string ids, lps;
+            for (uint32_t k = 0; k < req.top; ++k) {
+                ids += (k ? "," : "") + std::to_string(r.topTokens[i * req.top + k]);
+                lps += (k ? "," : "") + Number(r.topLogprobs[i * req.top + k]);
+            }
+            return "{\"tokens\":[" + ids + "],\"logprobs\":[" + lps + "]}";
+        });
+    j += ",\"total_logprob\":" + Number(float(total)) + ",\"engine\":" + std::to_string(slot) + "}";
+    return {200, j};
 }
 
 std::string Server::HealthJson() const {

@@ -35,6 +35,13 @@ struct GenerateRequest {
     uint64_t seed = 0;
 };
 
+// A parsed POST /score body.
+struct ScoreRequest {
+    std::vector<uint32_t> tokens;
+    uint32_t top = 0;
+};
+bool ParseScore(std::string_view body, uint32_t vocab, ScoreRequest &out, std::string &err);
+
 // Parses a /generate body. On failure returns false with the client-facing message in err
 // (the reference's wording where it has one). Validates every token against `vocab`
 // (0: unchecked) and clamps max_tokens and temperature as the reference does.
@@ -51,8 +58,8 @@ std::string JsonString(std::string_view s);
 
 class Server {
 public:
-    // engines: one per GPU, owned; may be empty (the routes still answer, /generate with
-    // 503). Binds 127.0.0.1:port (0: any free port) and starts one worker per engine (one
+    // engines: one per GPU, owned; may be empty (the routes still answer, /generate and
+    // /score with 503). Binds 127.0.0.1:port (0: any free port) and starts one worker per engine (one
     // when there are none) and an accept thread.
     Server(std::vector<std::unique_ptr<engine::VoxelEngine>> engines, uint16_t port);
     ~Server();
@@ -71,6 +78,7 @@ private:
     std::string HealthJson() const;
     std::string MetricsJson();
     Response Generate(const GenerateRequest &req, int slot);
+    Response Score(const ScoreRequest &req, int slot);
 
     std::vector<std::unique_ptr<engine::VoxelEngine>> engines_;
     int listenFd_ = -1;

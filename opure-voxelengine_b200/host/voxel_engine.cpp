@@ -2,6 +2,7 @@
 #include "voxel_engine.h"
 
 #include <algorithm>
+#include <bit>
 #include <cmath>
 #include <cstring>
 
@@ -45,7 +46,9 @@ void VoxelEngine::Shutdown() {
                     static_cast<void *>(buf_.sumsq), static_cast<void *>(buf_.mxNorm.codes),
                     static_cast<void *>(buf_.mxNorm.scales), static_cast<void *>(buf_.mxAttn.codes),
                     static_cast<void *>(buf_.mxAttn.scales), static_cast<void *>(buf_.mxAct.codes),
-                    static_cast<void *>(buf_.mxAct.scales), weights_})
+                    static_cast<void *>(buf_.mxAct.scales), static_cast<void *>(buf_.runSeq),
+                    static_cast<void *>(buf_.runLen), static_cast<void *>(buf_.runBegin),
+                    static_cast<void *>(buf_.scoreTokens), static_cast<void *>(buf_.scoreOut), weights_})
         if (p) opure_free(ctx_, p);
     for (auto &s : attnScratch_) opure_free(ctx_, s.second.first);
     attnScratch_.clear();
@@ -75,13 +78,14 @@ void VoxelEngine::Initialize(const std::string &modelDir, const EngineOptions &o
         ownsCtx_ = true;
     }
     graph::LayoutOptions lo;
-    lo.fusedLayouts = opts.path != 1;  // grouped o_proj and transposed down_proj
+    lo.fusedLayouts = opts.path != 1 && !opts.kvFp4;  // grouped o_proj and transposed down_proj
     lo.mxWeights = opts.mxWeights;
     comm_ = comm;
     if (comm) {
         OPURE_CUDA_CHECK(opure_comm_info(comm, &lo.tpSize, &lo.tpRank));
         lo.fusedLayouts = false;
         OPURE_CHECK(opts.path != 2, "the fused decode path does not run tensor-parallel");
+        OPURE_CHECK(!opts.kvFp4, "the 4-bit KV cache does not run tensor-parallel");
     }
     graph_.LoadConfigOnly(modelDir, lo);
     const graph::ModelConfig &cfg = graph_.Config();
@@ -98,7 +102,8 @@ void VoxelEngine::Initialize(const std::string &modelDir, const EngineOptions &o
     graph::ModelConfig kvCfg = cfg;
     kvCfg.numKvHeads = graph_.Local().kvHeads;  // a shard caches only its own KV heads
     kv_.Create(ctx_, kvCfg, opts.pageSize, pagesPerSeq * opts.maxBatch, opts.maxBatch, pagesPerSeq, opts.pageSeed,
-               ring);
+               ring, opts.kvFp4);
+    runs_ = longestRun_ = 0;
     maxVec_ = std::max(opts.maxBatch, opts.prefillChunk);
     AllocBuffers();
     // The fused GEMV + peer exchange (one kernel, tagged 8-byte words) took 8.5-9.4 us per
@@ -127,7 +132,7 @@ bool VoxelEngine::UsesFused(uint32_t n) const {
     const graph::ModelConfig &c = graph_.Config();
     const graph::VramPlan &p = graph_.Plan();
     const uint32_t hd = c.HeadDim(), G = c.KvGroupSize();
-    const bool shape = !comm_ && p.hasFused && !p.lmQuantized && G >= 1 && G <= 4 &&
+    const bool shape = !comm_ && !kv_.Fp4() && p.hasFused && !p.lmQuantized && G >= 1 && G <= 4 &&
                        (n == 1 || n == 2 || n == 4 || n == 8) && 3ull * c.hiddenSize * 2 <= 160 * 1024;
     if (p.wDtype == OPURE_W_Q8)  // GEMV_Quant weights: the persistent kernel only
         return shape && opts_.path != 1 && opts_.path != 3 && hd == 64 && c.numLayers <= 48 &&
@@ -199,6 +204,11 @@ void VoxelEngine::AllocBuffers() {
         buf_.packAct = packed(c.intermediateSize);
         buf_.sumsq = Alloc<float>(ctx_, size_t((c.hiddenSize + 127) / 128) * nv);
     }
+    if (kv_.Fp4()) {
+        buf_.runSeq = Alloc<int32_t>(ctx_, B);
+        buf_.runLen = Alloc<int32_t>(ctx_, B);
+        buf_.runBegin = Alloc<int32_t>(ctx_, size_t(B) + 1);
+    }
     if (comm_ && !buf_.partial) buf_.partial = Alloc<float>(ctx_, size_t(B) * c.hiddenSize);
     buf_.sync = Alloc<uint32_t>(ctx_, 3 * size_t(c.numLayers) + 1);
     if (opts_.phaseTrace) {
@@ -220,15 +230,18 @@ void VoxelEngine::AllocBuffers() {
 }
 
 void *VoxelEngine::AttnScratch(uint32_t n, size_t *bytes) {
-    auto it = attnScratch_.find(n);
+    const auto key = std::make_tuple(n, runs_, longestRun_);
+    auto it = attnScratch_.find(key);
     if (it == attnScratch_.end()) {
         const graph::ModelConfig &c = graph_.Config();
-        const size_t b = opure_attention_scratch_bytes(n, 1, c.numHeads, c.numKvHeads, c.HeadDim(), maxLen_, 0);
+        const size_t b = kv_.Fp4() ? opure_kv4_attention_scratch_bytes(runs_ ? runs_ : n, n, runs_ ? longestRun_ : 1, c.numHeads,
+                                                                       c.numKvHeads, c.HeadDim(), maxLen_, 0)
+                                   : opure_attention_scratch_bytes(n, 1, c.numHeads, c.numKvHeads, c.HeadDim(), maxLen_, 0);
         OPURE_CHECK(b > 0, "attention scratch size query failed");
         void *p = nullptr;
         OPURE_CUDA_CHECK(opure_alloc(ctx_, b, &p));
         OPURE_CUDA_CHECK(opure_fill(ctx_, p, 0, b));  // split counters start at zero
-        it = attnScratch_.emplace(n, std::make_pair(p, b)).first;
+        it = attnScratch_.emplace(key, std::make_pair(p, b)).first;
     }
     *bytes = it->second.second;
     return it->second.first;
@@ -257,6 +270,7 @@ opure_step_io VoxelEngine::StepIO(uint32_t n) const {
 // RoPE, the KV append and attention of the step's q;k;v rows; `packed` (or null) also receives
 // the attention output as a chained operand.
 void VoxelEngine::RecordAttention(uint32_t L, uint32_t n, uint32_t qkvRows, uint16_t *packed) {
+    if (kv_.Fp4()) return RecordAttention4(L, n, qkvRows, packed);
     const graph::ModelConfig &c = graph_.Config();
     const graph::LocalGeometry &lg = graph_.Local();
     const opure_kv_layout kv = kv_.Layout(L);
@@ -277,6 +291,45 @@ void VoxelEngine::RecordAttention(uint32_t L, uint32_t n, uint32_t qkvRows, uint
     a.kv = kv;
     a.out_packed = packed;
     OPURE_CUDA_CHECK(opure_attention(ctx_, &a));
+}
+
+// The same over the 4-bit cache. Vectors of neighbouring positions of a sequence (a chunk of a prompt, the
+// drafts of a verify step) are one entry of the attention call, whose keys are read once for all of them.
+void VoxelEngine::RecordAttention4(uint32_t L, uint32_t n, uint32_t qkvRows, uint16_t *packed) {
+    const graph::ModelConfig &c = graph_.Config();
+    const uint32_t qCols = c.numHeads * c.HeadDim();
+    const opure_kv4_layout kv = kv_.Layout4(L);
+    opure_kv4_append_args ap{};
+    ap.qkv = buf_.qkv;
+    ap.type = OPURE_F32;
+    ap.stride = qkvRows;
+    ap.q_out = buf_.q;
+    ap.q_stride = qCols;
+    ap.seq = buf_.seq;
+    ap.pos = buf_.pos;
+    ap.n = n;
+    ap.n_heads = c.numHeads;
+    ap.theta = c.ropeTheta;
+    ap.kv = kv;
+    OPURE_CUDA_CHECK(opure_kv4_append(ctx_, &ap));
+    opure_kv4_attn_args a{};
+    a.q = buf_.q;
+    a.out = buf_.attn;
+    a.type = OPURE_F32;
+    a.q_stride = a.out_stride = qCols;
+    a.seq = runs_ ? buf_.runSeq : buf_.seq;
+    a.seq_len = runs_ ? buf_.runLen : buf_.seqLen;
+    a.q_begin = runs_ ? buf_.runBegin : nullptr;
+    a.n = runs_ ? runs_ : n;
+    a.n_rows = n;
+    a.n_q = runs_ ? longestRun_ : 1;
+    a.n_heads = c.numHeads;
+    a.scale = opts_.attnScale;
+    a.max_ctx = maxLen_;
+    a.scratch = AttnScratch(n, &a.scratch_bytes);
+    a.kv = kv;
+    a.out_packed = packed;
+    OPURE_CUDA_CHECK(opure_kv4_attention(ctx_, &a));
 }
 
 // A layer over 4-bit microscaled weights: every linear layer takes 8-bit microscaled inputs, which
@@ -581,7 +634,7 @@ void VoxelEngine::RunSteps(uint32_t n, uint32_t steps, bool logits) {
         for (uint32_t s = 0; s < steps; ++s) RecordStep(n, logits);
         return;
     }
-    const auto key = std::make_pair(n, logits);
+    const auto key = std::make_tuple(n, logits, runs_, longestRun_);
     auto it = graphs_.find(key);
     if (it == graphs_.end()) {
         size_t dummy = 0;
@@ -658,6 +711,7 @@ void VoxelEngine::ResetSequences(const std::vector<std::vector<uint32_t>> &promp
     OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.flags, flags.data(), flags.size() * 4));
     hostDriven_ = !automatic;
     seqIdentity_ = true;
+    runs_ = longestRun_ = 0;
     OPURE_CUDA_CHECK(opure_fill(ctx_, buf_.keys, 0, n * 8));
     OPURE_CUDA_CHECK(opure_sync(ctx_, 60000));
 }
@@ -845,6 +899,31 @@ void VoxelEngine::SetVectors(const int32_t *seq, const int32_t *pos, const int32
     OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.pos, pos, n * 4));
     if (tok) OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.inTokens, tok, n * 4));
     seqIdentity_ = false;
+    runs_ = longestRun_ = 0;
+    if (kv_.Fp4()) {
+        std::vector<int32_t> slot, len, begin;
+        for (uint32_t v = 0; v < n; ++v)
+            if (v == 0 || seq[v] != seq[v - 1] || pos[v] != pos[v - 1] + 1) {
+                slot.push_back(seq[v]);
+                len.push_back(pos[v] + 1);
+                begin.push_back(int32_t(v));
+            }
+        begin.push_back(int32_t(n));
+        if (slot.size() < n) {
+            // Their number and longest length are part of the step graph's key: rounded up to powers of two
+            // (entries without queries behind the last), so that steps of mixed sequences share a few graphs.
+            uint32_t longest = 0;
+            for (size_t r = 0; r < slot.size(); ++r) longest = std::max(longest, uint32_t(begin[r + 1] - begin[r]));
+            runs_ = std::min(n, std::bit_ceil(uint32_t(slot.size())));
+            longestRun_ = std::min(n, std::bit_ceil(longest));
+            slot.resize(runs_, -1);
+            len.resize(runs_, 0);
+            begin.resize(runs_ + 1, int32_t(n));
+            OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.runSeq, slot.data(), slot.size() * 4));
+            OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.runLen, len.data(), len.size() * 4));
+            OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.runBegin, begin.data(), begin.size() * 4));
+        }
+    }
     // Every vector of the step takes its token from the host: clear the self-driving flag of
     // all n (earlier calls may have set flags for fewer vectors, e.g. one per prompt).
     const std::vector<uint32_t> zero(n, 0u);
@@ -869,6 +948,7 @@ void VoxelEngine::SetAutoVectors(const int32_t *pos, const int32_t *known, uint3
     OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.flags, flags.data(), n * 4));
     seqIdentity_ = true;
     hostDriven_ = false;
+    runs_ = longestRun_ = 0;
 }
 
 void VoxelEngine::WriteHistory(uint32_t slot, uint32_t pos, const int32_t *tokens, uint32_t count) {
@@ -928,6 +1008,76 @@ void VoxelEngine::ForwardLogits(const std::vector<uint32_t> &tokens, std::vector
     seqLen_ = uint32_t(tokens.size());
 }
 
+std::vector<SequenceScores> VoxelEngine::Score(const std::vector<std::vector<uint32_t>> &sequences, uint32_t top) {
+    OPURE_CHECK(ready_, "engine used before Initialize");
+    OPURE_CHECK(!comm_, "Score is not available on a tensor-parallel shard (logits are split)");
+    OPURE_CHECK(top <= OPURE_SCORE_MAX_TOP && top <= graph_.Config().vocabSize, "too many alternatives asked for");
+    const uint32_t n = uint32_t(sequences.size()), C = opts_.prefillChunk ? opts_.prefillChunk : opts_.maxBatch;
+    const uint32_t V = graph_.Config().vocabSize;
+    size_t longest = 0;
+    for (const auto &s : sequences) {
+        longest = std::max(longest, s.size());
+        OPURE_CHECK(!kv_.Ring() || s.size() <= kv_.Ring() * kv_.PageSize(), "Score needs the sequence to fit the KV window");
+    }
+    ResetSequences(sequences, uint32_t(longest), false);
+    std::vector<SequenceScores> out(n);
+    std::vector<int32_t> seq, pos, tok, given;
+    for (uint32_t s = 0; s < n; ++s) {
+        const size_t len = sequences[s].size();
+        out[s].logprobs.assign(len, 0.f);
+        out[s].entropies.assign(len, 0.f);
+        out[s].ranks.assign(len, 0);
+        out[s].topTokens.assign(len * top, -1);
+        out[s].topLogprobs.assign(len * top, -INFINITY);
+        for (size_t t = 0; t + 1 < len; ++t) {
+            seq.push_back(int32_t(s));
+            pos.push_back(int32_t(t));
+            tok.push_back(int32_t(sequences[s][t]));
+            given.push_back(int32_t(sequences[s][t + 1]));
+        }
+    }
+    // A step's results lie one behind another: log probabilities, entropies, ranks, top tokens and theirs.
+    const size_t per = 3 + 2 * size_t(OPURE_SCORE_MAX_TOP);
+    if (!buf_.scoreTokens) buf_.scoreTokens = Alloc<int32_t>(ctx_, maxVec_);
+    if (!buf_.scoreOut) buf_.scoreOut = Alloc<float>(ctx_, maxVec_ * per);
+    std::vector<float> host(C * per);
+    for (size_t i0 = 0; i0 < seq.size(); i0 += C) {
+        const uint32_t m = uint32_t(std::min<size_t>(C, seq.size() - i0));
+        SetVectors(seq.data() + i0, pos.data() + i0, tok.data() + i0, m);
+        RunSteps(m, 1, true);
+        OPURE_CUDA_CHECK(opure_h2d(ctx_, buf_.scoreTokens, given.data() + i0, m * 4));
+        opure_score_args a{};
+        a.logits = buf_.logits;
+        a.type = OPURE_F32;
+        a.vocab = V;
+        a.rows = m;
+        a.stride = V;
+        a.tokens = buf_.scoreTokens;
+        a.logprob = buf_.scoreOut;
+        a.entropy = a.logprob + m;
+        a.rank = reinterpret_cast<int32_t *>(a.entropy + m);
+        a.top = top;
+        a.top_tokens = a.rank + m;
+        a.top_logprobs = reinterpret_cast<float *>(a.top_tokens + size_t(m) * top);
+        OPURE_CUDA_CHECK(opure_token_scores(ctx_, &a));
+        OPURE_CUDA_CHECK(opure_d2h(ctx_, host.data(), buf_.scoreOut, m * (3 + 2 * size_t(top)) * 4));
+        Sync();
+        const float *lp = host.data(), *ent = lp + m, *best = ent + 2 * size_t(m) + size_t(m) * top;
+        const int32_t *rank = reinterpret_cast<const int32_t *>(ent + m), *ids = rank + m;
+        for (uint32_t j = 0; j < m; ++j) {
+            SequenceScores &o = out[uint32_t(seq[i0 + j])];
+            const size_t t = size_t(pos[i0 + j]) + 1;
+            o.logprobs[t] = lp[j];
+            o.entropies[t] = ent[j];
+            o.ranks[t] = rank[j];
+            std::copy_n(ids + size_t(j) * top, top, o.topTokens.begin() + t * top);
+            std::copy_n(best + size_t(j) * top, top, o.topLogprobs.begin() + t * top);
+        }
+    }
+    seqLen_ = uint32_t(longest);
+    return out;
+}
+
 void VoxelEngine::DecodeStepBatch(const int32_t *tokens, const int32_t *positions, uint32_t n, int32_t *next) {
     OPURE_CHECK(n >= 1 && n <= opts_.maxBatch, "batch exceeds maxBatch");
     auto *io = static_cast<int32_t *>(hostIo_);
@@ -941,6 +1091,7 @@ void VoxelEngine::DecodeStepBatch(const int32_t *tokens, const int32_t *position
         io[maxVec_ + v] = positions[v];
     }
     kv_.SyncTable();
+    runs_ = longestRun_ = 0;
     if (!seqIdentity_) {
         // SetVectors may have pointed vectors at other slots; vector v is slot v here.
         std::vector<int32_t> ident(opts_.maxBatch);
@@ -1040,6 +1191,38 @@ void VoxelEngine::LoadKv(uint32_t seq, const uint16_t *kvData, uint32_t len) {
     OPURE_CHECK(kv_.Reserve(seq, std::max(len, 1u)), "KV cache has no room for the sequence");
     kv_.SyncTable();
     const uint32_t P = kv_.PageSize(), hd = c.HeadDim(), nkv = c.numKvHeads;
+    if (kv_.Fp4()) {
+        // Rows [k | v] of every position, quantised by the append call (not rotated).
+        const size_t row = size_t(2) * nkv * hd;
+        std::vector<int32_t> seqs(len, int32_t(seq)), pos(len);
+        for (uint32_t t = 0; t < len; ++t) pos[t] = int32_t(t);
+        std::vector<uint16_t> rows(len * row);
+        struct Temp {
+            opure_ctx *ctx;
+            void *p;
+            ~Temp() { opure_free(ctx, p); }
+        } dRows{ctx_, Alloc<uint16_t>(ctx_, rows.size())}, dSeq{ctx_, Alloc<int32_t>(ctx_, len)}, dPos{ctx_, Alloc<int32_t>(ctx_, len)};
+        OPURE_CUDA_CHECK(opure_h2d(ctx_, dSeq.p, seqs.data(), seqs.size() * 4));
+        OPURE_CUDA_CHECK(opure_h2d(ctx_, dPos.p, pos.data(), pos.size() * 4));
+        for (uint32_t L = 0; L < c.numLayers; ++L) {
+            for (uint32_t sel = 0; sel < 2; ++sel)
+                for (uint32_t g = 0; g < nkv; ++g)
+                    for (uint32_t t = 0; t < len; ++t)
+                        std::copy_n(kvData + ((((size_t(L) * 2 + sel) * nkv + g) * len) + t) * hd, hd, rows.data() + t * row + (size_t(sel) * nkv + g) * hd);
+            OPURE_CUDA_CHECK(opure_h2d(ctx_, dRows.p, rows.data(), rows.size() * 2));
+            opure_kv4_append_args a{};
+            a.qkv = dRows.p;
+            a.type = OPURE_F16;
+            a.stride = row;
+            a.seq = static_cast<const int32_t *>(dSeq.p);
+            a.pos = static_cast<const int32_t *>(dPos.p);
+            a.n = len;
+            a.kv = kv_.Layout4(L);
+            OPURE_CUDA_CHECK(opure_kv4_append(ctx_, &a));
+            OPURE_CUDA_CHECK(opure_sync(ctx_, 600000));
+        }
+        return;
+    }
     const std::vector<int32_t> &table = kv_.HostTable();
     for (uint32_t L = 0; L < c.numLayers; ++L) {
         uint8_t *pool = reinterpret_cast<uint8_t *>(kv_.Pool(L));
@@ -1061,6 +1244,7 @@ void VoxelEngine::PrepareSynthetic(uint32_t n, uint32_t len, uint32_t reserve, u
     OPURE_CHECK(ready_, "engine used before Initialize");
     OPURE_CHECK(n >= 1 && n <= opts_.maxBatch, "batch exceeds maxBatch");
     OPURE_CHECK(len >= 1 && len < reserve && reserve <= maxLen_, "need 1 <= len < reserve <= maxLen");
+    OPURE_CHECK(!kv_.Fp4(), "synthetic contexts are made for the fp16 KV cache only");
     const graph::ModelConfig &c = graph_.Config();
     std::vector<int32_t> seq(n), pos(n, int32_t(len)), known(n, int32_t(len) + 1);
     std::vector<uint32_t> flags(n, uint32_t(OPURE_VEC_AUTO));

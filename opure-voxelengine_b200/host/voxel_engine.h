@@ -23,6 +23,7 @@
 #include <cstdint>
 #include <map>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -54,6 +55,7 @@ struct EngineOptions {
                                     // whole pages and its own
     uint32_t tpAllreduce = 0;       // tensor parallel: 0 auto (peer kernels when mappable), 1 NCCL, 2 peer
     bool mxWeights = false;         // layer matrices quantised to 4-bit microscaled form on upload
+    bool kvFp4 = false;             // keys and values cached in 4 bits (opure_kv4_layout)
 };
 
 struct GenerateResult {
@@ -69,6 +71,15 @@ struct StepTiming {
     double prefillMs = 0.0;   // device time of the prefill steps
     double decodeMs = 0.0;    // device time of the decode steps
     uint32_t prefillSteps = 0, decodeSteps = 0;
+};
+
+// Scores of a sequence's tokens after those before them (opure_engine_score); the first token's are
+// 0, 0, 0, -1 and -inf.
+struct SequenceScores {
+    std::vector<float> logprobs, entropies;
+    std::vector<int32_t> ranks;
+    std::vector<int32_t> topTokens;    // [tokens][top]
+    std::vector<float> topLogprobs;
 };
 
 // Reads the ctx's device status word; throws opure::Error naming the failing kernel site
@@ -110,6 +121,9 @@ public:
 
     uint32_t ForwardArgMax(const std::vector<uint32_t> &tokens);
     void ForwardLogits(const std::vector<uint32_t> &tokens, std::vector<float> &logitsOut);
+
+    // Scores the tokens of independent sequences (slots 0..n-1), with the `top` most likely ones each.
+    std::vector<SequenceScores> Score(const std::vector<std::vector<uint32_t>> &sequences, uint32_t top);
 
     // Host-driven steps, the reference's Prefill + DecodeStep contract: each DecodeStep
     // copies the token in, runs one step and reads the 8-byte argmax result back.
@@ -198,6 +212,12 @@ public:
         // squares for the consumer's RMSNorm.
         uint16_t *packAttn = nullptr, *packRes = nullptr, *packAct = nullptr;
         float *sumsq = nullptr;
+        // 4-bit KV cache: the runs of neighbouring positions among a step's vectors (slot, keys
+        // that the first one sees, first vector), each one entry of the attention call.
+        int32_t *runSeq = nullptr, *runLen = nullptr, *runBegin = nullptr;
+        // Score: a step's given tokens and results (logprob, entropy | rank | top tokens | top logprobs).
+        int32_t *scoreTokens = nullptr;
+        float *scoreOut = nullptr;
         // Microscaled weights: the inputs of q;k;v and gate;up (normed residual), of the o_proj
         // (attention output) and of the down_proj (SwiGLU activation), in 8 bits.
         opure_mx_matrix mxNorm{}, mxAttn{}, mxAct{};
@@ -216,7 +236,8 @@ private:
     void RecordAttention(uint32_t layer, uint32_t n, uint32_t qkvRows, uint16_t *packed);
     void TpGemvAllreduce(const void *w, float scale, uint32_t rows, uint32_t cols, const float *in,
                          uint32_t in_stride, uint32_t n);
-    // Split-K attention scratch for batch n (one zeroed buffer per batch size, so its
+    void RecordAttention4(uint32_t layer, uint32_t n, uint32_t qkvRows, uint16_t *packed);
+    // Attention scratch for a step of n vectors (one zeroed buffer per shape of the call, so its
     // split counters always start at zero).
     void *AttnScratch(uint32_t n, size_t *bytes);
     void ResetSequences(const std::vector<std::vector<uint32_t>> &prompts, uint32_t reserve, bool automatic);
@@ -236,8 +257,10 @@ private:
     uint32_t seqLen_ = 0;
     double lastTokenMs_ = 0.0;
     float specAcceptance_ = -1.0f;
-    std::map<std::pair<uint32_t, bool>, opure_graph *> graphs_;
-    std::map<uint32_t, std::pair<void *, size_t>> attnScratch_;
+    // By vectors, logits, and the step's runs and longest run (0: an entry per vector).
+    std::map<std::tuple<uint32_t, bool, uint32_t, uint32_t>, opure_graph *> graphs_;
+    std::map<std::tuple<uint32_t, uint32_t, uint32_t>, std::pair<void *, size_t>> attnScratch_;
+    uint32_t runs_ = 0, longestRun_ = 0;  // 4-bit KV cache: of the vectors that SetVectors described
     void *hostIo_ = nullptr;  // pinned staging of the host-driven step
     bool hostDriven_ = false; // step flags currently cleared for host-supplied tokens
     bool seqIdentity_ = true; // vector v currently maps to sequence slot v

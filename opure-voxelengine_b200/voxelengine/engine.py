@@ -17,11 +17,12 @@ class EngineOptions(C.Structure):
     _fields_ = [("max_new_tokens", u32), ("max_batch", u32), ("max_len", u32), ("page_size", u32),
                 ("page_seed", u64), ("use_graphs", u32), ("attn_scale", f32), ("path", u32),
                 ("phase_trace", u32), ("prefill_chunk", u32), ("kv_window", u32),
-                ("tp_allreduce", u32), ("weights", u32)]
+                ("tp_allreduce", u32), ("weights", u32), ("kv", u32)]
 
 
 PATH_AUTO, PATH_UNFUSED, PATH_FUSED, PATH_FUSED_LAYERS = 0, 1, 2, 3
 WEIGHTS_STORED, WEIGHTS_MXFP4 = 0, 1
+KV_FP16, KV_FP4 = 0, 1
 TP_AUTO, TP_NCCL, TP_PEER = 0, 1, 2
 
 
@@ -30,7 +31,7 @@ class EngineInfo(C.Structure):
                 ("kv_heads", u32), ("head_dim", u32), ("max_pos", u32), ("max_len", u32),
                 ("max_batch", u32), ("page_size", u32), ("w_dtype", u32), ("weight_bytes", u64),
                 ("stream_bytes", u64), ("kv_bytes_per_token", u64), ("tp_ranks", u32),
-                ("tp_peer", u32), ("weights", u32)]
+                ("tp_peer", u32), ("weights", u32), ("kv", u32)]
 
 
 class Timing(C.Structure):
@@ -89,6 +90,7 @@ def lib() -> C.CDLL:
             "opure_engine_create_tp": [C.c_char_p, P, P, P, P],
             "opure_engine_spec_generate": [P, P, P, u32, u32, u32, P, P, P, u32, P],
             "opure_engine_sample_generate": [P, P, u32, u32, u32, P, P, P, P],
+            "opure_engine_score": [P, P, P, u32, u32, P, P, P, P, P],
             "opure_engine_destroy": [P],
             "opure_engine_get_info": [P, P],
             "opure_engine_generate": [P, P, P, u32, u32, P, P],
@@ -214,17 +216,17 @@ class Engine:
                  attn_scale: float = 1.0, max_new_tokens: int = 256, path: int = PATH_AUTO,
                  share: "Engine | None" = None, comm: "cuda.Comm | None" = None,
                  phase_trace: bool = False, prefill_chunk: int = 0, kv_window: int = 0,
-                 tp_allreduce: int = TP_AUTO, weights: int = WEIGHTS_STORED):
+                 tp_allreduce: int = TP_AUTO, weights: int = WEIGHTS_STORED, kv: int = KV_FP16):
         """With `share`, the engine runs on that engine's ctx (stream), as the draft of a
         speculative pair must; it keeps a reference so the owner outlives it. With `comm`
         it is that communicator's tensor-parallel shard, on the communicator's ctx, whose
         all-reduces run as NCCL calls (`tp_allreduce` TP_NCCL, and TP_AUTO at 2 ranks) or
         as NVLink peer kernels (TP_PEER, and TP_AUTO at any rank count, when every pair of GPUs
         can map each other's memory). `weights` WEIGHTS_MXFP4 quantises the layer matrices to
-        4-bit microscaled form on upload."""
+        4-bit microscaled form on upload; `kv` KV_FP4 caches keys and values in 4 bits."""
         o = EngineOptions(max_new_tokens, max_batch, max_len, page_size, page_seed,
                           int(use_graphs), attn_scale, path, int(phase_trace), prefill_chunk, kv_window,
-                          tp_allreduce, weights)
+                          tp_allreduce, weights, kv)
         h = C.c_void_p()
         if comm is not None:
             st = lib().opure_engine_create_tp(model_dir.encode(), comm.ctx.h, comm.h, C.byref(o), C.byref(h))
@@ -328,6 +330,26 @@ class Engine:
             return out
         return (out,) + ((st,) if stats else ()) + ((lg,) if logits else ())
 
+    def score(self, sequences, top: int = 0) -> list[dict]:
+        """Scores the tokens of up to max_batch sequences, each after those before it. Per sequence a
+        dict of arrays of its length: logprobs, ranks, entropies, and with `top` the most likely tokens
+        top_tokens, top_logprobs [length][top]. A first token has 0, 0, 0, -1 and -inf."""
+        seqs = [np.ascontiguousarray(s, np.int32).ravel() for s in sequences]
+        lens = np.array([s.size for s in seqs], np.uint32)
+        toks = np.concatenate(seqs) if seqs else np.zeros(0, np.int32)
+        n = toks.size
+        lp, en, rk = np.zeros(n, np.float32), np.zeros(n, np.float32), np.zeros(n, np.int32)
+        tt, tl = np.zeros((n, top), np.int32), np.zeros((n, top), np.float32)
+        _check(lib().opure_engine_score(self.h, _p(toks), _p(lens), len(seqs), top, _p(lp), _p(rk), _p(en),
+                                        _p(tt) if top else None, _p(tl) if top else None), "score", self.h)
+        cut = np.cumsum(lens)[:-1]
+        out = [dict(logprobs=a, ranks=b, entropies=c)
+               for a, b, c in zip(np.split(lp, cut), np.split(rk, cut), np.split(en, cut))]
+        if top:
+            for o, a, b in zip(out, np.split(tt, cut), np.split(tl, cut)):
+                o["top_tokens"], o["top_logprobs"] = a, b
+        return out
+
     def prefill(self, tokens) -> int:
         """Prefill slot 0; returns the first generated token."""
         t = np.ascontiguousarray(tokens, np.int32)
@@ -399,15 +421,15 @@ class Engine:
 
 # ---- serving front end -------------------------------------------------------------
 class Server:
-    """The HTTP front end (GET /health, POST /generate, GET /metrics) on 127.0.0.1 with one
-    engine per device in `devices` (none: the routes answer, /generate with 503)."""
+    """The HTTP front end (GET /health, POST /generate, POST /score, GET /metrics) on 127.0.0.1
+    with one engine per device in `devices` (none: the routes answer, /generate and /score with 503)."""
 
     def __init__(self, model_dir: str | None = None, devices=(), port: int = 0, **engine_opts):
         devs = np.ascontiguousarray(list(devices), np.int32)
         o = EngineOptions(engine_opts.get("max_new_tokens", 256), engine_opts.get("max_batch", 1),
                           engine_opts.get("max_len", 0), engine_opts.get("page_size", 64),
-                          engine_opts.get("page_seed", 3), 1, 1.0, engine_opts.get("path", PATH_AUTO), 0, 0, 0, 0,
-                          engine_opts.get("weights", WEIGHTS_STORED))
+                          engine_opts.get("page_seed", 3), 1, 1.0, engine_opts.get("path", PATH_AUTO), 0, engine_opts.get("prefill_chunk", 0), 0, 0,
+                          engine_opts.get("weights", WEIGHTS_STORED), engine_opts.get("kv", KV_FP16))
         h = C.c_void_p()
         _check(lib().opure_server_start(model_dir.encode() if model_dir else None, _p(devs) if devs.size else None,
                                         int(devs.size), port, C.byref(o), C.byref(h)), "opure_server_start")
