@@ -442,11 +442,12 @@ opure_status opure_kv4_read(opure_ctx *ctx, const opure_kv4_read_args *a);
  * without keys (seq[i] < 0, or seq_len[i] + j <= 0) gets zeros. Query head h reads kv head
  * h / (n_heads / n_kv). Sums and the softmax are fp32; queries and probabilities are split into
  * fp16 pairs, so that products keep 22 bits, except that with 16-bit types the probabilities of
- * entries with more than 8 (query, head) rows per kv head may be rounded to fp16 once.
+ * entries with more than 16 (query, head) rows per kv head are rounded to fp16 once.
  *
  * scratch: opure_kv4_attention_scratch_bytes(...) bytes, 16-byte aligned, caller-owned. Zero before
- * the first call (opure_fill); every call leaves its counters zero. Calls that may run at the same
- * time need scratch of their own. */
+ * the first call (opure_fill); every call leaves its counters zero, at a place that depends on n, n_rows,
+ * n_q, the heads, max_ctx and split_tokens: zero it again before a call with other ones. Calls that may
+ * run at the same time need scratch of their own. */
 typedef struct opure_kv4_attn_args {
     const void *q;             /* [n_rows][q_stride] of type, rows [n_heads][head_dim] */
     void *out;                 /* [n_rows][out_stride] of type, apart from q           */
@@ -460,7 +461,8 @@ typedef struct opure_kv4_attn_args {
     uint32_t n_heads;
     float scale;
     uint32_t max_ctx;          /* upper bound of seq_len[i] + queries of i - 1          */
-    uint32_t split_tokens;     /* keys per split; 0 = choose                         */
+    uint32_t split_tokens;     /* keys per split (raised where there would be more than 64
+                                  splits); 0 = choose                              */
     void *scratch;
     size_t scratch_bytes;
     opure_kv4_layout kv;

@@ -6,17 +6,23 @@
 // comes. The row's log-sum-exp is then m + log z, its entropy log z - e / z, with m the row's largest:
 // with any other reference the two terms of the entropy would cancel.
 //
-// The most likely tokens: logits that reach a bound go to a buffer in shared memory as keys (orderable
-// value, ~index). The bound is a value that `top` logits of a row's first piece reach (the top-th largest of
-// 32 lanes' maxima, as many of each warp), then the top-th best key of that piece. Keys are put in order by
-// counting, for each, the larger ones.
+// The most likely tokens: a thread notes in which pieces of the row it saw a logit that reaches a bound,
+// a value that `top` logits of the first piece reach (the top-th largest of 32 lanes' maxima, as many of each
+// warp). When the row is through, the top-th largest of the threads' maxima over all of it is a bound that
+// little more than `top` logits reach. Another warp reads the pieces that the threads above it have noted once
+// more (from L2), 32 logits of one thread at a time, collects those that reach the bound as keys (orderable
+// value, ~index), and puts them in order by counting, for each, the larger ones.
 //
-// CTAs go from row to row while a warp of theirs copies the coming pieces into a ring of stages, so
-// that what a row needs after its last piece (joining the sums, ordering the keys) costs no memory time;
-// nothing in a piece but a row's first waits for other warps. A row with more keys than the buffer takes
-// (equal values at the bound, rising ones) is gone over once more for its keys alone, a few values a
-// thread at a time. Where there are few rows each is shared out over a cluster of up to 8 CTAs, whose
-// parts meet in distributed shared memory.
+// CTAs go from row to row with three kinds of warps: four that work on values, one that copies the coming
+// pieces into a ring of stages, and one that finishes a row (joins its sums, finds its best tokens, writes the
+// results) while the others are at the next. Nothing in a piece but a row's first waits for another of the
+// four. A row with more keys than the buffer takes (equal values at the bound, large ones all in one thread's
+// words) is gone over once more for its keys alone. Where there are few rows each is shared out over a
+// cluster of up to 8 CTAs, whose parts meet in distributed shared memory.
+// Bound by memory while there are many rows: 4096 rows of 49152 fp32 logits take 139-144 us without best
+// tokens and 165-170 us with 5 (5.6 and 4.8 TB/s of 6.5 measured), 203 us with 20. With the finishing done by
+// the four warps themselves it was 215 us with 5. A single row, a cluster of 8, is latency: 5.5 us, 13.6 us
+// with 20 best tokens (11.1 us when four warps finished it; kept, since one way serves all sizes).
 #include <algorithm>
 
 #include "attn_core.cuh"
@@ -29,7 +35,9 @@ namespace {
 constexpr uint32_t kThreads = 128, kWarps = kThreads / 32;
 constexpr uint32_t kCtasPerSm = 3;
 constexpr uint32_t kMaxCluster = 8;
-constexpr uint32_t kBuffer = 512;   // keys; more than a step of one key a thread and the best so far
+constexpr uint32_t kBuffer = 512;   // keys
+constexpr uint32_t kItems = 512;    // pieces of threads that are read again
+constexpr uint32_t kOnce = 32;      // so many of them at once
 constexpr uint32_t kValues = 32;    // of a thread in a piece
 template <typename T>
 constexpr uint32_t kWords = kValues * sizeof(T) / 16;  // 16-byte words of them
@@ -38,7 +46,7 @@ constexpr uint32_t kPiece = kThreads * kWords<T>;      // words of a piece
 template <typename T>
 constexpr uint32_t kStages = sizeof(T) == 4 ? 3 : 6;   // 48 KB a CTA
 constexpr uint32_t kMaxStages = 6;
-constexpr uint32_t kSort = 128;     // up to this many keys are put in order as they are
+constexpr uint32_t kSort = 96;      // up to this many keys are put in order as they are
 constexpr float kLowest = -3.4028234663852886e38f;  // of fp32: a row may hold nothing larger
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -200.f;                       // exp of it is 0, and 0 times it stays 0 (unlike -inf)
@@ -98,36 +106,40 @@ struct Sums {
 
 using Key = unsigned long long;
 
-// Barriers of the threads that work on values (all but the copying warp's).
+// A barrier of the threads that work on values.
 __device__ __forceinline__ void sync_values() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-__device__ __forceinline__ bool sync_values_or(bool v) {
-    uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
-                 : "=r"(r)
-                 : "r"(uint32_t(v)), "n"(kThreads)
-                 : "memory");
-    return r != 0;
-}
-
-struct RowShared {
-    __align__(16) Key buffer[2][kBuffer];  // what lies behind them may be read by sort_keys
-    Key best[kMaxCluster][OPURE_SCORE_MAX_TOP];  // each CTA's best in order, 0 for none (the first CTA's copy is used)
-    uint32_t count[2], valid[2];                 // of each buffer: keys asked for, and up to where they were all stored
+// What a row's finishing needs of the threads that worked on it.
+struct Handed {
+    float most[kThreads];        // each one's largest value
+    uint32_t noted[kThreads];    // bit i: pieces i, i + 32, .. have one that reaches the first piece's bound
     float m[kWarps], z[kWarps], e[kWarps];
     uint32_t ahead[kWarps];
-    __align__(16) uint32_t reach[32];            // the largest lanes' maxima, as many of each warp, as order bits
+};
+struct RowShared {
+    __align__(16) Key buffer[2][kBuffer];        // what lies behind them may be read by sort_keys
+    Key best[kMaxCluster][OPURE_SCORE_MAX_TOP];  // each CTA's best in order, 0 for none (the first CTA's copy is used)
+    uint32_t items[kItems];
+    __align__(16) uint4 again[kOnce * 32 / 4];   // a thread's words of so many pieces
+    __align__(16) uint32_t most[64];
+    Handed handed[2];
+    __align__(16) uint32_t reach[2][32];         // the largest lanes' maxima, as many of each warp, as order bits
     float cm[kMaxCluster], cz[kMaxCluster], ce[kMaxCluster];
     uint32_t cahead[kMaxCluster];
-    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t full[kMaxStages], empty[kMaxStages], given[2], taken[2];
 };
 
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
 // The largest value that `top` threads' values (order bits) are known to reach, 0 for none, and the
-// largest of all. All threads that work on values; one barrier.
+// largest of all. All threads that work on values; one barrier. A call may use the same `reach` as an
+// earlier one if there was another barrier between them.
 struct Reach {
     uint32_t bound, highest;
 };
 static_assert(OPURE_SCORE_MAX_TOP <= 32, "as many maxima are compared");
-__device__ __forceinline__ Reach reach_of(RowShared &sm, uint32_t o, uint32_t top) {
+__device__ __forceinline__ Reach reach_of(uint32_t *reach, uint32_t o, uint32_t top) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     // Of each warp one more than its share of `top`, for a bound with fewer values above it.
     const uint32_t each = min(top / kWarps + 1, 32 / kWarps);
@@ -137,24 +149,64 @@ __device__ __forceinline__ Reach reach_of(RowShared &sm, uint32_t o, uint32_t to
         if (lane == k) own = m;
         if (o == m) o = 0;  // equal ones in other lanes go too: the bound is no higher for it
     }
-    if (lane < 32 / kWarps) sm.reach[warp * (32 / kWarps) + lane] = own;
+    if (lane < 32 / kWarps) reach[warp * (32 / kWarps) + lane] = own;
     sync_values();
-    const uint32_t mine = sm.reach[lane];
+    const uint32_t mine = reach[lane];
     uint32_t as_large = 0;
 #pragma unroll
     for (uint32_t j = 0; j < 32; j += 4) {
-        const uint4 y = *reinterpret_cast<const uint4 *>(&sm.reach[j]);
+        const uint4 y = *reinterpret_cast<const uint4 *>(&reach[j]);
         as_large += (y.x >= mine) + (y.y >= mine) + (y.z >= mine) + (y.w >= mine);
     }
     return Reach{__reduce_max_sync(0xffffffffu, as_large >= top ? mine : 0u), __reduce_max_sync(0xffffffffu, mine)};
 }
 
-// The `top` largest of n different keys, in order (0 for none), to dst; both in shared memory, src 16-byte
-// aligned. All threads that work on values; no barrier. A thread counts the larger keys for each.
-__device__ __forceinline__ void sort_keys(const Key *src, uint32_t n, Key *dst, uint32_t top) {
-    if (threadIdx.x < top && threadIdx.x >= n) dst[threadIdx.x] = 0ull;
+// A value (order bits) that `top` of the warp's 4 x 32 values reach, the top-th largest of the two largest
+// of each lane; 0 for none.
+__device__ __noinline__ uint32_t nth_of(RowShared &sm, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t top) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t x = max(max(a, b), max(c, d)), y = max(max(min(a, b), min(c, d)), min(max(a, b), max(c, d)));
+    sm.most[lane] = x;
+    sm.most[32 + lane] = y;
+    __syncwarp();
+    uint32_t nx = 0, ny = 0;
+#pragma unroll 4
+    for (uint32_t k = 0; k < 64; k += 4) {
+        const uint4 o = *reinterpret_cast<const uint4 *>(&sm.most[k]);
+        nx += (o.x >= x) + (o.y >= x) + (o.z >= x) + (o.w >= x);
+        ny += (o.x >= y) + (o.y >= y) + (o.z >= y) + (o.w >= y);
+    }
+    __syncwarp();
+    return __reduce_max_sync(0xffffffffu, nx >= top ? x : ny >= top ? y : 0u);
+}
+
+// The `top` largest of n different keys of a buffer, in order (0 for none), to the other one; returns how many.
+// One warp. A lane counts the larger keys for each of its own, after those below a value that `top` of them
+// reach have dropped out.
+__device__ __noinline__ uint32_t sort_keys(RowShared &sm, Key *src, uint32_t n, Key *dst, uint32_t top) {
+    const uint32_t lane = threadIdx.x & 31u;
+    __syncwarp();
+    if (n > kSort) {
+        uint32_t o[4] = {};
+#pragma unroll
+        for (uint32_t b = 0; b < kBuffer / 32; ++b)
+            if (b * 32 + lane < n) o[b % 4] = max(o[b % 4], uint32_t(src[b * 32 + lane] >> 32));
+        const uint32_t bound = nth_of(sm, o[0], o[1], o[2], o[3], top);
+        uint32_t kept = 0;
+        for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+            const Key key = i0 + lane < n ? src[i0 + lane] : 0ull;
+            const bool keep = uint32_t(key >> 32) >= bound && key != 0;
+            const uint32_t who = __ballot_sync(0xffffffffu, keep);
+            if (keep) src[kept + __popc(who & ((1u << lane) - 1u))] = key;  // at or before where it was
+            kept += __popc(who);
+            __syncwarp();
+        }
+        n = kept;
+    }
+    if (lane < top) dst[lane] = 0ull;
+    __syncwarp();
     const uint32_t from = smem_addr(src);
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    for (uint32_t i = lane; i < n; i += 32) {
         const Key key = src[i];
         uint32_t place = 0;
         for (uint32_t j = 0; j < n; j += 8) {
@@ -167,45 +219,12 @@ __device__ __forceinline__ void sort_keys(const Key *src, uint32_t n, Key *dst, 
         }
         if (place < top) dst[place] = key;
     }
-}
-
-// Moves the `top` best keys of buffer `at`, in order, to the other one; returns the bound that a later
-// key has to reach. All threads that work on values.
-__device__ __noinline__ Key cut(RowShared &sm, uint32_t at, uint32_t top, Key least) {
-    sync_values();
-    uint32_t n = min(min(sm.count[at], sm.valid[at]), kBuffer);
-    Key *src = sm.buffer[at];
-    if (n > kSort) {
-        // Keys below a value that `top` of them reach drop out first.
-        uint32_t mine = 0;
-        for (uint32_t i = threadIdx.x; i < n; i += kThreads) mine = max(mine, uint32_t(src[i] >> 32));
-        const uint32_t bound = reach_of(sm, mine, top).bound;
-        if (threadIdx.x == 0) sm.count[at] = 0;
-        Key own[(kBuffer + kThreads - 1) / kThreads];
-#pragma unroll
-        for (uint32_t b = 0; b < (kBuffer + kThreads - 1) / kThreads; ++b) {
-            const uint32_t i = threadIdx.x + b * kThreads;
-            own[b] = i < n ? src[i] : 0ull;
-        }
-        sync_values();
-#pragma unroll
-        for (uint32_t b = 0; b < (kBuffer + kThreads - 1) / kThreads; ++b)
-            if (own[b] && uint32_t(own[b] >> 32) >= bound) src[atomicAdd(&sm.count[at], 1u)] = own[b];
-        sync_values();
-        n = sm.count[at];
-    }
-    Key *dst = sm.buffer[at ^ 1u];
-    sort_keys(src, n, dst, top);
-    if (threadIdx.x == 0) {
-        sm.count[at ^ 1u] = min(n, top);
-        sm.valid[at ^ 1u] = kBuffer;
-    }
-    sync_values();
-    return n >= top ? dst[top - 1] + 1 : least;  // keys to come go behind the first min(n, top)
+    __syncwarp();
+    return min(n, top);
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreParams p) {
+__global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) score_kernel(ScoreParams p) {
     constexpr uint32_t kVec = 16 / sizeof(T), W = kWords<T>, P = kPiece<T>, S = kStages<T>;
     extern __shared__ __align__(128) uint4 stages[];  // [S][P]
     __shared__ RowShared sm;
@@ -213,6 +232,10 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreP
     if (threadIdx.x < S) {
         mbar_init(&sm.full[threadIdx.x], 1);
         mbar_init(&sm.empty[threadIdx.x], kWarps);
+    }
+    if (threadIdx.x < 2) {
+        mbar_init(&sm.given[threadIdx.x], kWarps);
+        mbar_init(&sm.taken[threadIdx.x], 1);
     }
     __syncthreads();
     grid_dependency_wait();
@@ -269,25 +292,235 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreP
     }
 
     auto token_at = [&](uint32_t row) { return p.tokens && row < p.rows ? p.tokens[row] : -1; };
-    auto given_value = [&](uint32_t row, int32_t token) {
+    auto value_of = [&](uint32_t row, int32_t token) {
         return token >= 0 && uint32_t(token) < p.vocab ? to_f32(static_cast<const T *>(p.logits)[size_t(row) * p.stride + token]) : 0.f;
     };
+    auto key_of = [](float v, uint32_t i) { return static_cast<Key>(order_bits(v)) << 32 | (0xffffffffu - i); };
+    auto unpack = [](const uint4 &raw, float *v) {
+        if constexpr (sizeof(T) == 4) {
+            v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y);
+            v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
+        } else {
+            const T *h = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (uint32_t j = 0; j < kVec; ++j) v[j] = to_f32(h[j]);
+        }
+    };
+    // (Of the references, a warp's largest; as order bits, for one instruction.)
+    auto warp_join = [](Sums &a) {
+        a.rescale(order_value(__reduce_max_sync(0xffffffffu, order_bits(a.m))));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+            a.e += __shfl_xor_sync(0xffffffffu, a.e, o);
+        }
+    };
+    // The value outside whole words that is a lane's.
+    auto is_edge = [&](const Row &r) { return cr == 0 && lane < r.n_head + r.n_tail; };
+    auto edge_index = [&](const Row &r) { return lane < r.n_head ? lane : r.n_head + r.words * kVec + (lane - r.n_head); };
+
+    if (warp == kWarps + 1) {
+        uint32_t turn = 0;
+        bool ok = true;
+        for (uint32_t row = row0; row < p.rows; row += step, ++turn) {
+            const Row r = row_at(row);
+            const uint4 *body = reinterpret_cast<const uint4 *>(r.x + r.n_head);
+            const int32_t token = token_at(row);
+            const float xt = value_of(row, token);
+            const bool given = token >= 0 && uint32_t(token) < p.vocab;
+            const bool edge = is_edge(r);
+            const uint32_t edge_i = edge_index(r);
+            const float edge_v = TOP && edge ? to_f32(r.x[edge_i]) : -INFINITY;
+            if (ok && !mbar_wait(&sm.given[turn & 1u], turn / 2 & 1u)) {
+                if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 107, blockIdx.x);
+                ok = false;
+            }
+            const Handed &h = sm.handed[turn & 1u];
+            Sums t{lane < kWarps ? h.m[lane] : kLowest, lane < kWarps ? h.z[lane] : 0.f, lane < kWarps ? h.e[lane] : 0.f};
+            warp_join(t);
+            uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < kWarps ? h.ahead[lane] : 0u);
+            uint32_t most[4], noted[4];
+            if constexpr (TOP) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    most[i] = order_bits(h.most[i * 32 + lane]);
+                    noted[i] = h.noted[i * 32 + lane];
+                }
+            }
+            __syncwarp();
+            if (lane == 0) arrive(&sm.taken[turn & 1u]);
+            if constexpr (TOP) {
+                // A thread without values has no say: where only its -inf is reached there is no bound.
+                uint32_t bound = nth_of(sm, most[0], most[1], most[2], most[3], p.top);
+                if (bound <= order_bits(-INFINITY)) bound = 1;
+                // Pieces to read again: as many as each lane's four threads noted.
+                const uint32_t pieces = (r.end - r.begin + P - 1) / P;
+                uint32_t own = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (most[i] < bound) noted[i] = 0;
+                    if (pieces <= 32) own += __popc(noted[i]);
+                    else
+                        for (uint32_t bits = noted[i]; bits; bits &= bits - 1) own += (pieces + 32 - __ffs(bits)) / 32;
+                }
+                uint32_t upto = own;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= uint32_t(d)) upto += v;
+                }
+                const uint32_t n_items = __shfl_sync(0xffffffffu, upto, 31);
+                uint32_t count = 0, buf = 0;
+                auto collect = [&](Key key, bool want) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, want);
+                    if (want) sm.buffer[buf][count + __popc(who & ((1u << lane) - 1u))] = key;
+                    count += __popc(who);
+                };
+                bool lost = n_items > kItems;
+                if (!lost) {
+                    uint32_t at = upto - own;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        for (uint32_t bits = noted[i]; bits; bits &= bits - 1)
+                            for (uint32_t q = __ffs(bits) - 1; q < pieces; q += 32) sm.items[at++] = q * P + i * 32 + lane;
+                    __syncwarp();
+                    // A 16-byte word of an item is a lane's to copy, then one of its 32 values to look at. (Loops
+                    // as they stand: what runs once a row and is unrolled waits for its instructions instead.)
+#pragma unroll 1
+                    for (uint32_t k0 = 0; k0 < n_items && !lost; k0 += kOnce) {
+                        const uint32_t here = min(kOnce, n_items - k0);
+#pragma unroll 1
+                        for (uint32_t k = lane; k < here * W; k += 32) {
+                            const uint32_t w = r.begin + sm.items[k0 + k / W] + k % W * kThreads;
+                            if (w < r.end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(&sm.again[k])), "l"(body + w) : "memory");
+                        }
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t k0v = 0; k0v < here && !lost; k0v += 4) {
+                            float v[4];
+                            uint32_t w[4];
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                w[k] = k0v + k < here ? r.begin + sm.items[k0 + k0v + k] + lane / kVec * kThreads : r.end;
+                                v[k] = to_f32(reinterpret_cast<const T *>(&sm.again[(k0v + k) * W])[lane]);
+                            }
+                            if (count > kBuffer - 160) lost = true;  // 32 of these for the values outside whole words
+                            else
+#pragma unroll
+                                for (uint32_t k = 0; k < 4; ++k)
+                                    collect(key_of(v[k], r.n_head + w[k] * kVec + lane % kVec), w[k] < r.end && order_bits(v[k]) >= bound);
+                        }
+                        __syncwarp();
+                    }
+                    if (!lost) collect(key_of(edge_v, edge_i), edge && order_bits(edge_v) >= bound);
+                }
+                if (lost) {
+                    // Once more for the keys: every value, against the best so far.
+                    Key least = 1ull << 32;  // a key below it is not wanted (NaN's are)
+                    count = 0;
+                    __syncwarp();
+                    auto offer = [&](float v, uint32_t i, bool is) {
+                        if (count > kBuffer - 32) {
+                            count = sort_keys(sm, sm.buffer[buf], count, sm.buffer[buf ^ 1u], p.top);
+                            buf ^= 1u;
+                            if (count == p.top) least = sm.buffer[buf][p.top - 1] + 1;
+                        }
+                        const Key key = key_of(v, i);
+                        collect(key, is && key >= least);
+                    };
+                    offer(edge_v, edge_i, edge);
+                    constexpr uint32_t kWide = 4;
+#pragma unroll 1
+                    for (uint32_t w0 = r.begin + lane; w0 - lane < r.end; w0 += 32 * kWide) {
+                        uint4 raw[kWide];
+#pragma unroll
+                        for (uint32_t k = 0; k < kWide; ++k) raw[k] = w0 + 32 * k < r.end ? body[w0 + 32 * k] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                        for (uint32_t k = 0; k < kWide; ++k) {
+                            float v[kVec];
+                            unpack(raw[k], v);
+                            bool any = false;
+#pragma unroll
+                            for (uint32_t j = 0; j < kVec; ++j) any = any || order_bits(v[j]) >= uint32_t(least >> 32);
+                            if (!__any_sync(0xffffffffu, any && w0 + 32 * k < r.end)) continue;
+#pragma unroll
+                            for (uint32_t j = 0; j < kVec; ++j) offer(v[j], r.n_head + (w0 + 32 * k) * kVec + j, w0 + 32 * k < r.end);
+                        }
+                    }
+                }
+                sort_keys(sm, sm.buffer[buf], count, sm.best[cr], p.top);
+            }
+            if (p.cluster > 1) {
+                tc::cluster_wait();  // the first CTA runs by now
+                // Every CTA sends its part to the first one.
+                auto send = [&](const void *ptr, uint32_t v) {
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::map_rank(smem_addr(ptr), 0)), "r"(v) : "memory");
+                };
+                if (lane == 0) {
+                    send(&sm.cm[cr], __float_as_uint(t.m));
+                    send(&sm.cz[cr], __float_as_uint(t.z));
+                    send(&sm.ce[cr], __float_as_uint(t.e));
+                    send(&sm.cahead[cr], ahead);
+                }
+                if (TOP && cr != 0)
+                    for (uint32_t k = lane; k < 2 * p.top; k += 32) {
+                        const uint32_t *word = reinterpret_cast<const uint32_t *>(sm.best[cr]) + k;
+                        send(word, *word);
+                    }
+                tc::cluster_sync();
+                if (cr != 0) return;  // one row per cluster
+                t = Sums{sm.cm[0], sm.cz[0], sm.ce[0]};
+                ahead = sm.cahead[0];
+                for (uint32_t c = 1; c < p.cluster; ++c) {
+                    t.join(Sums{sm.cm[c], sm.cz[c], sm.ce[c]});
+                    ahead += sm.cahead[c];
+                }
+                if (TOP) {
+                    uint32_t count = 0;
+                    for (uint32_t c = 0; c < p.cluster; ++c) {
+                        const Key key = lane < p.top ? sm.best[c][lane] : 0ull;
+                        const uint32_t who = __ballot_sync(0xffffffffu, key != 0);
+                        if (key) sm.buffer[0][count + __popc(who & ((1u << lane) - 1u))] = key;
+                        count += __popc(who);
+                    }
+                    sort_keys(sm, sm.buffer[0], count, sm.best[0], p.top);
+                }
+            }
+            const float lz = logf(t.z);
+            const bool none = t.z == 0.f;  // a row of -inf alone
+            auto log_prob = [&](float v) { return none ? NAN : (v - t.m) - lz; };
+            if (lane == 0) {
+                if (p.lse) p.lse[row] = none ? -INFINITY : t.m + lz;
+                if (p.entropy) p.entropy[row] = none ? NAN : lz - t.e / t.z;
+                if (p.tokens) {
+                    if (token >= 0 && !given) report(p.st, OPURE_ERR_DEVICE_BOUNDS, 97, uint32_t(token));
+                    if (p.logprob) p.logprob[row] = given ? log_prob(xt) : token < 0 ? 0.f : NAN;
+                    if (p.rank) p.rank[row] = given ? int32_t(ahead) : 0;
+                }
+            }
+            if (TOP && lane < p.top) {
+                const Key key = sm.best[0][lane];
+                const size_t at = size_t(row) * p.top + lane;
+                p.top_tokens[at] = key ? int32_t(0xffffffffu - uint32_t(key)) : -1;
+                p.top_logprobs[at] = key ? log_prob(order_value(uint32_t(key >> 32))) : -INFINITY;
+            }
+            __syncwarp();
+        }
+        return;
+    }
+
     int32_t token = token_at(row0);
-    float xt = given_value(row0, token);
-    uint32_t it = 0;
+    float xt = value_of(row0, token);
+    uint32_t it = 0, turn = 0;
     bool ok = true;
-    for (uint32_t row = row0; row < p.rows; row += step) {
+    for (uint32_t row = row0; row < p.rows; row += step, ++turn) {
         const Row r = row_at(row);
         const int32_t next_token = token_at(row + step);
         const bool given = token >= 0 && uint32_t(token) < p.vocab;
         // The smallest value that counts as ahead of xt: itself before the token, the next above it after.
         const float above = xt != xt ? xt : order_value(order_bits(xt) + 1u);
         const uint32_t token_word = given && uint32_t(token) >= r.n_head ? (uint32_t(token) - r.n_head) / kVec : ~0u;
-        uint32_t buf = 0;  // the buffer that keys go to
-        if (threadIdx.x == 0) {
-            sm.count[0] = 0;
-            sm.valid[0] = kBuffer;
-        }
         Sums s{kLowest, 0.f, 0.f};
         float2 z2 = make_float2(0.f, 0.f), e2 = z2;  // s.z and s.e in two parts
         uint32_t ahead = 0;
@@ -308,55 +541,12 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreP
                 e2 = make_float2(s.e, 0.f);
             }
         };
-        Key least = 1ull << 32;   // a key below it is not wanted (NaN's are)
-        float floor = -INFINITY;  // nor a value below this
-        auto key_of = [](float v, uint32_t i) { return static_cast<Key>(order_bits(v)) << 32 | (0xffffffffu - i); };
-        auto cut_now = [&]() {
-            least = cut(sm, buf, p.top, least);
-            buf ^= 1u;
-            floor = least >> 32 > 1 ? order_value(uint32_t(least >> 32)) : -INFINITY;
-        };
-        // `n` keys of this lane go to the buffer (all lanes call it): where to, or ~0 without room.
-        auto room = [&](uint32_t n) -> uint32_t {
-            uint32_t upto = n;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= uint32_t(o)) upto += t;
-            }
-            const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
-            uint32_t base = 0;
-            if (lane == 0) base = atomicAdd(&sm.count[buf], all);
-            base = __shfl_sync(0xffffffffu, base, 0);
-            if (base + all > kBuffer) {
-                if (lane == 0) atomicMin(&sm.valid[buf], base);
-                return ~0u;
-            }
-            return base + upto - n;
-        };
-        auto unpack = [](const uint4 &raw, float *v) {
-            if constexpr (sizeof(T) == 4) {
-                v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y);
-                v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
-            } else {
-                const T *h = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-                for (uint32_t j = 0; j < kVec; ++j) v[j] = to_f32(h[j]);
-            }
-        };
-
-        // The values outside whole words: the first warp of the first CTA has one in each lane.
-        const bool edge = cr == 0 && warp == 0 && lane < r.n_head + r.n_tail;
-        const uint32_t edge_i = lane < r.n_head ? lane : r.n_head + r.words * kVec + (lane - r.n_head);
+        // The values outside whole words: the first warp has one in each lane.
+        const bool edge = warp == 0 && is_edge(r);
+        const uint32_t edge_i = edge_index(r);
         const float edge_v = edge ? to_f32(r.x[edge_i]) : -INFINITY;
-        auto offer_edge = [&]() -> bool {
-            const bool want = edge && edge_v >= floor && key_of(edge_v, edge_i) >= least;
-            const uint32_t at = room(want);
-            if (want && at != ~0u) sm.buffer[buf][at] = key_of(edge_v, edge_i);
-            return at != ~0u;
-        };
-
-        bool lost = false;  // keys of this warp found no room
+        float floor = -INFINITY, most = -INFINITY;  // bound of the first piece; largest of this thread's values
+        uint32_t noted = 0;
         for (uint32_t piece = r.begin; piece < r.end; piece += P, ++it) {
             const uint32_t st = it % S;
             if (ok && !mbar_wait(&sm.full[st], it / S & 1u)) {
@@ -379,30 +569,17 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreP
             for (uint32_t j = 1; j + 1 < kValues; j += 2) high = max3(high, v[j], v[j + 1]);
             high = fmaxf(high, v[kValues - 1]);
             if (piece == r.begin) {
-                const Reach reach = reach_of(sm, order_bits(high), p.top);
+                const Reach reach = reach_of(sm.reach[turn & 1u], order_bits(high), p.top);
                 s.m = fmaxf(kLowest, order_value(reach.highest));
                 // A thread without values has no say: where only its -inf is reached there is no bound.
-                if (TOP && reach.bound > order_bits(-INFINITY)) {
-                    least = static_cast<Key>(reach.bound) << 32;
-                    floor = order_value(reach.bound);
-                }
+                if (TOP && reach.bound > order_bits(-INFINITY)) floor = order_value(reach.bound);
             }
-            if (TOP && !lost && __any_sync(0xffffffffu, high >= floor)) {
-                uint32_t want = 0;
-#pragma unroll
-                for (uint32_t j = 0; j < kValues; ++j) want |= uint32_t(v[j] >= floor) << j;
-                want &= n_values < 32 ? (1u << n_values) - 1u : ~0u;
-                uint32_t at = room(__popc(want));
-                lost = at == ~0u;
-                if (!lost)
-                    for (; want; want &= want - 1) {
-                        const uint32_t j = __ffs(want) - 1, w = j / kVec * kThreads;
-                        sm.buffer[buf][at++] =
-                            key_of(to_f32(reinterpret_cast<const T *>(words + w)[j % kVec]), r.n_head + (piece + w + threadIdx.x) * kVec + j % kVec);
-                    }
+            if (TOP && high >= floor && n_values != 0) {
+                noted |= 1u << ((piece - r.begin) / P & 31u);
+                most = fmaxf(most, high);
             }
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&sm.empty[st])) : "memory");
+            if (lane == 0) arrive(&sm.empty[st]);
             raise(high);
             const float2 z0 = z2, e0 = e2;
 #pragma unroll
@@ -430,162 +607,41 @@ __global__ void __launch_bounds__(kThreads + 32, kCtasPerSm) score_kernel(ScoreP
                     }
                 }
             }
-            if (TOP && piece == r.begin) {
-                if (cr == 0 && warp == 0 && !lost) lost = !offer_edge();
-                if (left > P && !sync_values_or(lost)) cut_now();
-            }
         }
-        const float next_xt = given_value(row + step, next_token);
+        const float next_xt = value_of(row + step, next_token);
         if (edge) {
             raise(edge_v);
             add2(make_float2(edge_v, -INFINITY), true);
             if (given) ahead += edge_v >= (edge_i < uint32_t(token) ? xt : above) && edge_i != uint32_t(token);
         }
-        if (TOP && sync_values_or(lost || r.begin == r.end)) {
-            // Once more for the keys: a word a thread at a time, value by value where one is wanted.
-            if (threadIdx.x == 0) {
-                sm.count[buf] = 0;
-                sm.valid[buf] = kBuffer;
-            }
-            least = 1ull << 32;
-            floor = -INFINITY;
-            sync_values();
-            const uint4 *body = reinterpret_cast<const uint4 *>(r.x + r.n_head);
-#pragma unroll 1
-            for (uint32_t w0 = r.begin; w0 < r.end; w0 += kThreads) {
-                const uint32_t w = w0 + threadIdx.x;
-                const T *x = reinterpret_cast<const T *>(body + w);
-                bool any = false;
-                for (uint32_t j = 0; j < kVec && w < r.end; ++j) any = any || key_of(to_f32(x[j]), r.n_head + w * kVec + j) >= least;
-                if (!sync_values_or(any)) continue;
-#pragma unroll 1
-                for (uint32_t j = 0; j < kVec; ++j) {
-                    const Key key = w < r.end ? key_of(to_f32(x[j]), r.n_head + w * kVec + j) : 0ull;
-                    const bool want = key >= least;
-                    const uint32_t at = room(want);
-                    if (want && at != ~0u) sm.buffer[buf][at] = key;
-                    sync_values();
-                    if (sync_values_or(sm.count[buf] > kBuffer - kThreads)) cut_now();
-                }
-                cut_now();
-            }
-            if (cr == 0 && warp == 0) (void)offer_edge();
-        }
         s.z = z2.x + z2.y;
         s.e = e2.x + e2.y;
-
-        // Warp, CTA, cluster. (Of the references, a warp's largest; as order bits, for one instruction.)
-        auto warp_join = [](Sums &a) {
-            a.rescale(order_value(__reduce_max_sync(0xffffffffu, order_bits(a.m))));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
-                a.e += __shfl_xor_sync(0xffffffffu, a.e, o);
-            }
-        };
         warp_join(s);
         ahead = __reduce_add_sync(0xffffffffu, ahead);
-        if (lane == 0) {
-            sm.m[warp] = s.m;
-            sm.z[warp] = s.z;
-            sm.e[warp] = s.e;
-            sm.ahead[warp] = ahead;
+        // To the finishing warp.
+        if (turn >= 2 && ok && !mbar_wait(&sm.taken[turn & 1u], (turn / 2 - 1) & 1u)) {
+            if (lane == 0) report(p.st, OPURE_ERR_DEVICE_TIMEOUT, 107, blockIdx.x);
+            ok = false;
         }
+        Handed &h = sm.handed[turn & 1u];
         if (TOP) {
-            cut_now();
-            if (threadIdx.x < p.top) sm.best[cr][threadIdx.x] = sm.buffer[buf][threadIdx.x];
-        } else {
-            sync_values();
+            h.most[threadIdx.x] = most;
+            h.noted[threadIdx.x] = noted;
         }
-        if (warp == 0) {
-            Sums t{lane < kWarps ? sm.m[lane] : kLowest, lane < kWarps ? sm.z[lane] : 0.f, lane < kWarps ? sm.e[lane] : 0.f};
-            warp_join(t);
-            const uint32_t n = __reduce_add_sync(0xffffffffu, lane < kWarps ? sm.ahead[lane] : 0u);
-            if (lane == 0) {
-                sm.cm[cr] = t.m;
-                sm.cz[cr] = t.z;
-                sm.ce[cr] = t.e;
-                sm.cahead[cr] = n;
-            }
+        if (lane == 0) {
+            h.m[warp] = s.m;
+            h.z[warp] = s.z;
+            h.e[warp] = s.e;
+            h.ahead[warp] = ahead;
         }
-        if (p.cluster > 1) {
-            sync_values();
-            tc::cluster_wait();  // the first CTA runs by now
-            // Every CTA sends its part to the first one.
-            auto send = [&](const void *ptr, uint32_t v) {
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::map_rank(smem_addr(ptr), 0)), "r"(v) : "memory");
-            };
-            if (cr != 0) {
-                if (threadIdx.x == 0) {
-                    send(&sm.cm[cr], __float_as_uint(sm.cm[cr]));
-                    send(&sm.cz[cr], __float_as_uint(sm.cz[cr]));
-                    send(&sm.ce[cr], __float_as_uint(sm.ce[cr]));
-                    send(&sm.cahead[cr], sm.cahead[cr]);
-                }
-                if (TOP && threadIdx.x < 2 * p.top) {
-                    const uint32_t *word = reinterpret_cast<const uint32_t *>(sm.best[cr]) + threadIdx.x;
-                    send(word, *word);
-                }
-            }
-            tc::cluster_sync();
-            if (cr != 0) return;  // one row per cluster
-        }
-        const Key *best = sm.best[0];
-        if (TOP && p.cluster > 1) {
-            // Each key's place is the sum of its places in the CTAs' lists, which are in order.
-            for (uint32_t k = threadIdx.x; k < p.cluster * OPURE_SCORE_MAX_TOP; k += kThreads) {
-                const uint32_t own = k % OPURE_SCORE_MAX_TOP, list = k / OPURE_SCORE_MAX_TOP;
-                const Key key = own < p.top ? sm.best[list][own] : 0ull;
-                if (!key) continue;
-                uint32_t place = 0;
-#pragma unroll
-                for (uint32_t c = 0; c < kMaxCluster; ++c) {
-                    if (c >= p.cluster) continue;
-                    uint32_t larger = 0;
-#pragma unroll
-                    for (uint32_t half = OPURE_SCORE_MAX_TOP / 2; half > 0; half /= 2)
-                        if (larger + half <= p.top && sm.best[c][larger + half - 1] > key) larger += half;
-                    if (larger < p.top && sm.best[c][larger] > key) ++larger;
-                    place += larger;
-                }
-                if (place < p.top) sm.buffer[1][place] = key;
-            }
-            uint32_t n_keys = 0;  // fewer than top: none behind them
-            for (uint32_t c = 0; c < p.cluster; ++c) n_keys += __popc(__ballot_sync(0xffffffffu, lane < p.top && sm.best[c][lane] != 0));
-            if (threadIdx.x >= n_keys && threadIdx.x < p.top) sm.buffer[1][threadIdx.x] = 0ull;
-            sync_values();
-            best = sm.buffer[1];
-        }
-        if (warp == 0) {
-            __syncwarp();
-            Sums t{sm.cm[0], sm.cz[0], sm.ce[0]};
-            uint32_t n = sm.cahead[0];
-            for (uint32_t c = 1; c < p.cluster; ++c) {
-                t.join(Sums{sm.cm[c], sm.cz[c], sm.ce[c]});
-                n += sm.cahead[c];
-            }
-            const float lz = logf(t.z);
-            const bool none = t.z == 0.f;  // a row of -inf alone
-            auto log_prob = [&](float v) { return none ? NAN : (v - t.m) - lz; };
-            if (lane == 0) {
-                if (p.lse) p.lse[row] = none ? -INFINITY : t.m + lz;
-                if (p.entropy) p.entropy[row] = none ? NAN : lz - t.e / t.z;
-                if (p.tokens) {
-                    if (token >= 0 && !given) report(p.st, OPURE_ERR_DEVICE_BOUNDS, 97, uint32_t(token));
-                    if (p.logprob) p.logprob[row] = given ? log_prob(xt) : token < 0 ? 0.f : NAN;
-                    if (p.rank) p.rank[row] = given ? int32_t(n) : 0;
-                }
-            }
-            if (TOP && lane < p.top) {
-                const Key key = best[lane];
-                const size_t at = size_t(row) * p.top + lane;
-                p.top_tokens[at] = key ? int32_t(0xffffffffu - uint32_t(key)) : -1;
-                p.top_logprobs[at] = key ? log_prob(order_value(uint32_t(key >> 32))) : -INFINITY;
-            }
-        }
-        sync_values();  // the next row writes what this one's results were read from
+        __syncwarp();
+        if (lane == 0) arrive(&sm.given[turn & 1u]);
         token = next_token;
         xt = next_xt;
+    }
+    if (p.cluster > 1) {
+        tc::cluster_wait();
+        tc::cluster_sync();
     }
 }
 
@@ -616,7 +672,7 @@ extern "C" opure_status opure_token_scores(opure_ctx *ctx, const opure_score_arg
         constexpr uint32_t kSmem = kStages<T> * kPiece<T> * 16;
         OPURE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem)));
         cfg.gridDim = dim3(cluster > 1 ? a->rows * cluster : std::min(a->rows, slots));
-        cfg.blockDim = dim3(kThreads + 32);
+        cfg.blockDim = dim3(kThreads + 64);
         cfg.dynamicSmemBytes = kSmem;
         cfg.stream = ctx->stream;
         cudaLaunchAttribute attr[2];
