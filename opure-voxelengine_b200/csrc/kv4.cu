@@ -6,6 +6,10 @@
 // definition exactly: a rotated value comes out of double as an fp32 number with its last bit set
 // where bits were cut off (so that it lies on the same side of every rounding boundary), and
 // quotients that land on a boundary are moved to the side that their remainder is on.
+//
+// 8192 tokens of 32 + 64 heads of 64, fp16, appended and read back: 83 us for 239 MB, 37 us of memory at the copy
+// rate; the rotation's conversions between fp32 and fp64 (16 a clock an SM) and stores of 1 to 8 bytes bound
+// it. A block a thread is kept for its independence of other lanes: 64 tokens take 6.4 us, two launches' time.
 #include "kv4.cuh"
 
 namespace opure {

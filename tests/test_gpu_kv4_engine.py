@@ -171,11 +171,12 @@ def test_scores(model, chunk, top, weights):
                 assert np.abs(o["top_logprobs"][t] - np.sort(lp)[::-1][:top]).max() <= 2 * tol
 
 
-def test_scores_of_the_fp16_cache(model):
+@pytest.mark.parametrize("chunk", [0, 64])
+def test_scores_of_the_fp16_cache(model, chunk):
     """Scores need no 4-bit cache: those of every prefix's own logits."""
     path, spec = model
     s = prompt(5, spec, 12)
-    with ve.Engine(path, max_len=64, prefill_chunk=64) as eng:
+    with ve.Engine(path, max_len=64, prefill_chunk=chunk) as eng:
         got = eng.score([s], 3)[0]
         for t in range(1, len(s)):
             row = eng.forward_logits(s[:t]).astype(np.float64)

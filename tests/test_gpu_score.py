@@ -88,6 +88,39 @@ def test_scores(ctx, t, rows, cols, top, shift, pad):
     check(got, held, tokens, top)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols,top,stride", [(1000, 4099, 32, 4099), (900, 9001, 7, 9004), (2, 300007, 20, 300007), (3, 150000, 32, 150000)])
+def test_rows_of_every_kind_one_behind_another(ctx, t, rows, cols, top, stride):
+    """Rows whose best tokens are gathered in each way follow one another on a CTA: random ones, equal ones,
+    rising and falling, large ones that all lie in the words of one thread (32 and 128 threads' strides of words),
+    more equal largest ones than any buffer holds. Sizes of more pieces than a thread's 32 bits too."""
+    rng = np.random.default_rng(rows + cols)
+    vec = 4 if t == "f32" else 8
+    i = np.arange(cols)
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    for r in range(rows):
+        kind = r % 7
+        if kind == 1:
+            x[r] = 0.5
+        elif kind == 2:
+            x[r] = np.sort(x[r])
+        elif kind == 3:
+            x[r] = np.sort(x[r])[::-1]
+        elif kind == 4:
+            x[r][i // vec % 128 == r % 128] += 20
+        elif kind == 5:
+            x[r][i // vec % 32 == r % 32] += 20
+        elif kind == 6:
+            x[r][rng.permutation(cols)[:700]] = 9.0
+    rows_ = Rows(ctx, rows, cols, t, stride)
+    held = rows_.put(x)
+    tokens = np.where(rng.random(rows) < 0.5, held.argmax(1), rng.integers(0, cols, rows))
+    got = call(ctx, rows_, tokens, top)
+    again = call(ctx, rows_, tokens, top)
+    assert all(np.array_equal(got[k], again[k]) for k in got)
+    check(got, held, tokens, top, list(range(min(rows, 30))) + list(range(max(min(rows, 30), rows - 130), rows)))
+
+
 @pytest.mark.parametrize("size", [1e-3, 200.0, 3e4])
 def test_scores_of_any_size(ctx, size):
     rng = np.random.default_rng(1)
