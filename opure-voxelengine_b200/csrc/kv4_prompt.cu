@@ -594,13 +594,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     ok = false;
                 }
             };
-            // Tile i's scores, and the products of tile i - 2, over whose P the scores go.
+            // Tile i's scores, and the products of tile i - 2, over whose P the scores go. A stage is free after one
+            // arrival of each half's warp, so a warp whose half has no part in a tile (rows that are not there, keys
+            // that they do not see) waits for the tile all the same: its arrivals for two tiles would else fill
+            // one phase, and the stage be written again under the other half.
             for (uint32_t i = 0; i < n_tiles + 2; ++i) {
                 const uint32_t n = i - from_t;
                 const uint32_t s_col = tmem + (t * 2 + (n & 1u)) * KT;
+                if (i >= 2) wait(&v_full[(i - 2) % kStages], (i - 2) / kStages & 1u);
                 if (i >= from_t + 2 && i < upto_t + 2 && upto_t > from_t) {
                     const uint32_t st = (i - 2) % kStages, v = smem_addr(kv_smem + st * 2 * S::kTile + S::kTile);
-                    wait(&v_full[st], (i - 2) / kStages & 1u);
                     wait(&p_full[t][n & 1u], (n - 2) / 2 & 1u);
                     if (!ok) break;
                     tc::fence_after();
@@ -616,11 +619,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                         }
                     tc::commit(one, &o_full[t][n & 1u]);
                 }
+                if (!ok) break;
                 if (i >= 2) tc::commit(one, &v_empty[(i - 2) % kStages]);
+                if (i < n_tiles) wait(&k_full[i % kStages], i / kStages & 1u);
+                if (!ok) break;
                 if (i >= from_t && i < upto_t) {
                     const uint32_t st = i % kStages, kt = smem_addr(kv_smem + st * 2 * S::kTile);
-                    wait(&k_full[st], i / kStages & 1u);
-                    if (!ok) break;
                     tc::fence_after();
 #pragma unroll
                     for (uint32_t part = 0; part < (S::kPair ? 2 : 1); ++part) {

@@ -1,0 +1,129 @@
+"""Attention over the 4-bit KV cache where a kernel for prompts walks many tiles of 64 keys in one split:
+few queries over a long past, and blocks of 256 rows whose halves see different tiles, or one of which
+is empty. Against a plain 64-bit implementation, with the bounds of test_gpu_kv4.
+"""
+import numpy as np
+import pytest
+
+import kv4_reference as ref
+from test_gpu_kv4 import TYPES, Dev, attend, bound, ctx, release, tables  # noqa: F401 (fixtures)
+from test_gpu_kv4_engine import Forward, prompt
+from test_gpu_mx import Rows
+from voxelengine import engine as ve
+
+pytestmark = pytest.mark.gpu
+
+
+def random_cache(rng, seqs, pages, n_kv, hd, page, ring=0):
+    """Codes of any value, scales from 2^-3 to 1, in every page."""
+    table, n_pages = tables(rng, seqs, ring or pages)
+    cache = ref.Cache(n_pages, n_kv, hd, page, table, ring)
+    cache.pool[:] = rng.integers(0, 256, cache.pool.shape)
+    cache.pool[..., 16 * hd :] = rng.integers(0x20, 0x39, cache.pool[..., 16 * hd :].shape)
+    return cache
+
+
+def plain(q, k, v, seen, scale):
+    """ref.attention for all queries of a head at once; as it, also the largest score's size and value."""
+    m, heads, _ = q.shape
+    begin, end = (np.array([s[i] for s in seen])[:, None] for i in (0, 1))
+    t = np.arange(k.shape[1])[None]
+    there = (t >= begin) & (t < end)
+    out, size = np.zeros(q.shape), 0.0
+    for h in range(heads):
+        kk, vv = k[h // (heads // k.shape[0])], v[h // (heads // k.shape[0])]
+        x = np.where(there, q[:, h] @ kk.T * scale, -np.inf)
+        w = np.exp(x - x.max(1, keepdims=True))
+        out[:, h] = w @ vv / w.sum(1, keepdims=True)
+        size = max(size, float((np.abs(q[:, h]) @ np.abs(kk).T).max()) * abs(scale))
+    return out, size, float(np.abs(v).max())
+
+
+def check(ctx, t, group, n_kv, hd, page, past, queries, split=0, ring=0, seed=0, n_q=None, max_ctx=None):
+    """Entries of `queries` each after `past` positions; twice, with the same bits."""
+    rng = np.random.default_rng(seed)
+    heads, total = group * n_kv, [a + b for a, b in zip(past, queries)]
+    cache = random_cache(rng, len(past), max((n + page - 1) // page for n in total), n_kv, hd, page, ring)
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, sum(queries), heads * hd, t)
+    x = q.put(rng.standard_normal((sum(queries), heads * hd)) * 1.5).reshape(-1, heads, hd)
+    begin = np.concatenate(([0], np.cumsum(queries)))
+    outs = [attend(ctx, dev, q, np.arange(len(past)), np.array(past) + 1, begin, n_q or max(queries), heads, hd ** -0.5, max_ctx or max(total), split)
+            for _ in range(2)]
+    got = outs[0].get().reshape(-1, heads, hd)
+    assert np.array_equal(got, outs[1].get().reshape(-1, heads, hd))
+    for s, (n, m) in enumerate(zip(past, queries)):
+        a, b = begin[s], begin[s + 1]
+        k, v = cache.get(s, total[s])
+        want, size, top = plain(x[a:b], k, v, [(ref.window_begin(n + j, page, ring), n + j + 1) for j in range(m)], hd ** -0.5)
+        single = t != "f32" and (n_q or max(queries)) * group > 16
+        d = np.abs(got[a:b] - want)
+        assert (d <= bound(t, want, size, top, hd, total[s], single)).all(), (s, float(d.max()))
+
+
+# Rows (queries x group) of a kv head: 17, 88, 128, 129, 300, 360, 257; keys: tiles of 64 in one split.
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("tiles", [3, 5, 8, 9, 13, 40])
+@pytest.mark.parametrize("group,n_kv,queries", [(1, 1, 17), (8, 2, 11), (4, 1, 32), (3, 2, 43), (3, 1, 100), (5, 1, 72), (1, 2, 257)])
+def test_few_queries_over_a_long_past(ctx, t, hd, tiles, group, n_kv, queries):
+    check(ctx, t, group, n_kv, hd, 64, [max(tiles * 64 - queries - 5, 0)], [queries], split=1 << 20, seed=tiles + queries)
+
+
+@pytest.mark.parametrize("t,hd", [("f32", 64), ("f32", 128), ("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("split", [0, 640, 1 << 20])
+def test_entries_of_very_different_lengths(ctx, t, hd, split):
+    """Long pasts with few queries beside prompts, an entry of one query, and one that starts its sequence."""
+    check(ctx, t, 4, 2, hd, 32, [3000, 0, 700, 1500, 40], [20, 261, 1, 64, 33], split=split)
+
+
+@pytest.mark.parametrize("t,hd", [("f32", 64), ("f32", 128), ("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("page,ring", [(16, 40), (64, 12), (32, 150)])
+def test_windows_that_move_within_a_call(ctx, t, hd, page, ring):
+    """The second half of a block of rows begins, and ends, tiles later than the first. (What lies in a page
+    of the ring is read as it is now, by both sides.)"""
+    check(ctx, t, 1, 2, hd, page, [ring * page + 30, 100], [256, 230], ring=ring, split=1 << 20)
+
+
+@pytest.mark.parametrize("queries,group,n_q", [(5, 3, 8), (5, 4, 8), (9, 1, 16), (9, 2, 16)])
+def test_verify_steps_over_a_long_past(ctx, queries, group, n_q):
+    """Drafts of several sequences as the engine passes them: n_q a power of two above what any entry has,
+    max_ctx the cache's capacity."""
+    check(ctx, "f32", group, 8, 64, 64, [1000, 1700, 2040], [queries, queries, 1], n_q=n_q, max_ctx=4096)
+
+
+# ---- through the engine -----------------------------------------------------------------------------
+
+WIDE = dict(vocab=1000, hidden=2048, inter=512, layers=2, heads=32, kv_heads=8, max_pos=4096)
+
+
+@pytest.fixture(scope="module")
+def wide(tmp_path_factory):
+    path = ve.synth_model(str(tmp_path_factory.mktemp("kv4long") / "m"), seed=21, **WIDE)
+    return path, Forward(path, WIDE)
+
+
+@pytest.mark.parametrize("chunk,n", [(1024, 600), (512, 600), (512, 1037)])
+def test_scores_of_long_prompts(wide, chunk, n):
+    """A prompt in one chunk whose last block of rows is part-filled, and short last chunks after long ones.
+    Log probabilities differ by at most twice what logits do."""
+    path, fwd = wide
+    p = prompt(7, WIDE, n)
+    y, tol = fwd.bounded(p)
+    with ve.Engine(path, max_len=4096, kv=ve.KV_FP4, prefill_chunk=chunk) as eng:
+        got = eng.score([p])[0]["logprobs"]
+        tokens, _ = eng.generate([p], 3)
+    lp = y - y.max(1, keepdims=True)
+    lp -= np.log(np.exp(lp).sum(1, keepdims=True))
+    assert np.abs(got[1:] - lp[np.arange(n - 1), p[1:]]).max() <= 2 * tol
+    assert len(tokens[0]) == 3 and fwd.follows(p, tokens[0])
+
+
+def test_speculation_after_long_prompts(wide):
+    path, fwd = wide
+    prompts = [prompt(30 + i, WIDE, 1000) for i in range(3)]
+    with ve.Engine(path, max_batch=18, max_len=4096, kv=ve.KV_FP4, prefill_chunk=512) as t:
+        with ve.Engine(path, max_batch=18, max_len=4096, share=t, kv=ve.KV_FP4) as d:
+            got, _, _ = t.spec_generate(d, prompts, 12, k=5)
+    for p, g in zip(prompts, got):
+        assert len(g) == 12 and fwd.follows(p, g)
