@@ -402,7 +402,9 @@ def _own_run(s):
         return {k: s[k] for k in ("q", "k", "v")}
     if "scratch" not in s:  # made once and kept, as a program keeps it; its counters start at zero
         need = cu.kv4_attention_scratch_bytes(c["seqs"], s["rows"], c["new"], heads, kv, hd, s["max_keys"])
-        s["scratch"] = torch.zeros(max(need, 16), dtype=torch.uint8, device=DEV)
+        s["scratch"] = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+        # On the context's stream, which does not wait for torch's.
+        ctx.call("opure_fill", s["scratch"].data_ptr(), 0, s["scratch"].numel())
     ctx.kv4_attention(cu.Kv4AttnArgs(
         q=s["q"].data_ptr(), out=s["out"].data_ptr(), type=t, q_stride=heads * hd, out_stride=heads * hd, seq=s["seq"].data_ptr(),
         seq_len=s["seq_len"].data_ptr(), q_begin=s["begin"].data_ptr() if c["new"] > 1 else None, n=c["seqs"], n_rows=s["rows"], n_q=c["new"], n_heads=heads,
