@@ -14,7 +14,7 @@
 // the other half's thread keeps the exponentials going while it adds. With fp32 queries Q and P are
 // pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit types Q is exact in
 // fp16 and P is rounded to it once. A row's queries are scaled by a power of two to [1, 2) first. The
-// maximum is raised only when a score passes it by 2^8.
+// maximum is raised only when a score passes it by 2^4.
 //
 // What bounds it: 16,384 exponentials a tile of 64 keys and 256 rows at 16 a clock, 1,024 clocks; the
 // tensor cores need as long for fp32 (two MMAs for one), half for 16-bit types. A tile takes 2,200-2,600 clocks:
@@ -31,7 +31,11 @@ namespace {
 constexpr uint32_t kSoftmaxWarps = 8, kThreads = 512, kHalf = 128;
 constexpr uint32_t kMmaWarp = 12;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRaise = 8.f;
+// Log2 units by which a score may pass the running maximum, and by which probabilities are larger than
+// relative to it: together 2^15, what fp16 has. So a probability has all its bits down to 2^-25 of the
+// maximum's, and is off by 2^-36 at most below (2^-25 if the maximum's were 1: keys of 2^-24.5 and less, thousands
+// of them beside one of weight 1, counted 1.4 times, or not at all).
+constexpr float kRaise = 4.f, kLift = 11.f;
 constexpr uint32_t KT = 64;          // keys of a tile
 constexpr uint32_t kGroups = KT / kKv4Group;  // of 16 positions, one to each converting warp
 
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
                     for (uint32_t d = 0; d < HD; ++d) acc[d] *= raised;
                     rescale = true;
                 }
-                const float base = m == -INFINITY ? 0.f : m;
+                const float base = m == -INFINITY ? 0.f : m - kLift;
 #pragma unroll 1
                 for (uint32_t c = 0; c < KT; c += CH) {
                     if (CH < KT) {

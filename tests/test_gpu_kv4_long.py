@@ -8,7 +8,7 @@ import pytest
 import kv4_reference as ref
 from test_gpu_kv4 import TYPES, Dev, attend, bound, ctx, release, tables  # noqa: F401 (fixtures)
 from test_gpu_kv4_engine import Forward, prompt
-from test_gpu_mx import Rows
+from test_gpu_mx import HALF_ULP, TINY, Rows
 from voxelengine import engine as ve
 
 pytestmark = pytest.mark.gpu
@@ -90,6 +90,37 @@ def test_verify_steps_over_a_long_past(ctx, queries, group, n_q):
     """Drafts of several sequences as the engine passes them: n_q a power of two above what any entry has,
     max_ctx the cache's capacity."""
     check(ctx, "f32", group, 8, 64, 64, [1000, 1700, 2040], [queries, queries, 1], n_q=n_q, max_ctx=4096)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("far", [10.0, 15.0, 17.0])
+def test_many_small_probabilities_beside_a_large_one(ctx, t, hd, far):
+    """A first key with a score about `far` above all others', whose value is 0: the result is the others' sum, 40,000
+    probabilities of exp(-far) or so, each off by 2^-22 of itself (pairs) or 2^-11 (16-bit types) and by 2^-36 of the
+    largest, and the scores by the usual."""
+    rng = np.random.default_rng(int(far))
+    n, m = 40000, 40
+    table, n_pages = tables(rng, 1, (n + 127) // 128)
+    cache = ref.Cache(n_pages, 1, hd, 128, table)
+    for at, scales in ((0, cache.at[2]), (8 * hd, cache.at[3])):
+        cache.pool[..., at : at + 8 * hd] = 0x22  # 1.0
+        cache.pool[..., scales.ravel()] = 0x38    # 1.0
+    k, v = np.zeros((1, hd)), np.zeros((1, hd))
+    k[0, 0] = 2.0
+    k[0, 1:] = 1.0
+    cache.put(0, 0, k, v)
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, m, hd, t)
+    x = np.zeros((m, hd))
+    x[:, 0] = far  # exact in every type
+    q.put(x)
+    got = attend(ctx, dev, q, [0], [n - m + 1], [0, m], m, 1, 1.0, n).get()
+    # (The first key is kept as 2.0625: its score lies 1.0625 far above the others'.)
+    want = plain(x[:, None], *cache.get(0, n), [(0, n - m + 1 + j) for j in range(m)], 1.0)[0][:, 0]
+    # The score's own error, 2 far 2^-22 or so, is in all of the others alike; the sums' of n / 64 steps.
+    relative = 4 * far * 2.0 ** -22 + 2.0 ** -20 + 2 * (n / 64 + 64) * 2.0 ** -24 + (2.0 ** -11 if t != "f32" else 0.0)
+    assert (np.abs(got - want) <= (HALF_ULP[t] + relative) * want + n * 2.0 ** -36 + TINY[t]).all()
 
 
 # ---- through the engine -----------------------------------------------------------------------------
