@@ -12,9 +12,10 @@
 //                tensor cores, whose additions cut off, the sums drift)
 // S has two buffers a half, so a row's thread finds the next scores ready when it is done with a tile, and
 // the other half's thread keeps the exponentials going while it adds. With fp32 queries Q and P are
-// pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit types Q is exact in
-// fp16 and P is rounded to it once. A row's queries are scaled by a power of two to [1, 2) first. The
-// maximum is raised only when a score passes it by 2^4.
+// pairs of fp16 (hi, lo), two MMAs each, so that products keep 22 bits; with 16-bit types Q is a single fp16
+// (exact down to 2^-28 of the row's largest) and P is rounded to it once. A row's queries are scaled by a power
+// of two to [2^14, 2^15) first, so that they are held to 2^-39 of the largest at least. The maximum is raised
+// only when a score passes it by 2^4.
 //
 // What bounds it: 16,384 exponentials a tile of 64 keys and 256 rows at 16 a clock, 1,024 clocks; the
 // tensor cores need as long for fp32 (two MMAs for one), half for 16-bit types. A tile takes 2,200-2,600 clocks:
@@ -235,11 +236,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(Kv4AttnParams p) {
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
         }
-        const uint32_t e = __float_as_uint(m) >> 23;
-        const bool normal = e > 0 && e < 253;
-        // The factor is not negative: a negative scale goes to the queries.
-        const float down = (normal ? __uint_as_float((254u - e) << 23) : 1.f) * (p.factor < 0.f ? -1.f : 1.f);
-        factor = (normal ? __uint_as_float(e << 23) : 1.f) * fabsf(p.factor);
+        // To [2^14, 2^15), times 2^(d - 127), and back in the factor (rows whose largest is below 2^-112 come
+        // out smaller, an infinity or NaN stays one). The factor is not negative: a negative scale goes to the
+        // queries.
+        const uint32_t e = __float_as_uint(m) >> 23, d = min(268u - e, 253u);
+        const float down = __uint_as_float(d << 23) * (p.factor < 0.f ? -1.f : 1.f);
+        factor = __uint_as_float((254u - d) << 23) * fabsf(p.factor);
         uint8_t *dst = q_smem + half * (S::kQBytes / 2) + r * 128;
         const uint32_t q_col = tmem + ((warp % 4 * 32) << 16) + S::kQCol + half * HD;
 #pragma unroll 2

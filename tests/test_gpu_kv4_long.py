@@ -123,6 +123,31 @@ def test_many_small_probabilities_beside_a_large_one(ctx, t, hd, far):
     assert (np.abs(got - want) <= (HALF_ULP[t] + relative) * want + n * 2.0 ** -36 + TINY[t]).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", [2.0 ** -30, 1.0, 2.0 ** 12, 2.0 ** 126])
+def test_small_queries_beside_a_large_one(ctx, t, hd, size):
+    """Scores that come from columns of 2^-20 of the query's largest, whose own column is 0 in every key: held
+    to 2^-39 of the largest and so 2^-18 of themselves, where the bound has 2^-22. Up to fp32's largest."""
+    if t == "f16" and size not in (1.0, 2.0 ** 12):
+        pytest.skip("not values of fp16")
+    rng = np.random.default_rng(hd)
+    n, m = 300, 40
+    cache = random_cache(rng, 1, 5, 1, hd, 64)
+    cache.pool[..., cache.at[0][:, 0]] &= 0xF0  # column 0's codes
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, m, hd, t)
+    x = rng.uniform(1, 2, (m, hd)) * rng.choice([-1, 1], (m, hd)) * size
+    x[:, 1:] *= 2.0 ** -20
+    x = q.put(x)  # as the type has them
+    scale = float(np.float32(0.25 / size * 2.0 ** 20))
+    got = attend(ctx, dev, q, [0], [n - m + 1], [0, m], m, 1, scale, n).get()
+    want, biggest, top = plain(x[:, None], *cache.get(0, n), [(0, n - m + 1 + j) for j in range(m)], scale)
+    assert biggest < 100
+    d = np.abs(got[:, None] - want)
+    assert (d <= bound(t, want, biggest, top, hd, n, t != "f32") + top * 2 * biggest * 2.0 ** -18).all(), float(d.max())
+
+
 # ---- through the engine -----------------------------------------------------------------------------
 
 WIDE = dict(vocab=1000, hidden=2048, inter=512, layers=2, heads=32, kv_heads=8, max_pos=4096)
