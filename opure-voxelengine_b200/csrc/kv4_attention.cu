@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<HD, NT>) rows_kernel(Kv4A
     uint8_t *ring = smem + size_t(warp) * S * kStageBytes<HD>;
 
     if (warp < kWarps) {
-        // Queries: row r of this lane's column. Each row is scaled by a power of two to [1, 2).
+        // Queries: row r of this lane's column. Each row is scaled by a power of two to [2, 4).
         uint32_t qf[HD / 16][NT][2];
         float factor[NT];
         uint32_t row_end[NT], row_begin[NT];
@@ -198,10 +198,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm<HD, NT>) rows_kernel(Kv4A
             }
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            // 2^-floor(log2 m), and back in the factor (m 0, infinite or subnormal: 1).
-            const uint32_t e = __float_as_uint(m) >> 23;
-            const bool normal = e > 0 && e < 253;
-            const float down = normal ? __uint_as_float((254u - e) << 23) : 1.f, up = normal ? __uint_as_float(e << 23) : 1.f;
+            // Times 2^(d - 127), and back in the factor (rows whose largest is below 2^-125 come out smaller,
+            // one with an infinity or NaN is NaN).
+            const uint32_t e = __float_as_uint(m) >> 23, d = min(255u - e, 253u);
+            const float down = __uint_as_float(d << 23), up = __uint_as_float((254u - d) << 23);
 #pragma unroll
             for (uint32_t k = 0; k < HD / 4; k += 2) {
                 uint32_t pair[2];

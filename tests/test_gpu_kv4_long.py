@@ -148,6 +148,31 @@ def test_small_queries_beside_a_large_one(ctx, t, hd, size):
     assert (d <= bound(t, want, biggest, top, hd, n, t != "f32") + top * 2 * biggest * 2.0 ** -18).all(), float(d.max())
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [4, 15, 40])
+def test_queries_of_the_largest_size(ctx, t, hd, m):
+    """Queries up to fp32's largest and of its subnormals beside ordinary ones; a query with an infinity or NaN is
+    NaN, and no other."""
+    rng = np.random.default_rng(m)
+    n = 200
+    cache = random_cache(rng, 1, 4, 1, hd, 64)
+    dev = Dev(ctx, cache)
+    size = np.array([2.0 ** 125, 2.0 ** 126, 2.0 ** 127, 2.0 ** -128])
+    for s in size:
+        q = Rows(ctx, m, hd, t)
+        x = rng.uniform(0.9, 0.99, (m, hd)) * rng.choice([-1, 1], (m, hd)) * s * 2
+        x[1::4, 3], x[2::4, 5] = np.inf, np.nan
+        x = q.put(x)
+        scale = float(np.float32(2.0 ** -3 / s)) if s > 1 else 2.0 ** 124
+        got = attend(ctx, dev, q, [0], [n - m + 1], [0, m], m, 1, scale, n).get()
+        ok = np.isfinite(x).all(1)
+        want, biggest, top = plain(np.where(ok[:, None], x, 0)[:, None], *cache.get(0, n), [(0, n - m + 1 + j) for j in range(m)], scale)
+        # (2^-128 (1 + ..) has 21 bits: held exactly.)
+        assert (np.abs(got[ok] - want[ok, 0]) <= bound(t, want, biggest, top, hd, n, t != "f32" and m > 16)[ok, 0]).all()
+        assert np.isnan(got[~ok]).all()
+
+
 # ---- through the engine -----------------------------------------------------------------------------
 
 WIDE = dict(vocab=1000, hidden=2048, inter=512, layers=2, heads=32, kv_heads=8, max_pos=4096)
