@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) score_kernel(ScoreP
 
     int32_t token = token_at(row0);
     float xt = value_of(row0, token);
-    uint32_t it = 0, turn = 0;
+    uint32_t it = 0, turn = 0, reached = 0;  // reached: rows with a first piece, which alone meet at a barrier
     bool ok = true;
     for (uint32_t row = row0; row < p.rows; row += step, ++turn) {
         const Row r = row_at(row);
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads + 64, kCtasPerSm) score_kernel(ScoreP
             for (uint32_t j = 1; j + 1 < kValues; j += 2) high = max3(high, v[j], v[j + 1]);
             high = fmaxf(high, v[kValues - 1]);
             if (piece == r.begin) {
-                const Reach reach = reach_of(sm.reach[turn & 1u], order_bits(high), p.top);
+                const Reach reach = reach_of(sm.reach[reached++ & 1u], order_bits(high), p.top);
                 s.m = fmaxf(kLowest, order_value(reach.highest));
                 // A thread without values has no say: where only its -inf is reached there is no bound.
                 if (TOP && reach.bound > order_bits(-INFINITY)) floor = order_value(reach.bound);

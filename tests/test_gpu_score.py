@@ -121,6 +121,21 @@ def test_rows_of_every_kind_one_behind_another(ctx, t, rows, cols, top, stride):
     check(got, held, tokens, top, list(range(min(rows, 30))) + list(range(max(min(rows, 30), rows - 130), rows)))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("cols,stride", [(3, 3), (5, 5), (6, 7), (7, 9), (8, 9), (9, 9), (14, 15)])
+def test_short_rows_with_and_without_whole_words(ctx, t, cols, stride):
+    """Rows of some of which no aligned 16 bytes are there, in turn with others that have some: many of each on a CTA."""
+    rng = np.random.default_rng(cols)
+    rows = 6000
+    x = Rows(ctx, rows, cols, t, stride)
+    held = x.put(rng.standard_normal((rows, cols)) * 4)
+    tokens = rng.integers(0, cols, rows)
+    got = call(ctx, x, tokens, 3)
+    again = call(ctx, x, tokens, 3)
+    assert all(np.array_equal(got[k], again[k]) for k in got)
+    check(got, held, tokens, 3)
+
+
 @pytest.mark.parametrize("size", [1e-3, 200.0, 3e4])
 def test_scores_of_any_size(ctx, size):
     rng = np.random.default_rng(1)
