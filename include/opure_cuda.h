@@ -445,9 +445,9 @@ opure_status opure_kv4_read(opure_ctx *ctx, const opure_kv4_read_args *a);
  * entries with more than 16 (query, head) rows per kv head are rounded to fp16 once.
  *
  * scratch: opure_kv4_attention_scratch_bytes(...) bytes, 16-byte aligned, caller-owned. Zero before
- * the first call (opure_fill); every call leaves its counters zero, at a place that depends on n, n_rows,
- * n_q, the heads, max_ctx and split_tokens: zero it again before a call with other ones. Calls that may
- * run at the same time need scratch of their own. */
+ * the first call (opure_fill); every call leaves the counters at its start zero, so that calls of any
+ * shapes may use one buffer in turn, of the bytes that the largest asks for. Calls that may run at the
+ * same time need scratch of their own. */
 typedef struct opure_kv4_attn_args {
     const void *q;             /* [n_rows][q_stride] of type, rows [n_heads][head_dim] */
     void *out;                 /* [n_rows][out_stride] of type, apart from q           */
@@ -462,7 +462,7 @@ typedef struct opure_kv4_attn_args {
     float scale;
     uint32_t max_ctx;          /* upper bound of seq_len[i] + queries of i - 1          */
     uint32_t split_tokens;     /* keys per split (raised where there would be more than 64
-                                  splits); 0 = choose                              */
+                                  splits, or enough work without); 0 = choose      */
     void *scratch;
     size_t scratch_bytes;
     opure_kv4_layout kv;

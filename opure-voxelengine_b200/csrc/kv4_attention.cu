@@ -499,8 +499,13 @@ struct Plan {
     bool prompt;
     uint32_t tile_rows, row_tiles, split_tokens, n_splits;
     uint64_t units;
-    size_t counters_off, bytes;
+    size_t bytes;
 };
+// Scratch: a counter for each unit, then the splits' sums. As many counters for every shape, so that the sums
+// of one call never lie where the next one, of another shape, has its counters. More units than that
+// fill the SMs several times over and are not split.
+constexpr uint32_t kCounters = 2048;
+constexpr size_t kPartialsAt = kCounters * sizeof(uint32_t);
 // More than kFewRows (query, head) rows per kv head go to the kernel for prompts.
 constexpr uint32_t kFewRows = 16;
 Plan make_plan(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t split_tokens, int sms) {
@@ -525,12 +530,11 @@ Plan make_plan(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t
         want = std::max<uint64_t>(want, std::min<uint64_t>((slots * 3 + p.units - 1) / p.units, ctx / 2048));
     }
     want = std::min<uint64_t>(std::max<uint64_t>(want, 1), std::min<uint64_t>(kMaxSplits, (ctx + unit - 1) / unit));
-    const uint64_t per = split_tokens ? std::max<uint64_t>(split_tokens, (ctx + kMaxSplits - 1) / kMaxSplits) : (ctx + want - 1) / want;
+    uint64_t per = split_tokens ? std::max<uint64_t>(split_tokens, (ctx + kMaxSplits - 1) / kMaxSplits) : (ctx + want - 1) / want;
+    if (p.units > kCounters) per = ctx;
     p.split_tokens = uint32_t(std::min<uint64_t>((per + unit - 1) / unit * unit, 0xffffff80u));
     p.n_splits = ceil_div(ctx, p.split_tokens);
-    const size_t partials = p.n_splits > 1 ? size_t(p.units) * p.n_splits * p.tile_rows * (hd + 2) * sizeof(float) : 0;
-    p.counters_off = (partials + 255) & ~size_t(255);
-    p.bytes = p.counters_off + (p.n_splits > 1 ? size_t(p.units) * sizeof(uint32_t) : 0);
+    p.bytes = p.n_splits > 1 ? kPartialsAt + size_t(p.units) * p.n_splits * p.tile_rows * (hd + 2) * sizeof(float) : 0;
     return p;
 }
 
@@ -581,8 +585,8 @@ extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn
     p.v_scale = a->kv.v_scale == 0.f ? 1.f : a->kv.v_scale;
     p.split_tokens = pl.split_tokens;
     p.n_splits = pl.n_splits;
-    p.partials = static_cast<float *>(a->scratch);
-    p.counters = reinterpret_cast<uint32_t *>(static_cast<char *>(a->scratch) + pl.counters_off);
+    p.counters = static_cast<uint32_t *>(a->scratch);
+    p.partials = reinterpret_cast<float *>(static_cast<char *>(a->scratch) + kPartialsAt);
     p.kv = a->kv;
     p.st = ctx->status;
     p.out_packed = reinterpret_cast<__half *>(a->out_packed);

@@ -9,6 +9,7 @@ import kv4_reference as ref
 from test_gpu_kv4 import TYPES, Dev, attend, bound, ctx, release, tables  # noqa: F401 (fixtures)
 from test_gpu_kv4_engine import Forward, prompt
 from test_gpu_mx import HALF_ULP, TINY, Rows
+from voxelengine import cuda as cu
 from voxelengine import engine as ve
 
 pytestmark = pytest.mark.gpu
@@ -171,6 +172,26 @@ def test_queries_of_the_largest_size(ctx, t, hd, m):
         # (2^-128 (1 + ..) has 21 bits: held exactly.)
         assert (np.abs(got[ok] - want[ok, 0]) <= bound(t, want, biggest, top, hd, n, t != "f32" and m > 16)[ok, 0]).all()
         assert np.isnan(got[~ok]).all()
+
+
+def test_one_scratch_for_calls_of_any_shape(ctx):
+    """Zeroed once: each call leaves the counters as the next one needs them, whatever its shape."""
+    rng = np.random.default_rng(4)
+    n_kv, hd, keys = 2, 64, 1500
+    cache = random_cache(rng, 3, 24, n_kv, hd, 64)
+    dev = Dev(ctx, cache)
+    kv = [cache.get(s, keys) for s in range(3)]
+    shapes = [(3, 1, 2, 256), (1, 40, 4, 128), (3, 4, 2, 512), (3, 1, 6, 0), (2, 100, 2, 256), (1, 1, 2, 256), (3, 7, 4, 0), (1100, 1, 4, 256), (3, 1, 2, 256)]
+    need = max(cu.kv4_attention_scratch_bytes(n, n * m, m, heads, n_kv, hd, keys, split) for n, m, heads, split in shapes)
+    scratch = ctx.buffer(need).fill(0)
+    for n, m, heads, split in shapes:
+        q = Rows(ctx, n * m, heads * hd, "f32")
+        x = q.put(rng.standard_normal((n * m, heads * hd))).reshape(n, m, heads, hd)
+        seq = np.arange(n) % 3
+        got = attend(ctx, dev, q, seq, np.full(n, keys - m + 1), None, m, heads, 0.125, keys, split, scratch=scratch).get().reshape(n, m, heads, hd)
+        for i in list(range(min(n, 3))) + [n - 1]:
+            want, size, top = plain(x[i], *kv[seq[i]], [(0, keys - m + 1 + j) for j in range(m)], 0.125)
+            assert (np.abs(got[i] - want) <= bound("f32", want, size, top, hd, keys)).all(), (n, m, heads, split, i)
 
 
 # ---- through the engine -----------------------------------------------------------------------------
