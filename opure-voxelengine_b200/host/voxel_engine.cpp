@@ -230,14 +230,21 @@ void VoxelEngine::AllocBuffers() {
 }
 
 void *VoxelEngine::AttnScratch(uint32_t n, size_t *bytes) {
-    const auto key = std::make_tuple(n, runs_, longestRun_);
+    const graph::ModelConfig &c = graph_.Config();
+    // The 4-bit cache's calls share one buffer, whatever their shape. One that is too small for a new shape
+    // stays (graphs hold it) beside one of at least twice its size.
+    uint32_t key = n;
+    size_t need = 0, least = 0;
+    if (kv_.Fp4()) {
+        need = opure_kv4_attention_scratch_bytes(runs_ ? runs_ : n, n, runs_ ? longestRun_ : 1, c.numHeads, c.numKvHeads, c.HeadDim(), maxLen_, 0);
+        key = 0;
+        for (; attnScratch_.count(key) && attnScratch_[key].second < need; ++key) least = 2 * attnScratch_[key].second;
+    }
     auto it = attnScratch_.find(key);
     if (it == attnScratch_.end()) {
-        const graph::ModelConfig &c = graph_.Config();
-        const size_t b = kv_.Fp4() ? opure_kv4_attention_scratch_bytes(runs_ ? runs_ : n, n, runs_ ? longestRun_ : 1, c.numHeads,
-                                                                       c.numKvHeads, c.HeadDim(), maxLen_, 0)
-                                   : opure_attention_scratch_bytes(n, 1, c.numHeads, c.numKvHeads, c.HeadDim(), maxLen_, 0);
-        OPURE_CHECK(b > 0, "attention scratch size query failed");
+        if (!kv_.Fp4()) need = opure_attention_scratch_bytes(n, 1, c.numHeads, c.numKvHeads, c.HeadDim(), maxLen_, 0);
+        OPURE_CHECK(need > 0, "attention scratch size query failed");
+        const size_t b = std::max(need, least);
         void *p = nullptr;
         OPURE_CUDA_CHECK(opure_alloc(ctx_, b, &p));
         OPURE_CUDA_CHECK(opure_fill(ctx_, p, 0, b));  // split counters start at zero

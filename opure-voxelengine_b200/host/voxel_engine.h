@@ -237,8 +237,8 @@ private:
     void TpGemvAllreduce(const void *w, float scale, uint32_t rows, uint32_t cols, const float *in,
                          uint32_t in_stride, uint32_t n);
     void RecordAttention4(uint32_t layer, uint32_t n, uint32_t qkvRows, uint16_t *packed);
-    // Attention scratch for a step of n vectors (one zeroed buffer per shape of the call, so its
-    // split counters always start at zero).
+    // Attention scratch for a step of n vectors: with the fp16 cache one zeroed buffer per n, so its split
+    // counters always start at zero; with the 4-bit cache buffers 0, 1, .. each twice the last or larger.
     void *AttnScratch(uint32_t n, size_t *bytes);
     void ResetSequences(const std::vector<std::vector<uint32_t>> &prompts, uint32_t reserve, bool automatic);
     // Chunked prefill of slots 0..n-1 after ResetSequences(..., false); leaves them
@@ -259,7 +259,7 @@ private:
     float specAcceptance_ = -1.0f;
     // By vectors, logits, and the step's runs and longest run (0: an entry per vector).
     std::map<std::tuple<uint32_t, bool, uint32_t, uint32_t>, opure_graph *> graphs_;
-    std::map<std::tuple<uint32_t, uint32_t, uint32_t>, std::pair<void *, size_t>> attnScratch_;
+    std::map<uint32_t, std::pair<void *, size_t>> attnScratch_;
     uint32_t runs_ = 0, longestRun_ = 0;  // 4-bit KV cache: of the vectors that SetVectors described
     void *hostIo_ = nullptr;  // pinned staging of the host-driven step
     bool hostDriven_ = false; // step flags currently cleared for host-supplied tokens

@@ -4,6 +4,7 @@ is empty. Against a plain 64-bit implementation, with the bounds of test_gpu_kv4
 """
 import numpy as np
 import pytest
+import torch
 
 import kv4_reference as ref
 from test_gpu_kv4 import TYPES, Dev, attend, bound, ctx, release, tables  # noqa: F401 (fixtures)
@@ -229,3 +230,19 @@ def test_speculation_after_long_prompts(wide):
             got, _, _ = t.spec_generate(d, prompts, 12, k=5)
     for p, g in zip(prompts, got):
         assert len(g) == 12 and fwd.follows(p, g)
+
+
+def test_scores_of_many_lengths_share_their_scratch(wide):
+    """Chunks of 40 different lengths: the splits' sums of each take some 10 MB, in buffers that all share.
+    What is left to grow is the step graphs, below 2 MB each."""
+    path, _ = wide
+    p = prompt(9, WIDE, 300)
+    with ve.Engine(path, max_len=4096, kv=ve.KV_FP4, prefill_chunk=256) as eng:
+        first = eng.score([p])[0]["logprobs"]
+        eng.score([p[:258]])
+        free = torch.cuda.mem_get_info(0)[0]
+        for n in range(100, 260, 4):
+            got = eng.score([p[:n]])[0]["logprobs"]
+            assert np.abs(got - first[:n]).max() <= 2e-2
+        assert free - torch.cuda.mem_get_info(0)[0] < 40 * (2 << 20) + (40 << 20)
+        assert np.array_equal(eng.score([p])[0]["logprobs"], first)
