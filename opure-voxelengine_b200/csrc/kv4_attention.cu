@@ -508,13 +508,19 @@ constexpr uint32_t kCounters = 2048;
 constexpr size_t kPartialsAt = kCounters * sizeof(uint32_t);
 // More than kFewRows (query, head) rows per kv head go to the kernel for prompts.
 constexpr uint32_t kFewRows = 16;
-Plan make_plan(uint32_t n, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t split_tokens, int sms) {
+constexpr uint32_t kMaxUnits = 0x7fffffffu;  // a grid's, and a unit's rows
+Plan make_plan(uint32_t n, uint32_t n_rows, uint32_t n_q, uint32_t group, uint32_t n_kv, uint32_t hd, uint32_t max_ctx, uint32_t split_tokens, int sms) {
     Plan p{};
-    const uint64_t rows = uint64_t(n_q) * group;
+    const uint64_t rows = uint64_t(std::min(n_q, n_rows)) * group;  // no entry has more queries than there are
     p.prompt = rows > kFewRows;
     p.tile_rows = p.prompt ? kKv4PromptRows : rows <= 4 ? 4 : 8;
+    const uint64_t per_entry = (rows + p.tile_rows - 1) / p.tile_rows * n_kv;
+    if (rows > kMaxUnits || per_entry > kMaxUnits || n * per_entry > kMaxUnits) {
+        p.units = ~uint64_t(0);  // refused
+        return p;
+    }
     p.row_tiles = ceil_div(rows, p.tile_rows);
-    p.units = uint64_t(n) * p.row_tiles * n_kv;
+    p.units = n * per_entry;
     // Splits in steps of a chunk for each warp, or of prompts' tiles.
     const uint64_t unit = p.prompt ? kKv4PromptKeys : kWarps * kChunk, ctx = std::max(max_ctx, 1u);
     uint64_t want;
@@ -548,7 +554,8 @@ extern "C" size_t opure_kv4_attention_scratch_bytes(uint32_t n, uint32_t n_rows,
     if (!n || !n_rows || !n_q || !n_heads || !kv4_shape(n_kv, hd, 64) || n_heads % n_kv) return 0;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return std::max<size_t>(16, make_plan(n, n_q, n_heads / n_kv, n_kv, hd, max_ctx, split_tokens, sms).bytes);
+    const Plan p = make_plan(n, n_rows, n_q, n_heads / n_kv, n_kv, hd, max_ctx, split_tokens, sms);
+    return p.units > kMaxUnits ? 0 : std::max<size_t>(16, p.bytes);
 }
 
 extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn_args *a) {
@@ -564,9 +571,9 @@ extern "C" opure_status opure_kv4_attention(opure_ctx *ctx, const opure_kv4_attn
         return OPURE_ERR_INVALID_ARG;
     if (!a->q_begin && uint64_t(a->n) * a->n_q != a->n_rows) return OPURE_ERR_INVALID_ARG;
     if (cols > 0x7fffffffu || a->n_rows > 0x7fffffffu || a->max_ctx > 0x7fffffffu) return OPURE_ERR_UNSUPPORTED;
-    const Plan pl = make_plan(a->n, a->n_q, a->n_heads / a->kv.n_kv, a->kv.n_kv, hd, a->max_ctx, a->split_tokens, ctx->sm_count);
+    const Plan pl = make_plan(a->n, a->n_rows, a->n_q, a->n_heads / a->kv.n_kv, a->kv.n_kv, hd, a->max_ctx, a->split_tokens, ctx->sm_count);
+    if (pl.units > kMaxUnits) return OPURE_ERR_UNSUPPORTED;
     if (a->scratch_bytes < pl.bytes || reinterpret_cast<uintptr_t>(a->scratch) % 16) return OPURE_ERR_INVALID_ARG;
-    if (pl.units > 0x7fffffffu || pl.n_splits > 65535) return OPURE_ERR_UNSUPPORTED;
     Kv4AttnParams p{};
     p.q = a->q;
     p.out = a->out;

@@ -175,6 +175,11 @@ def test_queries_of_the_largest_size(ctx, t, hd, m):
         assert np.isnan(got[~ok]).all()
 
 
+def test_entries_without_a_limit_of_queries(ctx):
+    """n_q above what there are rows stands for no limit."""
+    check(ctx, "f32", 2, 2, 64, 64, [300, 500], [3, 4], n_q=2 ** 32 - 1)
+
+
 def test_one_scratch_for_calls_of_any_shape(ctx):
     """Zeroed once: each call leaves the counters as the next one needs them, whatever its shape."""
     rng = np.random.default_rng(4)

@@ -31,6 +31,18 @@ def test_page_bytes(n_kv, hd, page, want):
     assert cu.kv4_page_bytes(n_kv, hd, page) == want
 
 
+def test_scratch_of_any_sizes():
+    """No entry has more queries than there are rows; 0 for more work than a grid takes, at sizes that leave 32 bits
+    (or whose tiles are a multiple of 2^32)."""
+    size = cu.kv4_attention_scratch_bytes
+    assert size(1, 8, 2 ** 32 - 1, 4, 2, 64, 5000) == size(1, 8, 8, 4, 2, 64, 5000) > 16
+    assert size(1, 40, 2 ** 31, 512, 1, 64, 5000) == size(1, 40, 40, 512, 1, 64, 5000) > 16
+    assert size(1, 2 ** 31, 2 ** 31, 512, 1, 64, 5000) == 0
+    assert size(2 ** 32 - 1, 2 ** 31, 2 ** 20, 512, 64, 64, 5000) == 0
+    assert size(2 ** 32 - 1, 2 ** 32 - 1, 1, 1, 1, 64, 5000) == 0
+    assert size(2 ** 20, 2 ** 20, 1, 8, 8, 64, 5000, 256) == 16  # enough work without splits
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_offsets_cover_each_byte_once(hd):
     assert sorted(np.concatenate(ref.offsets(hd), 1).ravel()) == list(range(18 * hd))
