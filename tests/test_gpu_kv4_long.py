@@ -180,6 +180,27 @@ def test_entries_without_a_limit_of_queries(ctx):
     check(ctx, "f32", 2, 2, 64, 64, [300, 500], [3, 4], n_q=2 ** 32 - 1)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group,queries", [(3, 3), (4, 4), (16, 1), (17, 1), (1, 17)])
+def test_both_sides_of_the_choice_of_kernel(ctx, t, hd, group, queries):
+    """Up to 16 rows of a kv head probabilities of 16-bit types are pairs too, above one rounding to fp16."""
+    check(ctx, t, group, 2, hd, 32, [700, 90], [queries, 1], seed=group)
+
+
+@pytest.mark.parametrize("queries", [1, 30])
+@pytest.mark.parametrize("max_ctx", [0, 1, 256, 600])
+def test_an_understated_max_ctx_is_reported(ctx, queries, max_ctx):
+    """More keys than the splits that max_ctx asks for hold: reported; what was written is of the rows alone."""
+    rng = np.random.default_rng(1)
+    dev = Dev(ctx, random_cache(rng, 1, 20, 2, 64, 64))
+    q = Rows(ctx, queries, 2 * 64, "f32")
+    q.put(rng.standard_normal((queries, 128)))
+    out = attend(ctx, dev, q, [0], [1280 - queries + 1], [0, queries], queries, 2, 0.125, max_ctx)
+    assert ctx.last_error() == cu.ERR_DEVICE_BOUNDS
+    out.get()
+
+
 def test_one_scratch_for_calls_of_any_shape(ctx):
     """Zeroed once: each call leaves the counters as the next one needs them, whatever its shape."""
     rng = np.random.default_rng(4)
