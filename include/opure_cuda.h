@@ -441,8 +441,9 @@ opure_status opure_kv4_read(opure_ctx *ctx, const opure_kv4_read_args *a);
  * and left out); q_begin NULL: n_q rows each. Rows from q_begin[n] on are not touched. A query
  * without keys (seq[i] < 0, or seq_len[i] + j <= 0) gets zeros. Query head h reads kv head
  * h / (n_heads / n_kv). Sums and the softmax are fp32; queries and probabilities are split into
- * fp16 pairs, so that products keep 22 bits, except that with 16-bit types the probabilities of
- * entries with more than 16 (query, head) rows per kv head are rounded to fp16 once.
+ * fp16 pairs, so that products keep 22 bits (of what is far below a row's largest fewer: all are held
+ * to 2^-36 of it). With 16-bit types the probabilities of entries with more than 16 (query, head) rows
+ * per kv head, by n_q and n_rows, are rounded to fp16 once instead.
  *
  * scratch: opure_kv4_attention_scratch_bytes(...) bytes, 16-byte aligned, caller-owned. Zero before
  * the first call (opure_fill); every call leaves the counters at its start zero, so that calls of any

@@ -15,9 +15,10 @@
 // that a fifth fills by bulk copies: no barrier between warps until they merge their states. The running
 // maximum is raised only when a score passes it by 2^8 (probabilities stay below 2^8, the sums in fp32).
 //
-// What bounds it: issue of the conversions, some 366 instructions a warp for 32 positions, 67% of slots with DRAM at
-// 47%: 64 sequences of 32768 keys over 3 kv heads 125 us (3.6 TB/s), of 4096 over 32 heads 151 us (4.0 TB/s); one
-// sequence of 4000 8.5 us, which is the latency of a split and of joining the splits.
+// What bounds it: neither issue nor memory alone. Some 366 instructions a warp for 32 positions, most of them
+// conversions, take 67% of the issue slots with DRAM at 47%; the rest is waiting, with 16 working warps an SM.
+// 64 sequences of 32768 keys over 3 kv heads 125 us (3.6 TB/s), of 4096 over 32 heads 152 us (4.0 TB/s); one
+// sequence of 4000 8 us, which is the latency of a split and of joining the splits.
 #include <algorithm>
 
 #include "kv4_attention.cuh"

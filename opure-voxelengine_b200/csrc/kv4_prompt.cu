@@ -18,8 +18,9 @@
 // only when a score passes it by 2^4.
 //
 // What bounds it: 16,384 exponentials a tile of 64 keys and 256 rows at 16 a clock, 1,024 clocks; the
-// tensor cores need as long for fp32 (two MMAs for one), half for 16-bit types. A tile takes 2,200-2,600 clocks:
-// 4096 causal queries of 32 heads of 64 211 us with fp32, 173 with fp16; of 128 310 with fp32, 235 with bf16.
+// tensor cores need as long for fp32 (two MMAs for one), half for 16-bit types. A tile takes 2,200-2,600 clocks
+// (fp32: issue 49%, exponentials and conversions 32%, tensor cores 31% of the time):
+// 4096 causal queries of 32 heads of 64 214 us with fp32, 171 with fp16; of 128 318 with fp32, 241 with bf16.
 // (mma.sync took 980 us for the first of these, tiles of 128 keys with one score buffer a half 341.)
 #include <type_traits>
 
