@@ -175,6 +175,27 @@ def test_queries_of_the_largest_size(ctx, t, hd, m):
         assert np.isnan(got[~ok]).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k_scale,v_scale", [(2.0 ** -7, 8.0), (2.0 ** 40, 2.0 ** -60), (2.0 ** -60, 2.0 ** 10)])
+@pytest.mark.parametrize("queries", [3, 40])
+def test_tensor_scales(ctx, t, k_scale, v_scale, queries):
+    """Powers of two for all keys and all values, taken out of the call's scale again."""
+    rng = np.random.default_rng(queries)
+    n, heads, hd = 400, 2, 64
+    cache = random_cache(rng, 1, 7, 2, hd, 64)
+    k, v = cache.get(0, n)
+    cache.k_scale, cache.v_scale = k_scale, v_scale
+    dev = Dev(ctx, cache)
+    q = Rows(ctx, queries, heads * hd, t)
+    x = q.put(rng.standard_normal((queries, heads * hd))).reshape(queries, heads, hd)
+    got = attend(ctx, dev, q, [0], [n - queries + 1], [0, queries], queries, heads, 0.125 / k_scale, n, 256).get().reshape(queries, heads, hd)
+    want, size, top = plain(x, k, v, [(0, n - queries + 1 + j) for j in range(queries)], 0.125)
+    if t == "f16":  # as far as it holds them
+        want = np.clip(want * v_scale, -65504, 65504) / v_scale
+    tiny = 2.0 ** -25 / v_scale if t == "f16" else 0.0
+    assert (np.abs(got / v_scale - want) <= bound(t, want, size, top, hd, n, t != "f32") + tiny).all()
+
+
 def test_entries_without_a_limit_of_queries(ctx):
     """n_q above what there are rows stands for no limit."""
     check(ctx, "f32", 2, 2, 64, 64, [300, 500], [3, 4], n_q=2 ** 32 - 1)
@@ -272,3 +293,18 @@ def test_scores_of_many_lengths_share_their_scratch(wide):
             assert np.abs(got - first[:n]).max() <= 2e-2
         assert free - torch.cuda.mem_get_info(0)[0] < 40 * (2 << 20) + (40 << 20)
         assert np.array_equal(eng.score([p])[0]["logprobs"], first)
+
+
+def test_scores_of_a_window(wide):
+    """Sequences that fit the window score as without one; longer ones are refused."""
+    path, _ = wide
+    p = prompt(10, WIDE, 200)
+    with ve.Engine(path, max_len=1024, kv=ve.KV_FP4, prefill_chunk=64, page_size=32, kv_window=256) as eng:
+        got = eng.score([p], 3)[0]
+        with pytest.raises(cu.OpureError):
+            eng.score([prompt(11, WIDE, 400)])
+        again = eng.score([p], 3)[0]
+    with ve.Engine(path, max_len=1024, kv=ve.KV_FP4, prefill_chunk=64, page_size=32) as eng:
+        want = eng.score([p], 3)[0]
+    assert all(np.array_equal(got[k], again[k]) for k in got)
+    assert np.abs(got["logprobs"] - want["logprobs"]).max() <= 2e-2
