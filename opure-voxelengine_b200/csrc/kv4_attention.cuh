@@ -18,8 +18,8 @@ struct Kv4AttnParams {
     float factor;            // scale * log2(e) * k_scale
     float v_scale;
     uint32_t split_tokens, n_splits;
+    uint32_t *counters;      // [unit], at the scratch's start
     float *partials;         // [unit][split][row of the tile][HD + 2]
-    uint32_t *counters;      // [unit]
     opure_kv4_layout kv;
     DeviceStatus *st;
     __half *out_packed;

@@ -21,9 +21,10 @@
 // cluster of up to 8 CTAs, whose parts meet in distributed shared memory.
 // Bound by memory while there are many rows: 4096 rows of 49152 fp32 logits take 139-144 us without best
 // tokens and 165-170 us with 5 (5.6 and 4.8 TB/s of 6.5 measured), 203 us with 20. With the finishing done by
-// the four warps themselves it was 215 us with 5. In fp16, 158 us (2.5 TB/s), and rows of 4096 logits 54 us (fp32
-// 59): the finishing of a row, some 9,000 clocks whatever its length, bounds these. A single row, a cluster of 8, is latency: 5.5 us, 13.6 us
-// with 20 best tokens (11.1 us when four warps finished it; kept, since one way serves all sizes).
+// the four warps themselves it was 215 us with 5. In fp16 they take 158 us (2.5 TB/s), and 4096 rows of 4096
+// logits 54 us (fp32 59): the finishing of a row, some 9,000 clocks whatever its length, bounds these. A single
+// row, a cluster of 8, is latency: 5.5 us, 13.6 us with 20 best tokens (11.1 us when four warps finished it;
+// kept, since one way serves all sizes).
 #include <algorithm>
 
 #include "attn_core.cuh"
